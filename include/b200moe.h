@@ -46,6 +46,10 @@ enum {
 
 /* kinds of router input accepted by the top-k epilogue */
 enum { B200MOE_LOGITS_BF16 = 0, B200MOE_LOGITS_F32 = 1, B200MOE_SCORES_F32 = 2 };
+/* ... and by the group-limited top-k and the router losses: LOGITS_BF16, LOGITS_F32 and */
+enum { B200MOE_LOGITS_F16 = 3 };
+/* their scores */
+enum { B200MOE_SIGMOID = 0, B200MOE_SOFTMAX = 1 };
 
 const char* b200moe_version(void);
 const char* b200moe_last_error_string(void);
@@ -90,6 +94,31 @@ int b200moe_router_small_fwd(const void* x, const void* weight, const float* bia
 int b200moe_router_topk_bwd(const void* logits, int input_kind, const int64_t* idx,
                             const float* grad_w, int64_t T, int E, int k, int norm_topk, float scale,
                             void* grad_logits, b200moe_stream_t stream);
+
+/* Group-limited top-k (no counterpart in the reference): s = sigmoid(z) or softmax(z) of logits (T,E), v = s + bias; of `groups`
+ * equal groups of neighbouring experts the `open` best, by their largest v or (group_top2) the sum of their two largest; the k
+ * best experts of those, equal values to the lowest index, decided as for real numbers (values that fp32 does not tell apart are
+ * compared in 64 bits); w = s, optionally / (sum + 1e-20), * scale.  logits_type: B200MOE_LOGITS_BF16 / _F32 / _F16.
+ * bias (E, nullable): selection only.  A row of -inf scores 0 everywhere; NaN ranks first.  counts nullable. */
+int b200moe_group_topk_fwd(const void* logits, int logits_type, const float* bias, int64_t T, int E, int k, int groups, int open,
+                           int scoring, int group_top2, int norm_topk, float scale, int64_t* idx, float* w, int32_t* counts,
+                           b200moe_stream_t stream);
+/* grad_logits (T,E), in the logits' type, from grad_w (T,k) at the picks idx. */
+int b200moe_group_topk_bwd(const void* logits, int logits_type, const int64_t* idx, const float* grad_w, int64_t T, int E, int k,
+                           int scoring, int norm_topk, float scale, void* grad_logits, b200moe_stream_t stream);
+/* Router losses (no counterpart in the reference) of `segs` segments of S tokens each, logits (segs*S,E), picks idx (segs*S,k):
+ * losses[0] = mean over the segments that have tokens of sum_e f_e P_e, f_e = E / (k n) * picks of e, P_e = mean of p_e,
+ * p = softmax(z) or sigmoid(z) / sum sigmoid(z); losses[1] = mean over all tokens of (log sum exp z)^2.  A token counts unless
+ * mask (nullable, one byte a token) is 0 or all its logits are -inf.  coef (segs*E + 2 fp32): what the backward needs.
+ * ws: b200moe_router_losses_ws_bytes, 8-byte aligned. */
+size_t b200moe_router_losses_ws_bytes(int64_t S, int segs, int E);
+int b200moe_router_losses_fwd(const void* logits, int logits_type, const int64_t* idx, const uint8_t* mask, int64_t S, int segs,
+                              int E, int k, int scoring, void* ws, float* coef, float* losses, int32_t* status,
+                              b200moe_stream_t stream);
+/* grad_logits from the device scalars grad_balance, grad_z (nullable: 0). */
+int b200moe_router_losses_bwd(const void* logits, int logits_type, const uint8_t* mask, const float* coef,
+                              const float* grad_balance, const float* grad_z, int64_t S, int segs, int E, int scoring,
+                              void* grad_logits, b200moe_stream_t stream);
 
 /* Replaces router_bias_update (kernels/sm75/router.py:292-301): b += u*sign(mean(c)-c); no-op u<=0. */
 int b200moe_router_bias_update(float* bias, const int32_t* counts, int E, float u,

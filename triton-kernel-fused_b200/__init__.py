@@ -5,6 +5,7 @@ Requires the in-tree libb200moe.so (see _lib.build); there is no CPU or library 
 from ._lib import build, check_status, lib, LIB_PATH, EXPORTED
 from .moe import moe, moe_grouped, moe_per_expert, GROUPED_MIN_TOKENS
 from .router import fused_mlp_router, FusedMLPRouter, fused_router, FusedConvRouter, router_bias_update
+from .router import fused_group_router, group_topk, router_losses
 from .layer import MoELayer
 from .mxfp8 import moe_mxfp8
 from . import ops
@@ -14,4 +15,4 @@ from . import muon
 from .muon import DistributedMuon, FusedMuon, newton_schulz
 
 __all__ = ["moe", "moe_grouped", "moe_per_expert", "GROUPED_MIN_TOKENS", "fused_mlp_router", "fused_router", "FusedConvRouter",
-           "FusedMLPRouter", "router_bias_update", "MoELayer", "moe_mxfp8", "ExpertParallelMoELayer", "ep_moe", "FusedMuon", "DistributedMuon", "newton_schulz", "muon", "ops", "build", "lib", "check_status"]
+           "FusedMLPRouter", "router_bias_update", "fused_group_router", "group_topk", "router_losses", "MoELayer", "moe_mxfp8", "ExpertParallelMoELayer", "ep_moe", "FusedMuon", "DistributedMuon", "newton_schulz", "muon", "ops", "build", "lib", "check_status"]

@@ -5,6 +5,7 @@ fallback: if the library is missing or a call fails, a Python exception is raise
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import importlib
 import os
@@ -41,6 +42,11 @@ _SIGNATURES = {
     "b200moe_router_topk_bwd": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_int, c_int,
                                         c_float, c_void_p, c_void_p]),
     "b200moe_router_bias_update": (c_int, [c_void_p, c_void_p, c_int, c_float, c_void_p]),
+    "b200moe_group_topk_fwd": (c_int, [c_void_p, c_int, c_void_p, c_int64] + [c_int] * 7 + [c_float] + [c_void_p] * 4),
+    "b200moe_group_topk_bwd": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64] + [c_int] * 4 + [c_float] + [c_void_p] * 2),
+    "b200moe_router_losses_ws_bytes": (c_size_t, [c_int64, c_int, c_int]),
+    "b200moe_router_losses_fwd": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64] + [c_int] * 4 + [c_void_p] * 5),
+    "b200moe_router_losses_bwd": (c_int, [c_void_p, c_int] + [c_void_p] * 4 + [c_int64] + [c_int] * 3 + [c_void_p] * 2),
     "b200moe_conv_unfold": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p]),
     "b200moe_conv_fold": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p]),
     "b200moe_conv_gemm_fwd": (c_int, [c_void_p] * 3 + [c_int64] * 4 + [c_int, c_void_p, c_void_p]),
@@ -219,6 +225,14 @@ def stream_of(t: torch.Tensor):
     """The raw handle of the current stream of t's device (torch.cuda.current_stream builds a Stream object around it,
     which costs more than a launch)."""
     return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+_same_device = contextlib.nullcontext()
+
+
+def on_device_of(t: torch.Tensor):
+    """Context in which t's device is the current one: a launch on a stream of another device is an error."""
+    return _same_device if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def capturing(t: torch.Tensor) -> bool:

@@ -10,7 +10,9 @@ import torch
 
 from . import _lib as L
 
-LOGITS_BF16, LOGITS_F32, SCORES_F32 = 0, 1, 2
+LOGITS_BF16, LOGITS_F32, SCORES_F32, LOGITS_F16 = 0, 1, 2, 3
+SIGMOID, SOFTMAX = 0, 1
+_LOGITS = {torch.bfloat16: LOGITS_BF16, torch.float32: LOGITS_F32, torch.float16: LOGITS_F16}
 TILE_M = 256   # B200MOE_TILE_M: expert segments are padded to this many rows
 
 # Optional observer used by the benchmark: hook(name, kernel_launches, start_event, end_event) is
@@ -115,6 +117,65 @@ def router_topk_bwd(logits, idx, grad_w, norm_topk=True, scale=1.0):
     gl = torch.empty(N, E, dtype=torch.bfloat16, device=logits.device)
     L.check(L.lib().b200moe_router_topk_bwd(L.ptr(logits), _kind(logits, False), L.ptr(idx), L.ptr(gw), N, E, k,
                                             int(bool(norm_topk)), float(scale), L.ptr(gl), L.stream_of(logits)))
+    return gl
+
+
+def _logits_type(logits):
+    L.require(logits.is_cuda, "logits must be a CUDA tensor (this package has no CPU path)")
+    L.require(logits.dtype in _LOGITS, f"logits must be bfloat16, float16 or float32, got {logits.dtype}")
+    L.require(logits.is_contiguous(), "logits must be contiguous")
+    return _LOGITS[logits.dtype]
+
+
+@_op("group_topk_fwd", 1)
+def group_topk_fwd(logits, bias, top_k, groups, open_groups, scoring, top2, norm_topk=True, scale=1.0, want_counts=True):
+    """(N,E) logits -> idx int64 (N,k), w fp32 (N,k), counts int32 (E,) or None: the top-k of the `open_groups` best groups."""
+    kind, (N, E), dev = _logits_type(logits), logits.shape, logits.device
+    if bias is not None:
+        L.require(bias.device == dev and bias.dtype == torch.float32 and bias.numel() == E and bias.is_contiguous(),
+                  "bias must be a contiguous float32 tensor of E elements on the logits' device")
+    with L.on_device_of(logits):
+        idx = torch.empty(N, top_k, dtype=torch.int64, device=dev)
+        w = torch.empty(N, top_k, dtype=torch.float32, device=dev)
+        counts = torch.empty(E, dtype=torch.int32, device=dev) if want_counts else None
+        # no rows: the pointers of empty tensors are null, and only the counts are written
+        L.check(L.lib().b200moe_group_topk_fwd(logits.data_ptr() or 16, kind, L.ptr(bias), N, E, top_k, groups, open_groups, scoring,
+                                               int(top2), int(norm_topk), scale, idx.data_ptr() or 16, w.data_ptr() or 16,
+                                               L.ptr(counts), L.stream_of(logits)))
+    return idx, w, counts
+
+
+@_op("group_topk_bwd", 1)
+def group_topk_bwd(logits, idx, grad_w, scoring, norm_topk=True, scale=1.0):
+    kind, (N, E), gl = _logits_type(logits), logits.shape, torch.empty_like(logits)
+    if N:
+        with L.on_device_of(logits):
+            L.check(L.lib().b200moe_group_topk_bwd(logits.data_ptr(), kind, idx.data_ptr(), grad_w.data_ptr(), N, E, idx.shape[1], scoring,
+                                                   int(norm_topk), scale, gl.data_ptr(), L.stream_of(logits)))
+    return gl
+
+
+@_op("router_losses_fwd", 3)
+def router_losses_fwd(logits, idx, mask, segments, scoring):
+    """logits (N,E) and picks (N,k) of `segments` equal segments -> (losses (2,) fp32, coefficients for the backward)."""
+    kind, (N, E), dev = _logits_type(logits), logits.shape, logits.device
+    with L.on_device_of(logits):
+        coef = torch.empty(segments * E + 2, dtype=torch.float32, device=dev)
+        losses = torch.empty(2, dtype=torch.float32, device=dev)
+        lib, S = L.lib(), N // segments
+        ws = L.workspace(lib.b200moe_router_losses_ws_bytes(S, segments, E), dev)
+        L.check(lib.b200moe_router_losses_fwd(logits.data_ptr(), kind, idx.data_ptr(), L.ptr(mask), S, segments, E, idx.shape[1], scoring,
+                                              ws.data_ptr(), coef.data_ptr(), losses.data_ptr(), L.status_word(dev).data_ptr(),
+                                              L.stream_of(logits)))
+    return losses, coef
+
+
+@_op("router_losses_bwd", 1)
+def router_losses_bwd(logits, mask, coef, grad_balance, grad_z, segments, scoring):
+    kind, (N, E), gl = _logits_type(logits), logits.shape, torch.empty_like(logits)
+    with L.on_device_of(logits):
+        L.check(L.lib().b200moe_router_losses_bwd(logits.data_ptr(), kind, L.ptr(mask), coef.data_ptr(), L.ptr(grad_balance), L.ptr(grad_z),
+                                                  N // segments, segments, E, scoring, gl.data_ptr(), L.stream_of(logits)))
     return gl
 
 

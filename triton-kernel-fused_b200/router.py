@@ -12,7 +12,8 @@ import torch
 from . import _lib as L
 from . import ops
 
-__all__ = ["fused_mlp_router", "FusedMLPRouter", "fused_router", "FusedConvRouter", "router_bias_update"]
+__all__ = ["fused_mlp_router", "FusedMLPRouter", "fused_router", "FusedConvRouter", "router_bias_update", "group_topk", "fused_group_router",
+           "router_losses"]
 
 
 class FusedMLPRouter(torch.autograd.Function):
@@ -172,6 +173,162 @@ def fused_router(x, conv_weight, bias, top_k, num_experts, norm_topk_prob=True, 
     idx = idx.view(B, S, top_k)
     w = w.view(B, S, top_k)
     return (idx, w, counts) if return_counts else (idx, w)
+
+
+# ---------------------------------------------------------------------------- groups of experts, softmax scores, losses
+_SCORING = {"sigmoid": ops.SIGMOID, "softmax": ops.SOFTMAX}
+_GROUP_SCORE = {"top2": 1, "max": 0}
+
+
+class _GroupTopk(torch.autograd.Function):
+    """(idx (N,k) int64, weights (N,k) fp32, counts (E,) int32) of contiguous logits (N,E); only the weights are differentiable."""
+
+    @staticmethod
+    def forward(ctx, logits, bias, top_k, groups, opened, scoring, top2, norm, scale):
+        idx, w, counts = ops.group_topk_fwd(logits, bias, top_k, groups, opened, scoring, top2, norm, scale)
+        ctx.args = (scoring, norm, scale)
+        ctx.save_for_backward(logits, idx)
+        ctx.mark_non_differentiable(idx, counts)
+        ctx.set_materialize_grads(False)      # no zero-filled gradients for idx and counts
+        return idx, w, counts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_idx, grad_weights, grad_counts):
+        if grad_weights is None:
+            return (None,) * 9
+        logits, idx = ctx.saved_tensors
+        return (ops.group_topk_bwd(logits, idx, grad_weights.float().contiguous(), *ctx.args),) + (None,) * 8
+
+
+def group_topk(logits, top_k, bias=None, num_groups=1, topk_groups=None, scoring="sigmoid", group_score="top2", norm_topk_prob=True,
+               routed_scaling_factor=1.0, return_counts=False):
+    """Group-limited top-k of router logits (N,E) or (B,S,E), bf16, fp16 or fp32 -> (idx int64 (...,k), weights fp32 (...,k)
+    [, counts (E,) int32]).  Scores are sigmoid(logits) or softmax(logits); `bias` (E,) is added for selection only; the E experts form
+    `num_groups` (1..32) equal groups of neighbours, of which the `topk_groups` (default: all) with the largest value are open: the sum of
+    a group's two best experts, or its best one (group_score "max").  The k best experts of the open groups are the picks, in
+    descending order, equal values in the order of the experts, and their unbiased scores the weights: divided by their sum + 1e-20
+    where norm_topk_prob and k > 1, times routed_scaling_factor.  Picks are decided as for real numbers: without a bias by the logits
+    themselves, with one in 64 bits where fp32 would round.  A row of -inf scores 0 everywhere; NaN ranks first.
+    E <= 256, k <= 32 and at most the experts of the open groups.  Differentiable in the logits."""
+    L.require(scoring in _SCORING, f"scoring must be 'sigmoid' or 'softmax', got {scoring!r}")
+    L.require(group_score in _GROUP_SCORE, f"group_score must be 'top2' or 'max', got {group_score!r}")
+    L.require(logits.dim() in (2, 3), "logits must be (N,E) or (B,S,E)")
+    L.require(logits.is_cuda, "logits must be a CUDA tensor (this package has no CPU path)")
+    opened = int(num_groups) if topk_groups is None else int(topk_groups)
+    if bias is not None:
+        bias = bias.detach()
+        L.require(bias.device == logits.device and bias.numel() == logits.shape[-1], "bias must have E elements on the logits' device")
+        if bias.dtype != torch.float32 or not bias.is_contiguous():
+            bias = bias.float().contiguous()
+    flat = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
+    flat = flat.contiguous()
+    k = int(top_k)
+    L.require(k >= 1, f"top_k = {k} must be positive")
+    args = (bias, k, int(num_groups), opened, _SCORING[scoring], _GROUP_SCORE[group_score], bool(norm_topk_prob and k > 1),
+            float(routed_scaling_factor))
+    if torch.is_grad_enabled() and flat.requires_grad:
+        idx, w, counts = _GroupTopk.apply(flat, *args)
+    else:
+        idx, w, counts = ops.group_topk_fwd(flat, *args, want_counts=return_counts)
+    if logits.dim() == 3:
+        idx, w = idx.view(*logits.shape[:2], k), w.view(*logits.shape[:2], k)
+    return (idx, w, counts) if return_counts else (idx, w)
+
+
+class _RouterLogits(torch.autograd.Function):
+    """logits (N,E) = x (N,H) @ weight (E,H)^T in bf16, fp32 accumulation: the products of `FusedMLPRouter` by themselves."""
+
+    @staticmethod
+    def forward(ctx, x, weight):
+        if torch.is_autocast_enabled("cuda"):
+            dt = torch.get_autocast_dtype("cuda")
+            x, weight = x.to(dt), weight.to(dt)
+        L.require_cuda_bf16("x", x)
+        L.require_cuda_bf16("gate_weight", weight)
+        L.require(weight.dim() == 2 and weight.shape[1] == x.shape[1], "gate_weight must be (E,H)")
+        L.require(weight.device == x.device, "gate_weight must be on x's device")
+        x, weight = x.contiguous(), weight.contiguous()
+        ctx.save_for_backward(x, weight)
+        with L.on_device_of(x):
+            return ops.gemm_nt(x, weight)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, weight = ctx.saved_tensors
+        grad = grad.to(torch.bfloat16).contiguous()
+        with L.on_device_of(x):
+            return (ops.gemm_nn(grad, weight) if ctx.needs_input_grad[0] else None,
+                    ops.gemm_tn(grad, x) if ctx.needs_input_grad[1] else None)
+
+
+def fused_group_router(x, gate_weight, bias, top_k, num_experts, num_groups=1, topk_groups=None, scoring="sigmoid", group_score="top2",
+                       norm_topk_prob=True, routed_scaling_factor=1.0, return_counts=False, return_logits=False):
+    """`fused_mlp_router` with softmax or sigmoid scores and groups of experts (`group_topk`): x (B,S,H) or (N,H), gate_weight (E,H) ->
+    (idx, weights[, counts][, logits]).  The logits are bf16 and differentiable, for `router_losses`."""
+    L.require(num_experts is None or int(num_experts) == gate_weight.shape[0], "num_experts must equal gate_weight.shape[0]")
+    flat = x.reshape(-1, x.shape[-1])
+    if flat.shape[0] == 0:
+        logits = (flat[:, :1] + 0.0 * gate_weight.sum()).expand(0, gate_weight.shape[0]).contiguous()
+    else:
+        logits = _RouterLogits.apply(flat, gate_weight)
+    logits = logits.view(*x.shape[:-1], gate_weight.shape[0])
+    res = group_topk(logits, top_k, bias, num_groups, topk_groups, scoring, group_score, norm_topk_prob, routed_scaling_factor,
+                     return_counts)
+    return res + (logits,) if return_logits else res
+
+
+class _RouterLosses(torch.autograd.Function):
+    """(balance, z) of contiguous logits (N,E) and picks (N,k) of `segments` equal segments."""
+
+    @staticmethod
+    def forward(ctx, logits, idx, mask, segments, scoring):
+        losses, coef = ops.router_losses_fwd(logits, idx, mask, segments, scoring)
+        ctx.args = (segments, scoring)
+        ctx.save_for_backward(logits, mask, coef)
+        ctx.set_materialize_grads(False)
+        return losses[0], losses[1]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_balance, grad_z):
+        if grad_balance is None and grad_z is None:
+            return (None,) * 5
+        logits, mask, coef = ctx.saved_tensors
+        gb, gz = (None if g is None else g.float().contiguous() for g in (grad_balance, grad_z))
+        return (ops.router_losses_bwd(logits, mask, coef, gb, gz, *ctx.args),) + (None,) * 4
+
+
+def router_losses(logits, top_k_indices, scoring="softmax", mask=None, per_sequence=False):
+    """(balance, z): two fp32 scalars, differentiable in the logits (N,E) or (B,S,E), bf16, fp16 or fp32.
+
+    balance = sum_e f_e P_e with f_e = E / (k n) * (picks of e among the n tokens) and P_e the mean of p_e, p = softmax(logits) or
+    sigmoid(logits) / their sum: 1 for even routing.  per_sequence: of every sequence of (B,S,E) by itself, averaged over the
+    sequences that have tokens.  z = mean over the tokens of (log sum exp logits)^2.  `top_k_indices` (...,k): the picks, as the
+    router gave them (a pick outside [0,E) is not counted and raises the status word).  mask (...): tokens that count (None: all); one whose
+    logits are all -inf never does.  Tokens that do not count are not read and get a zero gradient; without any the losses are 0."""
+    L.require(scoring in _SCORING, f"scoring must be 'sigmoid' or 'softmax', got {scoring!r}")
+    L.require(logits.dim() in (2, 3), "logits must be (N,E) or (B,S,E)")
+    L.require(logits.is_cuda, "logits must be a CUDA tensor (this package has no CPU path)")
+    L.require(not per_sequence or logits.dim() == 3, "per_sequence needs logits (B,S,E)")
+    idx = top_k_indices
+    L.require(idx.device == logits.device and idx.dtype == torch.int64 and idx.dim() == logits.dim() and idx.shape[:-1] == logits.shape[:-1],
+              "top_k_indices must be int64 (...,k) on the logits' device")
+    E = logits.shape[-1]
+    if mask is not None:
+        L.require(mask.device == logits.device and mask.shape == logits.shape[:-1], "mask must have the tokens' shape, on the logits' device")
+        mask = (mask if mask.dtype == torch.bool else mask != 0).contiguous()
+    segments = logits.shape[0] if per_sequence and logits.shape[0] > 0 else 1
+    flat = (logits if logits.dim() == 2 else logits.reshape(-1, E)).contiguous()
+    idx = idx.reshape(-1, idx.shape[-1]).contiguous()
+    if flat.shape[0] == 0:
+        zero = flat.float().sum()
+        return zero, zero.clone()
+    if torch.is_grad_enabled() and flat.requires_grad:
+        return _RouterLosses.apply(flat, idx, mask, segments, _SCORING[scoring])
+    losses, _ = ops.router_losses_fwd(flat, idx, mask, segments, _SCORING[scoring])
+    return losses[0], losses[1]
 
 
 @torch.no_grad()
