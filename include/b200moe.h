@@ -349,6 +349,30 @@ int b200moe_mxfp8_expert_wgrad(const void* Atq, const void* Atsf, const void* Bt
                                const int32_t* poffs, const int32_t* counts, int64_t rows_cap, int E,
                                int64_t Na, int64_t Nb, void* out, int32_t* status, b200moe_stream_t stream);
 
+/* ---- e4m3 with an fp32 scale per block of 128 (no counterpart in the reference) -----------------
+ * Activations: a scale per row and 128 values; weights: one per 128 x 128 values, (groups, ceil(N/128), ceil(K/128)), as
+ * checkpoints hold them.  scale = max(|v|, 2^-100) / 448 of a block, code = nearest e4m3 to 448 v / max(|v|), ties to even;
+ * a block with NaN or infinity has such a scale, and what is computed from it is NaN.  Products add up each block of K in
+ * fp32, scale the sum and add it to an fp32 accumulator. */
+/* x (rows,K) bf16 -> q (rows, ldq bytes apart), scale [k-block][scale_pitch >= rows]; K % 8 == 0, ldq % 8 == 0. */
+int b200moe_fp8_block_quant(const void* x, int64_t rows, int64_t K, void* q, int64_t ldq, float* scale, int64_t scale_pitch,
+                            b200moe_stream_t stream);
+/* w (groups,N,K) bf16 -> q, scale as above; K % 8 == 0. */
+int b200moe_fp8_block_quant_weight(const void* w, int64_t groups, int64_t N, int64_t K, void* q, float* scale,
+                                   b200moe_stream_t stream);
+/* The weights w (N,K) e4m3, w_scale: out (M,N) bf16 = quantised x (M,K) * w^T, or (transposed) out (M,K) = quantised x (M,N) * w:
+ * the gradient of x from that of out.  x bf16; N % 8 == 0, K % 16 == 0; all 16-byte aligned.
+ * ws: b200moe_fp8_block_linear_ws_bytes(M, reduction length). */
+size_t b200moe_fp8_block_linear_ws_bytes(int64_t M, int64_t K);
+int b200moe_fp8_block_linear(const void* x, const void* w, const float* w_scale, int64_t M, int64_t N, int64_t K, int transposed,
+                             void* ws, void* out, int32_t* status, b200moe_stream_t stream);
+/* The experts on given picks, forward (SiLU-GLU): gate_up (E,2I,H) and down (E,H,I) e4m3 with their scales, x (T,H) bf16,
+ * idx (T,k) int64, w (T,k) fp32, out (T,H) bf16; H and I multiples of 128.  silu(gate) * up is requantised from fp32. */
+size_t b200moe_moe_fp8_block_ws_bytes(int64_t T, int64_t H, int64_t I, int E, int k);
+int b200moe_moe_fp8_block_forward(const void* x, const int64_t* idx, const float* w, const void* gate_up, const float* gate_up_scale,
+                                  const void* down, const float* down_scale, int64_t T, int64_t H, int64_t I, int E, int k,
+                                  void* ws, void* out, int32_t* status, b200moe_stream_t stream);
+
 /* ---- combine -------------------------------------------------------------------------------- */
 /* Replaces _combine_scatter_kernel / index_add_ (kernels/sm75/moe.py:673-682, :593-595):
  * out[t] = sum_j w[t,j] * rows[slot_row[t*k+j]], fp32 accumulate in slot order, bf16 store.

@@ -1,0 +1,908 @@
+// Products of e4m3 codes with fp32 scales per block of 128: rows of X carry a scale per row and 128 values of K, weights one per 128 x 128
+// values.  tcgen05.mma.kind::f8f6f4, dense and grouped by experts, and the experts' SwiGLU with requantisation in the epilogue.
+//
+//   out[t, n] = sum_kb  sx[t, kb] * sw[n / 128, kb] * sum_{k in kb} X[t, k] W[n, k]
+//
+// The scales are arbitrary fp32 numbers, so the tensor cores cannot apply them: every k-block of 128 is a sum of its own in tensor
+// memory, which the epilogue warps fetch and add to accumulators in registers, times its scales (one multiply-add a value).  Tensor memory
+// is a ring, so that the MMAs of the next k-blocks run meanwhile.
+#include <cuda.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "few_tiles.cuh"
+#include "fp8_block.cuh"
+#include "gemm_common.cuh"
+
+namespace b200moe {
+
+constexpr int kBBK = 128;                 // k-block in elements = bytes: one swizzle row, four MMAs
+constexpr int kBTile = 128 * kBBK;        // one operand box
+
+struct BlockParams {
+  GemmParams g;             // sched, M, N (SwiGLU: I), K, num_groups, tile_expert, poffs, counts, status
+  const float* sx;          // scales of X, [k-block][row]
+  long long sx_pitch;
+  long long rows;           // rows of X that exist
+  const float* sw;          // scales of the weights: group, column block, k-block
+  long long sw_group;
+  int sw_n, sw_k;           // elements between column blocks and between k-blocks
+  int n_blocks;             // column blocks of one matrix (SwiGLU: of the gate half)
+  uint8_t* q_out;           // SwiGLU: codes (rows, I) and their scales [column block][row]
+  float* q_scale;
+  long long q_pitch;
+  __nv_bfloat16* out;       // few rows: (rows, N)
+  int split;                // few rows: CTAs of a cluster that share a tile's k-blocks
+  int first_dense;          // few rows, dense: rows of X (no table)
+};
+
+__device__ __forceinline__ void umma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_f8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// e4m3 (format 0) operands, fp32 result; bit 16: B is MN-major
+__host__ __device__ constexpr uint32_t idesc_f8(int m, int n, int b_mn) {
+  return (1u << 4) | (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+// two multiply-adds in one instruction
+__device__ __forceinline__ void fma2(float2& d, uint32_t a0, uint32_t a1, float2 f) {
+  asm("{\n\t.reg .b64 a, f, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 f, {%4, %5};\n\tmov.b64 d, {%0, %1};\n\t"
+      "fma.rn.f32x2 d, a, f, d;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "+f"(d.x), "+f"(d.y)
+      : "r"(a0), "r"(a1), "f"(f.x), "f"(f.y));
+}
+// N of the warp's 32 lanes' consecutive fp32 columns
+template <int N>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[N]) {
+  if constexpr (N == 32) tmem_ld32(taddr, r);
+  else if constexpr (N == 16) tmem_ld16(taddr, r);
+  else
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
+
+// ------------------------------------------------------------------------------------------------ many rows: pairs of SMs
+// A cluster of two CTAs computes 256 rows x 256 columns with cta_group::2 MMAs: each stages its own 128 rows of X and 128 rows of W (SwiGLU: one
+// the gate, the other the up rows of the same 128 columns).  Two k-blocks' sums of 256 columns fill tensor memory.  An epilogue warp owns
+// 32 rows and 128 columns (SwiGLU: 64 of gate and the same 64 of up), so its scales are one number a thread and k-block, or two.
+constexpr int kBStages = 6;
+constexpr int kBStage = 2 * kBTile;
+template <int EPI> constexpr int kBEpiBytes = EPI == EPI_STORE ? kEpiWarps * kStageOutBytes : 0;     // SwiGLU stores its codes from registers
+template <int EPI> constexpr int kBSmemBytes = kBStages * kBStage + kBEpiBytes<EPI> + (2 * kBStages + 4) * 8 + 16 + 1024;
+
+template <int EPI, bool BMN>
+__global__ void __launch_bounds__(kThreads, 1)
+block_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmD,
+                  const BlockParams bp) {
+  const GemmParams& p = bp.g;
+  constexpr int TM = 256, TN = EPI == EPI_SWIGLU ? 128 : 256;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* epi_smem = smem + kBStages * kBStage;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(epi_smem + kBEpiBytes<EPI>);
+  const uint32_t bar_full = smem_u32(bars);
+  const uint32_t bar_empty = smem_u32(bars + kBStages);
+  const uint32_t bar_tfull = smem_u32(bars + 2 * kBStages);
+  const uint32_t bar_tempty = smem_u32(bars + 2 * kBStages + 2);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kBStages + 4);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  __shared__ uint32_t s_amax[2][2][128];
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int cta_rank = static_cast<int>(cluster_ctarank());
+  const int first_tile = static_cast<int>(cluster_id_x());
+  const int tile_step = static_cast<int>(num_clusters_x());
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kBStages; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar_tfull + 8 * b, 1);
+      mbar_init(bar_tempty + 8 * b, 2 * kEpiWarps);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    if (EPI == EPI_STORE) tma_prefetch_desc(&tmD);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_slot), 512);
+    tmem_relinquish_pair();
+  }
+  grid_dep_wait();
+  tc_fence_before();
+  __syncthreads();
+  __syncwarp();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int total = total_tiles(p, TN, TM);
+  const int nkb = (p.K + kBBK - 1) / kBBK;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------------------ producer (each CTA)
+    if (elect_one()) {
+      const uint32_t full0 = mapa_shared(bar_full, 0);
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int tile = first_tile; tile < total && ok; tile += tile_step) {
+        const Tile t = get_tile(p, tile, TN, TM, kBBK);
+        const int m0 = t.m0 + BM * cta_rank;
+        const int n0 = EPI == EPI_SWIGLU ? t.n0 + p.I * cta_rank : t.n0 + 128 * cta_rank;
+        for (int kb = 0; kb < nkb; ++kb) {
+          if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, ST_WAIT_PRODUCER)) {
+            ok = false;
+            break;
+          }
+          if (cta_rank == 0) mbar_arrive_expect_tx(bar_full + 8 * s, 2 * kBStage);
+          const uint32_t sa = smem_u32(smem + s * kBStage), full = full0 + 8 * s;
+          tma_load_3d_pair(sa, &tmA, full, kb * kBBK, m0, 0);
+          if (BMN) tma_load_3d_pair(sa + kBTile, &tmB, full, n0, kb * kBBK, t.g);
+          else tma_load_3d_pair(sa + kBTile, &tmB, full, kb * kBBK, n0, t.g);
+          if (++s == kBStages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+    }
+    grid_dep_launch();   // the last loads are on their way
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------------------ MMA issuer (leader)
+    if (cta_rank == 0 && elect_one()) {
+      constexpr uint32_t idesc = idesc_f8(256, 256, BMN);
+      int s = 0;
+      uint32_t ph = 0, it = 0;
+      bool ok = true;
+      for (int tile = first_tile; tile < total && ok; tile += tile_step) {
+        for (int kb = 0; kb < nkb; ++kb, ++it) {
+          const int buf = it & 1;
+          if (!mbar_wait(bar_tempty + 8 * buf, ((it >> 1) & 1) ^ 1, abort_flag, ST_WAIT_MMA_TMEM) ||
+              !mbar_wait(bar_full + 8 * s, ph, abort_flag, ST_WAIT_MMA_FULL)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + s * kBStage), sb = sa + kBTile;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f8_pair(tmem_base + 256 * buf, umma_desc_sw128(sa + 32 * k, 0, 1024),
+                         umma_desc_sw128(sb + (BMN ? 4096 : 32) * k, 0, 1024), idesc, k != 0);
+          umma_commit_pair(bar_empty + 8 * s);
+          umma_commit_pair(bar_tfull + 8 * buf);
+          if (++s == kBStages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------------------ epilogue
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t tempty_leader = mapa_shared(bar_tempty, 0);
+    uint8_t* sbuf = epi_smem + (warp - 2) * kStageOutBytes;
+    uint32_t it = 0;
+    int flip = 0;
+    bool ok = true;      // a warp that gave up goes on to the barriers of the others
+    for (int tile = first_tile; tile < total; tile += tile_step) {
+      const Tile t = get_tile(p, tile, TN, TM, kBBK);
+      const int row0 = t.m0 + BM * cta_rank + 32 * q;
+      const long long row = min(static_cast<long long>(row0 + lane), bp.rows - 1);
+      const bool live = p.sched != SCHED_GROUPED_M || row0 < p.poffs[t.g] + p.counts[t.g];   // else nothing but pad rows
+      // column blocks of this warp: its 128 columns, or 64 of gate and 64 of up
+      const int nb = EPI == EPI_SWIGLU ? t.n0 >> 7 : min((t.n0 >> 7) + half, bp.n_blocks - 1);
+      const float* sx = bp.sx + row;
+      const float* sw = bp.sw + t.g * bp.sw_group + static_cast<long long>(nb) * bp.sw_n;
+      const float* sw2 = sw + static_cast<long long>(bp.n_blocks) * bp.sw_n;     // SwiGLU: up
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + (EPI == EPI_SWIGLU ? 64 : 128) * half;
+      float2 acc[64];
+#pragma unroll
+      for (int i = 0; i < 64; ++i) acc[i] = make_float2(0.0f, 0.0f);
+      float fx[2], fw[2], fu[2];     // scales of the next two k-blocks
+      auto scales = [&](int kb, int u) {
+        if (kb < nkb) {
+          fx[u] = sx[kb * bp.sx_pitch];
+          fw[u] = sw[static_cast<long long>(kb) * bp.sw_k];
+          if (EPI == EPI_SWIGLU) fu[u] = sw2[static_cast<long long>(kb) * bp.sw_k];
+        }
+      };
+      scales(0, 0);
+      scales(1, 1);
+      for (int kb0 = 0; kb0 < nkb; kb0 += 2) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          if (kb0 + u >= nkb) break;
+          const int buf = it & 1;
+          ok = ok && mbar_wait(bar_tfull + 8 * buf, (it >> 1) & 1, abort_flag, ST_WAIT_EPILOGUE);
+          ++it;
+          __syncwarp();
+          tc_fence_after();
+          const float f = fx[u] * fw[u], f2 = EPI == EPI_SWIGLU ? fx[u] * fu[u] : f;
+          scales(kb0 + u + 2, u);
+          if (live) {
+            uint32_t r[2][16];
+            const uint32_t ta = taddr + 256 * buf;
+            tmem_ld16(ta, r[0]);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              tmem_ld_wait();
+              if (c < 7) {
+                tmem_ld16(ta + (EPI == EPI_SWIGLU && c + 1 >= 4 ? 64 : 0) + 16 * (c + 1), r[(c + 1) & 1]);
+              } else {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(tempty_leader + 8 * buf);
+              }
+              const float s = EPI == EPI_SWIGLU && c >= 4 ? f2 : f;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) fma2(acc[8 * c + i], r[c & 1][2 * i], r[c & 1][2 * i + 1], make_float2(s, s));
+            }
+          } else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(tempty_leader + 8 * buf);
+          }
+        }
+      }
+      if constexpr (EPI == EPI_STORE) {
+        if (live && ok) {
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc) {
+            const int c = t.n0 + 128 * half + 64 * cc;
+            if (c < p.N) {
+              uint32_t pk[32];
+#pragma unroll
+              for (int i = 0; i < 32; ++i) pk[i] = pack_bf16x2(acc[32 * cc + i].x, acc[32 * cc + i].y);
+              staging_free(lane);
+              stage_row(sbuf, lane, pk);
+              store_box(&tmD, sbuf, lane, c, row0, 0);
+            }
+          }
+        }
+      } else {
+        // acc[0, 32): gate, acc[32, 64): up of the same 64 columns
+        uint32_t amax = 0u;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          acc[i].x = silu_mul(acc[i].x, acc[32 + i].x);
+          acc[i].y = silu_mul(acc[i].y, acc[32 + i].y);
+          amax = max(amax, max(__float_as_uint(acc[i].x) & 0x7fffffffu, __float_as_uint(acc[i].y) & 0x7fffffffu));
+        }
+        // the other half of the row's 128 columns: two buffers, since the other warp may be a tile ahead
+        s_amax[flip][half][32 * q + lane] = amax;
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
+        amax = max(amax, s_amax[flip][half ^ 1][32 * q + lane]);
+        flip ^= 1;
+        if (live && ok) {
+          const float inv = block_factor(amax);
+          const long long orow = row0 + lane;
+          uint4* dst = reinterpret_cast<uint4*>(bp.q_out + orow * p.I + t.n0 + 64 * half);
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 a = acc[8 * v + 2 * j], b = acc[8 * v + 2 * j + 1];
+              w[j] = cvt4_e4m3(a.x * inv, a.y * inv, b.x * inv, b.y * inv);
+            }
+            dst[v] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          if (half == 0) bp.q_scale[scale_at(t.n0 >> 7, bp.q_pitch, orow)] = block_scale(amax);
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_all();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  __syncwarp();
+  cluster_sync_all();
+  if (threadIdx.x == 0 && *abort_flag != 0 && p.status != nullptr) atomicCAS(p.status, 0, *abort_flag);
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ few rows
+// The weights are the M operand, 128 rows of them a tile, and up to NT rows of X the N operand, so that every weight is read once for
+// the rows that want it.  A stage is 32 KB of weights: two k-blocks (store), or the gate and the up rows of one (SwiGLU).  Lanes of an
+// epilogue warp are output columns, its registers NT / 2 rows of X; the rows' scales come with the operands, through shared memory.
+// Bound: HBM, by the one read of the weights.  Where the tiles do not fill the SMs, the k-blocks of a tile are shared by the CTAs of a
+// cluster, which send their sums to the first one (in the order of the ranks: the same bits every time).
+template <int EPI, int NT>
+struct FewBlockCfg {
+  static constexpr int XB = EPI == EPI_SWIGLU ? 1 : 2;                 // k-blocks of a stage
+  static constexpr int X_BYTES = NT * kBBK;
+  static constexpr int STAGE = 2 * kBTile + XB * X_BYTES;
+  static constexpr int ACCS = EPI == EPI_SWIGLU ? NT : NT / 2;         // fp32 sums of a thread
+  static constexpr int RANK_BYTES = 32 * kEpiWarps * ACCS * 4;
+  static constexpr int MAX_SPLIT = ACCS <= 8 ? 8 : ACCS <= 16 ? 4 : ACCS <= 32 ? 2 : 1;
+  static constexpr int RED_BYTES = (MAX_SPLIT - 1) * RANK_BYTES;
+  static constexpr int SLOTS = 512 / (2 * NT) < 8 ? 512 / (2 * NT) : 8;   // tensor-memory ring, a stage each
+  static constexpr int kFit = (232448 - 8192 - RED_BYTES) / STAGE;
+  static constexpr int NSTAGE = kFit > 8 ? 8 : kFit;
+  static constexpr int SF = NSTAGE + SLOTS;                            // ring of the rows' scales, see the producer
+  static constexpr int SF_BYTES = XB * NT * 4;
+  static constexpr int TMEM_COLS = SLOTS * 2 * NT;                     // 256 or 512
+  static constexpr int BARS = 2 * NSTAGE + 2 * SLOTS + SF + 2;
+  static constexpr int SMEM_BYTES = NSTAGE * STAGE + RED_BYTES + SF * SF_BYTES + BARS * 8 + 16 + 1024;
+  static_assert(SMEM_BYTES <= 232448 - 4608, "shared memory");         // 4.5 KB are static
+  static_assert(TMEM_COLS == 256 || TMEM_COLS == 512, "a power of two");
+};
+
+// as mbar_wait, for a barrier that other CTAs of the cluster arrive on: their writes before it are visible
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
+  const long long t0 = clock64();
+  for (uint32_t it = 1;; ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((it & 0xff) == 0) {
+      if (*abort_flag != 0) return false;
+      if (clock64() - t0 > kWaitLimitCycles) {
+        *abort_flag = code;
+        return false;
+      }
+    }
+  }
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+template <int EPI, int NT>
+__global__ void __launch_bounds__(kThreads, 1)
+block_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const BlockParams bp) {
+  using C = FewBlockCfg<EPI, NT>;
+  const GemmParams& p = bp.g;
+  constexpr int NSTAGE = C::NSTAGE, SLOTS = C::SLOTS, XB = C::XB, HC = NT / 2;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  float* red = reinterpret_cast<float*>(smem + NSTAGE * C::STAGE);
+  float* sf = reinterpret_cast<float*>(smem + NSTAGE * C::STAGE + C::RED_BYTES);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + NSTAGE * C::STAGE + C::RED_BYTES + C::SF * C::SF_BYTES);
+  const uint32_t bar_full = smem_u32(bars);
+  const uint32_t bar_empty = smem_u32(bars + NSTAGE);
+  const uint32_t bar_tfull = smem_u32(bars + 2 * NSTAGE);
+  const uint32_t bar_tempty = smem_u32(bars + 2 * NSTAGE + SLOTS);
+  const uint32_t bar_sf = smem_u32(bars + 2 * NSTAGE + 2 * SLOTS);
+  const uint32_t bar_sums = smem_u32(bars + 2 * NSTAGE + 2 * SLOTS + C::SF);       // rank 0: the others' sums are here
+  const uint32_t bar_taken = bar_sums + 8;                                         // the others: rank 0 has read theirs
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::BARS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  __shared__ int pre[B200MOE_MAX_EXPERTS + 1];
+  __shared__ uint32_t s_amax[2][4][NT];
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int rank = bp.split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int first_tile = static_cast<int>(blockIdx.x) / bp.split, tile_step = static_cast<int>(gridDim.x) / bp.split;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < NSTAGE; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    for (int b = 0; b < SLOTS; ++b) {
+      mbar_init(bar_tfull + 8 * b, 1);
+      mbar_init(bar_tempty + 8 * b, kEpiWarps);
+    }
+    for (int b = 0; b < C::SF; ++b) mbar_init(bar_sf + 8 * b, 1);
+    mbar_init(bar_sums, bp.split > 1 ? (bp.split - 1) * kEpiWarps : 1);
+    mbar_init(bar_taken, kEpiWarps);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmX);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  grid_dep_wait();
+  if (warp == 2) {
+    if (p.counts != nullptr) few_prefix<NT>(p.counts, p.num_groups, lane, pre);
+    else if (lane == 0) {
+      pre[0] = 0;
+      pre[1] = (bp.first_dense + NT - 1) / NT;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (bp.split > 1) {
+    __syncwarp();
+    cluster_sync_all();
+  }
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int mt = (p.N + 127) >> 7;
+  const int total = pre[p.num_groups] * mt;
+  const int nkb = (p.K + kBBK - 1) / kBBK;
+  const int kb_lo = nkb * rank / bp.split, kb_hi = nkb * (rank + 1) / bp.split;
+  const int steps = (kb_hi - kb_lo + XB - 1) / XB;       // stages of a tile
+  auto tile_of = [&](int tile) {
+    if (p.counts != nullptr) return few_tile<NT, 128>(p.counts, p.poffs, p.num_groups, p.N, pre, tile);
+    FewTile t;
+    const int c = tile / mt;
+    t.e = 0;
+    t.m0 = (tile - c * mt) * 128;
+    t.row0 = c * NT;
+    t.live = min(NT, bp.first_dense - c * NT);
+    return t;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ producer
+    if (elect_one()) {
+      int s = 0, f = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int tile = first_tile; tile < total && ok; tile += tile_step) {
+        const FewTile t = tile_of(tile);
+        for (int kb = kb_lo; kb < kb_hi; kb += XB) {
+          const int n = min(XB, kb_hi - kb);
+          if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, ST_WAIT_PRODUCER)) {
+            ok = false;
+            break;
+          }
+          const uint32_t full = bar_full + 8 * s, st = smem_u32(smem + s * C::STAGE), xs = st + 2 * kBTile;
+          mbar_arrive_expect_tx(full, (EPI == EPI_SWIGLU ? 2 : n) * kBTile + n * C::X_BYTES);
+          if constexpr (EPI == EPI_SWIGLU) {
+            tma_load_3d(st, &tmW, full, kb * kBBK, t.m0, t.e);
+            tma_load_3d(st + kBTile, &tmW, full, kb * kBBK, p.I + t.m0, t.e);
+            tma_load_3d(xs, &tmX, full, kb * kBBK, t.row0, 0);
+          } else {
+            for (int i = 0; i < n; ++i) {
+              tma_load_3d(st + i * kBTile, &tmW, full, (kb + i) * kBBK, t.m0, t.e);
+              tma_load_3d(xs + i * C::X_BYTES, &tmX, full, (kb + i) * kBBK, t.row0, 0);
+            }
+          }
+          // The MMAs of the stage NSTAGE before are complete (bar_empty), so the epilogue has given back the tensor memory of the one SLOTS
+          // before that: it has read those scales, and this slot of a ring of NSTAGE + SLOTS is free.
+          const uint32_t bf = bar_sf + 8 * f;
+          mbar_arrive_expect_tx(bf, n * NT * 4);
+          for (int i = 0; i < n; ++i)
+            bulk_load_1d(smem_u32(sf + f * (XB * NT) + i * NT), bp.sx + scale_at(kb + i, bp.sx_pitch, t.row0), NT * 4, bf);
+          if (++f == C::SF) f = 0;
+          if (++s == NSTAGE) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+    }
+    grid_dep_launch();   // the last loads are on their way
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (elect_one()) {
+      constexpr uint32_t idesc = idesc_f8(128, NT, 0);
+      int s = 0, slot = 0;
+      uint32_t ph = 0, sph = 1;
+      bool ok = true;
+      for (int tile = first_tile; tile < total && ok; tile += tile_step) {
+        for (int kb = kb_lo; kb < kb_hi; kb += XB) {
+          const int n = EPI == EPI_SWIGLU ? 2 : min(XB, kb_hi - kb);
+          if (!mbar_wait(bar_tempty + 8 * slot, sph, abort_flag, ST_WAIT_MMA_TMEM) ||
+              !mbar_wait(bar_full + 8 * s, ph, abort_flag, ST_WAIT_MMA_FULL)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t st = smem_u32(smem + s * C::STAGE);
+          for (int i = 0; i < n; ++i) {
+            const uint32_t sw = st + i * kBTile, sx = st + 2 * kBTile + (EPI == EPI_SWIGLU ? 0 : i * C::X_BYTES);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_f8(tmem_base + (2 * slot + i) * NT, umma_desc_sw128(sw + 32 * k, 0, 1024), umma_desc_sw128(sx + 32 * k, 0, 1024), idesc,
+                      k != 0);
+          }
+          umma_commit(bar_empty + 8 * s);
+          umma_commit(bar_tfull + 8 * slot);
+          if (++slot == SLOTS) {
+            slot = 0;
+            sph ^= 1;
+          }
+          if (++s == NSTAGE) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue: lane = output column, register = row of X
+    const int q = warp & 3, half = (warp - 2) >> 2, tid = threadIdx.x - 64;
+    constexpr int CH = HC < 32 ? HC : 32;      // columns fetched at a time
+    int slot = 0, f = 0, flip = 0;
+    uint32_t sph = 0, fph = 0, tph = 0;
+    bool ok = true;                            // a warp that gave up goes on to the barriers of the others
+    for (int tile = first_tile; tile < total; tile += tile_step) {
+      const FewTile t = tile_of(tile);
+      const float* sw = bp.sw + t.e * bp.sw_group + static_cast<long long>(t.m0 >> 7) * bp.sw_n;
+      const float* sw2 = sw + static_cast<long long>(bp.n_blocks) * bp.sw_n;       // SwiGLU: up
+      const int col = t.m0 + 32 * q + lane;
+      float acc[EPI == EPI_SWIGLU ? 2 : 1][HC];
+#pragma unroll
+      for (int i = 0; i < HC; ++i) {
+        acc[0][i] = 0.0f;
+        if constexpr (EPI == EPI_SWIGLU) acc[1][i] = 0.0f;
+      }
+      // the weights' scales of the next stage: of its two k-blocks, or of gate and up
+      float w0 = 0.0f, w1 = 0.0f;
+      auto weights = [&](int kb) {
+        if (kb >= kb_hi) return;
+        w0 = sw[static_cast<long long>(kb) * bp.sw_k];
+        if constexpr (EPI == EPI_SWIGLU) w1 = sw2[static_cast<long long>(kb) * bp.sw_k];
+        else if (kb + 1 < kb_hi) w1 = sw[static_cast<long long>(kb + 1) * bp.sw_k];
+      };
+      weights(kb_lo);
+      for (int i = 0, kb = kb_lo; i < steps; ++i, kb += XB) {
+        ok = ok && mbar_wait(bar_sf + 8 * f, fph, abort_flag, ST_WAIT_EPILOGUE) &&
+             mbar_wait(bar_tfull + 8 * slot, sph, abort_flag, ST_WAIT_EPILOGUE);
+        __syncwarp();
+        tc_fence_after();
+        const float c0 = w0, c1 = w1;
+        weights(kb + XB);
+        const uint32_t ta = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + 2 * slot * NT + half * HC;
+        const int boxes = EPI == EPI_SWIGLU ? 2 : min(XB, kb_hi - kb);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          if (b < boxes) {
+            const float4* x4 = reinterpret_cast<const float4*>(sf + f * (XB * NT) + (EPI == EPI_SWIGLU ? 0 : b * NT) + half * HC);
+            const float c = b ? c1 : c0;
+            float(&a)[HC] = acc[EPI == EPI_SWIGLU ? b : 0];
+#pragma unroll
+            for (int j0 = 0; j0 < HC; j0 += CH) {
+              uint32_t r[CH];
+              tmem_ld_cols<CH>(ta + b * NT + j0, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < CH; j += 4) {
+                const float4 x = x4[(j0 + j) >> 2];
+                a[j0 + j] += __uint_as_float(r[j]) * (x.x * c);
+                a[j0 + j + 1] += __uint_as_float(r[j + 1]) * (x.y * c);
+                a[j0 + j + 2] += __uint_as_float(r[j + 2]) * (x.z * c);
+                a[j0 + j + 3] += __uint_as_float(r[j + 3]) * (x.w * c);
+              }
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_tempty + 8 * slot);
+        if (++slot == SLOTS) {
+          slot = 0;
+          sph ^= 1;
+        }
+        if (++f == C::SF) {
+          f = 0;
+          fph ^= 1;
+        }
+      }
+      if constexpr (C::MAX_SPLIT > 1) {
+        if (bp.split > 1) {
+          if (rank != 0) {
+            // wait until rank 0 has taken the last tile's, send, say so
+            ok = ok && mbar_wait_cluster(bar_taken, tph ^ 1, abort_flag, ST_WAIT_EPILOGUE);
+            const uint32_t to = mapa_shared(smem_u32(red), 0) + (rank - 1) * C::RANK_BYTES + 4 * tid;
+            if (ok) {
+#pragma unroll
+              for (int i = 0; i < C::ACCS; ++i) st_cluster(to + i * (32 * kEpiWarps * 4), acc[i / HC][i % HC]);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(mapa_shared(bar_sums, 0));
+            tph ^= 1;
+            continue;
+          }
+          ok = ok && mbar_wait_cluster(bar_sums, tph, abort_flag, ST_WAIT_EPILOGUE);
+          tph ^= 1;
+          __syncwarp();
+          if (ok) {
+            for (int o = 0; o < bp.split - 1; ++o)
+#pragma unroll
+              for (int i = 0; i < C::ACCS; ++i) acc[i / HC][i % HC] += red[o * (C::RANK_BYTES / 4) + i * (32 * kEpiWarps) + tid];
+          }
+          __syncwarp();
+          if (lane == 0)
+            for (int o = 1; o < bp.split; ++o) mbar_arrive_cluster(mapa_shared(bar_taken, o));
+        }
+      }
+      const int mine = min(HC, t.live - half * HC);       // rows of this warp
+      const long long row = t.row0 + half * HC;
+      if constexpr (EPI == EPI_STORE) {
+        if (ok && col < p.N) {
+#pragma unroll
+          for (int i = 0; i < HC; ++i)
+            if (i < mine) bp.out[(row + i) * p.N + col] = __float2bfloat16_rn(acc[0][i]);
+        }
+      } else {
+        // a row's largest value over the tile's 128 columns: 32 of this warp, the other three warps' through shared memory (two buffers,
+        // since a warp may be a tile ahead)
+#pragma unroll
+        for (int i = 0; i < HC; ++i) {
+          acc[0][i] = silu_mul(acc[0][i], acc[1][i]);
+          const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(acc[0][i]) & 0x7fffffffu);
+          if (lane == 0) s_amax[flip][q][half * HC + i] = m;
+        }
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+        if (ok) {
+#pragma unroll
+          for (int i = 0; i < HC; ++i) {
+            const int j = half * HC + i;
+            if (i < mine) {
+              const uint32_t m = max(max(s_amax[flip][0][j], s_amax[flip][1][j]), max(s_amax[flip][2][j], s_amax[flip][3][j]));
+              bp.q_out[(row + i) * p.I + col] = static_cast<uint8_t>(__nv_cvt_float_to_fp8(acc[0][i] * block_factor(m), __NV_SATFINITE, __NV_E4M3));
+              if (q == 0 && lane == 0) bp.q_scale[scale_at(t.m0 >> 7, bp.q_pitch, row + i)] = block_scale(m);
+            }
+          }
+        }
+        flip ^= 1;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (bp.split > 1) {
+    __syncwarp();
+    cluster_sync_all();      // nobody's shared memory goes before the others have sent to it
+  }
+  if (threadIdx.x == 0 && *abort_flag != 0 && p.status != nullptr) atomicCAS(p.status, 0, *abort_flag);
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem_base, C::TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+template <int EPI, bool BMN>
+static int launch_pair(const void* X, int64_t x_rows, int64_t ldx, const void* W, int64_t w_inner, int64_t w_rows, int64_t groups,
+                       const BlockParams& bp, int64_t max_tiles, cudaStream_t stream) {
+  static std::once_flag once;
+  static cudaError_t attr_err = cudaSuccess;
+  std::call_once(once, [] {
+    attr_err = cudaFuncSetAttribute(block_pair_kernel<EPI, BMN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBSmemBytes<EPI>);
+  });
+  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "cudaFuncSetAttribute(max dynamic smem)");
+  CUtensorMap tmA, tmB, tmD;
+  int rc = make_map(&tmA, X, bp.g.K, x_rows, 1, ldx, x_rows * ldx, kBBK, 128, 1);
+  if (rc == 0) rc = make_map(&tmB, W, w_inner, w_rows, groups, w_inner, w_rows * w_inner, 128, 128, 1);
+  tmD = tmA;
+  if (rc == 0 && EPI == EPI_STORE) rc = make_map(&tmD, bp.g.D, bp.g.N, x_rows, 1, bp.g.ldd, x_rows * bp.g.ldd, 64, 32);
+  if (rc) return rc;
+  const int pairs = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(gemm_cta_budget() / 2, max_tiles)));
+  B200_CUDA(launch_chained(block_pair_kernel<EPI, BMN>, pairs * 2, kThreads, kBSmemBytes<EPI>, stream, 2, tmA, tmB, tmD, bp));
+  return 0;
+}
+
+// CTAs that share a tile's k-blocks: as many as the idle SMs allow, each with four k-blocks at least
+static int few_split(int64_t tiles, int nkb, int most) {
+  int s = 1;
+  while (2 * s <= most && tiles * 2 * s <= gemm_cta_budget() && nkb >= 8 * s) s *= 2;
+  return s;
+}
+
+template <int EPI, int NT>
+static int launch_few(const void* X, int64_t x_rows, int64_t ldx, const void* W, int64_t w_rows, BlockParams bp, int64_t tiles,
+                      int64_t max_tiles, cudaStream_t stream) {
+  using C = FewBlockCfg<EPI, NT>;
+  static std::once_flag once;
+  static cudaError_t attr_err = cudaSuccess;
+  std::call_once(once, [] {
+    attr_err = cudaFuncSetAttribute(block_few_kernel<EPI, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+  });
+  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "cudaFuncSetAttribute(max dynamic smem)");
+  CUtensorMap tmW, tmX;
+  int rc = make_map(&tmW, W, bp.g.K, w_rows, bp.g.num_groups, bp.g.K, w_rows * bp.g.K, kBBK, 128, 1);
+  if (rc == 0) rc = make_map(&tmX, X, bp.g.K, x_rows, 1, ldx, x_rows * ldx, kBBK, NT, 1);
+  if (rc) return rc;
+  bp.split = few_split(tiles, static_cast<int>(ceil_div(bp.g.K, kBBK)), C::MAX_SPLIT);
+  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(gemm_cta_budget() / bp.split, max_tiles)) * bp.split;
+  B200_CUDA(launch_chained(block_few_kernel<EPI, NT>, static_cast<int>(grid), kThreads, C::SMEM_BYTES, stream, bp.split, tmW, tmX, bp));
+  return 0;
+}
+template <int EPI>
+static int launch_few_nt(int nt, const void* X, int64_t x_rows, int64_t ldx, const void* W, int64_t w_rows, const BlockParams& bp,
+                         int64_t tiles, int64_t max_tiles, cudaStream_t st) {
+  if (nt <= 16) return launch_few<EPI, 16>(X, x_rows, ldx, W, w_rows, bp, tiles, max_tiles, st);
+  if (nt <= 32) return launch_few<EPI, 32>(X, x_rows, ldx, W, w_rows, bp, tiles, max_tiles, st);
+  if (nt <= 64) return launch_few<EPI, 64>(X, x_rows, ldx, W, w_rows, bp, tiles, max_tiles, st);
+  return launch_few<EPI, 128>(X, x_rows, ldx, W, w_rows, bp, tiles, max_tiles, st);
+}
+
+constexpr int64_t kFewDense = 256;       // rows up to which a dense product runs with the weights as the M operand
+
+// out (M, N) = X (M, K) * W (N, K)^T, or (b_mn) out (M, K') = X (M, N') * W (N', K'): N and K of the params are of the product
+static int block_dense(const void* X, int64_t ldx, const float* sx, int64_t pitch, const void* W, const float* sw, int64_t M, int64_t N, int64_t K,
+                       int b_mn, void* out, int32_t* status, cudaStream_t st) {
+  BlockParams bp{};
+  bp.g.sched = SCHED_DENSE; bp.g.M = (int)M; bp.g.N = (int)N; bp.g.K = (int)K; bp.g.num_groups = 1;
+  bp.g.D = out; bp.g.ldd = N; bp.g.status = status;
+  bp.sx = sx; bp.sx_pitch = pitch; bp.rows = M; bp.sw = sw;
+  bp.n_blocks = (int)ceil_div(N, 128);
+  bp.sw_n = b_mn ? 1 : (int)ceil_div(K, 128);
+  bp.sw_k = b_mn ? (int)ceil_div(N, 128) : 1;
+  if (!b_mn && M <= kFewDense) {
+    bp.out = reinterpret_cast<__nv_bfloat16*>(out);
+    bp.first_dense = (int)M;
+    const int nt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+    const int64_t tiles = ceil_div(N, 128) * ceil_div(M, nt);
+    return launch_few_nt<EPI_STORE>(nt, X, M, ldx, W, N, bp, tiles, tiles, st);
+  }
+  const int64_t tiles = ceil_div(M, 256) * ceil_div(N, 256);
+  return b_mn ? launch_pair<EPI_STORE, true>(X, M, ldx, W, N, K, 1, bp, tiles, st)
+              : launch_pair<EPI_STORE, false>(X, M, ldx, W, K, N, 1, bp, tiles, st);
+}
+
+struct BlockCarver {
+  char* base;
+  size_t off = 0;
+  template <class T>
+  T* take(int64_t n) {
+    off = (off + 255) & ~static_cast<size_t>(255);
+    T* p = base != nullptr ? reinterpret_cast<T*>(base + off) : nullptr;
+    off += static_cast<size_t>(n) * sizeof(T);
+    return p;
+  }
+};
+
+struct BlockExperts {
+  int32_t *counts, *offs, *poffs, *slot_row, *row_slot, *tile_expert;
+  void* scratch;
+  size_t scratch_bytes;
+  uint8_t *xq, *iq;
+  float *xs, *is;
+  void* eo;
+};
+static BlockExperts carve_block(int64_t T, int64_t H, int64_t I, int E, int k, void* ws, size_t* bytes) {
+  BlockCarver c{static_cast<char*>(ws)};
+  BlockExperts f{};
+  const int64_t M = T * k, cap = b200moe_padded_rows_cap(M, E);
+  f.counts = c.take<int32_t>(E);
+  f.offs = c.take<int32_t>(E + 1);
+  f.poffs = c.take<int32_t>(E + 1);
+  f.slot_row = c.take<int32_t>(M);
+  f.row_slot = c.take<int32_t>(cap);
+  f.tile_expert = c.take<int32_t>(cap / B200MOE_TILE_M);
+  f.scratch_bytes = b200moe_permute_ws_bytes(M, E);
+  f.scratch = c.take<char>(f.scratch_bytes);
+  f.xq = c.take<uint8_t>(cap * H);
+  f.xs = c.take<float>(cap * (H / 128));
+  f.iq = c.take<uint8_t>(cap * I);
+  f.is = c.take<float>(cap * (I / 128));
+  f.eo = c.take<uint16_t>(cap * H);
+  *bytes = c.off;
+  return f;
+}
+
+}  // namespace b200moe
+
+using namespace b200moe;
+
+static int check_linear(const char* who, int64_t M, int64_t N, int64_t K) {
+  B200_CHECK_ARG(M >= 0 && M < (1LL << 31) - 256, B200MOE_E_BAD_SHAPE, "%s: %lld rows", who, (long long)M);
+  B200_CHECK_ARG(N > 0 && N % 8 == 0 && N < (1LL << 31) - 256, B200MOE_E_BAD_SHAPE, "%s: N = %lld must be a positive multiple of 8", who, (long long)N);
+  B200_CHECK_ARG(K > 0 && K % 16 == 0 && K < (1LL << 31) - 256, B200MOE_E_BAD_SHAPE, "%s: K = %lld must be a positive multiple of 16", who, (long long)K);
+  return 0;
+}
+
+extern "C" {
+
+size_t b200moe_fp8_block_linear_ws_bytes(int64_t M, int64_t K) {
+  if (M <= 0 || K <= 0) return 0;
+  BlockCarver c{nullptr};
+  c.take<uint8_t>(M * code_pitch(K));
+  c.take<float>(scale_pitch(M) * ceil_div(K, 128));
+  return c.off;
+}
+
+int b200moe_fp8_block_linear(const void* x, const void* w, const float* w_scale, int64_t M, int64_t N, int64_t K, int transposed, void* ws,
+                             void* out, int32_t* status, b200moe_stream_t stream) {
+  int rc = check_linear("fp8_block_linear", M, N, K);
+  if (rc) return rc;
+  if (M == 0) return 0;
+  B200_CHECK_ARG(x && w && w_scale && ws && out, B200MOE_E_NULL, "fp8_block_linear: null pointer");
+  B200_CHECK_ARG(aligned16(x) && aligned16(w) && aligned16(ws) && aligned16(out), B200MOE_E_ALIGN,
+                 "fp8_block_linear: tensors must be 16-byte aligned");
+  const int64_t red = transposed ? N : K, ldq = code_pitch(red), pitch = scale_pitch(M);
+  BlockCarver c{static_cast<char*>(ws)};
+  uint8_t* q = c.take<uint8_t>(M * ldq);
+  float* s = c.take<float>(pitch * ceil_div(red, 128));
+  rc = fp8_block_quant(x, M, red, M, nullptr, 1, q, ldq, s, pitch, stream);
+  if (rc) return rc;
+  return block_dense(q, ldq, s, pitch, w, w_scale, M, transposed ? K : N, red, transposed, out, status, (cudaStream_t)stream);
+}
+
+size_t b200moe_moe_fp8_block_ws_bytes(int64_t T, int64_t H, int64_t I, int E, int k) {
+  if (T <= 0 || H <= 0 || I <= 0 || E < 1 || k < 1) return 0;
+  size_t bytes = 0;
+  carve_block(T, H, I, E, k, nullptr, &bytes);
+  return bytes;
+}
+
+int b200moe_moe_fp8_block_forward(const void* x, const int64_t* idx, const float* w, const void* gate_up, const float* gate_up_scale,
+                                  const void* down, const float* down_scale, int64_t T, int64_t H, int64_t I, int E, int k, void* ws,
+                                  void* out, int32_t* status, b200moe_stream_t stream) {
+  B200_CHECK_ARG(T >= 0 && T < (1LL << 31) && H > 0 && I > 0 && H % 128 == 0 && I % 128 == 0, B200MOE_E_BAD_SHAPE,
+                 "moe_fp8_block: T = %lld, H = %lld, I = %lld (positive multiples of 128)", (long long)T, (long long)H, (long long)I);
+  B200_CHECK_ARG(E >= 1 && E <= B200MOE_MAX_EXPERTS, B200MOE_E_UNSUPPORTED, "moe_fp8_block: E = %d, supported 1..%d", E, B200MOE_MAX_EXPERTS);
+  B200_CHECK_ARG(k >= 1 && k <= B200MOE_MAX_TOPK, B200MOE_E_BAD_SHAPE, "moe_fp8_block: k = %d", k);
+  B200_CHECK_ARG(2 * I < (1LL << 31) && H < (1LL << 31) && b200moe_padded_rows_cap(T * k, E) < (1LL << 31) - 256, B200MOE_E_BAD_SHAPE,
+                 "moe_fp8_block: %lld routed rows do not fit int32 tables", (long long)(T * k));
+  if (T == 0) return 0;
+  B200_CHECK_ARG(x && idx && w && gate_up && gate_up_scale && down && down_scale && ws && out && status, B200MOE_E_NULL,
+                 "moe_fp8_block: null pointer");
+  B200_CHECK_ARG(aligned16(x) && aligned16(gate_up) && aligned16(down) && aligned16(ws) && aligned16(out), B200MOE_E_ALIGN,
+                 "moe_fp8_block: tensors must be 16-byte aligned");
+  size_t bytes;
+  const BlockExperts f = carve_block(T, H, I, E, k, ws, &bytes);
+  const int64_t M = T * k, cap = b200moe_padded_rows_cap(M, E);
+  cudaStream_t st = (cudaStream_t)stream;
+#define RUN(name, launches, call)     \
+  do {                                \
+    OpScope scope__(name, launches);  \
+    const int rc__ = (call);          \
+    if (rc__) return rc__;            \
+  } while (0)
+  RUN("permute_build", M > 1024 ? 2 : 1,
+      permute_build(idx, T, k, E, f.counts, f.offs, f.poffs, f.slot_row, f.row_slot, f.tile_expert, nullptr, nullptr, f.scratch, f.scratch_bytes,
+                    nullptr, nullptr, status, stream));
+  RUN("fp8_block_quant", 1, fp8_block_quant(x, T, H, cap, f.slot_row, k, f.xq, H, f.xs, cap, stream));
+  // gate and up
+  BlockParams up{};
+  up.g.sched = SCHED_GROUPED_M; up.g.N = up.g.I = (int)I; up.g.K = (int)H; up.g.num_groups = E;
+  up.g.tile_expert = f.tile_expert; up.g.poffs = f.poffs; up.g.counts = f.counts; up.g.status = status;
+  up.sx = f.xs; up.sx_pitch = cap; up.rows = cap; up.sw = gate_up_scale;
+  up.n_blocks = (int)(I / 128); up.sw_n = (int)(H / 128); up.sw_k = 1; up.sw_group = 2 * (I / 128) * (H / 128);
+  up.q_out = f.iq; up.q_scale = f.is; up.q_pitch = cap;
+  // down
+  BlockParams dn{};
+  dn.g.sched = SCHED_GROUPED_M; dn.g.N = (int)H; dn.g.K = (int)I; dn.g.num_groups = E;
+  dn.g.tile_expert = f.tile_expert; dn.g.poffs = f.poffs; dn.g.counts = f.counts; dn.g.status = status;
+  dn.g.D = f.eo; dn.g.ldd = H; dn.out = reinterpret_cast<__nv_bfloat16*>(f.eo);
+  dn.sx = f.is; dn.sx_pitch = cap; dn.rows = cap; dn.sw = down_scale;
+  dn.n_blocks = (int)(H / 128); dn.sw_n = (int)(I / 128); dn.sw_k = 1; dn.sw_group = (H / 128) * (I / 128);
+  const int64_t hit = std::min<int64_t>(E, M);           // experts that can have a row
+  const int64_t mean = ceil_div(M, E);
+  if (mean <= 96) {
+    const int nt = mean <= 12 ? 16 : mean <= 24 ? 32 : mean <= 48 ? 64 : 128;
+    const int64_t chunks = E + M / nt;                   // at most
+    RUN("fp8_block_gate_up", 1, launch_few_nt<EPI_SWIGLU>(nt, f.xq, cap, H, gate_up, 2 * I, up, hit * (I / 128), chunks * (I / 128), st));
+    RUN("fp8_block_down", 1, launch_few_nt<EPI_STORE>(nt, f.iq, cap, I, down, H, dn, hit * (H / 128), chunks * (H / 128), st));
+  } else {
+    const int64_t tiles = cap / 256;
+    RUN("fp8_block_gate_up", 1, (launch_pair<EPI_SWIGLU, false>(f.xq, cap, H, gate_up, H, 2 * I, E, up, tiles * (I / 128), st)));
+    RUN("fp8_block_down", 1, (launch_pair<EPI_STORE, false>(f.iq, cap, I, down, I, H, E, dn, tiles * ceil_div(H, 256), st)));
+  }
+  RUN("combine", 1, b200moe_combine(f.eo, w, f.slot_row, T, k, H, out, stream));
+#undef RUN
+  return 0;
+}
+
+}  // extern "C"
