@@ -62,6 +62,12 @@ __device__ __forceinline__ void fma2(float2& d, uint32_t a0, uint32_t a1, float2
       : "+f"(d.x), "+f"(d.y)
       : "r"(a0), "r"(a1), "f"(f.x), "f"(f.y));
 }
+// Arrive on a barrier of another CTA of the cluster that guards tensor memory alone: nothing in memory is handed over, and
+// tcgen05.fence orders the rest.  A release waits for the thread's own loads in flight (the scales ahead) twice a k-block: 8192 x 14336 x 4096
+// took 984 us with it and takes 494 without.
+__device__ __forceinline__ void mbar_arrive_tmem(uint32_t bar_cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
+}
 // N of the warp's 32 lanes' consecutive fp32 columns
 template <int N>
 __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[N]) {
@@ -250,7 +256,7 @@ block_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
               } else {
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(tempty_leader + 8 * buf);
+                if (lane == 0) mbar_arrive_tmem(tempty_leader + 8 * buf);
               }
               const float s = EPI == EPI_SWIGLU && c >= 4 ? f2 : f;
 #pragma unroll
@@ -259,7 +265,7 @@ block_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
           } else {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(tempty_leader + 8 * buf);
+            if (lane == 0) mbar_arrive_tmem(tempty_leader + 8 * buf);
           }
         }
       }
