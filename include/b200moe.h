@@ -107,13 +107,13 @@ int b200moe_group_topk_fwd(const void* logits, int logits_type, const float* bia
 int b200moe_group_topk_bwd(const void* logits, int logits_type, const int64_t* idx, const float* grad_w, int64_t T, int E, int k,
                            int scoring, int norm_topk, float scale, void* grad_logits, b200moe_stream_t stream);
 /* Router losses (no counterpart in the reference) of `segs` segments of S tokens each, logits (segs*S,E), picks idx (segs*S,k):
- * losses[0] = mean over the segments that have tokens of sum_e f_e P_e, f_e = E / (k n) * picks of e, P_e = mean of p_e,
- * p = softmax(z) or sigmoid(z) / sum sigmoid(z); losses[1] = mean over all tokens of (log sum exp z)^2.  A token counts unless
+ * *balance = mean over the segments that have tokens of sum_e f_e P_e, f_e = E / (k n) * picks of e, P_e = mean of p_e,
+ * p = softmax(z) or sigmoid(z) / sum sigmoid(z); *z = mean over all tokens of (log sum exp z)^2.  A token counts unless
  * mask (nullable, one byte a token) is 0 or all its logits are -inf.  coef (segs*E + 2 fp32): what the backward needs.
  * ws: b200moe_router_losses_ws_bytes, 8-byte aligned. */
 size_t b200moe_router_losses_ws_bytes(int64_t S, int segs, int E);
 int b200moe_router_losses_fwd(const void* logits, int logits_type, const int64_t* idx, const uint8_t* mask, int64_t S, int segs,
-                              int E, int k, int scoring, void* ws, float* coef, float* losses, int32_t* status,
+                              int E, int k, int scoring, void* ws, float* coef, float* balance, float* z, int32_t* status,
                               b200moe_stream_t stream);
 /* grad_logits from the device scalars grad_balance, grad_z (nullable: 0). */
 int b200moe_router_losses_bwd(const void* logits, int logits_type, const uint8_t* mask, const float* coef,

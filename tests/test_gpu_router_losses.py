@@ -68,8 +68,8 @@ def test_losses_and_gradient(pkg, dtype, scoring, masked, per_sequence):
         got = pkg.router_losses(z, idx, scoring, mask, per_sequence)
         (grad,) = torch.autograd.grad(got, z, (gb, gz))
         b, zl, rg, size = losses64(z.detach(), idx, scoring, mask, per_sequence, 0.7, 0.02)
-        assert abs(float(got[0]) - float(b)) <= 2.0 ** -12 * float(b), (B, S, E, float(got[0]), float(b))
-        assert abs(float(got[1]) - float(zl)) <= 2.0 ** -18 * (1 + float(zl)), (B, S, E)
+        assert abs(float(got[0].detach()) - float(b)) <= 2.0 ** -12 * float(b), (B, S, E, float(got[0]), float(b))
+        assert abs(float(got[1].detach()) - float(zl)) <= 2.0 ** -18 * (1 + float(zl)), (B, S, E)
         bound = 2.0 ** -17 * size + torch.finfo(dtype).eps / 2 * rg.abs() + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
         assert grad.dtype == dtype and ((grad.double() - rg).abs() <= bound).all(), (B, S, E, float(((grad.double() - rg).abs() / bound).max()))
         again = pkg.router_losses(z.detach(), idx, scoring, mask, per_sequence)
@@ -135,7 +135,7 @@ def test_far_logits_and_picks_out_of_range(pkg):
         got = pkg.router_losses(z, idx, scoring)
         b, zl, rg, size = losses64(z.detach()[None], idx[None], scoring, None, False, 1.0, 1.0)
         (g,) = torch.autograd.grad(got[0] + got[1], z)
-        assert abs(float(got[0]) - float(b)) <= 2.0 ** -12 * float(b) and abs(float(got[1]) - float(zl)) <= 2.0 ** -18 * (1 + float(zl))
+        assert abs(float(got[0].detach()) - float(b)) <= 2.0 ** -12 * float(b) and abs(float(got[1].detach()) - float(zl)) <= 2.0 ** -18 * (1 + float(zl))
         # exponents of 300 carry 300 * 2^-24 of their own
         assert ((g.double() - rg[0]).abs() <= 2.0 ** -14 * size[0] + 1e-12).all()
     pkg.check_status()

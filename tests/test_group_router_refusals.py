@@ -27,7 +27,7 @@ def test_router_losses_refusals():
     lib = load_pkg().lib()
 
     def call(kind=0, S=4, segs=2, E=64, k=6, scoring=1, ws=P, logits=P):
-        return lib.b200moe_router_losses_fwd(logits, kind, P, None, S, segs, E, k, scoring, ws, P, P, None, None)
+        return lib.b200moe_router_losses_fwd(logits, kind, P, None, S, segs, E, k, scoring, ws, P, P, P, None, None)
 
     assert call(ws=None) == -6 and call(logits=None) == -6
     assert call(kind=2) == -3 and call(E=257) == -3 and call(scoring=3) == -3

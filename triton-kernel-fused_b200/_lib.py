@@ -45,7 +45,7 @@ _SIGNATURES = {
     "b200moe_group_topk_fwd": (c_int, [c_void_p, c_int, c_void_p, c_int64] + [c_int] * 7 + [c_float] + [c_void_p] * 4),
     "b200moe_group_topk_bwd": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64] + [c_int] * 4 + [c_float] + [c_void_p] * 2),
     "b200moe_router_losses_ws_bytes": (c_size_t, [c_int64, c_int, c_int]),
-    "b200moe_router_losses_fwd": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64] + [c_int] * 4 + [c_void_p] * 5),
+    "b200moe_router_losses_fwd": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64] + [c_int] * 4 + [c_void_p] * 6),
     "b200moe_router_losses_bwd": (c_int, [c_void_p, c_int] + [c_void_p] * 4 + [c_int64] + [c_int] * 3 + [c_void_p] * 2),
     "b200moe_conv_unfold": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p]),
     "b200moe_conv_fold": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p]),

@@ -1,4 +1,4 @@
-// Autograd functions of the layer, of the experts on given picks and of the conv router as compiled code: the host side of the
+// Autograd functions of the layer, of the experts on given picks, of the routers' top-k and losses and of the block-scaled 8-bit products as compiled code: the host side of the
 // Python Functions of the same name (layer.py, moe.py, router.py) for plain calls.  Each function returns None for a call
 // that is not plain (a tensor that would have to be cast or made contiguous, autocast, functorch transforms, forward-mode
 // gradients, dispatch modes, tensor subclasses, a shape that is an error), and the caller then takes the Python Function, which
@@ -7,7 +7,7 @@
 // Why: between two small passes the host was the bound.  A Python Function costs the caller 8 us to enter, its allocations and
 // argument checks 15 to 30 more each way, and in the backward the autograd engine's thread waits for the interpreter lock before
 // it can call it.  us a pass, Python / compiled: one token through 64 experts of 2048 x 1408 62 / 39; forward and backward of 512 tokens
-// at width 256 237 / 148; conv router of 16 384 tokens 145 / 118.
+// at width 256 237 / 148; conv router of 16 384 tokens 145 / 118.  HOSTTIMES
 //
 // Nothing is kept between calls but what autograd saves (saved-tensor hooks see it); the workspace of a forward is a saved tensor.
 #include <ATen/autocast_mode.h>
@@ -274,6 +274,211 @@ optional<std::tuple<Tensor, Tensor, Tensor>> conv_router(const Tensor& x, const 
   return std::make_tuple(r[0], r[1], r[2]);
 }
 
+// ---------------------------------------------------------------------------- group-limited top-k
+// of the logits' types
+optional<int> logits_type(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return B200MOE_LOGITS_BF16;
+    case at::kFloat: return B200MOE_LOGITS_F32;
+    case at::kHalf: return B200MOE_LOGITS_F16;
+    default: return std::nullopt;
+  }
+}
+
+struct GroupArgs {
+  optional<Tensor> bias;
+  int type;
+  int64_t k, groups, open, scoring, top2, norm;
+  double scale;
+  bool counts;
+};
+
+variable_list group_forward(const Tensor& z, const GroupArgs& a) {
+  const int64_t E = z.size(-1), T = z.numel() / E;
+  std::vector<int64_t> shape(z.sizes().begin(), z.sizes().end());
+  shape.back() = a.k;
+  Tensor idx = at::empty(shape, z.options().dtype(at::kLong)), w = at::empty(shape, z.options().dtype(at::kFloat));
+  Tensor counts = a.counts ? at::empty({E}, z.options().dtype(at::kInt)) : Tensor();
+  check(b200moe_group_topk_fwd(ptr(z), a.type, static_cast<const float*>(ptr(a.bias)), T, E, a.k, a.groups, a.open, a.scoring, a.top2, a.norm,
+                               static_cast<float>(a.scale), idx.data_ptr<int64_t>(), w.data_ptr<float>(), static_cast<int32_t*>(ptr(counts)),
+                               stream_of(z)));
+  return {idx, w, counts};
+}
+
+struct GroupTopk : torch::autograd::Function<GroupTopk> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& z, const GroupArgs& a) {
+    variable_list r = group_forward(z, a);
+    ctx->save_for_backward({z, r[0]});
+    ctx->saved_data["scoring"] = a.scoring;
+    ctx->saved_data["norm"] = a.norm;
+    ctx->saved_data["scale"] = a.scale;
+    ctx->mark_non_differentiable({r[0], r[2]});
+    ctx->set_materialize_grads(false);
+    return r;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list res(2);
+    if (!grads[1].defined()) return res;
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &z = s[0], &idx = s[1];
+    const c10::cuda::CUDAGuard guard(z.device());
+    const Tensor gw = grads[1].contiguous().to(at::kFloat);
+    const int64_t E = z.size(-1);
+    res[0] = at::empty_like(z);
+    check(b200moe_group_topk_bwd(ptr(z), *logits_type(z), idx.data_ptr<int64_t>(), gw.data_ptr<float>(), z.numel() / E, E, idx.size(-1),
+                                 ctx->saved_data["scoring"].toInt(), ctx->saved_data["norm"].toInt(),
+                                 static_cast<float>(ctx->saved_data["scale"].toDouble()), ptr(res[0]), stream_of(z)));
+    return res;
+  }
+};
+
+// (idx (...,k) int64, weights (...,k) fp32, counts (E,) int32 or None), or None
+optional<std::tuple<Tensor, Tensor, optional<Tensor>>> group_topk(const Tensor& z, const optional<Tensor>& bias, int64_t k, int64_t groups,
+                                                                  int64_t open, int64_t scoring, int64_t top2, bool norm, double scale,
+                                                                  bool counts) {
+  if (!plain_call(z)) return std::nullopt;
+  const auto dev = z.device();
+  const auto type = logits_type(z);
+  if (!type.has_value() || !plain(z, z.scalar_type(), dev) || !plain_or_none(bias, at::kFloat, dev)) return std::nullopt;
+  if (z.dim() < 2 || z.dim() > 3 || z.numel() == 0 || k < 1 || k > B200MOE_MAX_TOPK || (bias.has_value() && bias->numel() != z.size(-1)))
+    return std::nullopt;
+  const c10::cuda::CUDAGuard guard(dev);
+  const bool grad = at::GradMode::is_enabled() && z.requires_grad();
+  const GroupArgs a{bias, *type, k, groups, open, scoring, top2, norm, scale, counts || grad};
+  variable_list r = grad ? GroupTopk::apply(z, a) : group_forward(z, a);
+  return std::make_tuple(r[0], r[1], r[2].defined() ? optional<Tensor>(r[2]) : std::nullopt);
+}
+
+// ---------------------------------------------------------------------------- router losses
+struct LossArgs {
+  Tensor idx, status;
+  optional<Tensor> mask;
+  int type;
+  int64_t segs, scoring;
+};
+
+variable_list losses_forward(const Tensor& z, const LossArgs& a) {
+  const int64_t E = z.size(-1), S = z.numel() / E / a.segs;
+  Tensor balance = at::empty({}, z.options().dtype(at::kFloat)), zl = at::empty({}, z.options().dtype(at::kFloat));
+  Tensor coef = at::empty({a.segs * E + 2}, z.options().dtype(at::kFloat)), ws = bytes(b200moe_router_losses_ws_bytes(S, a.segs, E), z);
+  check(b200moe_router_losses_fwd(ptr(z), a.type, a.idx.data_ptr<int64_t>(), static_cast<const uint8_t*>(ptr(a.mask)), S, a.segs, E, a.idx.size(-1),
+                                  a.scoring, ptr(ws), coef.data_ptr<float>(), balance.data_ptr<float>(), zl.data_ptr<float>(),
+                                  status_ptr(a.status), stream_of(z)));
+  return {balance, zl, coef};
+}
+
+struct RouterLosses : torch::autograd::Function<RouterLosses> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& z, const LossArgs& a) {
+    variable_list r = losses_forward(z, a);
+    variable_list saved{z, r[2]};
+    if (a.mask.has_value()) saved.push_back(*a.mask);
+    ctx->save_for_backward(std::move(saved));
+    ctx->saved_data["segs"] = a.segs;
+    ctx->saved_data["scoring"] = a.scoring;
+    ctx->set_materialize_grads(false);
+    return {r[0], r[1]};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list res(2);
+    if (!grads[0].defined() && !grads[1].defined()) return res;
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &z = s[0], &coef = s[1];
+    const c10::cuda::CUDAGuard guard(z.device());
+    Tensor g[2];
+    for (int i = 0; i < 2; ++i)
+      if (grads[i].defined()) g[i] = grads[i].to(at::kFloat);
+    const int64_t E = z.size(-1), segs = ctx->saved_data["segs"].toInt();
+    res[0] = at::empty_like(z);
+    check(b200moe_router_losses_bwd(ptr(z), *logits_type(z), s.size() > 2 ? static_cast<const uint8_t*>(ptr(s[2])) : nullptr,
+                                    coef.data_ptr<float>(), static_cast<const float*>(ptr(g[0])), static_cast<const float*>(ptr(g[1])),
+                                    z.numel() / E / segs, segs, E, ctx->saved_data["scoring"].toInt(), ptr(res[0]), stream_of(z)));
+    return res;
+  }
+};
+
+// (balance, z), or None
+optional<std::tuple<Tensor, Tensor>> router_losses(const Tensor& z, const Tensor& idx, const optional<Tensor>& mask, const Tensor& status,
+                                                   int64_t scoring, bool per_sequence) {
+  if (!plain_call(z)) return std::nullopt;
+  const auto dev = z.device();
+  const auto type = logits_type(z);
+  if (!type.has_value() || !plain(z, z.scalar_type(), dev) || !plain(idx, at::kLong, dev) || !plain_or_none(mask, at::kBool, dev))
+    return std::nullopt;
+  if (z.dim() < 2 || z.dim() > 3 || z.numel() == 0 || idx.dim() != z.dim() || (per_sequence && z.dim() != 3)) return std::nullopt;
+  const auto rows = z.sizes().slice(0, z.dim() - 1);
+  if (idx.sizes().slice(0, z.dim() - 1) != rows || (mask.has_value() && mask->sizes() != rows)) return std::nullopt;
+  const c10::cuda::CUDAGuard guard(dev);
+  const LossArgs a{idx, status, mask, *type, per_sequence ? z.size(0) : 1, scoring};
+  variable_list r = at::GradMode::is_enabled() && z.requires_grad() ? RouterLosses::apply(z, a) : losses_forward(z, a);
+  return std::make_tuple(r[0], r[1]);
+}
+
+// ---------------------------------------------------------------------------- e4m3 weights with block scales
+bool codes(const Tensor& w, const Tensor& scale, int64_t dim, c10::Device dev) {
+  if (!plain(w, at::kFloat8_e4m3fn, dev) || !plain(scale, at::kFloat, dev) || w.dim() != dim || scale.dim() != dim || w.numel() == 0) return false;
+  if (dim == 3 && scale.size(0) != w.size(0)) return false;
+  return scale.size(-2) == (w.size(-2) + 127) / 128 && scale.size(-1) == (w.size(-1) + 127) / 128;
+}
+bool aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+
+Tensor block_product(const Tensor& x, const Tensor& w, const Tensor& scale, const Tensor& status, bool transposed) {
+  const int64_t N = w.size(0), K = w.size(1), M = x.numel() / (transposed ? N : K);
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = transposed ? K : N;
+  Tensor out = at::empty(shape, x.options()), ws = bytes(b200moe_fp8_block_linear_ws_bytes(M, transposed ? N : K), x);
+  check(b200moe_fp8_block_linear(ptr(x), ptr(w), scale.data_ptr<float>(), M, N, K, transposed, ptr(ws), ptr(out), status_ptr(status), stream_of(x)));
+  return out;
+}
+
+struct BlockLinear : torch::autograd::Function<BlockLinear> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& scale, const Tensor& status) {
+    ctx->save_for_backward({w, scale});
+    ctx->saved_data["status"] = status;
+    return block_product(x, w, scale, status, false);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const c10::cuda::CUDAGuard guard(s[0].device());
+    Tensor g = grads[0].to(at::kBFloat16).contiguous();
+    if (!aligned(g)) g = g.clone();
+    return {block_product(g, s[0], s[1], ctx->saved_data["status"].toTensor(), true), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// (..., N) bf16, or None
+optional<Tensor> fp8_block_linear(const Tensor& x, const Tensor& w, const Tensor& scale, const Tensor& status) {
+  if (!plain_call(x)) return std::nullopt;
+  const auto dev = x.device();
+  if (!plain(x, at::kBFloat16, dev) || !codes(w, scale, 2, dev) || x.dim() < 1 || x.numel() == 0 || x.size(-1) != w.size(1)) return std::nullopt;
+  if (w.size(0) % 8 != 0 || w.size(1) % 16 != 0 || !aligned(x) || !aligned(w)) return std::nullopt;
+  const c10::cuda::CUDAGuard guard(dev);
+  if (at::GradMode::is_enabled() && x.requires_grad()) return BlockLinear::apply(x, w, scale, status);
+  return block_product(x, w, scale, status, false);
+}
+
+// (N,H) bf16, or None
+optional<Tensor> moe_fp8_block(const Tensor& x, const Tensor& idx, const Tensor& w, const Tensor& gate_up, const Tensor& gate_up_scale,
+                               const Tensor& down, const Tensor& down_scale, const Tensor& status) {
+  if (!plain_call(x)) return std::nullopt;
+  const auto dev = x.device();
+  if (!plain(x, at::kBFloat16, dev) || !plain(idx, at::kLong, dev) || !plain(w, at::kFloat, dev) || !codes(gate_up, gate_up_scale, 3, dev) ||
+      !codes(down, down_scale, 3, dev))
+    return std::nullopt;
+  if (x.dim() != 2 || idx.dim() != 2 || x.size(0) == 0 || (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad()))) return std::nullopt;
+  const int64_t T = x.size(0), H = x.size(1), E = gate_up.size(0), I = down.size(2), k = idx.size(1);
+  if (gate_up.size(1) != 2 * I || gate_up.size(2) != H || down.size(0) != E || down.size(1) != H || idx.size(0) != T || w.sizes() != idx.sizes() ||
+      H % 128 != 0 || I % 128 != 0 || k < 1 || !aligned(x) || !aligned(gate_up) || !aligned(down))
+    return std::nullopt;
+  const c10::cuda::CUDAGuard guard(dev);
+  Tensor out = at::empty({T, H}, x.options()), ws = bytes(b200moe_moe_fp8_block_ws_bytes(T, H, I, E, k), x);
+  check(b200moe_moe_fp8_block_forward(ptr(x), idx.data_ptr<int64_t>(), w.data_ptr<float>(), ptr(gate_up), gate_up_scale.data_ptr<float>(),
+                                      ptr(down), down_scale.data_ptr<float>(), T, H, I, E, k, ptr(ws), ptr(out), status_ptr(status), stream_of(x)));
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -281,4 +486,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layer", torch::wrap_pybind_function_no_gil(layer));
   m.def("experts", torch::wrap_pybind_function_no_gil(experts));
   m.def("conv_router", torch::wrap_pybind_function_no_gil(conv_router));
+  m.def("group_topk", torch::wrap_pybind_function_no_gil(group_topk));
+  m.def("router_losses", torch::wrap_pybind_function_no_gil(router_losses));
+  m.def("fp8_block_linear", torch::wrap_pybind_function_no_gil(fp8_block_linear));
+  m.def("moe_fp8_block", torch::wrap_pybind_function_no_gil(moe_fp8_block));
 }

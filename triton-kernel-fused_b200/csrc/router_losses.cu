@@ -31,7 +31,7 @@ struct LossParams {
   double* part_z;
   float* coef;              // (segs, E): f / n, then [1 / live segments, 1 / N]
   double* seg_out;          // per segment: balance, sum lse^2, tokens
-  float* losses;            // balance, z
+  float *balance, *z;       // the two losses
   int* status;
 };
 
@@ -96,8 +96,8 @@ __device__ __forceinline__ void put_losses(const LossParams& p, double balance, 
   float* scalars = p.coef + static_cast<long long>(p.segs) * p.E;
   scalars[0] = live > 0.0 ? static_cast<float>(1.0 / live) : 0.0f;
   scalars[1] = n > 0.0 ? static_cast<float>(1.0 / n) : 0.0f;
-  p.losses[0] = live > 0.0 ? static_cast<float>(balance / live) : 0.0f;
-  p.losses[1] = n > 0.0 ? static_cast<float>(z / n) : 0.0f;
+  *p.balance = live > 0.0 ? static_cast<float>(balance / live) : 0.0f;
+  *p.z = n > 0.0 ? static_cast<float>(z / n) : 0.0f;
 }
 
 template <class T, bool SIGMOID, int V>
@@ -317,8 +317,8 @@ size_t b200moe_router_losses_ws_bytes(int64_t S, int segs, int E) {
 }
 
 int b200moe_router_losses_fwd(const void* logits, int logits_type, const int64_t* idx, const uint8_t* mask, int64_t S, int segs, int E, int k,
-                              int scoring, void* ws, float* coef, float* losses, int32_t* status, b200moe_stream_t stream) {
-  B200_CHECK_ARG(ws && coef && losses && (S == 0 || (logits && idx)), B200MOE_E_NULL, "router_losses_fwd: null pointer");
+                              int scoring, void* ws, float* coef, float* balance, float* z, int32_t* status, b200moe_stream_t stream) {
+  B200_CHECK_ARG(ws && coef && balance && z && (S == 0 || (logits && idx)), B200MOE_E_NULL, "router_losses_fwd: null pointer");
   CHECK_LOSSES("router_losses_fwd");
   B200_CHECK_ARG(k >= 1 && k <= B200MOE_MAX_TOPK, B200MOE_E_BAD_SHAPE, "router_losses_fwd: top_k = %d, supported 1..%d", k, B200MOE_MAX_TOPK);
   LossParams p{};
@@ -329,7 +329,7 @@ int b200moe_router_losses_fwd(const void* logits, int logits_type, const int64_t
   p.seg_out = p.part_z + 2 * n;
   p.part_p = reinterpret_cast<float*>(p.seg_out + 3 * static_cast<long long>(segs));
   p.part_hits = reinterpret_cast<int*>(p.part_p + n * E);
-  p.coef = coef; p.losses = losses; p.status = status;
+  p.coef = coef; p.balance = balance; p.z = z; p.status = status;
   cudaError_t err = cudaSuccess;
   by_values((E + 31) / 32, [&](auto v) {
     constexpr int V = v.value;

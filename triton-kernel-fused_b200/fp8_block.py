@@ -77,7 +77,7 @@ def _product(x, w, scale, transposed):
 
 
 class _Fp8BlockLinear(torch.autograd.Function):
-    """x (M,K) through frozen weights; the gradient of x is the product of its own gradient, quantised like x, with the same codes."""
+    """Plain calls take its compiled form (csrc/fast.cpp).  x (M,K) through frozen weights; the gradient of x is the product of its own gradient, quantised like x, with the same codes."""
 
     @staticmethod
     def forward(ctx, x, w, scale):
@@ -94,6 +94,11 @@ class _Fp8BlockLinear(torch.autograd.Function):
 def fp8_block_linear(x, weight, weight_scale):
     """x (..., K) bf16 times weight (N, K) float8_e4m3fn with weight_scale (ceil(N/128), ceil(K/128)) fp32 -> (..., N) bf16.
     N a multiple of 8, K of 16.  Differentiable in x (its gradient is quantised along N); the weights are frozen."""
+    fast = L.fast() if x.is_cuda else None
+    if fast is not None:
+        out = fast.fp8_block_linear(x, weight, weight_scale, L.status_word(x.device))
+        if out is not None:
+            return out
     if torch.is_autocast_enabled("cuda") and x.is_floating_point():
         x = x.to(torch.get_autocast_dtype("cuda"))
     L.require_cuda_bf16("x", x)
@@ -115,6 +120,12 @@ def moe_fp8_block(hidden, top_k_indices, top_k_weights, gate_up_proj, gate_up_sc
     float8_e4m3fn with scales (E, 2I/128, H/128) and (E, H/128, I/128) fp32 -> (N,H) bf16.  SiLU-GLU experts; H and I multiples of
     128; silu(gate) * up is requantised from fp32.  No backward: an input that requires a gradient is refused in grad mode (`moe` and
     `moe_mxfp8` train)."""
+    fast = L.fast() if hidden.is_cuda else None
+    if fast is not None:
+        out = fast.moe_fp8_block(hidden, top_k_indices, top_k_weights, gate_up_proj, gate_up_scale, down_proj, down_scale,
+                                 L.status_word(hidden.device))
+        if out is not None:
+            return out
     (hidden,) = (hidden.to(torch.get_autocast_dtype("cuda")),) if torch.is_autocast_enabled("cuda") else (hidden,)
     L.require_cuda_bf16("hidden", hidden)
     L.require(not (torch.is_grad_enabled() and (hidden.requires_grad or top_k_weights.requires_grad)),

@@ -157,17 +157,17 @@ def group_topk_bwd(logits, idx, grad_w, scoring, norm_topk=True, scale=1.0):
 
 @_op("router_losses_fwd", 3)
 def router_losses_fwd(logits, idx, mask, segments, scoring):
-    """logits (N,E) and picks (N,k) of `segments` equal segments -> (losses (2,) fp32, coefficients for the backward)."""
+    """logits (N,E) and picks (N,k) of `segments` equal segments -> (balance, z, coefficients for the backward), fp32."""
     kind, (N, E), dev = _logits_type(logits), logits.shape, logits.device
     with L.on_device_of(logits):
         coef = torch.empty(segments * E + 2, dtype=torch.float32, device=dev)
-        losses = torch.empty(2, dtype=torch.float32, device=dev)
+        balance, z = (torch.empty((), dtype=torch.float32, device=dev) for _ in range(2))
         lib, S = L.lib(), N // segments
         ws = L.workspace(lib.b200moe_router_losses_ws_bytes(S, segments, E), dev)
         L.check(lib.b200moe_router_losses_fwd(logits.data_ptr(), kind, idx.data_ptr(), L.ptr(mask), S, segments, E, idx.shape[1], scoring,
-                                              ws.data_ptr(), coef.data_ptr(), losses.data_ptr(), L.status_word(dev).data_ptr(),
+                                              ws.data_ptr(), coef.data_ptr(), balance.data_ptr(), z.data_ptr(), L.status_word(dev).data_ptr(),
                                               L.stream_of(logits)))
-    return losses, coef
+    return balance, z, coef
 
 
 @_op("router_losses_bwd", 1)

@@ -181,7 +181,7 @@ _GROUP_SCORE = {"top2": 1, "max": 0}
 
 
 class _GroupTopk(torch.autograd.Function):
-    """(idx (N,k) int64, weights (N,k) fp32, counts (E,) int32) of contiguous logits (N,E); only the weights are differentiable."""
+    """Plain calls take the compiled form of this Function and of `_RouterLosses` (csrc/fast.cpp).  (idx (N,k) int64, weights (N,k) fp32, counts (E,) int32) of contiguous logits (N,E); only the weights are differentiable."""
 
     @staticmethod
     def forward(ctx, logits, bias, top_k, groups, opened, scoring, top2, norm, scale):
@@ -216,6 +216,12 @@ def group_topk(logits, top_k, bias=None, num_groups=1, topk_groups=None, scoring
     L.require(logits.dim() in (2, 3), "logits must be (N,E) or (B,S,E)")
     L.require(logits.is_cuda, "logits must be a CUDA tensor (this package has no CPU path)")
     opened = int(num_groups) if topk_groups is None else int(topk_groups)
+    fast = L.fast()
+    if fast is not None:
+        res = fast.group_topk(logits, bias, int(top_k), int(num_groups), opened, _SCORING[scoring], _GROUP_SCORE[group_score],
+                              bool(norm_topk_prob and top_k > 1), float(routed_scaling_factor), bool(return_counts))
+        if res is not None:
+            return res if return_counts else res[:2]
     if bias is not None:
         bias = bias.detach()
         L.require(bias.device == logits.device and bias.numel() == logits.shape[-1], "bias must have E elements on the logits' device")
@@ -284,11 +290,11 @@ class _RouterLosses(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, idx, mask, segments, scoring):
-        losses, coef = ops.router_losses_fwd(logits, idx, mask, segments, scoring)
+        balance, z, coef = ops.router_losses_fwd(logits, idx, mask, segments, scoring)
         ctx.args = (segments, scoring)
         ctx.save_for_backward(logits, mask, coef)
         ctx.set_materialize_grads(False)
-        return losses[0], losses[1]
+        return balance, z
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -313,6 +319,11 @@ def router_losses(logits, top_k_indices, scoring="softmax", mask=None, per_seque
     L.require(logits.is_cuda, "logits must be a CUDA tensor (this package has no CPU path)")
     L.require(not per_sequence or logits.dim() == 3, "per_sequence needs logits (B,S,E)")
     idx = top_k_indices
+    fast = L.fast()
+    if fast is not None:
+        res = fast.router_losses(logits, idx, mask, L.status_word(logits.device), _SCORING[scoring], bool(per_sequence))
+        if res is not None:
+            return res
     L.require(idx.device == logits.device and idx.dtype == torch.int64 and idx.dim() == logits.dim() and idx.shape[:-1] == logits.shape[:-1],
               "top_k_indices must be int64 (...,k) on the logits' device")
     E = logits.shape[-1]
@@ -327,8 +338,7 @@ def router_losses(logits, top_k_indices, scoring="softmax", mask=None, per_seque
         return zero, zero.clone()
     if torch.is_grad_enabled() and flat.requires_grad:
         return _RouterLosses.apply(flat, idx, mask, segments, _SCORING[scoring])
-    losses, _ = ops.router_losses_fwd(flat, idx, mask, segments, _SCORING[scoring])
-    return losses[0], losses[1]
+    return ops.router_losses_fwd(flat, idx, mask, segments, _SCORING[scoring])[:2]
 
 
 @torch.no_grad()
