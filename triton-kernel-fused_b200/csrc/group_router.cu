@@ -27,12 +27,14 @@ constexpr int kGroupWarps = 8;
 template <bool SOFTMAX>
 constexpr float kNear = SOFTMAX ? 3.814697265625e-6f : 1.9073486328125e-6f;   // 2^-18, 2^-19
 
-// A value as a key of the same order: 0 lies below every value, NaN above infinity, the zeros are one
-__device__ __forceinline__ uint32_t key_of(float v) {
-  const uint32_t u = __float_as_uint(v + 0.0f);
-  return v != v ? 0xffffffffu : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+// A value (no NaN) as a signed integer of the same order, and back; kNone lies below every value
+constexpr int kNone = static_cast<int>(0x80000000u);
+__device__ __forceinline__ int key_of(float v) {
+  const int i = __float_as_int(v);
+  return i ^ ((i >> 31) & 0x7fffffff);
 }
-__device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k); }
+__device__ __forceinline__ float value_of(int k) { return __int_as_float(k ^ ((k >> 31) & 0x7fffffff)); }
+// ... and in 64 bits, with NaN above infinity; 0 lies below every value, the zeros are one
 __device__ __forceinline__ unsigned long long key_of(double v) {
   const unsigned long long u = __double_as_longlong(v + 0.0);
   return v != v ? ~0ull : (u >> 63) ? ~u : (u | (1ull << 63));
@@ -51,35 +53,18 @@ struct GroupParams {
   int count_direct;   // one CTA does all: counts are written, not added to
 };
 
-// The scores of a lane's experts in 64 bits; m: the row's largest logit
-template <bool SOFTMAX, int V>
-__device__ __forceinline__ void scores64(const float (&z)[V], int live, float m, double (&s)[V]) {
-  if constexpr (SOFTMAX) {
-    double sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      s[i] = i < live ? exp(static_cast<double>(z[i]) - static_cast<double>(m)) : 0.0;
-      sum += s[i];
-    }
-    sum = warp_sum(sum);
-#pragma unroll
-    for (int i = 0; i < V; ++i) s[i] = m == -INFINITY ? 0.0 : s[i] / sum;
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) s[i] = 1.0 / (1.0 + exp(-static_cast<double>(z[i])));
-  }
-}
-
 // The two largest of a group's values, over the lanes it owns; NaN counts as infinity
-template <class F, int V>
-__device__ __forceinline__ void group_best(const F (&v)[V], int live, int lanes_log, F& a, F& b) {
-  a = b = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const F x = i >= live ? static_cast<F>(-INFINITY) : v[i] != v[i] ? static_cast<F>(INFINITY) : v[i];
-    b = x > a ? a : (x > b ? x : b);
-    a = x > a ? x : a;
-  }
+__device__ __forceinline__ void best_of(float x, float& a, float& b) {      // no NaN
+  b = fmaxf(b, fminf(a, x));
+  a = fmaxf(a, x);
+}
+__device__ __forceinline__ void best_of(double x, double& a, double& b) {
+  x = x != x ? static_cast<double>(INFINITY) : x;
+  b = x > a ? a : (x > b ? x : b);
+  a = x > a ? x : a;
+}
+template <class F>
+__device__ __forceinline__ void group_best(int lanes_log, F& a, F& b) {
   for (int off = 1; off < (1 << lanes_log); off <<= 1) {
     const F oa = __shfl_xor_sync(0xffffffffu, a, off), ob = __shfl_xor_sync(0xffffffffu, b, off);
     const F lo = oa > a ? a : oa;
@@ -92,26 +77,110 @@ __device__ __forceinline__ void group_best(const F (&v)[V], int live, int lanes_
 template <class F>
 __device__ __forceinline__ bool group_open(F value, int g, int groups, int lanes_log, int open, F near, bool& close) {
   int rank = 0;
-  bool below = false;
   for (int j = 0; j < groups; ++j) {
     const F o = __shfl_sync(0xffffffffu, value, j << lanes_log);
-    const bool ahead = o > value || (o == value && j < g);
-    rank += ahead ? 1 : 0;
-    below = below || (!ahead && j != g && value - o <= near);
+    rank += o > value || (o == value && j < g) ? 1 : 0;
   }
-  close = __any_sync(0xffffffffu, g < groups && rank == open - 1 && below);
-  return g < groups && rank < open;
+  const bool in = g < groups;
+  const int last = __ffs(__ballot_sync(0xffffffffu, in && rank == open - 1)) - 1;
+  const F border = __shfl_sync(0xffffffffu, value, last < 0 ? 0 : last);
+  close = __any_sync(0xffffffffu, in && rank >= open && border - value <= near);
+  return in && rank < open;
+}
+
+// The rest is for tokens that fp32 does not decide.  Out of line, with the logits read again one by one: inlined, its 64-bit arithmetic
+// doubled the kernel's registers (32 768 tokens, 8 of 256 experts in 4 of 8 groups: 128 us with it inside, whether it ran or not).
+template <class T, bool SOFTMAX>
+struct Exact {
+  const GroupParams& p;
+  const T* z;          // the lane's logits
+  int first, live;
+  double m, sum;       // softmax: the row's largest logit, its denominator
+  __device__ __forceinline__ Exact(const GroupParams& p_, long long t, int first_, int live_, float m_)
+      : p(p_), z(reinterpret_cast<const T*>(p_.logits) + t * p_.E + first_), first(first_), live(live_), m(m_), sum(1.0) {
+    if constexpr (SOFTMAX) {
+      double s = 0.0;
+#pragma unroll 1
+      for (int i = 0; i < live; ++i) s += exp(static_cast<double>(to_f32(z[i])) - m);
+      sum = warp_sum(s);
+    }
+  }
+  __device__ __forceinline__ double score(float logit) const {
+    if constexpr (SOFTMAX) return m == -INFINITY ? 0.0 : exp(static_cast<double>(logit) - m) / sum;
+    else return 1.0 / (1.0 + exp(-static_cast<double>(logit)));
+  }
+  __device__ __forceinline__ double value(int i) const {      // what selection compares
+    if (p.bias == nullptr) return score(to_f32(z[i]));
+    return score(to_f32(z[i])) + static_cast<double>(p.bias[first + i]);
+  }
+};
+
+template <class T, bool SOFTMAX>
+__device__ __noinline__ bool open_exactly(const GroupParams& p, long long t, int g, int first, int live, float m) {
+  const Exact<T, SOFTMAX> x(p, t, first, live, m);
+  double a = -INFINITY, b = -INFINITY;
+#pragma unroll 1
+  for (int i = 0; i < live; ++i) best_of(x.value(i), a, b);
+  group_best(p.lanes_log, a, b);
+  bool close;
+  return group_open(p.top2 && p.per_group > 1 ? a + b : a, g, p.groups, p.lanes_log, p.open, -1.0, close);
+}
+
+// the rank of a lane's candidate (its logit and bias) among n
+template <class T, bool SOFTMAX>
+__device__ __noinline__ int rank_exactly(const GroupParams& p, long long t, int first, int live, float m, int n, float logit, float bias) {
+  const Exact<T, SOFTMAX> x(p, t, first, live, m);
+  const unsigned long long key = key_of(x.score(logit) + static_cast<double>(bias));
+  const int lane = threadIdx.x & 31;
+  int rank = 0;
+#pragma unroll 1
+  for (int j = 0; j < n; ++j) {
+    const unsigned long long o = __shfl_sync(0xffffffffu, key, j);
+    rank += o > key || (o == key && j < lane) ? 1 : 0;
+  }
+  return rank;
+}
+
+// More than 32 candidates (rows of equal logits): k rounds of argmax over keys in shared memory.  live: 0 for a closed group
+template <class T, bool SOFTMAX>
+__device__ __noinline__ void pick_exactly(const GroupParams& p, long long t, int first, int live, int open_live, float m, unsigned long long* keys,
+                                          float2* pick) {
+  const Exact<T, SOFTMAX> x(p, t, first, live, m);
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int i = 0; i < open_live; ++i)
+    keys[first + i] = key_of(p.bias == nullptr ? static_cast<double>(to_f32(x.z[i])) : x.value(i));
+#pragma unroll 1
+  for (int j = 0; j < p.k; ++j) {
+    unsigned long long best = 0ull;
+    int at = 0;
+#pragma unroll 1
+    for (int i = 0; i < open_live; ++i)
+      if (keys[first + i] > best) {
+        best = keys[first + i];
+        at = i;
+      }
+    const uint32_t hi = static_cast<uint32_t>(best >> 32), lo = static_cast<uint32_t>(best);
+    const uint32_t th = __reduce_max_sync(0xffffffffu, hi);
+    const uint32_t tl = __reduce_max_sync(0xffffffffu, hi == th ? lo : 0u);
+    const int owner = __ffs(__ballot_sync(0xffffffffu, hi == th && lo == tl)) - 1;   // lanes hold ascending experts
+    if (lane == owner) {
+      pick[j] = make_float2(__int_as_float(first + at), to_f32(x.z[at]));
+      keys[first + at] = 0ull;
+    }
+    __syncwarp();
+  }
 }
 
 template <class T, bool SOFTMAX, int V>
-__global__ void __launch_bounds__(32 * kGroupWarps)
-group_topk_kernel(const GroupParams p) {
+__global__ void __launch_bounds__(32 * kGroupWarps, V > 8 ? 1 : 4)
+group_topk_kernel(const __grid_constant__ GroupParams p) {
   grid_dep_begin();
   __shared__ int hist[B200MOE_MAX_EXPERTS];
-  __shared__ float4 cand_s[kGroupWarps][32];     // value, logit, bias, expert
+  __shared__ int2 cand_s[kGroupWarps][32];       // key, expert
   __shared__ float2 pick_s[kGroupWarps][32];     // expert, logit
+  __shared__ unsigned long long key_s[kGroupWarps][B200MOE_MAX_EXPERTS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const unsigned lower = (1u << lane) - 1u;
   if (p.counts != nullptr) {
     for (int e = threadIdx.x; e < p.E; e += blockDim.x) hist[e] = 0;
     __syncthreads();
@@ -126,155 +195,143 @@ group_topk_kernel(const GroupParams p) {
     span = fmaxf(span, 1.0f + fabsf(bias[i]));
   }
   const bool by_logit = p.bias == nullptr;
-  const float near = by_logit ? -1.0f : kNear<SOFTMAX> * warp_max(span);
-  float4* cand = cand_s[warp];
+  const float near = kNear<SOFTMAX> * warp_max(span);
+  int2* cand = cand_s[warp];
   float2* pick = pick_s[warp];
 
   for (long long t = static_cast<long long>(blockIdx.x) * kGroupWarps + warp; t < p.T;
        t += static_cast<long long>(gridDim.x) * kGroupWarps) {
-    float z[V], v[V];
-    load_values<T, V>(reinterpret_cast<const T*>(p.logits) + t * p.E + first, live, p.vec, z);
-    // ---- scores and selection values
+    const T* row = reinterpret_cast<const T*>(p.logits) + t * p.E;
+    float v[V];
+    load_values<T, V>(row + first, live, p.vec, v);
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < V; ++i) odd = odd || v[i] != v[i];
+    odd = __any_sync(0xffffffffu, odd);          // a row with NaN
+    // ---- what selection compares: the logits, or scores + bias (groups by two: the scores, until a group is chosen)
+    const bool sums = p.open < p.groups && p.top2;
+    int key[V];
     float m = 0.0f, inv = 0.0f;
     if constexpr (SOFTMAX) {
-      m = z[0];
+      m = v[0];
 #pragma unroll
-      for (int i = 1; i < V; ++i) m = fmaxf(m, z[i]);
+      for (int i = 1; i < V; ++i) m = fmaxf(m, v[i]);
       m = warp_max(m);
-      float sum = 0.0f;
+    }
+    if (by_logit) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        v[i] = i < live ? __expf(z[i] - m) : 0.0f;
-        sum += v[i];
+      for (int i = 0; i < V; ++i) key[i] = i < live ? key_of(v[i] + 0.0f) : kNone;
+    }
+    if (SOFTMAX || !by_logit || sums) {
+      if constexpr (SOFTMAX) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          v[i] = m == -INFINITY ? 0.0f : __expf(v[i] - m);       // a value that does not exist is -inf
+          sum += v[i];
+        }
+        sum = warp_sum(sum);
+        inv = m == -INFINITY ? 0.0f : 1.0f / sum;
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = v[i] * inv + bias[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = __fdividef(1.0f, 1.0f + __expf(-v[i])) + bias[i];
       }
-      sum = warp_sum(sum);
-      inv = m == -INFINITY ? 0.0f : 1.0f / sum;
+    }
+    if (!by_logit) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = m == -INFINITY ? bias[i] : v[i] * inv + bias[i];
-    } else if (!by_logit || p.top2) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = __fdividef(1.0f, 1.0f + __expf(-z[i])) + bias[i];
+      for (int i = 0; i < V; ++i) key[i] = i < live ? key_of(v[i]) : kNone;
     }
     // ---- the open groups
     bool mine = live > 0;
     if (p.open < p.groups) {
-      float a, b;
-      const bool direct = by_logit && !p.top2;           // the largest logit decides
-      if (direct) group_best(z, live, p.lanes_log, a, b);
-      else group_best(v, live, p.lanes_log, a, b);
-      bool close;
-      mine = group_open(p.top2 && p.per_group > 1 ? a + b : a, g, p.groups, p.lanes_log, p.open,
-                        direct ? -1.0f : 2.0f * (by_logit ? kNear<SOFTMAX> : near), close) && live > 0;
-      if (close) {                                        // two groups that fp32 does not tell apart
-        double s[V], a2, b2;
-        scores64<SOFTMAX, V>(z, live, m, s);
+      bool close = odd;
+      if (!odd) {
+        float a = -INFINITY, b = -INFINITY;
+        const bool direct = by_logit && !p.top2;           // the largest logit decides
+        if (direct) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) s[i] += static_cast<double>(bias[i]);
-        group_best(s, live, p.lanes_log, a2, b2);
-        mine = group_open(p.top2 && p.per_group > 1 ? a2 + b2 : a2, g, p.groups, p.lanes_log, p.open, -1.0, close) && live > 0;
+          for (int i = 0; i < V; ++i)
+            if (i < live) a = fmaxf(a, value_of(key[i]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            if (i < live) best_of(v[i], a, b);
+        }
+        group_best(p.lanes_log, a, b);
+        mine = group_open(p.top2 && p.per_group > 1 ? a + b : a, g, p.groups, p.lanes_log, p.open, direct ? -1.0f : 2.0f * near, close) && mine;
+      }
+      if (close) mine = open_exactly<T, SOFTMAX>(p, t, g, first, live, m) && live > 0;
+      if (!mine) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) key[i] = kNone;
       }
     }
     // ---- candidates: every expert that reaches the k-th largest of the lanes' maxima (less `near`)
-    uint32_t key[V], best = 0u;
+    int best = key[0];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      key[i] = mine && i < live ? key_of(by_logit ? z[i] : v[i]) : 0u;
-      best = max(best, key[i]);
-    }
-    uint32_t floor_key = 1u;
-    for (int n = 0;;) {
-      const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-      if (top == 0u) {       // fewer than k lanes with an expert: all of them
-        floor_key = 1u;
-        break;
-      }
-      const bool at = best == top;
-      n += __popc(__ballot_sync(0xffffffffu, at));
-      if (at) best = 0u;
+    for (int i = 1; i < V; ++i) best = max(best, key[i]);
+    int floor_key = kNone + 1;
+    for (int n = 0; n < p.k;) {
+      const int top = __reduce_max_sync(0xffffffffu, best);
       floor_key = top;
-      if (n >= p.k) break;
+      if (top == kNone) break;
+      const unsigned at = __ballot_sync(0xffffffffu, best == top);
+      n += __popc(at);
+      if (best == top) best = kNone;
     }
-    if (!by_logit && floor_key != 1u) {
-      const float f = value_of(floor_key);
-      floor_key = f == f && fabsf(f) < INFINITY ? key_of(f - near) : floor_key;
-    }
-    int n = 0;
+    // fewer than k lanes with an expert: all of them; else what `near` may hide below it too
+    if (floor_key == kNone) floor_key = kNone + 1;
+    else if (!by_logit) floor_key = min(floor_key, key_of(value_of(floor_key) - near));
+    // collected in the order of the experts, so that of equal ones the first collected wins
+    int have = 0;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const bool in = key[i] >= floor_key;
-      const unsigned b = __ballot_sync(0xffffffffu, in);
-      const int at = n + __popc(b & lower);
-      if (in && at < 32) cand[at] = make_float4(by_logit ? z[i] : v[i], z[i], bias[i], __int_as_float(first + i));
-      n += __popc(b);
-    }
-    __syncwarp();
-    if (n <= 32) {
-      const float4 c = lane < n ? cand[lane] : make_float4(0.f, 0.f, 0.f, 0.f);
-      const uint32_t ck = key_of(c.x);
-      const int ce = __float_as_int(c.w);
-      int rank = 0;
-      bool close = false;
-      for (int j = 0; j < n; ++j) {
-        const float4 o = cand[j];
-        const uint32_t ok = key_of(o.x);
-        rank += ok > ck || (ok == ck && __float_as_int(o.w) < ce) ? 1 : 0;
-        close = close || (fabsf(o.x - c.x) <= near && (o.y != c.y || o.z != c.z));
-      }
-      if (__any_sync(0xffffffffu, lane < n && rank < p.k && close)) {     // picks that fp32 does not tell apart
-        double d;
-        if constexpr (SOFTMAX) {
-          double s[V], sum = 0.0;
+    for (int i = 0; i < V; ++i) have += key[i] >= floor_key ? 1 : 0;
+    int at = have;
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            s[i] = i < live ? exp(static_cast<double>(z[i]) - static_cast<double>(m)) : 0.0;
-            sum += s[i];
-          }
-          sum = warp_sum(sum);
-          d = m == -INFINITY ? 0.0 : exp(static_cast<double>(c.y) - static_cast<double>(m)) / sum;
-        } else {
-          d = 1.0 / (1.0 + exp(-static_cast<double>(c.y)));
-        }
-        const unsigned long long dk = key_of(d + static_cast<double>(c.z));
-        rank = 0;
-        for (int j = 0; j < n; ++j) {
-          const unsigned long long ok = __shfl_sync(0xffffffffu, dk, j);
-          const int oe = __shfl_sync(0xffffffffu, ce, j);
-          rank += ok > dk || (ok == dk && oe < ce) ? 1 : 0;
-        }
-      }
-      if (lane < n && rank < p.k) pick[rank] = make_float2(__int_as_float(ce), c.y);
-    } else {
-      // more than 32 candidates (rows of equal logits): k rounds of argmax, in 64 bits where there is a bias
-      unsigned long long k64[V];
-      double s[V];
-      if (!by_logit) scores64<SOFTMAX, V>(z, live, m, s);
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, at, off);
+      if (lane >= off) at += o;
+    }
+    const int n = __shfl_sync(0xffffffffu, at, 31);
+    if (n <= 32 && !odd) {
+      at -= have;
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        k64[i] = mine && i < live ? key_of(by_logit ? static_cast<double>(z[i]) : s[i] + static_cast<double>(bias[i])) : 0ull;
-      for (int j = 0; j < p.k; ++j) {
-        unsigned long long bk = k64[0];
-        int bi = 0;
-#pragma unroll
-        for (int i = 1; i < V; ++i)
-          if (k64[i] > bk) {
-            bk = k64[i];
-            bi = i;
+        if (key[i] >= floor_key) cand[at++] = make_int2(key[i], first + i);
+      __syncwarp();
+      const int2 c = lane < n ? cand[lane] : make_int2(kNone, 0);
+      const float logit = to_f32(row[c.y]);
+      const float value = lane < n ? value_of(c.x) : -INFINITY;
+      int rank = 0, level = 0;                     // level: candidates within `near` of this one, itself among them
+      if (by_logit) {
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) {
+          const int o = __shfl_sync(0xffffffffu, c.x, j);
+          rank += o > c.x || (o == c.x && j < lane) ? 1 : 0;
+        }
+      } else {
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) {
+          const float o = __shfl_sync(0xffffffffu, value, j);
+          rank += o > value || (o == value && j < lane) ? 1 : 0;
+          level += fabsf(o - value) <= near ? 1 : 0;
+        }
+        if (__any_sync(0xffffffffu, lane < n && rank < p.k && level > 1)) {
+          // the same logit and bias is a tie; others are compared in 64 bits
+          const float b = p.bias[c.y];
+          bool close = false;
+          for (int j = 0; j < n; ++j) {
+            const float o = __shfl_sync(0xffffffffu, value, j), oz = __shfl_sync(0xffffffffu, logit, j), ob = __shfl_sync(0xffffffffu, b, j);
+            close = close || (fabsf(o - value) <= near && (oz != logit || ob != b));
           }
-        const uint32_t hi = static_cast<uint32_t>(bk >> 32), lo = static_cast<uint32_t>(bk);
-        const uint32_t th = __reduce_max_sync(0xffffffffu, hi);
-        const uint32_t tl = __reduce_max_sync(0xffffffffu, hi == th ? lo : 0u);
-        const int owner = __ffs(__ballot_sync(0xffffffffu, hi == th && lo == tl)) - 1;   // lanes hold ascending experts
-        if (lane == owner) {
-          float zi = z[0];
-#pragma unroll
-          for (int i = 0; i < V; ++i)
-            if (i == bi) {
-              zi = z[i];
-              k64[i] = 0ull;
-            }
-          pick[j] = make_float2(__int_as_float(first + bi), zi);
+          if (__any_sync(0xffffffffu, lane < n && rank < p.k && close)) rank = rank_exactly<T, SOFTMAX>(p, t, first, live, m, n, logit, b);
         }
       }
+      if (lane < n && rank < p.k) pick[rank] = make_float2(__int_as_float(c.y), logit);
+    } else {
+      pick_exactly<T, SOFTMAX>(p, t, first, live, mine ? live : 0, m, key_s[warp], pick);
     }
     __syncwarp();
     // ---- lane j < k: pick j and its weight
