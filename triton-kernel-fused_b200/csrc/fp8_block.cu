@@ -2,57 +2,99 @@
 //
 //   scale = max(|x|) / 448 (a block's largest value becomes 448, e4m3's largest), code = nearest e4m3 to 448 x / max(|x|)
 //
-// Sixteen lanes a block, eight values each: one 16-byte load and one 8-byte store a lane.  Bound by HBM: 2 bytes in and one out a value.
-// With a table of rows (experts) a token's codes are made once and written to each of its rows.
+// Eight lanes a block, sixteen values each, kQuantAhead blocks of a lane on their way.  Bound by HBM, 2 bytes in and one out a value, and close
+// behind by issue: 8192 x 14336 in QT us (with sixteen lanes a block and quotients by division 120).  With a table of rows (experts) a
+// token's codes are made once and written to each of its rows.
 #include <algorithm>
 
 #include "fp8_block.cuh"
 
 namespace b200moe {
 
+constexpr int kQuantAhead = 3;
+
+// 16 values -> their codes
+__device__ __forceinline__ void block_codes(const uint4 (&v)[2], float factor, bool finite, uint2 (&o)[2]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t words[4] = {v[h].x, v[h].y, v[h].z, v[h].w};
+    float a[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[2 * i] = bf16_lo(words[i]) * factor;
+      a[2 * i + 1] = bf16_hi(words[i]) * factor;
+    }
+    if (finite) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] = block_snap(a[i]);
+    }
+    o[h] = make_uint2(cvt4_e4m3(a[0], a[1], a[2], a[3]), cvt4_e4m3(a[4], a[5], a[6], a[7]));
+  }
+}
+__device__ __forceinline__ uint32_t absmax8(uint32_t m, const uint4& v) {
+  return __vmaxu2(m, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+}
+
 __global__ void __launch_bounds__(256)
 fp8_block_quant_kernel(const __nv_bfloat16* x, long long rows, int K, const int* slot_row, int k, uint8_t* q, long long ldq, float* scale,
                        long long pitch) {
   grid_dep_begin();
-  const int lane16 = threadIdx.x & 15;
-  const unsigned half = 0xffffu << (threadIdx.x & 16);      // the lanes of this block
+  const int lane8 = threadIdx.x & 7;
   const int blocks = (K + kBlockK - 1) / kBlockK;
-  const long long total = rows * blocks;
-  for (long long i = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 4; i < total;
-       i += (static_cast<long long>(gridDim.x) * blockDim.x) >> 4) {
-    const long long r = i / blocks;
-    const int kb = static_cast<int>(i - r * blocks), c = kb * kBlockK + 8 * lane16;
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (c < K) v = *reinterpret_cast<const uint4*>(x + r * K + c);       // K is a multiple of 8
-    uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
-    m = max(m & 0xffffu, m >> 16) << 16;                                 // the bits of the largest |x|
-    m = __reduce_max_sync(half, m);
-    const float f = block_factor(m);
-    const bool finite = m < 0x7f800000u;
-    auto code = [&](uint32_t w, float& a, float& b) {
-      a = bf16_lo(w) * f;
-      b = bf16_hi(w) * f;
-      if (finite) {
-        a = block_snap(a);
-        b = block_snap(b);
+  // the first block of these eight lanes and their step, as (row, block of the row)
+  const long long begin = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 3;
+  const long long step = (static_cast<long long>(gridDim.x) * blockDim.x) >> 3;
+  const long long step_r = step / blocks;
+  const int step_b = static_cast<int>(step - step_r * blocks);
+  long long r = begin / blocks;
+  int b = static_cast<int>(begin - r * blocks);
+  while (__any_sync(0xffffffffu, r < rows)) {      // all four blocks of a warp, for the shuffles
+    uint4 v[kQuantAhead][2];
+    long long row[kQuantAhead];
+    int kb[kQuantAhead];
+#pragma unroll
+    for (int u = 0; u < kQuantAhead; ++u) {
+      row[u] = r;
+      kb[u] = b;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = b * kBlockK + 64 * h + 8 * lane8;
+        v[u][h] = make_uint4(0u, 0u, 0u, 0u);
+        if (r < rows && c < K) v[u][h] = *reinterpret_cast<const uint4*>(x + r * K + c);       // K is a multiple of 8
       }
-    };
-    float a[8];
-    code(v.x, a[0], a[1]);
-    code(v.y, a[2], a[3]);
-    code(v.z, a[4], a[5]);
-    code(v.w, a[6], a[7]);
-    const uint2 o = make_uint2(cvt4_e4m3(a[0], a[1], a[2], a[3]), cvt4_e4m3(a[4], a[5], a[6], a[7]));
-    const float s = block_scale(m);
-    if (slot_row == nullptr) {
-      if (c < K) *reinterpret_cast<uint2*>(q + r * ldq + c) = o;
-      if (lane16 == 0) scale[scale_at(kb, pitch, r)] = s;
-    } else {
-      for (int j = 0; j < k; ++j) {
-        const long long to = slot_row[r * k + j];
-        if (to < 0) continue;            // a pick that names no expert has no row
-        if (c < K) *reinterpret_cast<uint2*>(q + to * ldq + c) = o;
-        if (lane16 == 0) scale[scale_at(kb, pitch, to)] = s;
+      r += step_r;
+      b += step_b;
+      if (b >= blocks) {
+        b -= blocks;
+        ++r;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kQuantAhead; ++u) {
+      uint32_t m = absmax8(absmax8(0u, v[u][0]), v[u][1]);
+#pragma unroll
+      for (int off = 4; off > 0; off >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, off));
+      m = max(m & 0xffffu, m >> 16) << 16;                                 // the bits of the largest |x|
+      if (row[u] >= rows) continue;
+      float s, f;
+      block_scale_factor(m, s, f);
+      uint2 o[2];
+      block_codes(v[u], f, m < 0x7f800000u, o);
+      const int c = kb[u] * kBlockK + 8 * lane8;
+      if (slot_row == nullptr) {
+        uint8_t* to = q + row[u] * ldq + c;
+        if (c < K) *reinterpret_cast<uint2*>(to) = o[0];
+        if (c + 64 < K) *reinterpret_cast<uint2*>(to + 64) = o[1];
+        if (lane8 == 0) scale[scale_at(kb[u], pitch, row[u])] = s;
+      } else {
+        for (int j = 0; j < k; ++j) {
+          const long long rr = slot_row[row[u] * k + j];
+          if (rr < 0) continue;            // a pick that names no expert has no row
+          uint8_t* to = q + rr * ldq + c;
+          if (c < K) *reinterpret_cast<uint2*>(to) = o[0];
+          if (c + 64 < K) *reinterpret_cast<uint2*>(to + 64) = o[1];
+          if (lane8 == 0) scale[scale_at(kb[u], pitch, rr)] = s;
+        }
       }
     }
   }
@@ -67,8 +109,8 @@ int fp8_block_quant(const void* x, int64_t rows, int64_t K, int64_t out_rows, co
                  (long long)ldq, (long long)pitch);
   B200_CHECK_ARG(aligned16(x) && reinterpret_cast<uintptr_t>(q) % 8 == 0, B200MOE_E_ALIGN, "fp8_block_quant: x must be 16-byte, q 8-byte aligned");
   if (rows == 0) return 0;
-  const int64_t blocks = (rows * ((K + kBlockK - 1) / kBlockK) + 15) / 16;
-  B200_LAUNCH(fp8_block_quant_kernel, static_cast<int>(std::min<int64_t>(blocks, static_cast<int64_t>(num_sms()) * 16)), 256, 0, stream,
+  const int64_t blocks = rows * ((K + kBlockK - 1) / kBlockK), ctas = std::max<int64_t>((blocks + 32 * kQuantAhead - 1) / (32 * kQuantAhead), std::min<int64_t>((blocks + 31) / 32, num_sms()));
+  B200_LAUNCH(fp8_block_quant_kernel, static_cast<int>(std::min<int64_t>(ctas, static_cast<int64_t>(num_sms()) * 16)), 256, 0, stream,
               reinterpret_cast<const __nv_bfloat16*>(x), static_cast<long long>(rows), static_cast<int>(K), slot_row, k,
               reinterpret_cast<uint8_t*>(q), static_cast<long long>(ldq), scale, static_cast<long long>(pitch));
   return 0;
@@ -92,30 +134,25 @@ fp8_block_quant_weight_kernel(const __nv_bfloat16* w, long long N, int K, uint8_
   for (int i = 0; i < 8; ++i) {
     v[i] = make_uint4(0u, 0u, 0u, 0u);
     if (c < K && r0 + 16 * i < N) v[i] = *reinterpret_cast<const uint4*>(w + (g * N + r0 + 16 * i) * K + c);
-    m = __vmaxu2(m, __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu), __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu)));
+    m = absmax8(m, v[i]);
   }
   m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16) << 16);
   if ((threadIdx.x & 31) == 0) warp_max_s[threadIdx.x >> 5] = m;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 8; ++i) m = max(m, warp_max_s[i]);
-  const float f = block_factor(m);
-  const bool finite = m < 0x7f800000u;
+  float sc, f;
+  block_scale_factor(m, sc, f);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (c >= K || r0 + 16 * i >= N) continue;
-    const uint32_t words[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-    uint32_t o[2];
+  for (int i = 0; i < 8; i += 2) {
+    const uint4 two[2] = {v[i], v[i + 1]};
+    uint2 o[2];
+    block_codes(two, f, m < 0x7f800000u, o);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float a[4] = {bf16_lo(words[2 * h]) * f, bf16_hi(words[2 * h]) * f, bf16_lo(words[2 * h + 1]) * f, bf16_hi(words[2 * h + 1]) * f};
-      if (finite)
-        for (int j = 0; j < 4; ++j) a[j] = block_snap(a[j]);
-      o[h] = cvt4_e4m3(a[0], a[1], a[2], a[3]);
-    }
-    *reinterpret_cast<uint2*>(q + (g * N + r0 + 16 * i) * K + c) = make_uint2(o[0], o[1]);
+    for (int h = 0; h < 2; ++h)
+      if (c < K && r0 + 16 * (i + h) < N) *reinterpret_cast<uint2*>(q + (g * N + r0 + 16 * (i + h)) * K + c) = o[h];
   }
-  if (threadIdx.x == 0) scale[blockIdx.x] = block_scale(m);
+  if (threadIdx.x == 0) scale[blockIdx.x] = sc;
 }
 
 }  // namespace b200moe

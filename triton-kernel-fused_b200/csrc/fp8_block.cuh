@@ -14,9 +14,23 @@ constexpr int kBlockK = 128;                            // values that share a s
 constexpr uint32_t kAmaxFloor = 0x0d800000u;            // 2^-100: a block below it (of zeros) still has a scale
 constexpr float kE4m3Max = 448.0f;
 
-// scale = max(amax, 2^-100) / 448 and the factor 448 / amax that codes are made with; amax as the bits of |x|, so that NaN is above all
-__device__ __forceinline__ float block_scale(uint32_t amax_bits) { return __fdiv_rn(__uint_as_float(max(amax_bits, kAmaxFloor)), kE4m3Max); }
-__device__ __forceinline__ float block_factor(uint32_t amax_bits) { return __fdiv_rn(kE4m3Max, __uint_as_float(max(amax_bits, kAmaxFloor))); }
+// scale = max(amax, 2^-100) / 448, correctly rounded, and the factor 448 / amax that codes are made with; amax as the bits of |x|, so that NaN
+// is above all.  The quotient a / 448 = a / 7 / 64 is never nearer than 1/14 of a step to the middle between two fp32 numbers, so a product
+// with 1 / 448, corrected once by its remainder, rounds to the right one.
+__device__ __forceinline__ void block_scale_factor(uint32_t amax_bits, float& scale, float& factor) {
+  const float a = __uint_as_float(max(amax_bits, kAmaxFloor));
+  if (a < 1e30f) {
+    constexpr float kInv = 1.0f / kE4m3Max;
+    const float s = a * kInv;
+    scale = fmaf(fmaf(-s, kE4m3Max, a), kInv, s);
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a));
+    factor = kE4m3Max * r;
+  } else {                 // the reciprocal may be too small for a normal number; infinity and NaN
+    scale = __fdiv_rn(a, kE4m3Max);
+    factor = __fdiv_rn(kE4m3Max, a);
+  }
+}
 
 // A code is the e4m3 value nearest to 448 x / amax.  For bf16 x and amax, both of 8 bits, that quotient is either exactly half way between
 // two codes or at least 2^-13 away from there (relative), while x * (448 / amax) is off by 2^-23: rounded to 20 bits first, it is half

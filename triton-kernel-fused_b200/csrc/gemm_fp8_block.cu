@@ -299,7 +299,8 @@ block_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         amax = max(amax, s_amax[flip][half ^ 1][32 * q + lane]);
         flip ^= 1;
         if (live && ok) {
-          const float inv = block_factor(amax);
+          float scale, inv;
+          block_scale_factor(amax, scale, inv);
           const long long orow = row0 + lane;
           uint4* dst = reinterpret_cast<uint4*>(bp.q_out + orow * p.I + t.n0 + 64 * half);
 #pragma unroll
@@ -312,7 +313,7 @@ block_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
             }
             dst[v] = make_uint4(w[0], w[1], w[2], w[3]);
           }
-          if (half == 0) bp.q_scale[scale_at(t.n0 >> 7, bp.q_pitch, orow)] = block_scale(amax);
+          if (half == 0) bp.q_scale[scale_at(t.n0 >> 7, bp.q_pitch, orow)] = scale;
         }
       }
     }
@@ -663,8 +664,10 @@ block_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
             const int j = half * HC + i;
             if (i < mine) {
               const uint32_t m = max(max(s_amax[flip][0][j], s_amax[flip][1][j]), max(s_amax[flip][2][j], s_amax[flip][3][j]));
-              bp.q_out[(row + i) * p.I + col] = static_cast<uint8_t>(__nv_cvt_float_to_fp8(acc[0][i] * block_factor(m), __NV_SATFINITE, __NV_E4M3));
-              if (q == 0 && lane == 0) bp.q_scale[scale_at(t.m0 >> 7, bp.q_pitch, row + i)] = block_scale(m);
+              float scale, inv;
+              block_scale_factor(m, scale, inv);
+              bp.q_out[(row + i) * p.I + col] = static_cast<uint8_t>(__nv_cvt_float_to_fp8(acc[0][i] * inv, __NV_SATFINITE, __NV_E4M3));
+              if (q == 0 && lane == 0) bp.q_scale[scale_at(t.m0 >> 7, bp.q_pitch, row + i)] = scale;
             }
           }
         }
