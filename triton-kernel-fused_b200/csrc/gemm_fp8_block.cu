@@ -84,29 +84,44 @@ __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(
 // ------------------------------------------------------------------------------------------------ many rows: pairs of SMs
 // A cluster of two CTAs computes 256 rows x 256 columns with cta_group::2 MMAs: each stages its own 128 rows of X and 128 rows of W (SwiGLU: one
 // the gate, the other the up rows of the same 128 columns).  Two k-blocks' sums of 256 columns fill tensor memory.  An epilogue warp owns
-// 32 rows and 128 columns (SwiGLU: 64 of gate and the same 64 of up), so its scales are one number a thread and k-block, or two.
-constexpr int kBStages = 6;
+// 32 rows and 128 columns (SwiGLU: 64 of gate and the same 64 of up), 128 accumulators a thread.
+//
+// Bound: the MMAs of a k-block take 512 cycles, the multiply-adds of the epilogue 386 beside them, but between the two lie four signals of 130
+// to 220 cycles each, for two k-blocks: some 900 cycles in all (1635 MHz under the power cap).  So what counts is how long the epilogue holds
+// tensor memory.  8192 x 14336 x 4096, us: arrivals as releases 984 (mbar_arrive_tmem), scales from global memory by the epilogue's threads 488,
+// by a warp that prepares them 455; 2112 TFLOP/s.  Slower: 16 epilogue warps 519; columns 32 at a time 485; plain multiply-adds in place of
+// packed ones 466; the other CTA's arrivals passed on by one thread 500; tensor memory as four half k-blocks 535.  Each of the 128 + 16
+// registers counts: twelve warps could have 168 each, at which every form spilled in the loop (500 to 900 us), so the four that issue
+// loads and MMAs hand theirs over, 4 x 72 + 8 x 216 = 12 x 168.
+constexpr int kBEpi = 8;                       // epilogue warps
+constexpr int kBParts = kBEpi / 4;             // ... that share a tile's columns
+constexpr int kBCols = 256 / kBParts;          // columns of one
+constexpr int kBThreads = 32 * (4 + kBEpi);
+template <int EPI> constexpr int kBStages = EPI == EPI_STORE ? 5 : 6;
+constexpr int kBRing = 8;                      // k-blocks whose scales are in shared memory
 constexpr int kBStage = 2 * kBTile;
-template <int EPI> constexpr int kBEpiBytes = EPI == EPI_STORE ? kEpiWarps * kStageOutBytes : 0;     // SwiGLU stores its codes from registers
-template <int EPI> constexpr int kBSmemBytes = kBStages * kBStage + kBEpiBytes<EPI> + (2 * kBStages + 4) * 8 + 16 + 1024;
+template <int EPI> constexpr int kBEpiBytes = EPI == EPI_STORE ? kBEpi * 2048 : 0;     // SwiGLU stores its codes from registers
+template <int EPI> constexpr int kBSmemBytes = kBStages<EPI> * kBStage + kBEpiBytes<EPI> + kBRing * 1024 + (2 * kBStages<EPI> + 4) * 8 + 16 + 1024;
 
 template <int EPI, bool BMN>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kBThreads, 1)
 block_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmD,
                   const BlockParams bp) {
   const GemmParams& p = bp.g;
+  constexpr int kStages = kBStages<EPI>;
   constexpr int TM = 256, TN = EPI == EPI_SWIGLU ? 128 : 256;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* epi_smem = smem + kBStages * kBStage;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(epi_smem + kBEpiBytes<EPI>);
+  uint8_t* epi_smem = smem + kStages * kBStage;
+  float* ring = reinterpret_cast<float*>(epi_smem + kBEpiBytes<EPI>);      // [k-block % kBRing][column block][row]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + kBRing * 256);
   const uint32_t bar_full = smem_u32(bars);
-  const uint32_t bar_empty = smem_u32(bars + kBStages);
-  const uint32_t bar_tfull = smem_u32(bars + 2 * kBStages);
-  const uint32_t bar_tempty = smem_u32(bars + 2 * kBStages + 2);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kBStages + 4);
+  const uint32_t bar_empty = smem_u32(bars + kStages);
+  const uint32_t bar_tfull = smem_u32(bars + 2 * kStages);
+  const uint32_t bar_tempty = smem_u32(bars + 2 * kStages + 2);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  __shared__ uint32_t s_amax[2][2][128];
+  __shared__ uint32_t s_amax[2][4][128];
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int cta_rank = static_cast<int>(cluster_ctarank());
@@ -114,13 +129,13 @@ block_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
   const int tile_step = static_cast<int>(num_clusters_x());
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kBStages; ++s) {
+    for (int s = 0; s < kStages; ++s) {
       mbar_init(bar_full + 8 * s, 1);
       mbar_init(bar_empty + 8 * s, 1);
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(bar_tfull + 8 * b, 1);
-      mbar_init(bar_tempty + 8 * b, 2 * kEpiWarps);
+      mbar_init(bar_tfull + 8 * b, 2);      // the MMAs and the scales
+      mbar_init(bar_tempty + 8 * b, 2 * kBEpi);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -142,178 +157,207 @@ block_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
   const int total = total_tiles(p, TN, TM);
   const int nkb = (p.K + kBBK - 1) / kBBK;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------------------------ producer (each CTA)
-    if (elect_one()) {
-      const uint32_t full0 = mapa_shared(bar_full, 0);
-      int s = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      for (int tile = first_tile; tile < total && ok; tile += tile_step) {
-        const Tile t = get_tile(p, tile, TN, TM, kBBK);
-        const int m0 = t.m0 + BM * cta_rank;
-        const int n0 = EPI == EPI_SWIGLU ? t.n0 + p.I * cta_rank : t.n0 + 128 * cta_rank;
-        for (int kb = 0; kb < nkb; ++kb) {
-          if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, ST_WAIT_PRODUCER)) {
-            ok = false;
-            break;
-          }
-          if (cta_rank == 0) mbar_arrive_expect_tx(bar_full + 8 * s, 2 * kBStage);
-          const uint32_t sa = smem_u32(smem + s * kBStage), full = full0 + 8 * s;
-          tma_load_3d_pair(sa, &tmA, full, kb * kBBK, m0, 0);
-          if (BMN) tma_load_3d_pair(sa + kBTile, &tmB, full, n0, kb * kBBK, t.g);
-          else tma_load_3d_pair(sa + kBTile, &tmB, full, kb * kBBK, n0, t.g);
-          if (++s == kBStages) {
-            s = 0;
-            ph ^= 1;
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 0) {
+      // ------------------------------------------------------------------------------ producer (each CTA)
+      if (elect_one()) {
+        const uint32_t full0 = mapa_shared(bar_full, 0);
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int tile = first_tile; tile < total && ok; tile += tile_step) {
+          const Tile t = get_tile(p, tile, TN, TM, kBBK);
+          const int m0 = t.m0 + BM * cta_rank;
+          const int n0 = EPI == EPI_SWIGLU ? t.n0 + p.I * cta_rank : t.n0 + 128 * cta_rank;
+          for (int kb = 0; kb < nkb; ++kb) {
+            if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, ST_WAIT_PRODUCER)) {
+              ok = false;
+              break;
+            }
+            if (cta_rank == 0) mbar_arrive_expect_tx(bar_full + 8 * s, 2 * kBStage);
+            const uint32_t sa = smem_u32(smem + s * kBStage), full = full0 + 8 * s;
+            tma_load_3d_pair(sa, &tmA, full, kb * kBBK, m0, 0);
+            if (BMN) tma_load_3d_pair(sa + kBTile, &tmB, full, n0, kb * kBBK, t.g);
+            else tma_load_3d_pair(sa + kBTile, &tmB, full, kb * kBBK, n0, t.g);
+            if (++s == kStages) {
+              s = 0;
+              ph ^= 1;
+            }
           }
         }
       }
-    }
-    grid_dep_launch();   // the last loads are on their way
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------------------ MMA issuer (leader)
-    if (cta_rank == 0 && elect_one()) {
-      constexpr uint32_t idesc = idesc_f8(256, 256, BMN);
-      int s = 0;
-      uint32_t ph = 0, it = 0;
-      bool ok = true;
-      for (int tile = first_tile; tile < total && ok; tile += tile_step) {
-        for (int kb = 0; kb < nkb; ++kb, ++it) {
-          const int buf = it & 1;
-          if (!mbar_wait(bar_tempty + 8 * buf, ((it >> 1) & 1) ^ 1, abort_flag, ST_WAIT_MMA_TMEM) ||
-              !mbar_wait(bar_full + 8 * s, ph, abort_flag, ST_WAIT_MMA_FULL)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t sa = smem_u32(smem + s * kBStage), sb = sa + kBTile;
+      grid_dep_launch();   // the last loads are on their way
+    } else if (warp == 1) {
+      // ------------------------------------------------------------------------------ MMA issuer (leader)
+      if (cta_rank == 0 && elect_one()) {
+        constexpr uint32_t idesc = idesc_f8(256, 256, BMN);
+        int s = 0;
+        uint32_t ph = 0, it = 0;
+        bool ok = true;
+        for (int tile = first_tile; tile < total && ok; tile += tile_step) {
+          for (int kb = 0; kb < nkb; ++kb, ++it) {
+            const int buf = it & 1;
+            if (!mbar_wait(bar_tempty + 8 * buf, ((it >> 1) & 1) ^ 1, abort_flag, ST_WAIT_MMA_TMEM) ||
+                !mbar_wait(bar_full + 8 * s, ph, abort_flag, ST_WAIT_MMA_FULL)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t sa = smem_u32(smem + s * kBStage), sb = sa + kBTile;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_f8_pair(tmem_base + 256 * buf, umma_desc_sw128(sa + 32 * k, 0, 1024),
-                         umma_desc_sw128(sb + (BMN ? 4096 : 32) * k, 0, 1024), idesc, k != 0);
-          umma_commit_pair(bar_empty + 8 * s);
-          umma_commit_pair(bar_tfull + 8 * buf);
-          if (++s == kBStages) {
-            s = 0;
-            ph ^= 1;
+            for (int k = 0; k < 4; ++k)
+              umma_f8_pair(tmem_base + 256 * buf, umma_desc_sw128(sa + 32 * k, 0, 1024),
+                           umma_desc_sw128(sb + (BMN ? 4096 : 32) * k, 0, 1024), idesc, k != 0);
+            umma_commit_pair(bar_empty + 8 * s);
+            umma_commit_pair(bar_tfull + 8 * buf);
+            if (++s == kStages) {
+              s = 0;
+              ph ^= 1;
+            }
+          }
+        }
+      }
+    } else if (warp == 2) {
+      // ------------------------------------------------------------------------------ scales
+      // This warp multiplies the scales of 128 rows and of the tile's two column blocks, k-block by k-block, for the epilogue, whose warps have
+      // neither the registers nor the time to wait for global memory.  The MMAs of k-block i are complete only after the epilogue gave back
+      // the tensor memory of i - 2, having read its scales: once they are, the slot of i - 2 is free.  The arrival for k-block i has to follow
+      // the phase of i - 2 of the same barrier.
+      constexpr int kAhead = 4;
+      uint32_t it = 0;
+      bool ok = true;
+      for (int tile = first_tile; tile < total; tile += tile_step) {
+        const Tile t = get_tile(p, tile, TN, TM, kBBK);
+        const int nb = t.n0 >> 7;
+        const long long row = t.m0 + BM * cta_rank;
+        const bool rows = row < bp.rows;         // else none of these 128 exists
+        const float4* sx = reinterpret_cast<const float4*>(bp.sx + (rows ? row : 0)) + lane;
+        const float* sw = bp.sw + t.g * bp.sw_group + static_cast<long long>(nb) * bp.sw_n;
+        const float* sw2 = sw + static_cast<long long>(EPI == EPI_SWIGLU ? bp.n_blocks : nb + 1 < bp.n_blocks ? 1 : 0) * bp.sw_n;
+        float4 x[kAhead];
+        float w[kAhead], w2[kAhead];
+        auto get = [&](int kb, int u) {
+          if (kb < nkb) {
+            x[u] = sx[static_cast<long long>(kb) * (bp.sx_pitch >> 2)];
+            w[u] = sw[static_cast<long long>(kb) * bp.sw_k];
+            w2[u] = sw2[static_cast<long long>(kb) * bp.sw_k];
+          }
+        };
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) get(u, u);
+        for (int kb0 = 0; kb0 < nkb; kb0 += kAhead) {
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            if (kb0 + u >= nkb) break;
+            if (it >= 2) ok = ok && mbar_wait(bar_tfull + 8 * (it & 1), ((it >> 1) & 1) ^ 1, abort_flag, ST_WAIT_EPILOGUE);
+            float4* to = reinterpret_cast<float4*>(ring + (it & (kBRing - 1)) * 256) + lane;
+            to[0] = make_float4(x[u].x * w[u], x[u].y * w[u], x[u].z * w[u], x[u].w * w[u]);
+            to[32] = make_float4(x[u].x * w2[u], x[u].y * w2[u], x[u].z * w2[u], x[u].w * w2[u]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_tfull + 8 * (it & 1));
+            get(kb0 + u + kAhead, u);
+            ++it;
           }
         }
       }
     }
   } else {
     // ------------------------------------------------------------------------------ epilogue
-    const int q = warp & 3, half = (warp - 2) >> 2;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int q = warp & 3, part = (warp - 4) >> 2;
+    constexpr int HC = kBCols / 2;     // SwiGLU: columns of gate, and of up
     const uint32_t tempty_leader = mapa_shared(bar_tempty, 0);
-    uint8_t* sbuf = epi_smem + (warp - 2) * kStageOutBytes;
+    uint8_t* sbuf = epi_smem + (warp - 4) * 2048;
     uint32_t it = 0;
     int flip = 0;
     bool ok = true;      // a warp that gave up goes on to the barriers of the others
+    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + (EPI == EPI_SWIGLU ? HC : kBCols) * part;
     for (int tile = first_tile; tile < total; tile += tile_step) {
       const Tile t = get_tile(p, tile, TN, TM, kBBK);
       const int row0 = t.m0 + BM * cta_rank + 32 * q;
-      const long long row = min(static_cast<long long>(row0 + lane), bp.rows - 1);
       const bool live = p.sched != SCHED_GROUPED_M || row0 < p.poffs[t.g] + p.counts[t.g];   // else nothing but pad rows
-      // column blocks of this warp: its 128 columns, or 64 of gate and 64 of up
-      const int nb = EPI == EPI_SWIGLU ? t.n0 >> 7 : min((t.n0 >> 7) + half, bp.n_blocks - 1);
-      const float* sx = bp.sx + row;
-      const float* sw = bp.sw + t.g * bp.sw_group + static_cast<long long>(nb) * bp.sw_n;
-      const float* sw2 = sw + static_cast<long long>(bp.n_blocks) * bp.sw_n;     // SwiGLU: up
-      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + (EPI == EPI_SWIGLU ? 64 : 128) * half;
-      float2 acc[64];
+      float2 acc[kBCols / 2];
 #pragma unroll
-      for (int i = 0; i < 64; ++i) acc[i] = make_float2(0.0f, 0.0f);
-      float fx[2], fw[2], fu[2];     // scales of the next two k-blocks
-      auto scales = [&](int kb, int u) {
-        if (kb < nkb) {
-          fx[u] = sx[kb * bp.sx_pitch];
-          fw[u] = sw[static_cast<long long>(kb) * bp.sw_k];
-          if (EPI == EPI_SWIGLU) fu[u] = sw2[static_cast<long long>(kb) * bp.sw_k];
-        }
-      };
-      scales(0, 0);
-      scales(1, 1);
-      for (int kb0 = 0; kb0 < nkb; kb0 += 2) {
+      for (int i = 0; i < kBCols / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
+      for (int kb = 0; kb < nkb; ++kb, ++it) {
+        const int buf = it & 1;
+        ok = ok && mbar_wait(bar_tfull + 8 * buf, (it >> 1) & 1, abort_flag, ST_WAIT_EPILOGUE);
+        __syncwarp();
+        tc_fence_after();
+        const float* fs = ring + (it & (kBRing - 1)) * 256 + 32 * q + lane;
+        const float f = EPI == EPI_SWIGLU ? fs[0] : fs[2 * part >= kBParts ? 128 : 0], f2 = EPI == EPI_SWIGLU ? fs[128] : f;
+        if (live) {
+          const uint32_t ta = taddr + 256 * buf;
+          constexpr int NC = kBCols / 16;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          if (kb0 + u >= nkb) break;
-          const int buf = it & 1;
-          ok = ok && mbar_wait(bar_tfull + 8 * buf, (it >> 1) & 1, abort_flag, ST_WAIT_EPILOGUE);
-          ++it;
-          __syncwarp();
-          tc_fence_after();
-          const float f = fx[u] * fw[u], f2 = EPI == EPI_SWIGLU ? fx[u] * fu[u] : f;
-          scales(kb0 + u + 2, u);
-          if (live) {
-            uint32_t r[2][16];
-            const uint32_t ta = taddr + 256 * buf;
-            tmem_ld16(ta, r[0]);
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              tmem_ld_wait();
-              if (c < 7) {
-                tmem_ld16(ta + (EPI == EPI_SWIGLU && c + 1 >= 4 ? 64 : 0) + 16 * (c + 1), r[(c + 1) & 1]);
-              } else {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_tmem(tempty_leader + 8 * buf);
-              }
-              const float s = EPI == EPI_SWIGLU && c >= 4 ? f2 : f;
-#pragma unroll
-              for (int i = 0; i < 8; ++i) fma2(acc[8 * c + i], r[c & 1][2 * i], r[c & 1][2 * i + 1], make_float2(s, s));
+          for (int c = 0; c < NC; ++c) {
+            uint32_t r[16];
+            tmem_ld16(ta + (EPI == EPI_SWIGLU && 2 * c >= NC ? 128 - HC : 0) + 16 * c, r);
+            tmem_ld_wait();
+            if (c == NC - 1) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_tmem(tempty_leader + 8 * buf);
             }
-          } else {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_tmem(tempty_leader + 8 * buf);
+            const float s = EPI == EPI_SWIGLU && 2 * c >= NC ? f2 : f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) fma2(acc[8 * c + i], r[2 * i], r[2 * i + 1], make_float2(s, s));
           }
+        } else {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_tmem(tempty_leader + 8 * buf);
         }
       }
       if constexpr (EPI == EPI_STORE) {
         if (live && ok) {
 #pragma unroll
-          for (int cc = 0; cc < 2; ++cc) {
-            const int c = t.n0 + 128 * half + 64 * cc;
+          for (int cc = 0; cc < kBCols / 32; ++cc) {
+            const int c = t.n0 + kBCols * part + 32 * cc;
             if (c < p.N) {
-              uint32_t pk[32];
-#pragma unroll
-              for (int i = 0; i < 32; ++i) pk[i] = pack_bf16x2(acc[32 * cc + i].x, acc[32 * cc + i].y);
               staging_free(lane);
-              stage_row(sbuf, lane, pk);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {      // 32 columns of a row, 64-byte swizzle
+                const float2* x = acc + 16 * cc + 4 * j;
+                *reinterpret_cast<uint4*>(sbuf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
+                    make_uint4(pack_bf16x2(x[0].x, x[0].y), pack_bf16x2(x[1].x, x[1].y), pack_bf16x2(x[2].x, x[2].y), pack_bf16x2(x[3].x, x[3].y));
+              }
               store_box(&tmD, sbuf, lane, c, row0, 0);
             }
           }
         }
       } else {
-        // acc[0, 32): gate, acc[32, 64): up of the same 64 columns
+        // acc: gate, then up of the same HC columns
         uint32_t amax = 0u;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          acc[i].x = silu_mul(acc[i].x, acc[32 + i].x);
-          acc[i].y = silu_mul(acc[i].y, acc[32 + i].y);
+        for (int i = 0; i < HC / 2; ++i) {
+          acc[i].x = silu_mul(acc[i].x, acc[HC / 2 + i].x);
+          acc[i].y = silu_mul(acc[i].y, acc[HC / 2 + i].y);
           amax = max(amax, max(__float_as_uint(acc[i].x) & 0x7fffffffu, __float_as_uint(acc[i].y) & 0x7fffffffu));
         }
-        // the other half of the row's 128 columns: two buffers, since the other warp may be a tile ahead
-        s_amax[flip][half][32 * q + lane] = amax;
-        asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
-        amax = max(amax, s_amax[flip][half ^ 1][32 * q + lane]);
+        // the other parts of the row's 128 columns: two buffers, since another warp may be a tile ahead
+        s_amax[flip][part][32 * q + lane] = amax;
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + q), "n"(32 * kBParts) : "memory");
+#pragma unroll
+        for (int o = 0; o < kBParts; ++o) amax = max(amax, s_amax[flip][o][32 * q + lane]);
         flip ^= 1;
         if (live && ok) {
           float scale, inv;
           block_scale_factor(amax, scale, inv);
           const long long orow = row0 + lane;
-          uint4* dst = reinterpret_cast<uint4*>(bp.q_out + orow * p.I + t.n0 + 64 * half);
+          uint4* dst = reinterpret_cast<uint4*>(bp.q_out + orow * p.I + t.n0 + HC * part);
 #pragma unroll
-          for (int v = 0; v < 4; ++v) {
+          for (int v = 0; v < HC / 16; ++v) {
             uint32_t w[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const float2 a = acc[8 * v + 2 * j], b = acc[8 * v + 2 * j + 1];
-              w[j] = cvt4_e4m3(a.x * inv, a.y * inv, b.x * inv, b.y * inv);
+              const float2 x = acc[8 * v + 2 * j], y = acc[8 * v + 2 * j + 1];
+              w[j] = cvt4_e4m3(x.x * inv, x.y * inv, y.x * inv, y.y * inv);
             }
             dst[v] = make_uint4(w[0], w[1], w[2], w[3]);
           }
-          if (half == 0) bp.q_scale[scale_at(t.n0 >> 7, bp.q_pitch, orow)] = scale;
+          if (part == 0) bp.q_scale[scale_at(t.n0 >> 7, bp.q_pitch, orow)] = scale;
         }
       }
     }
@@ -703,10 +747,10 @@ static int launch_pair(const void* X, int64_t x_rows, int64_t ldx, const void* W
   int rc = make_map(&tmA, X, bp.g.K, x_rows, 1, ldx, x_rows * ldx, kBBK, 128, 1);
   if (rc == 0) rc = make_map(&tmB, W, w_inner, w_rows, groups, w_inner, w_rows * w_inner, 128, 128, 1);
   tmD = tmA;
-  if (rc == 0 && EPI == EPI_STORE) rc = make_map(&tmD, bp.g.D, bp.g.N, x_rows, 1, bp.g.ldd, x_rows * bp.g.ldd, 64, 32);
+  if (rc == 0 && EPI == EPI_STORE) rc = make_map(&tmD, bp.g.D, bp.g.N, x_rows, 1, bp.g.ldd, x_rows * bp.g.ldd, 32, 32, 2, 64);
   if (rc) return rc;
   const int pairs = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(gemm_cta_budget() / 2, max_tiles)));
-  B200_CUDA(launch_chained(block_pair_kernel<EPI, BMN>, pairs * 2, kThreads, kBSmemBytes<EPI>, stream, 2, tmA, tmB, tmD, bp));
+  B200_CUDA(launch_chained(block_pair_kernel<EPI, BMN>, pairs * 2, kBThreads, kBSmemBytes<EPI>, stream, 2, tmA, tmB, tmD, bp));
   return 0;
 }
 
