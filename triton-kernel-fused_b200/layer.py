@@ -8,10 +8,11 @@ import torch.nn as nn
 
 from . import _lib as L
 from .moe import FUSED_CODES, _amp_cast, _code_info, _codes_on, _float32, moe
+from .fp8_block import fp8_block_quantize_weight, moe_fp8_block
 from .mxfp8 import moe_mxfp8
-from .router import fused_mlp_router, router_bias_update
+from .router import fused_group_router, fused_mlp_router, router_bias_update, router_losses
 
-__all__ = ["MoELayer", "LoadBalanceMixin"]
+__all__ = ["MoELayer", "Fp8BlockMoELayer", "LoadBalanceMixin"]
 
 
 class LoadBalanceMixin:
@@ -138,10 +139,13 @@ class _Layer(torch.autograd.Function):
 
 class MoELayer(LoadBalanceMixin, nn.Module):
     def __init__(self, H, I, E, top_k=2, norm_topk_prob=True, routed_scaling_factor=1.0, init_std=0.02,
-                 precision="bf16", act_codes=None, learnable_situ=False):
+                 precision="bf16", act_codes=None, learnable_situ=False, scoring="sigmoid", num_groups=1, topk_groups=None,
+                 group_score="top2", balance_loss=0.0, z_loss=0.0, balance_per_sequence=False):
         """act_codes: one activation code per expert (default all 0 = SiLU-GLU); Identity (3) / Zero (4)
         experts come last and carry no weights.  learnable_situ adds an (E,2) [alpha,gamma] parameter
-        for the code-5 experts."""
+        for the code-5 experts.  scoring, num_groups, topk_groups, group_score: the router's scores and groups of experts (`group_topk`).
+        balance_loss, z_loss: the coefficients of `router_losses`; a training forward leaves balance_loss * balance + z_loss * z of its
+        batch in `aux_loss` (None otherwise), for the caller to add to the loss."""
         super().__init__()
         if precision not in ("bf16", "mxfp8"):
             raise ValueError("precision must be 'bf16' or 'mxfp8'")
@@ -162,7 +166,25 @@ class MoELayer(LoadBalanceMixin, nn.Module):
         self.num_experts = E
         self.norm_topk_prob = norm_topk_prob
         self.routed_scaling_factor = routed_scaling_factor
+        self.scoring, self.num_groups, self.topk_groups, self.group_score = scoring, num_groups, topk_groups, group_score
+        self.balance_loss, self.z_loss, self.balance_per_sequence = balance_loss, z_loss, balance_per_sequence
+        self.aux_loss = None      # a plain attribute: a tensor of the last training forward's graph
         self._init_load(E)
+
+    def _plain_router(self):
+        return self.scoring == "sigmoid" and self.num_groups == 1 and not self.balance_loss and not self.z_loss
+
+    def _route(self, x, mask):
+        """(idx, w, counts) of x (...,H), flat; leaves the losses of a training forward in aux_loss."""
+        idx, w, counts, logits = fused_group_router(x, self.gate.weight, self.bias, self.top_k, self.num_experts, self.num_groups,
+                                                    self.topk_groups, self.scoring, self.group_score, self.norm_topk_prob,
+                                                    self.routed_scaling_factor, return_counts=True, return_logits=True)
+        aux = None
+        if self.training and (self.balance_loss or self.z_loss):
+            balance, z = router_losses(logits, idx, self.scoring, mask, self.balance_per_sequence)
+            aux = self.balance_loss * balance + self.z_loss * z
+        self.__dict__["aux_loss"] = aux
+        return idx.reshape(-1, self.top_k), w.reshape(-1, self.top_k), counts
 
     def _apply(self, fn, *a, **kw):
         super()._apply(fn, *a, **kw)
@@ -171,14 +193,19 @@ class MoELayer(LoadBalanceMixin, nn.Module):
             self.act_params.data = self.act_params.data.float()
         return self
 
-    def forward(self, x):                               # x: (B,S,H) or (N,H)
+    def forward(self, x, mask=None):                    # x: (B,S,H) or (N,H); mask (B,S) or (N,): the tokens that the losses count
         shape = x.shape
+        plain = self._plain_router()
+        # the last forward's graph goes before this one's is built: alive, its gradient accumulators would tie a backward that is
+        # captured now to the stream they were made on
+        self.__dict__["aux_loss"] = None
+        L.require(mask is None or self.balance_loss or self.z_loss, "mask is for the router's losses, which this layer does not have")
         flat = x if x.dim() == 2 else x.reshape(-1, shape[-1])
         # an nn.Module resolves each of its parameters and buffers by name: once each
         weight, bias, gate_up, down, codes, params = (self.gate.weight, self.bias, self.gate_up_proj, self.down_proj,
                                                       self.act_codes, self.act_params)
         infos, n_glu = _code_info(codes)
-        if (self.precision == "bf16" and params is None and flat.shape[0] > 0 and n_glu == len(infos) == self.num_experts
+        if (plain and self.precision == "bf16" and params is None and flat.shape[0] > 0 and n_glu == len(infos) == self.num_experts
                 and all(c in FUSED_CODES for c in infos)):
             load = self._load_tensor(flat.device) if self.training and flat.is_cuda else None
             codes_dev = _codes_on(codes, flat.device) if any(infos) else None
@@ -193,9 +220,69 @@ class MoELayer(LoadBalanceMixin, nn.Module):
                 res = _Layer.apply(flat, weight, bias, gate_up, down, codes_dev, load, k, norm, scale, int(keep))
             out, self.__dict__["last_counts"] = res       # a plain attribute: nn.Module.__setattr__ would look for parameters first
             return out if out.dim() == len(shape) else out.reshape(shape)
-        idx, w, counts = fused_mlp_router(flat, weight, bias, self.top_k, self.num_experts, self.norm_topk_prob,
-                                          self.routed_scaling_factor, return_counts=True)
+        if plain:
+            idx, w, counts = fused_mlp_router(flat, weight, bias, self.top_k, self.num_experts, self.norm_topk_prob,
+                                              self.routed_scaling_factor, return_counts=True)
+        else:
+            idx, w, counts = self._route(x, mask)
         self._record_counts(counts)
         fn = moe_mxfp8 if self.precision == "mxfp8" else moe
         out = fn(flat, idx, w, gate_up, down, codes, params)
         return out.reshape(shape)
+
+
+class Fp8BlockMoELayer(nn.Module):
+    """A layer for serving with 8-bit experts (`moe_fp8_block`): e4m3 stacks with fp32 scales per 128 x 128 block, as buffers, under
+    the names that `MoELayer` has for its parameters, so a checkpoint of them loads by `load_state_dict`; `from_layer` quantises a bf16 one.
+    Routes like `MoELayer`.  The gate, in bf16, is the one parameter and takes no gradient; `to(dtype)` and the like leave codes and scales as
+    they are."""
+
+    _KEPT = ("gate_up_proj", "gate_up_scale", "down_proj", "down_scale", "bias")
+
+    def __init__(self, H, I, E, top_k=2, norm_topk_prob=True, routed_scaling_factor=1.0, scoring="sigmoid", num_groups=1, topk_groups=None,
+                 group_score="top2", device=None):
+        super().__init__()
+        if H % 128 or I % 128:
+            raise ValueError(f"d_model and d_ff must be multiples of 128, got {H}, {I}")
+        self.gate = nn.Linear(H, E, bias=False, device=device, dtype=torch.bfloat16).requires_grad_(False)
+        for name, shape in (("gate_up", (E, 2 * I, H)), ("down", (E, H, I))):
+            self.register_buffer(name + "_proj", torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn))
+            self.register_buffer(name + "_scale", torch.ones(E, shape[1] // 128, shape[2] // 128, device=device))
+        self.register_buffer("bias", torch.zeros(E, device=device))
+        self.top_k, self.num_experts, self.norm_topk_prob, self.routed_scaling_factor = top_k, E, norm_topk_prob, routed_scaling_factor
+        self.scoring, self.num_groups, self.topk_groups, self.group_score = scoring, num_groups, topk_groups, group_score
+
+    @classmethod
+    @torch.no_grad()
+    def from_layer(cls, layer):
+        """The 8-bit copy of a `MoELayer` of SiLU-GLU experts in bf16 on the GPU."""
+        if any(_code_info(layer.act_codes)[0]) or layer.act_params is not None:
+            raise ValueError("8-bit experts are pure SiLU-GLU stacks (act code 0)")
+        E, twoI, H = layer.gate_up_proj.shape
+        self = cls(H, twoI // 2, E, layer.top_k, layer.norm_topk_prob, layer.routed_scaling_factor, layer.scoring, layer.num_groups,
+                   layer.topk_groups, layer.group_score, device=layer.gate_up_proj.device)
+        self.gate.weight.copy_(layer.gate.weight)
+        self.bias.copy_(layer.bias)
+        self.gate_up_proj, self.gate_up_scale = fp8_block_quantize_weight(layer.gate_up_proj)
+        self.down_proj, self.down_scale = fp8_block_quantize_weight(layer.down_proj)
+        return self.train(layer.training)
+
+    def _apply(self, fn, *a, **kw):
+        kept = {n: getattr(self, n) for n in self._KEPT}
+        super()._apply(fn, *a, **kw)
+        for n, t in kept.items():                      # moved, never cast
+            moved = getattr(self, n)
+            if moved.dtype != t.dtype:
+                setattr(self, n, t.to(moved.device))
+        return self
+
+    @torch.no_grad()
+    def forward(self, x):                              # x: (B,S,H) or (N,H)
+        flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+        if self.scoring == "sigmoid" and self.num_groups == 1:
+            idx, w = fused_mlp_router(flat, self.gate.weight, self.bias, self.top_k, self.num_experts, self.norm_topk_prob,
+                                      self.routed_scaling_factor)
+        else:
+            idx, w = fused_group_router(flat, self.gate.weight, self.bias, self.top_k, self.num_experts, self.num_groups, self.topk_groups,
+                                        self.scoring, self.group_score, self.norm_topk_prob, self.routed_scaling_factor)
+        return moe_fp8_block(flat, idx, w, self.gate_up_proj, self.gate_up_scale, self.down_proj, self.down_scale).reshape(x.shape)
