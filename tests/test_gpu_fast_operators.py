@@ -75,6 +75,22 @@ def test_same_bits(pkg, seen, kind, grad):
         assert a.requires_grad == b.requires_grad
 
 
+@pytest.mark.parametrize("compiled", [True, False])
+def test_a_second_derivative_is_refused(pkg, seen, compiled):
+    """The gradients are right under create_graph, and going through them is an error, not a zero."""
+    seen.off = not compiled
+    z = torch.randn(20, 64, device=DEV, generator=torch.Generator(device=DEV).manual_seed(0), requires_grad=True)
+    x = torch.randn(20, 128, device=DEV).to(torch.bfloat16).requires_grad_(True)
+    w, s = torch.ones(64, 128, device=DEV).to(torch.float8_e4m3fn), torch.ones(1, 1, device=DEV)
+    idx, weights = pkg.group_topk(z, 4)
+    for out, leaf in ((weights.square().sum(), z), (sum(pkg.router_losses(z, idx)), z), (pkg.fp8_block_linear(x, w, s).float().square().sum(), x)):
+        (plain,) = torch.autograd.grad(out, leaf, retain_graph=True)
+        (g,) = torch.autograd.grad(out, leaf, create_graph=True)
+        assert torch.equal(plain, g)
+        with pytest.raises(RuntimeError, match="once_differentiable|does not require grad"):
+            g.float().sum().backward()
+
+
 class Noting(TorchDispatchMode):
     def __torch_dispatch__(self, func, types, args=(), kwargs=None):
         return func(*args, **(kwargs or {}))

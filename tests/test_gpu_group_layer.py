@@ -39,7 +39,7 @@ def test_layer_is_its_parts(pkg, kw):
     if aux is not None:
         balance, z = pkg.router_losses(logits, idx, layer.scoring, mask, layer.balance_per_sequence)
         total = total + 3 * (layer.balance_loss * balance + layer.z_loss * z)
-        assert torch.equal(aux, layer.balance_loss * balance + layer.z_loss * z) and float(aux) > 0
+        assert torch.equal(aux, layer.balance_loss * balance + layer.z_loss * z) and float(aux.detach()) > 0
     assert torch.equal(out, ref) and torch.equal(layer.last_counts, counts)
     for a, b in zip(got, torch.autograd.grad(total, params)):
         assert torch.equal(a, b)

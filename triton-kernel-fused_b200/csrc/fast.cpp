@@ -1,5 +1,6 @@
-// Autograd functions of the layer, of the experts on given picks, of the routers' top-k and losses and of the block-scaled 8-bit products as compiled code: the host side of the
-// Python Functions of the same name (layer.py, moe.py, router.py) for plain calls.  Each function returns None for a call
+// Autograd functions of the layer, of the experts on given picks, of the conv router, of the group top-k, of the router losses and of
+// the block-scaled 8-bit products as compiled code: the host side of the Python Functions of the same name (layer.py, moe.py, router.py,
+// fp8_block.py) for plain calls.  Each function returns None for a call
 // that is not plain (a tensor that would have to be cast or made contiguous, autocast, functorch transforms, forward-mode
 // gradients, dispatch modes, tensor subclasses, a shape that is an error), and the caller then takes the Python Function, which
 // casts, refuses or raises as it always did.
@@ -7,7 +8,8 @@
 // Why: between two small passes the host was the bound.  A Python Function costs the caller 8 us to enter, its allocations and
 // argument checks 15 to 30 more each way, and in the backward the autograd engine's thread waits for the interpreter lock before
 // it can call it.  us a pass, Python / compiled: one token through 64 experts of 2048 x 1408 62 / 39; forward and backward of 512 tokens
-// at width 256 237 / 148; conv router of 16 384 tokens 145 / 118.  HOSTTIMES
+// at width 256 237 / 148; conv router of 16 384 tokens 145 / 118.
+// Of the operators below, host time of a call of 512 tokens, forward and backward: top-k 118 / 75, losses 141 / 84, an 8-bit product 154 / 89.
 //
 // Nothing is kept between calls but what autograd saves (saved-tensor hooks see it); the workspace of a forward is a saved tensor.
 #include <ATen/autocast_mode.h>
@@ -15,6 +17,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 #include <torch/version.h>
 
@@ -274,6 +277,18 @@ optional<std::tuple<Tensor, Tensor, Tensor>> conv_router(const Tensor& x, const 
   return std::make_tuple(r[0], r[1], r[2]);
 }
 
+// Gradients that are not differentiable themselves: where a graph of the backward is being made, going through them is an error, as with the
+// Python Functions' once_differentiable
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  const auto error = std::make_shared<torch::autograd::DelayedError>(
+      "trying to differentiate twice a function that was marked with @once_differentiable", static_cast<int>(grads.size()));
+  variable_list in(grads.size());
+  for (size_t i = 0; i < grads.size(); ++i)
+    if (grads[i].defined()) in[i] = grads[i].detach().requires_grad_(true);
+  return (*error)(std::move(in));
+}
+
 // ---------------------------------------------------------------------------- group-limited top-k
 // of the logits' types
 optional<int> logits_type(const Tensor& t) {
@@ -329,7 +344,7 @@ struct GroupTopk : torch::autograd::Function<GroupTopk> {
     check(b200moe_group_topk_bwd(ptr(z), *logits_type(z), idx.data_ptr<int64_t>(), gw.data_ptr<float>(), z.numel() / E, E, idx.size(-1),
                                  ctx->saved_data["scoring"].toInt(), ctx->saved_data["norm"].toInt(),
                                  static_cast<float>(ctx->saved_data["scale"].toDouble()), ptr(res[0]), stream_of(z)));
-    return res;
+    return once(std::move(res));
   }
 };
 
@@ -394,7 +409,7 @@ struct RouterLosses : torch::autograd::Function<RouterLosses> {
     check(b200moe_router_losses_bwd(ptr(z), *logits_type(z), s.size() > 2 ? static_cast<const uint8_t*>(ptr(s[2])) : nullptr,
                                     coef.data_ptr<float>(), static_cast<const float*>(ptr(g[0])), static_cast<const float*>(ptr(g[1])),
                                     z.numel() / E / segs, segs, E, ctx->saved_data["scoring"].toInt(), ptr(res[0]), stream_of(z)));
-    return res;
+    return once(std::move(res));
   }
 };
 
@@ -444,7 +459,7 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
     const c10::cuda::CUDAGuard guard(s[0].device());
     Tensor g = grads[0].to(at::kBFloat16).contiguous();
     if (!aligned(g)) g = g.clone();
-    return {block_product(g, s[0], s[1], ctx->saved_data["status"].toTensor(), true), Tensor(), Tensor(), Tensor()};
+    return once({block_product(g, s[0], s[1], ctx->saved_data["status"].toTensor(), true), Tensor(), Tensor(), Tensor()});
   }
 };
 

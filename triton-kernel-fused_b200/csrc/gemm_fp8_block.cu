@@ -121,7 +121,7 @@ block_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
   const uint32_t bar_tempty = smem_u32(bars + 2 * kStages + 2);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  __shared__ uint32_t s_amax[2][4][128];
+  __shared__ uint32_t s_amax[2][kBParts][128];
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int cta_rank = static_cast<int>(cluster_ctarank());
@@ -785,11 +785,30 @@ static int launch_few_nt(int nt, const void* X, int64_t x_rows, int64_t ldx, con
                          int64_t tiles, int64_t max_tiles, cudaStream_t st) {
   if (nt <= 16) return launch_few<EPI, 16>(X, x_rows, ldx, W, w_rows, bp, tiles, max_tiles, st);
   if (nt <= 32) return launch_few<EPI, 32>(X, x_rows, ldx, W, w_rows, bp, tiles, max_tiles, st);
-  if (nt <= 64) return launch_few<EPI, 64>(X, x_rows, ldx, W, w_rows, bp, tiles, max_tiles, st);
-  return launch_few<EPI, 128>(X, x_rows, ldx, W, w_rows, bp, tiles, max_tiles, st);
+  return launch_few<EPI, 64>(X, x_rows, ldx, W, w_rows, bp, tiles, max_tiles, st);
 }
 
-constexpr int64_t kFewDense = 256;       // rows up to which a dense product runs with the weights as the M operand
+// Rows of a chunk of the few-rows kernel for a dense product, 0 for row tiles: the fewest whose tiles are one wave of CTAs, since more CTAs
+// that read the weights once more out of L2 beat fewer; or all rows in one chunk.  Weights of 32 MB and more want fewer reads.  us with
+// chunks of 16, 32, 64 / row tiles, L2 flushed.  4096 x 4096, 64 rows 17.4, 19.5, 21.5 / 25.6; 128 rows 23.6, 19.5, 21.5 / 27.6; 256 rows 37.9,
+// 27.6, 23.6 / 27.6; 384 rows 50.2, 35.8, 35.8 / 29.7.  1408 x 2048, 192 rows 13.3, 15.4, 17.4 / 19.5; 768 rows 25.6, 19.5, 17.4 / 21.5;
+// 1024 rows 29.7, 25.6, 25.6 / 21.5.  4096 x 14336, 16 rows 25.6, 27.6, 33.8 / 58.4; 64 rows 37.9, 31.8, 35.8 / 58.4; 256 rows 101, 66.6, 50.2 /
+// 62.5; 384 rows 144, 93.2, 85.0 / 66.4.  (Chunks of 128 rows, whose accumulators spill, were never the best.)
+static int few_dense(int64_t M, int64_t N, int64_t K) {
+  const int64_t columns = ceil_div(N, 128);
+  const int least = N * K < (32LL << 20) || M <= 16 ? 16 : M <= 64 ? 32 : 64;
+  for (int nt = least; nt <= 64; nt *= 2)
+    if (M <= nt || columns * ceil_div(M, nt) <= gemm_cta_budget()) return nt;
+  return 0;
+}
+
+// The same for experts, by their mean rows, as the host knows them.  us of a whole block with chunks of 16, 32, 64 / row tiles, L2 flushed, even
+// and rank^-1.1 routing.  64 experts of 2048 x 1408: 12 rows each 133, 135, 150 / 170, 119, 115, 125 / 133; 24 rows 152, 137, 156 / 170 and 162,
+// 145, 147 / 156; 32 rows 172, 150, 160 / 174 and 193, 164, 162 / 164; 48 rows 223, 182, 164 / 176 and 240, 199, 201 / 172.  8 of 4096 x 14336:
+// 8 rows 242, 248, 272 / 340 and 236, 227, 256 / 309; 24 rows 356, 254, 287 / 342 and 352, 303, 279 / 344; 32 rows 424, 307, 291 / 344 and 383,
+// 303, 283 / 342; 48 rows 537, 363, 293 / 348 and 514, 371, 361 / 346; 64 rows 635, 459, 381 / 346.  128 of 512 x 512: 8 rows 59, 64, 80 / 80; 32 rows
+// 78, 70, 84 / 80 and 72, 68, 74 / 66; 48 rows 90, 82, 84 / 80.
+static int few_experts(int64_t mean) { return mean <= 12 ? 16 : mean <= 28 ? 32 : mean <= 40 ? 64 : 0; }
 
 // out (M, N) = X (M, K) * W (N, K)^T, or (b_mn) out (M, K') = X (M, N') * W (N', K'): N and K of the params are of the product
 static int block_dense(const void* X, int64_t ldx, const float* sx, int64_t pitch, const void* W, const float* sw, int64_t M, int64_t N, int64_t K,
@@ -801,10 +820,9 @@ static int block_dense(const void* X, int64_t ldx, const float* sx, int64_t pitc
   bp.n_blocks = (int)ceil_div(N, 128);
   bp.sw_n = b_mn ? 1 : (int)ceil_div(K, 128);
   bp.sw_k = b_mn ? (int)ceil_div(N, 128) : 1;
-  if (!b_mn && M <= kFewDense) {
+  if (const int nt = b_mn ? 0 : few_dense(M, N, K); nt > 0) {
     bp.out = reinterpret_cast<__nv_bfloat16*>(out);
     bp.first_dense = (int)M;
-    const int nt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
     const int64_t tiles = ceil_div(N, 128) * ceil_div(M, nt);
     return launch_few_nt<EPI_STORE>(nt, X, M, ldx, W, N, bp, tiles, tiles, st);
   }
@@ -942,9 +960,7 @@ int b200moe_moe_fp8_block_forward(const void* x, const int64_t* idx, const float
   dn.sx = f.is; dn.sx_pitch = cap; dn.rows = cap; dn.sw = down_scale;
   dn.n_blocks = (int)(H / 128); dn.sw_n = (int)(I / 128); dn.sw_k = 1; dn.sw_group = (H / 128) * (I / 128);
   const int64_t hit = std::min<int64_t>(E, M);           // experts that can have a row
-  const int64_t mean = ceil_div(M, E);
-  if (mean <= 96) {
-    const int nt = mean <= 12 ? 16 : mean <= 24 ? 32 : mean <= 48 ? 64 : 128;
+  if (const int nt = few_experts(ceil_div(M, E)); nt > 0) {
     const int64_t chunks = E + M / nt;                   // at most
     RUN("fp8_block_gate_up", 1, launch_few_nt<EPI_SWIGLU>(nt, f.xq, cap, H, gate_up, 2 * I, up, hit * (I / 128), chunks * (I / 128), st));
     RUN("fp8_block_down", 1, launch_few_nt<EPI_STORE>(nt, f.iq, cap, I, down, H, dn, hit * (H / 128), chunks * (H / 128), st));
