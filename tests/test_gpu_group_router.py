@@ -168,6 +168,55 @@ def test_equal_logits_infinities_and_nan(pkg, scoring, bias):
     assert torch.isnan(w[9, 0]) and torch.isfinite(w[8]).all() and torch.isfinite(w[10]).all()
 
 
+@pytest.mark.parametrize("E,k,groups,opened", [(8, 3, 1, 1), (24, 4, 1, 1), (24, 4, 4, 2), (64, 6, 8, 3), (256, 8, 8, 4)])
+@pytest.mark.parametrize("scoring", ("sigmoid", "softmax"))
+def test_scores_and_biases_that_are_not_finite(pkg, scoring, E, k, groups, opened):
+    """Infinite biases open and close experts; NaN, of a bias or of a softmax over +infinity, ranks first and counts as infinity in a group."""
+    z, b, _ = make(70, E, torch.float32, 5, True)
+
+    def check(z, b):
+        v = scores64(z, scoring) + b.double()
+        for by in ("top2", "max"):
+            idx, w, counts = pkg.group_topk(z, k, b, groups, opened, scoring, by, return_counts=True)
+            if opened < groups:
+                top = v.nan_to_num(nan=torch.inf, posinf=torch.inf, neginf=-torch.inf).view(-1, groups, E // groups).sort(dim=2, descending=True).values
+                value = top[..., 0] if by == "max" else (top[..., 0] + top[..., 1]).nan_to_num(nan=torch.inf, posinf=torch.inf, neginf=-torch.inf)
+                keep = torch.zeros(z.shape[0], groups, dtype=torch.bool, device=DEV)
+                keep.scatter_(1, value.sort(dim=1, descending=True, stable=True).indices[:, :opened], True)
+                open_ = keep.repeat_interleave(E // groups, 1)
+            else:
+                open_ = torch.ones_like(v, dtype=torch.bool)
+            # NaN first, then by value, in the order of the experts; closed ones last
+            order = v.nan_to_num(nan=0.0, posinf=torch.inf, neginf=-torch.inf).sort(dim=1, descending=True, stable=True).indices
+            for first in (v.isnan(), open_):
+                rank = (~first).gather(1, order).long().sort(dim=1, stable=True).indices
+                order = order.gather(1, rank)
+            assert torch.equal(idx, order[:, :k]), (by, (idx != order[:, :k]).any(1).nonzero().flatten().tolist()[:5])
+            assert int(counts.sum()) == z.shape[0] * k
+            s = scores64(z, scoring).gather(1, idx)
+            s = s / (s.sum(1, keepdim=True) + 1e-20)
+            assert torch.equal(w.isnan(), s.isnan())
+            assert ((w - s).abs() <= 2.0 ** -18 * s)[~s.isnan()].all()
+
+    closed = b.clone()
+    closed[::3] = -torch.inf
+    check(z, closed)
+    both = closed.clone()
+    both[E // 2 + 1] = torch.inf
+    check(z, both)
+    if groups > 1:                             # one group has nothing but +infinity and -infinity
+        both[-(E // groups):] = -torch.inf
+        both[-1] = torch.inf
+        check(z, both)
+    nan = b.clone()
+    nan[E - 2] = torch.nan
+    check(z, nan)
+    if scoring == "softmax":
+        z = z.clone()
+        z[::2, 5] = torch.inf
+        check(z, b)
+
+
 def test_empty_strided_unaligned_and_three_dimensional(pkg):
     z, b, _ = make(400, 64, torch.bfloat16, 3, True)
     ref = pkg.group_topk(z, 6, b, 8, 3, return_counts=True)

@@ -63,6 +63,12 @@ __device__ __forceinline__ void best_of(double x, double& a, double& b) {
   b = x > a ? a : (x > b ? x : b);
   a = x > a ? x : a;
 }
+// A group's value from them; infinity less infinity counts as infinity too
+template <class F>
+__device__ __forceinline__ F group_value(const GroupParams& p, F a, F b) {
+  const F v = p.top2 && p.per_group > 1 ? a + b : a;
+  return v != v ? static_cast<F>(INFINITY) : v;
+}
 template <class F>
 __device__ __forceinline__ void group_best(int lanes_log, F& a, F& b) {
   for (int off = 1; off < (1 << lanes_log); off <<= 1) {
@@ -123,7 +129,7 @@ __device__ __noinline__ bool open_exactly(const GroupParams& p, long long t, int
   for (int i = 0; i < live; ++i) best_of(x.value(i), a, b);
   group_best(p.lanes_log, a, b);
   bool close;
-  return group_open(p.top2 && p.per_group > 1 ? a + b : a, g, p.groups, p.lanes_log, p.open, -1.0, close);
+  return group_open(group_value(p, a, b), g, p.groups, p.lanes_log, p.open, -1.0, close);
 }
 
 // the rank of a lane's candidate (its logit and bias) among n
@@ -192,7 +198,8 @@ group_topk_kernel(const __grid_constant__ GroupParams p) {
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     bias[i] = p.bias != nullptr && i < live ? p.bias[first + i] : 0.0f;
-    span = fmaxf(span, 1.0f + fabsf(bias[i]));
+    const float size = fabsf(bias[i]);
+    span = fmaxf(span, 1.0f + (size < INFINITY ? size : 0.0f));      // sums with an infinite one are exact
   }
   const bool by_logit = p.bias == nullptr;
   const float near = kNear<SOFTMAX> * warp_max(span);
@@ -207,7 +214,7 @@ group_topk_kernel(const __grid_constant__ GroupParams p) {
     bool odd = false;
 #pragma unroll
     for (int i = 0; i < V; ++i) odd = odd || v[i] != v[i];
-    odd = __any_sync(0xffffffffu, odd);          // a row with NaN
+    odd = __any_sync(0xffffffffu, odd);          // a row with NaN, or with scores or sums that are NaN (below)
     // ---- what selection compares: the logits, or scores + bias (groups by two: the scores, until a group is chosen)
     const bool sums = p.open < p.groups && p.top2;
     int key[V];
@@ -238,6 +245,11 @@ group_topk_kernel(const __grid_constant__ GroupParams p) {
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = __fdividef(1.0f, 1.0f + __expf(-v[i])) + bias[i];
       }
+      // a softmax over +infinity, a bias of NaN: NaN is neither above nor below a value, and fp32 finds no pick
+      bool nan = odd;
+#pragma unroll
+      for (int i = 0; i < V; ++i) nan = nan || v[i] != v[i];
+      odd = __any_sync(0xffffffffu, nan);
     }
     if (!by_logit) {
 #pragma unroll
@@ -260,7 +272,7 @@ group_topk_kernel(const __grid_constant__ GroupParams p) {
             if (i < live) best_of(v[i], a, b);
         }
         group_best(p.lanes_log, a, b);
-        mine = group_open(p.top2 && p.per_group > 1 ? a + b : a, g, p.groups, p.lanes_log, p.open, direct ? -1.0f : 2.0f * near, close) && mine;
+        mine = group_open(group_value(p, a, b), g, p.groups, p.lanes_log, p.open, direct ? -1.0f : 2.0f * near, close) && mine;
       }
       if (close) mine = open_exactly<T, SOFTMAX>(p, t, g, first, live, m) && live > 0;
       if (!mine) {
