@@ -1,4 +1,6 @@
 """GPU: the operators behind the layers: `MoELayer` with groups of experts, softmax scores and the routers' losses, and `Fp8BlockMoELayer`."""
+import copy
+
 import pytest
 import torch
 
@@ -63,6 +65,16 @@ def test_a_plain_layer_is_what_it_was(pkg):
         make(pkg, num_groups=5)(x)
     with pytest.raises(ValueError, match="scoring"):
         make(pkg, scoring="tanh")(x)
+
+
+def test_a_layer_is_copied_after_a_training_forward(pkg):
+    layer = make(pkg, scoring="softmax", balance_loss=0.1)
+    x = hidden(70, 256)
+    out = layer(x)
+    other = copy.deepcopy(layer)
+    assert other.aux_loss is None and layer.aux_loss is not None and torch.equal(other(x), out)
+    layer.aux_loss.backward()
+    assert layer.gate.weight.grad is not None
 
 
 def test_losses_balance_the_router(pkg):

@@ -171,6 +171,9 @@ class MoELayer(LoadBalanceMixin, nn.Module):
         self.aux_loss = None      # a plain attribute: a tensor of the last training forward's graph
         self._init_load(E)
 
+    def __getstate__(self):         # a copy has no part in the last forward's graph, and could not be made with it
+        return {**self.__dict__, "aux_loss": None}
+
     def _plain_router(self):
         return self.scoring == "sigmoid" and self.num_groups == 1 and not self.balance_loss and not self.z_loss
 
