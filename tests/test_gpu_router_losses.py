@@ -144,6 +144,9 @@ def test_far_logits_and_picks_out_of_range(pkg):
     with pytest.raises(RuntimeError, match="expert index"):
         pkg.check_status()
     assert torch.isfinite(got[0])
+    for none in (idx[:, :0], idx.repeat(1, 2)[:, ::2][:, :0]):
+        with pytest.raises(ValueError):
+            pkg.router_losses(z.detach(), none)
 
 
 def test_strides_other_stream_and_captured_graph(pkg):

@@ -326,6 +326,7 @@ def router_losses(logits, top_k_indices, scoring="softmax", mask=None, per_seque
             return res
     L.require(idx.device == logits.device and idx.dtype == torch.int64 and idx.dim() == logits.dim() and idx.shape[:-1] == logits.shape[:-1],
               "top_k_indices must be int64 (...,k) on the logits' device")
+    L.require(idx.shape[-1] >= 1, "top_k_indices must have at least one pick a token")
     E = logits.shape[-1]
     if mask is not None:
         L.require(mask.device == logits.device and mask.shape == logits.shape[:-1], "mask must have the tokens' shape, on the logits' device")
