@@ -969,6 +969,8 @@ int b200moe_moe_fp8_block_forward(const void* x, const int64_t* idx, const float
     RUN("fp8_block_gate_up", 1, (launch_pair<EPI_SWIGLU, false>(f.xq, cap, H, gate_up, H, 2 * I, E, up, tiles * (I / 128), st)));
     RUN("fp8_block_down", 1, (launch_pair<EPI_STORE, false>(f.iq, cap, I, down, I, H, E, dn, tiles * ceil_div(H, 256), st)));
   }
+  // A row's result is rounded to bf16 before the sum over a token's k, as in the bf16 block: kept in fp32 it would be 2 H bytes a row more,
+  // written and read (16 384 tokens of 2048, top-6: 120 us beside 1210), for an error of 0.0017 instead of 0.0024.
   RUN("combine", 1, b200moe_combine(f.eo, w, f.slot_row, T, k, H, out, stream));
 #undef RUN
   return 0;
