@@ -15,24 +15,8 @@ constexpr int kQuantAhead = 3;
 
 // 16 values -> their codes
 __device__ __forceinline__ void block_codes(const uint4 (&v)[2], float factor, bool finite, uint2 (&o)[2]) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint32_t words[4] = {v[h].x, v[h].y, v[h].z, v[h].w};
-    float a[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[2 * i] = bf16_lo(words[i]) * factor;
-      a[2 * i + 1] = bf16_hi(words[i]) * factor;
-    }
-    if (finite) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) a[i] = block_snap(a[i]);
-    }
-    o[h] = make_uint2(cvt4_e4m3(a[0], a[1], a[2], a[3]), cvt4_e4m3(a[4], a[5], a[6], a[7]));
-  }
-}
-__device__ __forceinline__ uint32_t absmax8(uint32_t m, const uint4& v) {
-  return __vmaxu2(m, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+  o[0] = block_codes8(v[0], factor, finite);
+  o[1] = block_codes8(v[1], factor, finite);
 }
 
 __global__ void __launch_bounds__(256)

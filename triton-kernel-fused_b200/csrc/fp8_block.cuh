@@ -37,6 +37,25 @@ __device__ __forceinline__ void block_scale_factor(uint32_t amax_bits, float& sc
 // way exactly where the quotient is, and ties go to even as they should.  (Without, one value in some hundred goes the other way.)
 __device__ __forceinline__ float block_snap(float q) { return __uint_as_float((__float_as_uint(q) + 8u) & ~15u); }
 
+// 8 bf16 values -> their codes; and the larger of m and their |x|, as bits, in each half of a word
+__device__ __forceinline__ uint2 block_codes8(const uint4& v, float factor, bool finite) {
+  const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+  float a[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    a[2 * i] = bf16_lo(words[i]) * factor;
+    a[2 * i + 1] = bf16_hi(words[i]) * factor;
+  }
+  if (finite) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = block_snap(a[i]);
+  }
+  return make_uint2(cvt4_e4m3(a[0], a[1], a[2], a[3]), cvt4_e4m3(a[4], a[5], a[6], a[7]));
+}
+__device__ __forceinline__ uint32_t absmax8(uint32_t m, const uint4& v) {
+  return __vmaxu2(m, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+}
+
 // First row of scales of k-block kb: scales lie block by block, rows in order (a warp's rows are one line)
 __device__ __forceinline__ long long scale_at(int kb, long long pitch, long long row) { return kb * pitch + row; }
 

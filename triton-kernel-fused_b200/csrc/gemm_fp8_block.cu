@@ -35,6 +35,9 @@ struct BlockParams {
   __nv_bfloat16* out;       // few rows: (rows, N)
   int split;                // few rows: CTAs of a cluster that share a tile's k-blocks
   int first_dense;          // few rows, dense: rows of X (no table)
+  const __nv_bfloat16* x;   // few rows, quantised on the way: X in bf16, its rows those of the product or (row_slot) of the tokens, k slots each
+  const int* row_slot;
+  int k;
 };
 
 __device__ __forceinline__ void umma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -382,6 +385,10 @@ block_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
 // epilogue warp are output columns, its registers NT / 2 rows of X; the rows' scales come with the operands, through shared memory.
 // Bound: HBM, by the one read of the weights.  Where the tiles do not fill the SMs, the k-blocks of a tile are shared by the CTAs of a
 // cluster, which send their sums to the first one (in the order of the ranks: the same bits every time).
+//
+// QUANT: X comes in bf16, and eight more warps write its codes and scales into the stages, the live rows alone, with the bits of the quantiser, which
+// needs no launch then.  Every tile makes them again: see quant_inside.
+constexpr int kQuantWarps = 8;
 template <int EPI, int NT>
 struct FewBlockCfg {
   static constexpr int XB = EPI == EPI_SWIGLU ? 1 : 2;                 // k-blocks of a stage
@@ -429,8 +436,8 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
-template <int EPI, int NT>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int EPI, int NT, bool QUANT>
+__global__ void __launch_bounds__(kThreads + (QUANT ? 32 * kQuantWarps : 0), 1)
 block_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const BlockParams bp) {
   using C = FewBlockCfg<EPI, NT>;
   const GemmParams& p = bp.g;
@@ -457,20 +464,20 @@ block_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
   const int first_tile = static_cast<int>(blockIdx.x) / bp.split, tile_step = static_cast<int>(gridDim.x) / bp.split;
   if (threadIdx.x == 0) {
     for (int s = 0; s < NSTAGE; ++s) {
-      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_full + 8 * s, QUANT ? 1 + kQuantWarps : 1);
       mbar_init(bar_empty + 8 * s, 1);
     }
     for (int b = 0; b < SLOTS; ++b) {
       mbar_init(bar_tfull + 8 * b, 1);
       mbar_init(bar_tempty + 8 * b, kEpiWarps);
     }
-    for (int b = 0; b < C::SF; ++b) mbar_init(bar_sf + 8 * b, 1);
+    for (int b = 0; b < C::SF; ++b) mbar_init(bar_sf + 8 * b, QUANT ? kQuantWarps : 1);
     mbar_init(bar_sums, bp.split > 1 ? (bp.split - 1) * kEpiWarps : 1);
     mbar_init(bar_taken, kEpiWarps);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmW);
-    tma_prefetch_desc(&tmX);
+    if (!QUANT) tma_prefetch_desc(&tmX);
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
@@ -523,24 +530,26 @@ block_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
             break;
           }
           const uint32_t full = bar_full + 8 * s, st = smem_u32(smem + s * C::STAGE), xs = st + 2 * kBTile;
-          mbar_arrive_expect_tx(full, (EPI == EPI_SWIGLU ? 2 : n) * kBTile + n * C::X_BYTES);
+          mbar_arrive_expect_tx(full, (EPI == EPI_SWIGLU ? 2 : n) * kBTile + (QUANT ? 0 : n * C::X_BYTES));
           if constexpr (EPI == EPI_SWIGLU) {
             tma_load_3d(st, &tmW, full, kb * kBBK, t.m0, t.e);
             tma_load_3d(st + kBTile, &tmW, full, kb * kBBK, p.I + t.m0, t.e);
-            tma_load_3d(xs, &tmX, full, kb * kBBK, t.row0, 0);
+            if (!QUANT) tma_load_3d(xs, &tmX, full, kb * kBBK, t.row0, 0);
           } else {
             for (int i = 0; i < n; ++i) {
               tma_load_3d(st + i * kBTile, &tmW, full, (kb + i) * kBBK, t.m0, t.e);
-              tma_load_3d(xs + i * C::X_BYTES, &tmX, full, (kb + i) * kBBK, t.row0, 0);
+              if (!QUANT) tma_load_3d(xs + i * C::X_BYTES, &tmX, full, (kb + i) * kBBK, t.row0, 0);
             }
           }
           // The MMAs of the stage NSTAGE before are complete (bar_empty), so the epilogue has given back the tensor memory of the one SLOTS
           // before that: it has read those scales, and this slot of a ring of NSTAGE + SLOTS is free.
-          const uint32_t bf = bar_sf + 8 * f;
-          mbar_arrive_expect_tx(bf, n * NT * 4);
-          for (int i = 0; i < n; ++i)
-            bulk_load_1d(smem_u32(sf + f * (XB * NT) + i * NT), bp.sx + scale_at(kb + i, bp.sx_pitch, t.row0), NT * 4, bf);
-          if (++f == C::SF) f = 0;
+          if constexpr (!QUANT) {
+            const uint32_t bf = bar_sf + 8 * f;
+            mbar_arrive_expect_tx(bf, n * NT * 4);
+            for (int i = 0; i < n; ++i)
+              bulk_load_1d(smem_u32(sf + f * (XB * NT) + i * NT), bp.sx + scale_at(kb + i, bp.sx_pitch, t.row0), NT * 4, bf);
+            if (++f == C::SF) f = 0;
+          }
           if (++s == NSTAGE) {
             s = 0;
             ph ^= 1;
@@ -582,6 +591,73 @@ block_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
           if (++s == NSTAGE) {
             s = 0;
             ph ^= 1;
+          }
+        }
+      }
+    }
+  } else if (QUANT && warp >= 2 + kEpiWarps) {
+    // ------------------------------------------------------------------ codes and scales of X, kQAhead stages' values on their way
+    // kQLanes lanes a row and k-block.  A slot of the scales is free when the stage's is, as for the producer.  Rows that are not live are left as
+    // they are: what they make of a stage goes nowhere.
+    if constexpr (QUANT) {
+      constexpr int kQLanes = 32 * kQuantWarps / (XB * NT), kQVec = 16 / kQLanes, kQAhead = 8 / kQVec;
+      static_assert(kQLanes * kQVec == 16 && kQVec <= 2, "a block of 128 is 16 vectors");
+      const int at = threadIdx.x - kThreads, ql = at % kQLanes, box = at / kQLanes / NT, r = at / kQLanes % NT;
+      int s = 0, f = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int tile = first_tile; tile < total && ok; tile += tile_step) {
+        const FewTile t = tile_of(tile);
+        const bool live = r < t.live;
+        long long row = t.row0 + r;
+        if (live && bp.row_slot != nullptr) row = bp.row_slot[row] / bp.k;
+        const __nv_bfloat16* x = bp.x + row * p.K;
+        uint4 v[kQAhead][2];
+        auto get = [&](int kb, uint4 (&to)[2]) {
+#pragma unroll
+          for (int h = 0; h < kQVec; ++h) {
+            const int c = kb * kBBK + 64 * h + 8 * ql;
+            to[h] = make_uint4(0u, 0u, 0u, 0u);
+            if (live && kb < kb_hi && c < p.K) to[h] = *reinterpret_cast<const uint4*>(x + c);      // K is a multiple of 16
+          }
+        };
+#pragma unroll
+        for (int u = 0; u < kQAhead; ++u) get(kb_lo + u * XB + box, v[u]);
+        for (int kb0 = kb_lo; kb0 < kb_hi && ok; kb0 += kQAhead * XB) {
+#pragma unroll
+          for (int u = 0; u < kQAhead; ++u) {
+            const int kb = kb0 + u * XB;
+            if (kb >= kb_hi || !ok) break;
+            uint32_t m = absmax8(0u, v[u][0]);
+            if (kQVec == 2) m = absmax8(m, v[u][1]);
+#pragma unroll
+            for (int off = kQLanes / 2; off > 0; off >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, off));
+            m = max(m & 0xffffu, m >> 16) << 16;
+            float scale, factor;
+            block_scale_factor(m, scale, factor);
+            uint2 o[kQVec];
+#pragma unroll
+            for (int h = 0; h < kQVec; ++h) o[h] = block_codes8(v[u][h], factor, m < 0x7f800000u);
+            ok = mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, ST_WAIT_PRODUCER);
+            __syncwarp();
+            if (live && ok && kb + box < kb_hi) {
+              uint8_t* to = smem + s * C::STAGE + 2 * kBTile + box * C::X_BYTES + r * kBBK + 8 * (ql & 1);      // 128-byte swizzle
+#pragma unroll
+              for (int h = 0; h < kQVec; ++h) *reinterpret_cast<uint2*>(to + ((((ql >> 1) + 4 * h) ^ (r & 7)) << 4)) = o[h];
+              if (ql == 0) sf[f * (XB * NT) + box * NT + r] = scale;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(bar_full + 8 * s);
+              mbar_arrive(bar_sf + 8 * f);
+            }
+            get(kb + kQAhead * XB + box, v[u]);
+            if (++f == C::SF) f = 0;
+            if (++s == NSTAGE) {
+              s = 0;
+              ph ^= 1;
+            }
           }
         }
       }
@@ -761,28 +837,31 @@ static int few_split(int64_t tiles, int nkb, int most) {
   return s;
 }
 
-template <int EPI, int NT>
+template <int EPI, int NT, bool QUANT = false>
 static int launch_few(const void* X, int64_t x_rows, int64_t ldx, const void* W, int64_t w_rows, BlockParams bp, int64_t tiles,
                       int64_t max_tiles, cudaStream_t stream) {
   using C = FewBlockCfg<EPI, NT>;
   static std::once_flag once;
   static cudaError_t attr_err = cudaSuccess;
   std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(block_few_kernel<EPI, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+    attr_err = cudaFuncSetAttribute(block_few_kernel<EPI, NT, QUANT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
   });
   if (attr_err != cudaSuccess) return cuda_fail(attr_err, "cudaFuncSetAttribute(max dynamic smem)");
   CUtensorMap tmW, tmX;
   int rc = make_map(&tmW, W, bp.g.K, w_rows, bp.g.num_groups, bp.g.K, w_rows * bp.g.K, kBBK, 128, 1);
-  if (rc == 0) rc = make_map(&tmX, X, bp.g.K, x_rows, 1, ldx, x_rows * ldx, kBBK, NT, 1);
+  tmX = tmW;
+  if (rc == 0 && !QUANT) rc = make_map(&tmX, X, bp.g.K, x_rows, 1, ldx, x_rows * ldx, kBBK, NT, 1);
   if (rc) return rc;
   bp.split = few_split(tiles, static_cast<int>(ceil_div(bp.g.K, kBBK)), C::MAX_SPLIT);
   const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(gemm_cta_budget() / bp.split, max_tiles)) * bp.split;
-  B200_CUDA(launch_chained(block_few_kernel<EPI, NT>, static_cast<int>(grid), kThreads, C::SMEM_BYTES, stream, bp.split, tmW, tmX, bp));
+  B200_CUDA(launch_chained(block_few_kernel<EPI, NT, QUANT>, static_cast<int>(grid), kThreads + (QUANT ? 32 * kQuantWarps : 0), C::SMEM_BYTES,
+                           stream, bp.split, tmW, tmX, bp));
   return 0;
 }
 template <int EPI>
 static int launch_few_nt(int nt, const void* X, int64_t x_rows, int64_t ldx, const void* W, int64_t w_rows, const BlockParams& bp,
                          int64_t tiles, int64_t max_tiles, cudaStream_t st) {
+  if (bp.x != nullptr) return launch_few<EPI, 16, true>(X, x_rows, ldx, W, w_rows, bp, tiles, max_tiles, st);
   if (nt <= 16) return launch_few<EPI, 16>(X, x_rows, ldx, W, w_rows, bp, tiles, max_tiles, st);
   if (nt <= 32) return launch_few<EPI, 32>(X, x_rows, ldx, W, w_rows, bp, tiles, max_tiles, st);
   return launch_few<EPI, 64>(X, x_rows, ldx, W, w_rows, bp, tiles, max_tiles, st);
@@ -810,27 +889,6 @@ static int few_dense(int64_t M, int64_t N, int64_t K) {
 // 78, 70, 84 / 80 and 72, 68, 74 / 66; 48 rows 90, 82, 84 / 80.
 static int few_experts(int64_t mean) { return mean <= 12 ? 16 : mean <= 28 ? 32 : mean <= 40 ? 64 : 0; }
 
-// out (M, N) = X (M, K) * W (N, K)^T, or (b_mn) out (M, K') = X (M, N') * W (N', K'): N and K of the params are of the product
-static int block_dense(const void* X, int64_t ldx, const float* sx, int64_t pitch, const void* W, const float* sw, int64_t M, int64_t N, int64_t K,
-                       int b_mn, void* out, int32_t* status, cudaStream_t st) {
-  BlockParams bp{};
-  bp.g.sched = SCHED_DENSE; bp.g.M = (int)M; bp.g.N = (int)N; bp.g.K = (int)K; bp.g.num_groups = 1;
-  bp.g.D = out; bp.g.ldd = N; bp.g.status = status;
-  bp.sx = sx; bp.sx_pitch = pitch; bp.rows = M; bp.sw = sw;
-  bp.n_blocks = (int)ceil_div(N, 128);
-  bp.sw_n = b_mn ? 1 : (int)ceil_div(K, 128);
-  bp.sw_k = b_mn ? (int)ceil_div(N, 128) : 1;
-  if (const int nt = b_mn ? 0 : few_dense(M, N, K); nt > 0) {
-    bp.out = reinterpret_cast<__nv_bfloat16*>(out);
-    bp.first_dense = (int)M;
-    const int64_t tiles = ceil_div(N, 128) * ceil_div(M, nt);
-    return launch_few_nt<EPI_STORE>(nt, X, M, ldx, W, N, bp, tiles, tiles, st);
-  }
-  const int64_t tiles = ceil_div(M, 256) * ceil_div(N, 256);
-  return b_mn ? launch_pair<EPI_STORE, true>(X, M, ldx, W, N, K, 1, bp, tiles, st)
-              : launch_pair<EPI_STORE, false>(X, M, ldx, W, K, N, 1, bp, tiles, st);
-}
-
 struct BlockCarver {
   char* base;
   size_t off = 0;
@@ -842,6 +900,47 @@ struct BlockCarver {
     return p;
   }
 };
+
+// Whether the few-rows kernel quantises X itself: where its rows are few and its weights no long read, the launch saved is worth more than
+// what the tiles do over again.  us with the quantiser / inside, L2 flushed.  A block of 64 experts of 2048 x 1408: 1 token 36.9 / 34.8, 4 rows an expert 125 /
+// 123, 12 rows under rank^-1.1 routing 119 / 125; of 128 of 512 x 512, 4 rows 55.3 / 53.2; of 8 of 4096 x 14336, 1 row 194.6 / 196.6, 4 rows 239.6 / 241.7.
+// Dense (one chunk is all rows): 4 x 4096 x 4096 16.4 / 14.3 and 2.4 less on the host, 16 x 4096 x 14336 24.6 / 22.5; 64 x 4096 x 4096 in four
+// chunks 16.4 / 18.5.
+static bool quant_inside(int64_t mean, int64_t weights) { return mean <= 4 && weights < (32LL << 20); }
+
+// out (M, N) = x (M, K) * w (N, K)^T, or (b_mn) out (M, K') = x (M, N') * w (N', K'): N and K of the params are of the product
+static int block_dense(const void* x, const void* w, const float* sw, int64_t M, int64_t N, int64_t K, int b_mn, void* ws, void* out, int32_t* status,
+                       cudaStream_t st) {
+  BlockParams bp{};
+  bp.g.sched = SCHED_DENSE; bp.g.M = (int)M; bp.g.N = (int)N; bp.g.K = (int)K; bp.g.num_groups = 1;
+  bp.g.D = out; bp.g.ldd = N; bp.g.status = status;
+  bp.rows = M; bp.sw = sw;
+  bp.n_blocks = (int)ceil_div(N, 128);
+  bp.sw_n = b_mn ? 1 : (int)ceil_div(K, 128);
+  bp.sw_k = b_mn ? (int)ceil_div(N, 128) : 1;
+  const int nt = b_mn ? 0 : few_dense(M, N, K);
+  const int64_t ldq = code_pitch(K);
+  BlockCarver c{static_cast<char*>(ws)};
+  uint8_t* q = c.take<uint8_t>(M * ldq);
+  float* sx = c.take<float>(scale_pitch(M) * ceil_div(K, 128));
+  if (nt == 16 && M <= 16) {
+    bp.x = reinterpret_cast<const __nv_bfloat16*>(x);
+  } else {
+    bp.sx = sx;
+    bp.sx_pitch = scale_pitch(M);
+    const int rc = fp8_block_quant(x, M, K, M, nullptr, 1, q, ldq, sx, bp.sx_pitch, st);
+    if (rc) return rc;
+  }
+  if (nt > 0) {
+    bp.out = reinterpret_cast<__nv_bfloat16*>(out);
+    bp.first_dense = (int)M;
+    const int64_t tiles = ceil_div(N, 128) * ceil_div(M, nt);
+    return launch_few_nt<EPI_STORE>(nt, q, M, ldq, w, N, bp, tiles, tiles, st);
+  }
+  const int64_t tiles = ceil_div(M, 256) * ceil_div(N, 256);
+  return b_mn ? launch_pair<EPI_STORE, true>(q, M, ldq, w, N, K, 1, bp, tiles, st)
+              : launch_pair<EPI_STORE, false>(q, M, ldq, w, K, N, 1, bp, tiles, st);
+}
 
 struct BlockExperts {
   int32_t *counts, *offs, *poffs, *slot_row, *row_slot, *tile_expert;
@@ -901,13 +1000,7 @@ int b200moe_fp8_block_linear(const void* x, const void* w, const float* w_scale,
   B200_CHECK_ARG(x && w && w_scale && ws && out, B200MOE_E_NULL, "fp8_block_linear: null pointer");
   B200_CHECK_ARG(aligned16(x) && aligned16(w) && aligned16(ws) && aligned16(out), B200MOE_E_ALIGN,
                  "fp8_block_linear: tensors must be 16-byte aligned");
-  const int64_t red = transposed ? N : K, ldq = code_pitch(red), pitch = scale_pitch(M);
-  BlockCarver c{static_cast<char*>(ws)};
-  uint8_t* q = c.take<uint8_t>(M * ldq);
-  float* s = c.take<float>(pitch * ceil_div(red, 128));
-  rc = fp8_block_quant(x, M, red, M, nullptr, 1, q, ldq, s, pitch, stream);
-  if (rc) return rc;
-  return block_dense(q, ldq, s, pitch, w, w_scale, M, transposed ? K : N, red, transposed, out, status, (cudaStream_t)stream);
+  return block_dense(x, w, w_scale, M, transposed ? K : N, transposed ? N : K, transposed, ws, out, status, (cudaStream_t)stream);
 }
 
 size_t b200moe_moe_fp8_block_ws_bytes(int64_t T, int64_t H, int64_t I, int E, int k) {
@@ -944,13 +1037,16 @@ int b200moe_moe_fp8_block_forward(const void* x, const int64_t* idx, const float
   RUN("permute_build", M > 1024 ? 2 : 1,
       permute_build(idx, T, k, E, f.counts, f.offs, f.poffs, f.slot_row, f.row_slot, f.tile_expert, nullptr, nullptr, f.scratch, f.scratch_bytes,
                     nullptr, nullptr, status, stream));
-  RUN("fp8_block_quant", 1, fp8_block_quant(x, T, H, cap, f.slot_row, k, f.xq, H, f.xs, cap, stream));
+  const int nt = few_experts(ceil_div(M, E));
+  const bool inside = quant_inside(ceil_div(M, E), H * I);
+  if (!inside) RUN("fp8_block_quant", 1, fp8_block_quant(x, T, H, cap, f.slot_row, k, f.xq, H, f.xs, cap, stream));
   // gate and up
   BlockParams up{};
   up.g.sched = SCHED_GROUPED_M; up.g.N = up.g.I = (int)I; up.g.K = (int)H; up.g.num_groups = E;
   up.g.tile_expert = f.tile_expert; up.g.poffs = f.poffs; up.g.counts = f.counts; up.g.status = status;
   up.sx = f.xs; up.sx_pitch = cap; up.rows = cap; up.sw = gate_up_scale;
   up.n_blocks = (int)(I / 128); up.sw_n = (int)(H / 128); up.sw_k = 1; up.sw_group = 2 * (I / 128) * (H / 128);
+  if (inside) { up.x = reinterpret_cast<const __nv_bfloat16*>(x); up.row_slot = f.row_slot; up.k = k; }
   up.q_out = f.iq; up.q_scale = f.is; up.q_pitch = cap;
   // down
   BlockParams dn{};
@@ -960,7 +1056,7 @@ int b200moe_moe_fp8_block_forward(const void* x, const int64_t* idx, const float
   dn.sx = f.is; dn.sx_pitch = cap; dn.rows = cap; dn.sw = down_scale;
   dn.n_blocks = (int)(H / 128); dn.sw_n = (int)(I / 128); dn.sw_k = 1; dn.sw_group = (H / 128) * (I / 128);
   const int64_t hit = std::min<int64_t>(E, M);           // experts that can have a row
-  if (const int nt = few_experts(ceil_div(M, E)); nt > 0) {
+  if (nt > 0) {
     const int64_t chunks = E + M / nt;                   // at most
     RUN("fp8_block_gate_up", 1, launch_few_nt<EPI_SWIGLU>(nt, f.xq, cap, H, gate_up, 2 * I, up, hit * (I / 128), chunks * (I / 128), st));
     RUN("fp8_block_down", 1, launch_few_nt<EPI_STORE>(nt, f.iq, cap, I, down, H, dn, hit * (H / 128), chunks * (H / 128), st));
