@@ -344,3 +344,20 @@ def test_router_then_experts_and_losses(pkg):
     gx, gW = torch.autograd.grad(balance + 1e-2 * z + w.sum() * 0.1 + shared.float().mean(), (xt, Wt))
     assert torch.isfinite(gx).all() and torch.isfinite(gW).all() and gW.abs().max() > 0 and gx.abs().max() > 0
     pkg.check_status()
+
+
+def test_quantised_inside_and_before(pkg):
+    """Few rows are quantised by the product itself, more of them by a launch before it: a row's result is the same to the bit."""
+    g = gen(7)
+    x = torch.randn(32, 2048, generator=g, device=DEV).to(torch.bfloat16)
+    x[3] = 0
+    x[5, 300] = torch.inf
+    w, s = weights(g, 1408, 2048)
+    few, more = pkg.fp8_block_linear(x[:16], w, s), pkg.fp8_block_linear(x[:17], w, s)
+    assert torch.equal(few.view(torch.int16), more[:16].view(torch.int16))
+    gu, gs = weights(g, 8, 768, 2048, std=0.1)
+    dn, ds = weights(g, 8, 2048, 384, std=0.1)
+    idx = torch.rand(32, 8, generator=g, device=DEV).topk(2, dim=1).indices
+    wt = torch.rand(32, 2, generator=g, device=DEV)
+    few, more = (pkg.moe_fp8_block(x[:n], idx[:n], wt[:n], gu, gs, dn, ds) for n in (16, 32))
+    assert torch.equal(few.view(torch.int16), more[:16].view(torch.int16))
