@@ -89,8 +89,9 @@ __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(
 // the gate, the other the up rows of the same 128 columns).  Two k-blocks' sums of 256 columns fill tensor memory.  An epilogue warp owns
 // 32 rows and 128 columns (SwiGLU: 64 of gate and the same 64 of up), 128 accumulators a thread.
 //
-// Bound: the MMAs of a k-block take 512 cycles, the multiply-adds of the epilogue 386 beside them, but between the two lie four signals of 130
-// to 220 cycles each, for two k-blocks: some 900 cycles in all (1635 MHz under the power cap).  So what counts is how long the epilogue holds
+// Bound: the MMAs of a k-block take 512 cycles, the multiply-adds of the epilogue 386 after them, and between the two lie four signals of 130 to 220
+// cycles each, so a slot of tensor memory comes round in some 1700 cycles and, with two of them, a k-block takes 870: the tensor cores are
+// busy for 60 % of the time.  So what counts is how long the epilogue holds
 // tensor memory.  8192 x 14336 x 4096, us: arrivals as releases 984 (mbar_arrive_tmem), scales from global memory by the epilogue's threads 488,
 // by a warp that prepares them 455; 2112 TFLOP/s.  Slower: 16 epilogue warps 519; columns 32 at a time 485; plain multiply-adds in place of
 // packed ones 466; the other CTA's arrivals passed on by one thread 500; tensor memory as four half k-blocks 535.  Each of the 128 + 16
