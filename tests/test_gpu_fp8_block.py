@@ -361,3 +361,29 @@ def test_quantised_inside_and_before(pkg):
     wt = torch.rand(32, 2, generator=g, device=DEV)
     few, more = (pkg.moe_fp8_block(x[:n], idx[:n], wt[:n], gu, gs, dn, ds) for n in (16, 32))
     assert torch.equal(few.view(torch.int16), more[:16].view(torch.int16))
+
+
+def test_few_rows_captured_and_replayed(pkg):
+    """A graph of a product and a block of four rows, replayed on other inputs, gives what plain calls give."""
+    g = gen(9)
+    w, s = weights(g, 512, 512)
+    gu, gs = weights(g, 16, 512, 512, std=0.1)
+    dn, ds = weights(g, 16, 512, 256, std=0.1)
+    x, idx = torch.zeros(4, 512, dtype=torch.bfloat16, device=DEV), torch.zeros(4, 3, dtype=torch.int64, device=DEV)
+    wt = torch.rand(4, 3, generator=g, device=DEV)
+
+    def run():
+        return pkg.moe_fp8_block(pkg.fp8_block_linear(x, w, s), idx, wt, gu, gs, dn, ds)
+
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for _ in range(3):
+        x.copy_(torch.randn(4, 512, generator=g, device=DEV))
+        idx.copy_(torch.rand(4, 16, generator=g, device=DEV).topk(3, dim=1).indices)
+        graph.replay()
+        got = out.clone()
+        assert torch.equal(got, run()) and got.abs().sum() > 0
+    pkg.check_status()
