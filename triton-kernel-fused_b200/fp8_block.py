@@ -34,33 +34,58 @@ def _aligned(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+class _Frozen(torch.autograd.Function):
+    """Functions whose results take no gradient.  They are Functions all the same: a tracer records them as calls, where it would otherwise
+    record nothing but the allocation of their results, and a forward-mode gradient, which they cannot carry on, is refused."""
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("the products of frozen 8-bit weights and their quantisers have no backward (moe and moe_mxfp8 train)")
+
+
+class _Quantize(_Frozen):
+    """(codes (N,K), scales (ceil(K/128), N)) of rows (N,K)"""
+
+    @staticmethod
+    def forward(ctx, rows):
+        (N, K), rows = rows.shape, _aligned(rows)
+        with L.on_device_of(rows):
+            q = torch.empty(rows.shape, dtype=torch.float8_e4m3fn, device=rows.device)
+            scale = torch.empty(_blocks(K), N, dtype=torch.float32, device=rows.device)
+            if N:
+                L.check(L.lib().b200moe_fp8_block_quant(rows.data_ptr(), N, K, q.data_ptr(), K, scale.data_ptr(), N, L.stream_of(rows)))
+        ctx.mark_non_differentiable(q, scale)
+        return q, scale
+
+
+class _QuantizeWeight(_Frozen):
+    """(codes, scales) of matrices (...,N,K)"""
+
+    @staticmethod
+    def forward(ctx, w):
+        (N, K), w = w.shape[-2:], _aligned(w)
+        with L.on_device_of(w):
+            q = torch.empty(w.shape, dtype=torch.float8_e4m3fn, device=w.device)
+            scale = torch.empty(*w.shape[:-2], _blocks(N), _blocks(K), dtype=torch.float32, device=w.device)
+            L.check(L.lib().b200moe_fp8_block_quant_weight(w.data_ptr(), w.numel() // (N * K), N, K, q.data_ptr(), scale.data_ptr(),
+                                                           L.stream_of(w)))
+        ctx.mark_non_differentiable(q, scale)
+        return q, scale
+
+
 def fp8_block_quantize(x):
     """bf16 (..., K), K a multiple of 8 -> (codes float8_e4m3fn (..., K), scales fp32 (..., ceil(K/128))), the values being code * scale."""
     L.require_cuda_bf16("x", x)
     L.require(x.dim() >= 1 and x.shape[-1] > 0 and x.shape[-1] % 8 == 0, "the last dimension of x must be a positive multiple of 8")
-    K = x.shape[-1]
-    rows = _aligned(x.detach().reshape(-1, K).contiguous())
-    with L.on_device_of(rows):
-        q = torch.empty(rows.shape, dtype=torch.float8_e4m3fn, device=x.device)
-        scale = torch.empty(_blocks(K), rows.shape[0], dtype=torch.float32, device=x.device)
-        if rows.shape[0]:
-            L.check(L.lib().b200moe_fp8_block_quant(rows.data_ptr(), rows.shape[0], K, q.data_ptr(), K, scale.data_ptr(), rows.shape[0],
-                                                    L.stream_of(rows)))
-    return q.view(x.shape), scale.t().reshape(*x.shape[:-1], _blocks(K))
+    q, scale = _Quantize.apply(x.reshape(-1, x.shape[-1]).contiguous())
+    return q.view(x.shape), scale.t().reshape(*x.shape[:-1], _blocks(x.shape[-1]))
 
 
 def fp8_block_quantize_weight(w):
     """bf16 (..., N, K), K a multiple of 8 -> (codes float8_e4m3fn (..., N, K), scales fp32 (..., ceil(N/128), ceil(K/128)))."""
     L.require_cuda_bf16("w", w)
     L.require(w.dim() >= 2 and w.numel() > 0 and w.shape[-1] % 8 == 0, "w must be (..., N, K) with K a positive multiple of 8")
-    N, K = w.shape[-2:]
-    w = _aligned(w.detach().contiguous())
-    with L.on_device_of(w):
-        q = torch.empty(w.shape, dtype=torch.float8_e4m3fn, device=w.device)
-        scale = torch.empty(*w.shape[:-2], _blocks(N), _blocks(K), dtype=torch.float32, device=w.device)
-        L.check(L.lib().b200moe_fp8_block_quant_weight(w.data_ptr(), w.numel() // (N * K), N, K, q.data_ptr(), scale.data_ptr(),
-                                                       L.stream_of(w)))
-    return q, scale
+    return _QuantizeWeight.apply(w.contiguous())
 
 
 def _product(x, w, scale, transposed):
@@ -81,6 +106,7 @@ class _Fp8BlockLinear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, scale):
+        x, w = _aligned(x), _aligned(w)      # in here: a tracer would keep the choice it saw
         ctx.save_for_backward(w, scale)
         return _product(x, w, scale, False)
 
@@ -106,13 +132,26 @@ def fp8_block_linear(x, weight, weight_scale):
     N, K = w.shape
     L.require(x.dim() >= 1 and x.shape[-1] == K, f"x must be (..., {K}), got {tuple(x.shape)}")
     L.require(N % 8 == 0 and K % 16 == 0 and N > 0 and K > 0, f"weight must be (N, K) with N a multiple of 8 and K of 16, got ({N}, {K})")
-    rows = _aligned(x.reshape(-1, K).contiguous())
-    w = _aligned(w)
-    if torch.is_grad_enabled() and rows.requires_grad:
-        out = _Fp8BlockLinear.apply(rows, w, scale)
-    else:
-        out = _product(rows, w, scale, False)
+    out = _Fp8BlockLinear.apply(x.reshape(-1, K).contiguous(), w, scale)
     return out if x.dim() == 2 else out.view(*x.shape[:-1], N)
+
+
+class _Experts(_Frozen):
+    """`moe_fp8_block` on checked and contiguous tensors."""
+
+    @staticmethod
+    def forward(ctx, hidden, idx, w, gu, gs, dn, ds):
+        (T, H), (E, twoI, _), k, dev, lib = hidden.shape, gu.shape, idx.shape[1], hidden.device, L.lib()
+        I = twoI // 2
+        hidden, gu, dn = _aligned(hidden), _aligned(gu), _aligned(dn)
+        with L.on_device_of(hidden):
+            out = torch.empty(T, H, dtype=torch.bfloat16, device=dev)
+            if T:
+                ws = L.workspace(lib.b200moe_moe_fp8_block_ws_bytes(T, H, I, E, k), dev)
+                L.check(lib.b200moe_moe_fp8_block_forward(hidden.data_ptr(), idx.data_ptr(), w.data_ptr(), gu.data_ptr(), gs.data_ptr(),
+                                                          dn.data_ptr(), ds.data_ptr(), T, H, I, E, k, ws.data_ptr(), out.data_ptr(),
+                                                          L.status_word(dev).data_ptr(), L.stream_of(hidden)))
+        return out
 
 
 def moe_fp8_block(hidden, top_k_indices, top_k_weights, gate_up_proj, gate_up_scale, down_proj, down_scale):
@@ -141,16 +180,5 @@ def moe_fp8_block(hidden, top_k_indices, top_k_weights, gate_up_proj, gate_up_sc
     L.require(H > 0 and I > 0 and H % BLOCK == 0 and I % BLOCK == 0, f"d_model and d_ff must be positive multiples of {BLOCK}, got {H}, {I}")
     L.require(idx.device == dev and idx.dtype == torch.int64 and idx.dim() == 2 and idx.shape[0] == T, "top_k_indices must be int64 (N,k)")
     L.require(w.device == dev and w.shape == idx.shape, "top_k_weights must be (N,k) on hidden's device")
-    k = idx.shape[1]
-    L.require(k >= 1, "top_k_indices must have at least one pick a token")
-    hidden, gu, dn = (_aligned(t) for t in (hidden.detach().contiguous(), gu, dn))
-    idx, w = idx.contiguous(), w.detach().float().contiguous()
-    lib = L.lib()
-    with L.on_device_of(hidden):
-        out = torch.empty(T, H, dtype=torch.bfloat16, device=dev)
-        if T:
-            ws = L.workspace(lib.b200moe_moe_fp8_block_ws_bytes(T, H, I, E, k), dev)
-            L.check(lib.b200moe_moe_fp8_block_forward(hidden.data_ptr(), idx.data_ptr(), w.data_ptr(), gu.data_ptr(), gs.data_ptr(),
-                                                      dn.data_ptr(), ds.data_ptr(), T, H, I, E, k, ws.data_ptr(), out.data_ptr(),
-                                                      L.status_word(dev).data_ptr(), L.stream_of(hidden)))
-    return out
+    L.require(idx.shape[1] >= 1, "top_k_indices must have at least one pick a token")
+    return _Experts.apply(hidden.contiguous(), idx.contiguous(), w.float().contiguous(), gu, gs, dn, ds)

@@ -233,10 +233,8 @@ def group_topk(logits, top_k, bias=None, num_groups=1, topk_groups=None, scoring
     L.require(k >= 1, f"top_k = {k} must be positive")
     args = (bias, k, int(num_groups), opened, _SCORING[scoring], _GROUP_SCORE[group_score], bool(norm_topk_prob and k > 1),
             float(routed_scaling_factor))
-    if torch.is_grad_enabled() and flat.requires_grad:
-        idx, w, counts = _GroupTopk.apply(flat, *args)
-    else:
-        idx, w, counts = ops.group_topk_fwd(flat, *args, want_counts=return_counts)
+    # also where nothing requires a gradient: a tracer records the Function, and forward-mode gradients are refused by it
+    idx, w, counts = _GroupTopk.apply(flat, *args)
     if logits.dim() == 3:
         idx, w = idx.view(*logits.shape[:2], k), w.view(*logits.shape[:2], k)
     return (idx, w, counts) if return_counts else (idx, w)
@@ -286,11 +284,13 @@ def fused_group_router(x, gate_weight, bias, top_k, num_experts, num_groups=1, t
 
 
 class _RouterLosses(torch.autograd.Function):
-    """(balance, z) of contiguous logits (N,E) and picks (N,k) of `segments` equal segments."""
+    """(balance, z) of contiguous logits (N,E) or (B,S,E) and picks (N,k); per_sequence: over B segments, which are counted in here, so
+    that a traced call takes another batch."""
 
     @staticmethod
-    def forward(ctx, logits, idx, mask, segments, scoring):
-        balance, z, coef = ops.router_losses_fwd(logits, idx, mask, segments, scoring)
+    def forward(ctx, logits, idx, mask, per_sequence, scoring):
+        segments = logits.shape[0] if per_sequence else 1
+        balance, z, coef = ops.router_losses_fwd(logits.view(-1, logits.shape[-1]), idx, mask, segments, scoring)
         ctx.args = (segments, scoring)
         ctx.save_for_backward(logits, mask, coef)
         ctx.set_materialize_grads(False)
@@ -303,7 +303,8 @@ class _RouterLosses(torch.autograd.Function):
             return (None,) * 5
         logits, mask, coef = ctx.saved_tensors
         gb, gz = (None if g is None else g.float().contiguous() for g in (grad_balance, grad_z))
-        return (ops.router_losses_bwd(logits, mask, coef, gb, gz, *ctx.args),) + (None,) * 4
+        grad = ops.router_losses_bwd(logits.view(-1, logits.shape[-1]), mask, coef, gb, gz, *ctx.args)
+        return (grad.view(logits.shape),) + (None,) * 4
 
 
 def router_losses(logits, top_k_indices, scoring="softmax", mask=None, per_sequence=False):
@@ -327,19 +328,14 @@ def router_losses(logits, top_k_indices, scoring="softmax", mask=None, per_seque
     L.require(idx.device == logits.device and idx.dtype == torch.int64 and idx.dim() == logits.dim() and idx.shape[:-1] == logits.shape[:-1],
               "top_k_indices must be int64 (...,k) on the logits' device")
     L.require(idx.shape[-1] >= 1, "top_k_indices must have at least one pick a token")
-    E = logits.shape[-1]
     if mask is not None:
         L.require(mask.device == logits.device and mask.shape == logits.shape[:-1], "mask must have the tokens' shape, on the logits' device")
         mask = (mask if mask.dtype == torch.bool else mask != 0).contiguous()
-    segments = logits.shape[0] if per_sequence and logits.shape[0] > 0 else 1
-    flat = (logits if logits.dim() == 2 else logits.reshape(-1, E)).contiguous()
     idx = idx.reshape(-1, idx.shape[-1]).contiguous()
-    if flat.shape[0] == 0:
-        zero = flat.float().sum()
+    if logits.shape[0] == 0 or logits.shape[-2] == 0:
+        zero = logits.float().sum()
         return zero, zero.clone()
-    if torch.is_grad_enabled() and flat.requires_grad:
-        return _RouterLosses.apply(flat, idx, mask, segments, _SCORING[scoring])
-    return ops.router_losses_fwd(flat, idx, mask, segments, _SCORING[scoring])[:2]
+    return _RouterLosses.apply(logits.contiguous(), idx, mask, bool(per_sequence), _SCORING[scoring])
 
 
 @torch.no_grad()
