@@ -138,6 +138,10 @@ class _Layer(torch.autograd.Function):
 
 
 class MoELayer(LoadBalanceMixin, nn.Module):
+    # what a layer that was pickled without these has: the plain router
+    scoring, num_groups, topk_groups, group_score = "sigmoid", 1, None, "top2"
+    balance_loss, z_loss, balance_per_sequence, aux_loss = 0.0, 0.0, False, None
+
     def __init__(self, H, I, E, top_k=2, norm_topk_prob=True, routed_scaling_factor=1.0, init_std=0.02,
                  precision="bf16", act_codes=None, learnable_situ=False, scoring="sigmoid", num_groups=1, topk_groups=None,
                  group_score="top2", balance_loss=0.0, z_loss=0.0, balance_per_sequence=False):
