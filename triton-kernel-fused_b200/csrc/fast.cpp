@@ -433,6 +433,7 @@ optional<std::tuple<Tensor, Tensor>> router_losses(const Tensor& z, const Tensor
 // ---------------------------------------------------------------------------- e4m3 weights with block scales
 bool codes(const Tensor& w, const Tensor& scale, int64_t dim, c10::Device dev) {
   if (!plain(w, at::kFloat8_e4m3fn, dev) || !plain(scale, at::kFloat, dev) || w.dim() != dim || scale.dim() != dim || w.numel() == 0) return false;
+  if (at::GradMode::is_enabled() && (w.requires_grad() || scale.requires_grad())) return false;      // refused
   if (dim == 3 && scale.size(0) != w.size(0)) return false;
   return scale.size(-2) == (w.size(-2) + 127) / 128 && scale.size(-1) == (w.size(-1) + 127) / 128;
 }

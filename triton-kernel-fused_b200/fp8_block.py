@@ -24,6 +24,8 @@ def _weight(name, w, scale, device, dim):
     """Codes and scales as the kernels read them: contiguous, 16-byte aligned."""
     L.require(w.dtype == torch.float8_e4m3fn and w.dim() == dim, f"{name} must be a float8_e4m3fn tensor of {dim} dimensions")
     L.require(w.device == device and scale.device == device, f"{name} and its scale must be on the input's device")
+    L.require(not (torch.is_grad_enabled() and (w.requires_grad or scale.requires_grad)),
+              f"{name} and its scale are frozen, they take no gradient: requires_grad_(False) on both, or torch.no_grad() around the call")
     want = (*w.shape[:-2], _blocks(w.shape[-2]), _blocks(w.shape[-1]))
     L.require(scale.dtype == torch.float32 and tuple(scale.shape) == want, f"the scale of {name} must be float32 {want}, got "
               f"{scale.dtype} {tuple(scale.shape)}")
@@ -119,7 +121,8 @@ class _Fp8BlockLinear(torch.autograd.Function):
 
 def fp8_block_linear(x, weight, weight_scale):
     """x (..., K) bf16 times weight (N, K) float8_e4m3fn with weight_scale (ceil(N/128), ceil(K/128)) fp32 -> (..., N) bf16.
-    N a multiple of 8, K of 16.  Differentiable in x (its gradient is quantised along N); the weights are frozen."""
+    N a multiple of 8, K of 16.  Differentiable in x (its gradient is quantised along N); the weights are frozen: one that
+    requires a gradient is refused in grad mode."""
     fast = L.fast() if x.is_cuda else None
     if fast is not None:
         out = fast.fp8_block_linear(x, weight, weight_scale, L.status_word(x.device))
