@@ -7,6 +7,7 @@
 #include <type_traits>
 
 #include "../../include/b200moe.h"
+#include "per_device.h"
 
 namespace b200moe {
 

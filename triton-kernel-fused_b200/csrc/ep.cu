@@ -16,7 +16,6 @@
 // that the host side issues (the kernels themselves never wait on a peer).
 #include <cuda_bf16.h>
 
-#include <mutex>
 
 #include "common.cuh"
 #include "ptx.cuh"
@@ -701,12 +700,8 @@ int b200moe_ep_combine_pull(const void* const* rows_peers, const float* w, const
   if (nslots > 16) nslots = 16;
   B200_CHECK_ARG(nslots >= 2, B200MOE_E_UNSUPPORTED, "ep_combine_pull: k = %d rows of 4 KB do not fit twice in shared memory", k);
   const size_t smem = nslots * per_slot + 128 + 16;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(ep_combine_pull_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
-  });
-  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "cudaFuncSetAttribute(max dynamic smem)");
+  static PerDevice smem_allowed;
+  B200_CUDA(allow_smem(smem_allowed, ep_combine_pull_kernel, 232448));
   const long long row_bytes = H * 2;
   const long long items = T * ((row_bytes + kPullChunk - 1) / kPullChunk);
   long long grid = exchange_sm_budget();

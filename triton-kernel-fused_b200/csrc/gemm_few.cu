@@ -21,7 +21,6 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
-#include <mutex>
 #include <type_traits>
 
 #include "few_tiles.cuh"
@@ -500,13 +499,8 @@ router_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
 template <int EPI, int NT, int HALVES>
 static int launch_few(const void* x, const void* w, int64_t rows_cap, const FewParams& p, cudaStream_t stream) {
   using C = FewCfg<EPI, NT, HALVES>;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(few_rows_kernel<EPI, NT, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    C::SMEM_BYTES);
-  });
-  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "cudaFuncSetAttribute(max dynamic smem)");
+  static PerDevice smem_allowed;
+  B200_CUDA(allow_smem(smem_allowed, few_rows_kernel<EPI, NT, HALVES>, C::SMEM_BYTES));
   CUtensorMap tmW, tmX, tmXbig;
   int rc = EPI == EPI_SWIGLU ? make_map_gate_up(&tmW, w, p.K, p.N, p.E, 8)
                              : make_map(&tmW, w, p.K, p.N, p.E, p.K, static_cast<uint64_t>(p.N) * p.K, kFewBK, 128);
@@ -526,12 +520,8 @@ static int launch_few(const void* x, const void* w, int64_t rows_cap, const FewP
 template <int VPL>
 static int launch_router_few(const void* x, const void* weight, const RouterFewParams& p, cudaStream_t stream) {
   using C = RouterFewCfg;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(router_few_kernel<VPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
-  });
-  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "cudaFuncSetAttribute(max dynamic smem)");
+  static PerDevice smem_allowed;
+  B200_CUDA(allow_smem(smem_allowed, router_few_kernel<VPL>, C::SMEM_BYTES));
   CUtensorMap tmW, tmX;   // a weight box of E rows: what the MMA reads past them ends in lanes nobody reads
   int rc = make_map(&tmW, weight, p.H, p.E, 1, p.H, static_cast<uint64_t>(p.E) * p.H, kFewBK, p.E);
   if (rc) return rc;

@@ -9,7 +9,6 @@
 #include <cuda.h>
 
 #include <algorithm>
-#include <mutex>
 
 #include "few_tiles.cuh"
 #include "fp8_block.cuh"
@@ -814,12 +813,8 @@ block_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
 template <int EPI, bool BMN>
 static int launch_pair(const void* X, int64_t x_rows, int64_t ldx, const void* W, int64_t w_inner, int64_t w_rows, int64_t groups,
                        const BlockParams& bp, int64_t max_tiles, cudaStream_t stream) {
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(block_pair_kernel<EPI, BMN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBSmemBytes<EPI>);
-  });
-  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "cudaFuncSetAttribute(max dynamic smem)");
+  static PerDevice smem_allowed;
+  B200_CUDA(allow_smem(smem_allowed, block_pair_kernel<EPI, BMN>, kBSmemBytes<EPI>));
   CUtensorMap tmA, tmB, tmD;
   int rc = make_map(&tmA, X, bp.g.K, x_rows, 1, ldx, x_rows * ldx, kBBK, 128, 1);
   if (rc == 0) rc = make_map(&tmB, W, w_inner, w_rows, groups, w_inner, w_rows * w_inner, 128, 128, 1);
@@ -842,12 +837,8 @@ template <int EPI, int NT, bool QUANT = false>
 static int launch_few(const void* X, int64_t x_rows, int64_t ldx, const void* W, int64_t w_rows, BlockParams bp, int64_t tiles,
                       int64_t max_tiles, cudaStream_t stream) {
   using C = FewBlockCfg<EPI, NT>;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(block_few_kernel<EPI, NT, QUANT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
-  });
-  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "cudaFuncSetAttribute(max dynamic smem)");
+  static PerDevice smem_allowed;
+  B200_CUDA(allow_smem(smem_allowed, block_few_kernel<EPI, NT, QUANT>, C::SMEM_BYTES));
   CUtensorMap tmW, tmX;
   int rc = make_map(&tmW, W, bp.g.K, w_rows, bp.g.num_groups, bp.g.K, w_rows * bp.g.K, kBBK, 128, 1);
   tmX = tmW;

@@ -959,12 +959,8 @@ template <int EPI, bool FWD>
 static int launch_fp8_pair(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmSFA,
                            const CUtensorMap& tmSFB, const CUtensorMap& tmD, const CUtensorMap& tmD2,
                            const Fp8Params& fp, int max_tiles, cudaStream_t stream) {
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(gemm_mxfp8_pair_kernel<EPI, FWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg<EPI>::kSmemBytes);
-  });
-  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "cudaFuncSetAttribute(max dynamic smem)");
+  static PerDevice smem_allowed;
+  B200_CUDA(allow_smem(smem_allowed, gemm_mxfp8_pair_kernel<EPI, FWD>, PairCfg<EPI>::kSmemBytes));
   int pairs = gemm_cta_budget() / 2;
   if (max_tiles > 0 && max_tiles < pairs) pairs = max_tiles;
   if (pairs < 1) pairs = 1;
@@ -987,12 +983,8 @@ static bool fp8_pairs_enabled() {
 template <int EPI>
 static int launch_fp8(const CUtensorMap& tmA, const CUtensorMap& tmB, const Fp8Params& fp, int max_tiles,
                       cudaStream_t stream) {
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(gemm_mxfp8_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFSmemBytes);
-  });
-  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "cudaFuncSetAttribute(max dynamic smem)");
+  static PerDevice smem_allowed;
+  B200_CUDA(allow_smem(smem_allowed, gemm_mxfp8_kernel<EPI>, kFSmemBytes));
   int grid = gemm_cta_budget();
   if (max_tiles > 0 && max_tiles < grid) grid = max_tiles;
   if (grid < 1) grid = 1;
@@ -1010,12 +1002,8 @@ static int launch_few_fp8(const void* Xq, const void* Wq, int64_t rows_cap, cons
   using C = FewFp8Cfg<EPI, NT>;
   int rc = check_scales(p.sfx, p.sfw);
   if (rc) return rc;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(few_mxfp8_kernel<EPI, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
-  });
-  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "cudaFuncSetAttribute(max dynamic smem)");
+  static PerDevice smem_allowed;
+  B200_CUDA(allow_smem(smem_allowed, few_mxfp8_kernel<EPI, NT>, C::SMEM_BYTES));
   CUtensorMap tmW, tmX, tmXbig;
   rc = map_fp8(&tmW, Wq, p.N, p.K, p.E);
   if (rc) return rc;
