@@ -63,10 +63,10 @@ __device__ __forceinline__ void best_of(double x, double& a, double& b) {
   b = x > a ? a : (x > b ? x : b);
   a = x > a ? x : a;
 }
-// A group's value from them; infinity less infinity counts as infinity too
+// A group's value from them, halved, so that the sum of two finite values is finite; infinity less infinity counts as infinity too
 template <class F>
-__device__ __forceinline__ F group_value(const GroupParams& p, F a, F b) {
-  const F v = p.top2 && p.per_group > 1 ? a + b : a;
+__device__ __forceinline__ F group_value(F a, F b) {
+  const F v = static_cast<F>(0.5) * a + static_cast<F>(0.5) * b;
   return v != v ? static_cast<F>(INFINITY) : v;
 }
 template <class F>
@@ -129,7 +129,7 @@ __device__ __noinline__ bool open_exactly(const GroupParams& p, long long t, int
   for (int i = 0; i < live; ++i) best_of(x.value(i), a, b);
   group_best(p.lanes_log, a, b);
   bool close;
-  return group_open(group_value(p, a, b), g, p.groups, p.lanes_log, p.open, -1.0, close);
+  return group_open(group_value(a, p.top2 && p.per_group > 1 ? b : a), g, p.groups, p.lanes_log, p.open, -1.0, close);
 }
 
 // the rank of a lane's candidate (its logit and bias) among n
@@ -272,7 +272,8 @@ group_topk_kernel(const __grid_constant__ GroupParams p) {
             if (i < live) best_of(v[i], a, b);
         }
         group_best(p.lanes_log, a, b);
-        mine = group_open(group_value(p, a, b), g, p.groups, p.lanes_log, p.open, direct ? -1.0f : 2.0f * near, close) && mine;
+        if (!p.top2 || p.per_group == 1) b = a;
+        mine = group_open(direct ? a : group_value(a, b), g, p.groups, p.lanes_log, p.open, direct ? -1.0f : near, close) && mine;
       }
       if (close) mine = open_exactly<T, SOFTMAX>(p, t, g, first, live, m) && live > 0;
       if (!mine) {
