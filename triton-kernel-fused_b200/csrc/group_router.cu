@@ -6,7 +6,7 @@
 //
 // A pick is a comparison of real numbers, and two of 256 experts are often closer than fp32 resolves (32 768 tokens, 8 of 256: some
 // hundred picks a step), so which one an fp32 kernel takes is left to its rounding.  Here the picks are those of the real numbers:
-// without a bias s rises with z, and z itself is compared; with one, values closer than the error of the fp32 ones (kNear) are
+// without a bias s rises with z, and z itself is compared; with one, values closer than the error of the fp32 ones (kErr) are
 // computed again in 64 bits and compared there, unless logit and bias are the same, which is a tie.
 //
 // One warp a token.  A lane holds V neighbouring experts of one group (groups own lanes, so a group's value is a reduction over
@@ -21,11 +21,19 @@
 namespace b200moe {
 
 constexpr int kGroupWarps = 8;
-// At least twice the error of an fp32 value v = s + b, relative to 1 + |b|.  In steps of 2^-23: the exponential of x is off by
-// 2 + 1.17 |x| of its own, of which a sigmoid keeps the share s (1 - s), 0.7 at most, the quotient 2, the sums 0.5 and 0.5 (1 + |b|):
-// below 4 and 8.  A softmax keeps 2 of the exponentials, 2 of those in its sum, 6.5 of 13 additions, 1.5 of the quotient: 12.5 and 32.
+// Two fp32 values v = s + b whose distance is above the sum of their kErr * max(1, |v|) are in the order of the real numbers.  In steps of 2^-23,
+// relative to max(1, |v|): a sigmoid is off by 0.7 (its exponential, 2 + 1.17 |x| of itself, times s (1 - s)), 2 (quotient) and 0.5 (sum), v by 0.5 more and
+// the sum of a group's two values by 0.5: 4.2, and 8 are allowed.  A softmax value is off by 2 (the exponential of x <= 0: 2 + 1.67 |x| of itself with the
+// rounding of x, times at most e^x), 0.5 (product), 0.5 and 0.5: 3.5 of its own.  What the denominator is off by is common to the two values and
+// counts with their distance, below 1: 0.5 (quotient), 2 + 2.5 (its exponentials; the mean of 1.67 |x|, times the largest share), 6 or 10 (12 or 20 additions, at
+// 8 or 16 values a lane): 15 a pair.  7 + 15 = 22, and 32 are allowed.
 template <bool SOFTMAX>
-constexpr float kNear = SOFTMAX ? 3.814697265625e-6f : 1.9073486328125e-6f;   // 2^-18, 2^-19
+constexpr float kErr = SOFTMAX ? 1.9073486328125e-6f : 9.5367431640625e-7f;   // 2^-19, 2^-20
+// of v, finite for an infinite one too (a sum with infinity is exact)
+template <bool SOFTMAX>
+__device__ __forceinline__ float err_of(float v) {
+  return kErr<SOFTMAX> * fminf(fmaxf(fabsf(v), 1.0f), 3.402823466e38f);
+}
 
 // A value (no NaN) as a signed integer of the same order, and back; kNone lies below every value
 constexpr int kNone = static_cast<int>(0x80000000u);
@@ -79,19 +87,21 @@ __device__ __forceinline__ void group_best(int lanes_log, F& a, F& b) {
     b = b > lo ? b : lo;
   }
 }
-// Whether a lane's group is among the `open` best.  close: the last one that is and one that is not lie within `near` of one another
+// Whether a lane's group is among the `open` best
 template <class F>
-__device__ __forceinline__ bool group_open(F value, int g, int groups, int lanes_log, int open, F near, bool& close) {
+__device__ __forceinline__ bool group_open(F value, int g, int groups, int lanes_log, int open) {
   int rank = 0;
   for (int j = 0; j < groups; ++j) {
     const F o = __shfl_sync(0xffffffffu, value, j << lanes_log);
     rank += o > value || (o == value && j < g) ? 1 : 0;
   }
-  const bool in = g < groups;
-  const int last = __ffs(__ballot_sync(0xffffffffu, in && rank == open - 1)) - 1;
-  const F border = __shfl_sync(0xffffffffu, value, last < 0 ? 0 : last);
-  close = __any_sync(0xffffffffu, in && rank >= open && border - value <= near);
-  return in && rank < open;
+  return g < groups && rank < open;
+}
+// Whether an open and a closed group may be the other way round, each value off by `err` at most.  (Infinite ones are equal as they are.)
+__device__ __forceinline__ bool groups_close(float value, float err, bool opened, bool closed) {
+  const float lo = value_of(__reduce_min_sync(0xffffffffu, opened ? key_of(value - err) : 0x7fffffff));
+  const float hi = value_of(__reduce_max_sync(0xffffffffu, closed ? key_of(value + err) : kNone));
+  return hi >= lo && fabsf(lo) < INFINITY;
 }
 
 // The rest is for tokens that fp32 does not decide.  Out of line, with the logits read again one by one: inlined, its 64-bit arithmetic
@@ -128,8 +138,7 @@ __device__ __noinline__ bool open_exactly(const GroupParams& p, long long t, int
 #pragma unroll 1
   for (int i = 0; i < live; ++i) best_of(x.value(i), a, b);
   group_best(p.lanes_log, a, b);
-  bool close;
-  return group_open(group_value(a, p.top2 && p.per_group > 1 ? b : a), g, p.groups, p.lanes_log, p.open, -1.0, close);
+  return group_open(group_value(a, p.top2 && p.per_group > 1 ? b : a), g, p.groups, p.lanes_log, p.open);
 }
 
 // the rank of a lane's candidate (its logit and bias) among n
@@ -194,15 +203,10 @@ group_topk_kernel(const __grid_constant__ GroupParams p) {
   const int g = lane >> p.lanes_log, sub = lane & ((1 << p.lanes_log) - 1);
   const int live = g < p.groups ? max(0, min(V, p.per_group - sub * V)) : 0;
   const int first = live > 0 ? g * p.per_group + sub * V : 0;
-  float bias[V], span = 1.0f;
+  float bias[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    bias[i] = p.bias != nullptr && i < live ? p.bias[first + i] : 0.0f;
-    const float size = fabsf(bias[i]);
-    span = fmaxf(span, 1.0f + (size < INFINITY ? size : 0.0f));      // sums with an infinite one are exact
-  }
+  for (int i = 0; i < V; ++i) bias[i] = p.bias != nullptr && i < live ? p.bias[first + i] : 0.0f;
   const bool by_logit = p.bias == nullptr;
-  const float near = kNear<SOFTMAX> * warp_max(span);
   int2* cand = cand_s[warp];
   float2* pick = pick_s[warp];
 
@@ -273,7 +277,10 @@ group_topk_kernel(const __grid_constant__ GroupParams p) {
         }
         group_best(p.lanes_log, a, b);
         if (!p.top2 || p.per_group == 1) b = a;
-        mine = group_open(direct ? a : group_value(a, b), g, p.groups, p.lanes_log, p.open, direct ? -1.0f : near, close) && mine;
+        const float value = direct ? a : group_value(a, b);
+        const bool opened = group_open(value, g, p.groups, p.lanes_log, p.open);
+        close = !direct && groups_close(value, 0.5f * (err_of<SOFTMAX>(a) + err_of<SOFTMAX>(b)), opened, g < p.groups && !opened);
+        mine = mine && opened;
       }
       if (close) mine = open_exactly<T, SOFTMAX>(p, t, g, first, live, m) && live > 0;
       if (!mine) {
@@ -281,7 +288,7 @@ group_topk_kernel(const __grid_constant__ GroupParams p) {
         for (int i = 0; i < V; ++i) key[i] = kNone;
       }
     }
-    // ---- candidates: every expert that reaches the k-th largest of the lanes' maxima (less `near`)
+    // ---- candidates: every expert that reaches the k-th largest of the lanes' maxima (less what the two may be off by)
     int best = key[0];
 #pragma unroll
     for (int i = 1; i < V; ++i) best = max(best, key[i]);
@@ -294,9 +301,9 @@ group_topk_kernel(const __grid_constant__ GroupParams p) {
       n += __popc(at);
       if (best == top) best = kNone;
     }
-    // fewer than k lanes with an expert: all of them; else what `near` may hide below it too
+    // fewer than k lanes with an expert: all of them; else what may be hidden below it too
     if (floor_key == kNone) floor_key = kNone + 1;
-    else if (!by_logit) floor_key = min(floor_key, key_of(value_of(floor_key) - near));
+    else if (!by_logit) floor_key = min(floor_key, key_of(value_of(floor_key) - 2.0f * err_of<SOFTMAX>(value_of(floor_key))));
     // collected in the order of the experts, so that of equal ones the first collected wins
     int have = 0;
 #pragma unroll
@@ -317,6 +324,7 @@ group_topk_kernel(const __grid_constant__ GroupParams p) {
       const int2 c = lane < n ? cand[lane] : make_int2(kNone, 0);
       const float logit = to_f32(row[c.y]);
       const float value = lane < n ? value_of(c.x) : -INFINITY;
+      const float near = 2.0f * err_of<SOFTMAX>(value);      // values this close are of one size
       int rank = 0, level = 0;                     // level: candidates within `near` of this one, itself among them
       if (by_logit) {
 #pragma unroll 4
