@@ -72,3 +72,17 @@ def test_near_ties_at_sixteen_values_a_lane(pkg, groups, opened, by):
         z = z.expand(T, E).contiguous()
         z[1:, 2:] += torch.randn(T - 1, E - 2, generator=g, device=DEV) * 1e-6
         check(pkg, z, k, b, groups, opened, scoring, by)
+
+
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+def test_groups_of_one_expert(pkg, scoring):
+    """Without a bias the logits decide, also where the scores are equal in 64 bits: a group of one expert is worth its best one."""
+    z = torch.arange(60.0, 68.0, device=DEV).repeat(5, 1)
+    z[1] = z[1].flip(0)
+    z[2] = -torch.arange(8, device=DEV) * 900.0
+    z[3] = -z[2]
+    z[4] = 3.0
+    for by in ("top2", "max"):
+        for opened in (3, 8):
+            idx, _ = pkg.group_topk(z, 3, None, 8, opened, scoring, by)
+            assert idx.tolist() == [[7, 6, 5], [0, 1, 2], [0, 1, 2], [7, 6, 5], [0, 1, 2]], (by, opened)

@@ -138,7 +138,7 @@ __device__ __noinline__ bool open_exactly(const GroupParams& p, long long t, int
 #pragma unroll 1
   for (int i = 0; i < live; ++i) best_of(x.value(i), a, b);
   group_best(p.lanes_log, a, b);
-  return group_open(group_value(a, p.top2 && p.per_group > 1 ? b : a), g, p.groups, p.lanes_log, p.open);
+  return group_open(group_value(a, p.top2 ? b : a), g, p.groups, p.lanes_log, p.open);
 }
 
 // the rank of a lane's candidate (its logit and bias) among n
@@ -276,7 +276,7 @@ group_topk_kernel(const __grid_constant__ GroupParams p) {
             if (i < live) best_of(v[i], a, b);
         }
         group_best(p.lanes_log, a, b);
-        if (!p.top2 || p.per_group == 1) b = a;
+        if (!p.top2) b = a;
         const float value = direct ? a : group_value(a, b);
         const bool opened = group_open(value, g, p.groups, p.lanes_log, p.open);
         close = !direct && groups_close(value, 0.5f * (err_of<SOFTMAX>(a) + err_of<SOFTMAX>(b)), opened, g < p.groups && !opened);
@@ -486,7 +486,7 @@ int b200moe_group_topk_fwd(const void* logits, int logits_type, const float* bia
   GroupParams p{};
   p.logits = logits; p.bias = bias; p.T = T; p.E = E; p.k = k; p.groups = groups; p.open = open; p.per_group = E / groups;
   while ((2 << p.lanes_log) * groups <= 32) ++p.lanes_log;
-  p.top2 = group_top2; p.norm = norm_topk; p.scale = scale;
+  p.top2 = group_top2 && p.per_group > 1; p.norm = norm_topk; p.scale = scale;
   p.idx = reinterpret_cast<long long*>(idx); p.w = w; p.counts = counts; p.count_direct = grid == 1;
   const int lanes = 1 << p.lanes_log;
   cudaError_t err = cudaSuccess;
