@@ -241,13 +241,15 @@ class MoELayer(LoadBalanceMixin, nn.Module):
 class Fp8BlockMoELayer(nn.Module):
     """A layer for serving with 8-bit experts (`moe_fp8_block`): e4m3 stacks with fp32 scales per 128 x 128 block, as buffers, under
     the names that `MoELayer` has for its parameters, so a checkpoint of them loads by `load_state_dict`; `from_layer` quantises a bf16 one.
-    Routes like `MoELayer`.  The gate, in bf16, is the one parameter and takes no gradient; `to(dtype)` and the like leave codes and scales as
+    Routes like `MoELayer`: by `fused_mlp_router` where scores are sigmoid over one group of experts, else by `fused_group_router`, which
+    exact_picks asks for in either case; `from_layer` does so for a layer with losses, whose router that is.  The gate, in bf16, is the one parameter and takes no gradient; `to(dtype)` and the like leave codes and scales as
     they are."""
 
+    exact_picks = False
     _KEPT = ("gate_up_proj", "gate_up_scale", "down_proj", "down_scale", "bias")
 
     def __init__(self, H, I, E, top_k=2, norm_topk_prob=True, routed_scaling_factor=1.0, scoring="sigmoid", num_groups=1, topk_groups=None,
-                 group_score="top2", device=None):
+                 group_score="top2", device=None, exact_picks=False):
         super().__init__()
         if H % 128 or I % 128:
             raise ValueError(f"d_model and d_ff must be multiples of 128, got {H}, {I}")
@@ -258,6 +260,7 @@ class Fp8BlockMoELayer(nn.Module):
         self.register_buffer("bias", torch.zeros(E, device=device))
         self.top_k, self.num_experts, self.norm_topk_prob, self.routed_scaling_factor = top_k, E, norm_topk_prob, routed_scaling_factor
         self.scoring, self.num_groups, self.topk_groups, self.group_score = scoring, num_groups, topk_groups, group_score
+        self.exact_picks = exact_picks
 
     @classmethod
     @torch.no_grad()
@@ -267,7 +270,7 @@ class Fp8BlockMoELayer(nn.Module):
             raise ValueError("8-bit experts are pure SiLU-GLU stacks (act code 0)")
         E, twoI, H = layer.gate_up_proj.shape
         self = cls(H, twoI // 2, E, layer.top_k, layer.norm_topk_prob, layer.routed_scaling_factor, layer.scoring, layer.num_groups,
-                   layer.topk_groups, layer.group_score, device=layer.gate_up_proj.device)
+                   layer.topk_groups, layer.group_score, layer.gate_up_proj.device, exact_picks=not layer._plain_router())
         self.gate.weight.copy_(layer.gate.weight)
         self.bias.copy_(layer.bias)
         self.gate_up_proj, self.gate_up_scale = fp8_block_quantize_weight(layer.gate_up_proj)
@@ -286,7 +289,7 @@ class Fp8BlockMoELayer(nn.Module):
     @torch.no_grad()
     def forward(self, x):                              # x: (B,S,H) or (N,H)
         flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-        if self.scoring == "sigmoid" and self.num_groups == 1:
+        if self.scoring == "sigmoid" and self.num_groups == 1 and not self.exact_picks:
             idx, w = fused_mlp_router(flat, self.gate.weight, self.bias, self.top_k, self.num_experts, self.norm_topk_prob,
                                       self.routed_scaling_factor)
         else:
