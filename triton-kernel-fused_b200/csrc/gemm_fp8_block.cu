@@ -314,6 +314,7 @@ block_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         }
       }
       if constexpr (EPI == EPI_STORE) {
+        ok = __all_sync(0xffffffffu, ok);      // the lanes meet in there
         if (live && ok) {
 #pragma unroll
           for (int cc = 0; cc < kBCols / 32; ++cc) {
@@ -638,8 +639,8 @@ block_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
             uint2 o[kQVec];
 #pragma unroll
             for (int h = 0; h < kQVec; ++h) o[h] = block_codes8(v[u][h], factor, m < 0x7f800000u);
-            ok = mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, ST_WAIT_PRODUCER);
-            __syncwarp();
+            // all lanes give up or none does: those that went on would wait in the next shuffle for those that left
+            ok = __all_sync(0xffffffffu, mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, ST_WAIT_PRODUCER));
             if (live && ok && kb + box < kb_hi) {
               uint8_t* to = smem + s * C::STAGE + 2 * kBTile + box * C::X_BYTES + r * kBBK + 8 * (ql & 1);      // 128-byte swizzle
 #pragma unroll
