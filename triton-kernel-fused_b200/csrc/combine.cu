@@ -59,6 +59,44 @@ combine_kernel(const uint4* rows, int pitch, const float* w, const int* slot_row
   }
 }
 
+// The same of fp32 rows that lie at their slots, without gaps; slot_row tells the slots that have one.
+template <int TPR>
+__global__ void __launch_bounds__(256)
+combine_f32_kernel(const float4* rows, const float* w, const int* slot_row, long long T, int k, int vec_per_row, uint4* out) {
+  grid_dep_begin();
+  constexpr int G = 256 / TPR;
+  for (long long t = static_cast<long long>(blockIdx.x) * G + threadIdx.x / TPR; t < T;
+       t += static_cast<long long>(gridDim.x) * G) {
+    const int* slots = slot_row + t * k;
+    const float4* src = rows + t * k * (2LL * vec_per_row);
+    for (int c = threadIdx.x % TPR; c < vec_per_row; c += TPR) {
+      float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      for (int j0 = 0; j0 < k; j0 += 4) {
+        float4 v[4][2];
+        float wt[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[i][0] = v[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+          wt[i] = 0.0f;
+          if (j0 + i < k && slots[j0 + i] >= 0) {
+            const float4* r = src + (j0 + i) * (2LL * vec_per_row) + 2 * c;
+            v[i][0] = r[0];
+            v[i][1] = r[1];
+            wt[i] = w[t * k + j0 + i];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          acc[0] += wt[i] * v[i][0].x; acc[1] += wt[i] * v[i][0].y; acc[2] += wt[i] * v[i][0].z; acc[3] += wt[i] * v[i][0].w;
+          acc[4] += wt[i] * v[i][1].x; acc[5] += wt[i] * v[i][1].y; acc[6] += wt[i] * v[i][1].z; acc[7] += wt[i] * v[i][1].w;
+        }
+      }
+      out[t * vec_per_row + c] = make_uint4(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]), pack_bf16x2(acc[4], acc[5]),
+                                            pack_bf16x2(acc[6], acc[7]));
+    }
+  }
+}
+
 // grad_eo[r] = bf16(go[tok] * w[slot]);  grad_w[slot] = sum_h go[tok,h] * eo[r,h]  (fp32)
 // One warp per routed row, 2 * kVecBatch independent 16-byte loads in flight per lane; the dot product is
 // reduced by shuffles in a fixed order.
@@ -172,6 +210,19 @@ int combine_add(const void* rows, int64_t ldh, const float* w, const int32_t* sl
                          (cudaStream_t)stream, 1,
                          reinterpret_cast<const uint4*>(rows), static_cast<int>(ldh / 8), w, slot_row, reinterpret_cast<const uint4*>(add), T, k,
                          static_cast<int>(H / 8), reinterpret_cast<uint4*>(out));
+  });
+  B200_CUDA(err);
+  return 0;
+}
+
+int combine_f32(const float* rows, const float* w, const int32_t* slot_row, int64_t T, int k, int64_t H, void* out, b200moe_stream_t stream) {
+  cudaError_t err = cudaSuccess;
+  by_row_threads(static_cast<int>(H / 8), [&](auto tpr) {
+    constexpr int G = 256 / tpr.value;
+    const long long grid = std::min<long long>((T + G - 1) / G, static_cast<long long>(num_sms()) * 16);
+    err = launch_chained(combine_f32_kernel<tpr.value>, static_cast<int>(grid), 256, 0, (cudaStream_t)stream, 1,
+                         reinterpret_cast<const float4*>(rows), w, slot_row, static_cast<long long>(T), k, static_cast<int>(H / 8),
+                         reinterpret_cast<uint4*>(out));
   });
   B200_CUDA(err);
   return 0;

@@ -51,6 +51,8 @@ int gather_rows(const void* x, const int32_t* row_slot, const int32_t* total_row
                 b200moe_stream_t stream);
 int combine_add(const void* rows, int64_t ldh, const float* w, const int32_t* slot_row, const void* add, int64_t T, int k, int64_t H, void* out,
                 b200moe_stream_t stream);
+// combine.cu: out[t] = sum_j w[t,j] * rows[t*k+j] of fp32 rows at their slots; H a multiple of 8, all 16-byte aligned
+int combine_f32(const float* rows, const float* w, const int32_t* slot_row, int64_t T, int k, int64_t H, void* out, b200moe_stream_t stream);
 int combine_bwd(const void* grad_out, const void* eo, const float* w, const int32_t* row_slot, const int32_t* total_rows, int k, int64_t H,
                 int64_t ldh, int64_t rows_cap, void* grad_eo, float* grad_w, b200moe_stream_t stream);
 int glu_fwd_rows(const void* gate_up, int64_t ld2, const int32_t* tile_expert, const int32_t* act_codes, const float* act_params,

@@ -31,11 +31,12 @@ struct BlockParams {
   uint8_t* q_out;           // SwiGLU: codes (rows, I) and their scales [column block][row]
   float* q_scale;
   long long q_pitch;
-  __nv_bfloat16* out;       // few rows: (rows, N)
+  __nv_bfloat16* out;       // few rows: (rows, N), or
+  float* out_slots;         // ... (experts) the rows in fp32 at their slots of row_slot
   int split;                // few rows: CTAs of a cluster that share a tile's k-blocks
   int first_dense;          // few rows, dense: rows of X (no table)
   const __nv_bfloat16* x;   // few rows, quantised on the way: X in bf16, its rows those of the product or (row_slot) of the tokens, k slots each
-  const int* row_slot;
+  const int* row_slot;      // the slots, token and pick, of the rows
   int k;
 };
 
@@ -675,6 +676,8 @@ block_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
       const float* sw = bp.sw + t.e * bp.sw_group + static_cast<long long>(t.m0 >> 7) * bp.sw_n;
       const float* sw2 = sw + static_cast<long long>(bp.n_blocks) * bp.sw_n;       // SwiGLU: up
       const int col = t.m0 + 32 * q + lane;
+      int slot_of = 0;      // lane i: of this warp's row i
+      if (EPI == EPI_STORE && bp.out_slots != nullptr && lane < min(HC, t.live - half * HC)) slot_of = bp.row_slot[t.row0 + half * HC + lane];
       float acc[EPI == EPI_SWIGLU ? 2 : 1][HC];
 #pragma unroll
       for (int i = 0; i < HC; ++i) {
@@ -764,7 +767,13 @@ block_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
       const int mine = min(HC, t.live - half * HC);       // rows of this warp
       const long long row = t.row0 + half * HC;
       if constexpr (EPI == EPI_STORE) {
-        if (ok && col < p.N) {
+        if (bp.out_slots != nullptr) {
+#pragma unroll
+          for (int i = 0; i < HC; ++i) {
+            const long long to = __shfl_sync(0xffffffffu, slot_of, i);
+            if (i < mine && ok) bp.out_slots[to * p.N + col] = acc[0][i];      // N is a multiple of 128
+          }
+        } else if (ok && col < p.N) {
 #pragma unroll
           for (int i = 0; i < HC; ++i)
             if (i < mine) bp.out[(row + i) * p.N + col] = __float2bfloat16_rn(acc[0][i]);
@@ -941,7 +950,7 @@ struct BlockExperts {
   size_t scratch_bytes;
   uint8_t *xq, *iq;
   float *xs, *is;
-  void* eo;
+  void* eo;                 // the experts' results: bf16 rows as the products have them, or (few rows) fp32 at their slots
 };
 static BlockExperts carve_block(int64_t T, int64_t H, int64_t I, int E, int k, void* ws, size_t* bytes) {
   BlockCarver c{static_cast<char*>(ws)};
@@ -959,7 +968,8 @@ static BlockExperts carve_block(int64_t T, int64_t H, int64_t I, int E, int k, v
   f.xs = c.take<float>(cap * (H / 128));
   f.iq = c.take<uint8_t>(cap * I);
   f.is = c.take<float>(cap * (I / 128));
-  f.eo = c.take<uint16_t>(cap * H);
+  if (few_experts(ceil_div(M, E)) > 0) f.eo = c.take<float>(M * H);
+  else f.eo = c.take<uint16_t>(cap * H);
   *bytes = c.off;
   return f;
 }
@@ -1045,7 +1055,8 @@ int b200moe_moe_fp8_block_forward(const void* x, const int64_t* idx, const float
   BlockParams dn{};
   dn.g.sched = SCHED_GROUPED_M; dn.g.N = (int)H; dn.g.K = (int)I; dn.g.num_groups = E;
   dn.g.tile_expert = f.tile_expert; dn.g.poffs = f.poffs; dn.g.counts = f.counts; dn.g.status = status;
-  dn.g.D = f.eo; dn.g.ldd = H; dn.out = reinterpret_cast<__nv_bfloat16*>(f.eo);
+  if (nt > 0) { dn.out_slots = static_cast<float*>(f.eo); dn.row_slot = f.row_slot; }
+  else { dn.g.D = f.eo; dn.g.ldd = H; }
   dn.sx = f.is; dn.sx_pitch = cap; dn.rows = cap; dn.sw = down_scale;
   dn.n_blocks = (int)(H / 128); dn.sw_n = (int)(I / 128); dn.sw_k = 1; dn.sw_group = (H / 128) * (I / 128);
   const int64_t hit = std::min<int64_t>(E, M);           // experts that can have a row
@@ -1058,9 +1069,12 @@ int b200moe_moe_fp8_block_forward(const void* x, const int64_t* idx, const float
     RUN("fp8_block_gate_up", 1, (launch_pair<EPI_SWIGLU, false>(f.xq, cap, H, gate_up, H, 2 * I, E, up, tiles * (I / 128), st)));
     RUN("fp8_block_down", 1, (launch_pair<EPI_STORE, false>(f.iq, cap, I, down, I, H, E, dn, tiles * ceil_div(H, 256), st)));
   }
-  // A row's result is rounded to bf16 before the sum over a token's k, as in the bf16 block: kept in fp32 it would be 2 H bytes a row more,
-  // written and read (16 384 tokens of 2048, top-6: 120 us beside 1210), for an error of 0.0017 instead of 0.0024.
-  RUN("combine", 1, b200moe_combine(f.eo, w, f.slot_row, T, k, H, out, stream));
+  // Of few rows the results stay in fp32 until the sum over a token's k is rounded, which costs nothing (us a block, bf16 rows / fp32: 1 token
+  // of top-6 through 64 experts of 2048 x 1408 34.9 / 34.8, 256 tokens 137 / 139, 400 tokens 162 / 156; 64 tokens of top-2 through 8 of 4096 x 14336 258 / 258).
+  // Row tiles store them in bf16, as the bf16 block does: in fp32 they would be 2 H bytes a row more, written and read (16 384 tokens of 2048, top-6: 120 us
+  // beside 1210), for an error of 0.0017 instead of 0.0024.
+  if (nt > 0) RUN("combine", 1, combine_f32(static_cast<const float*>(f.eo), w, f.slot_row, T, k, H, out, stream));
+  else RUN("combine", 1, b200moe_combine(f.eo, w, f.slot_row, T, k, H, out, stream));
 #undef RUN
   return 0;
 }

@@ -2,7 +2,8 @@
 
 Weights carry one scale per 128 x 128 values, (..., ceil(N/128), ceil(K/128)); rows of activations are quantised on the way, one scale
 per 128 values, nearest e4m3 to 448 x / max |x|.  Every block of 128 is summed in fp32 by the tensor cores, scaled, and added in fp32;
-results are rounded to bf16 once.  MXFP8 (`moe_mxfp8`) is the other 8-bit format here: power-of-two scales per 32 values, bf16
+a product is rounded to bf16 once.  (So is what `moe_fp8_block` gives at few rows an expert; from 40 rows on an expert's results are bf16 before they
+are weighted and summed, as in `moe`.)  MXFP8 (`moe_mxfp8`) is the other 8-bit format here: power-of-two scales per 32 values, bf16
 masters, training.  These weights have no master: they are frozen, so `fp8_block_linear` gives the gradient of its input alone,
 and `moe_fp8_block` serves.  The reference has no 8-bit path."""
 from __future__ import annotations
