@@ -93,7 +93,10 @@ int fp8_block_quant(const void* x, int64_t rows, int64_t K, int64_t out_rows, co
                  (long long)ldq, (long long)pitch);
   B200_CHECK_ARG(aligned16(x) && reinterpret_cast<uintptr_t>(q) % 8 == 0, B200MOE_E_ALIGN, "fp8_block_quant: x must be 16-byte, q 8-byte aligned");
   if (rows == 0) return 0;
-  const int64_t blocks = rows * ((K + kBlockK - 1) / kBlockK), ctas = std::max<int64_t>((blocks + 32 * kQuantAhead - 1) / (32 * kQuantAhead), std::min<int64_t>((blocks + 31) / 32, num_sms()));
+  OpScope scope("fp8_block_quant", 1);
+  // three blocks of 128 for each eight lanes, but a CTA an SM where there is work for them
+  const int64_t blocks = rows * ((K + kBlockK - 1) / kBlockK);
+  const int64_t ctas = std::max<int64_t>((blocks + 32 * kQuantAhead - 1) / (32 * kQuantAhead), std::min<int64_t>((blocks + 31) / 32, num_sms()));
   B200_LAUNCH(fp8_block_quant_kernel, static_cast<int>(std::min<int64_t>(ctas, static_cast<int64_t>(num_sms()) * 16)), 256, 0, stream,
               reinterpret_cast<const __nv_bfloat16*>(x), static_cast<long long>(rows), static_cast<int>(K), slot_row, k,
               reinterpret_cast<uint8_t*>(q), static_cast<long long>(ldq), scale, static_cast<long long>(pitch));
@@ -152,6 +155,7 @@ int b200moe_fp8_block_quant_weight(const void* w, int64_t groups, int64_t N, int
                  "fp8_block_quant_weight: %lld matrices of %lld x %lld (a positive multiple of 8)", (long long)groups, (long long)N, (long long)K);
   B200_CHECK_ARG(aligned16(w) && reinterpret_cast<uintptr_t>(q) % 8 == 0, B200MOE_E_ALIGN,
                  "fp8_block_quant_weight: w must be 16-byte, q 8-byte aligned");
+  OpScope scope("fp8_block_quant_weight", 1);
   B200_LAUNCH(fp8_block_quant_weight_kernel, static_cast<int>(blocks), 256, 0, stream, reinterpret_cast<const __nv_bfloat16*>(w),
               static_cast<long long>(N), static_cast<int>(K), reinterpret_cast<uint8_t*>(q), scale);
   return 0;

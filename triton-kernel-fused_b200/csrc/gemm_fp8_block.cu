@@ -933,6 +933,7 @@ static int block_dense(const void* x, const void* w, const float* sw, int64_t M,
     const int rc = fp8_block_quant(x, M, K, M, nullptr, 1, q, ldq, sx, bp.sx_pitch, st);
     if (rc) return rc;
   }
+  OpScope scope("fp8_block_linear", 1);
   if (nt > 0) {
     bp.out = reinterpret_cast<__nv_bfloat16*>(out);
     bp.first_dense = (int)M;
@@ -1042,7 +1043,10 @@ int b200moe_moe_fp8_block_forward(const void* x, const int64_t* idx, const float
                     nullptr, nullptr, status, stream));
   const int nt = few_experts(ceil_div(M, E));
   const bool inside = quant_inside(ceil_div(M, E), H * I);
-  if (!inside) RUN("fp8_block_quant", 1, fp8_block_quant(x, T, H, cap, f.slot_row, k, f.xq, H, f.xs, cap, stream));
+  if (!inside) {
+    const int rc = fp8_block_quant(x, T, H, cap, f.slot_row, k, f.xq, H, f.xs, cap, stream);
+    if (rc) return rc;
+  }
   // gate and up
   BlockParams up{};
   up.g.sched = SCHED_GROUPED_M; up.g.N = up.g.I = (int)I; up.g.K = (int)H; up.g.num_groups = E;

@@ -489,6 +489,7 @@ int b200moe_group_topk_fwd(const void* logits, int logits_type, const float* bia
   p.top2 = group_top2 && p.per_group > 1; p.norm = norm_topk; p.scale = scale;
   p.idx = reinterpret_cast<long long*>(idx); p.w = w; p.counts = counts; p.count_direct = grid == 1;
   const int lanes = 1 << p.lanes_log;
+  OpScope scope("group_topk_fwd", 1);
   cudaError_t err = cudaSuccess;
   by_values((p.per_group + lanes - 1) / lanes, [&](auto v) {
     constexpr int V = v.value;
@@ -514,6 +515,7 @@ int b200moe_group_topk_bwd(const void* logits, int logits_type, const int64_t* i
   B200_CHECK_ARG(scoring == B200MOE_SIGMOID || scoring == B200MOE_SOFTMAX, B200MOE_E_UNSUPPORTED, "group_topk_bwd: unknown scoring %d",
                  scoring);
   if (T <= 0) return 0;
+  OpScope scope("group_topk_bwd", 1);
   cudaError_t err = cudaSuccess;
   by_values((E + 31) / 32, [&](auto v) {
     constexpr int V = v.value;

@@ -346,6 +346,7 @@ int b200moe_router_losses_fwd(const void* logits, int logits_type, const int64_t
   p.part_p = reinterpret_cast<float*>(p.seg_out + 3 * static_cast<long long>(segs));
   p.part_hits = reinterpret_cast<int*>(p.part_p + n * E);
   p.coef = coef; p.balance = balance; p.z = z; p.status = status;
+  OpScope scope("router_losses_fwd", p.blocks == 1 && segs == 1 ? 1 : segs == 1 ? 2 : 3);
   cudaError_t err = cudaSuccess;
   by_values((E + 31) / 32, [&](auto v) {
     constexpr int V = v.value;
@@ -372,6 +373,7 @@ int b200moe_router_losses_bwd(const void* logits, int logits_type, const uint8_t
   const int64_t rows = S * segs;
   if (rows == 0) return 0;
   const int grid = static_cast<int>(std::min<int64_t>((rows + 7) / 8, static_cast<int64_t>(num_sms()) * 8));
+  OpScope scope("router_losses_bwd", 1);
   cudaError_t err = cudaSuccess;
   by_values((E + 31) / 32, [&](auto v) {
     constexpr int V = v.value;

@@ -16,7 +16,8 @@ _LOGITS = {torch.bfloat16: LOGITS_BF16, torch.float32: LOGITS_F32, torch.float16
 TILE_M = 256   # B200MOE_TILE_M: expert segments are padded to this many rows
 
 # Optional observer used by the benchmark: hook(name, kernel_launches, start_event, end_event) is
-# called for every op below, and for every operation inside the native sequences (block.cu), with CUDA events recorded on
+# called for every op below, and for every operation that the native library tells of itself (the sequences of block.cu; the group
+# top-k, the router losses and the block-scaled products, which are reached past this module too), with CUDA events recorded on
 # the launching stream around it.
 _hook = None
 _native_observer = None
@@ -127,7 +128,6 @@ def _logits_type(logits):
     return _LOGITS[logits.dtype]
 
 
-@_op("group_topk_fwd", 1)
 def group_topk_fwd(logits, bias, top_k, groups, open_groups, scoring, top2, norm_topk=True, scale=1.0, want_counts=True):
     """(N,E) logits -> idx int64 (N,k), w fp32 (N,k), counts int32 (E,) or None: the top-k of the `open_groups` best groups."""
     kind, (N, E), dev = _logits_type(logits), logits.shape, logits.device
@@ -145,7 +145,6 @@ def group_topk_fwd(logits, bias, top_k, groups, open_groups, scoring, top2, norm
     return idx, w, counts
 
 
-@_op("group_topk_bwd", 1)
 def group_topk_bwd(logits, idx, grad_w, scoring, norm_topk=True, scale=1.0):
     kind, (N, E), gl = _logits_type(logits), logits.shape, torch.empty_like(logits)
     if N:
@@ -155,7 +154,6 @@ def group_topk_bwd(logits, idx, grad_w, scoring, norm_topk=True, scale=1.0):
     return gl
 
 
-@_op("router_losses_fwd", 3)
 def router_losses_fwd(logits, idx, mask, segments, scoring):
     """logits (N,E) and picks (N,k) of `segments` equal segments -> (balance, z, coefficients for the backward), fp32."""
     kind, (N, E), dev = _logits_type(logits), logits.shape, logits.device
@@ -170,7 +168,6 @@ def router_losses_fwd(logits, idx, mask, segments, scoring):
     return balance, z, coef
 
 
-@_op("router_losses_bwd", 1)
 def router_losses_bwd(logits, mask, coef, grad_balance, grad_z, segments, scoring):
     kind, (N, E), gl = _logits_type(logits), logits.shape, torch.empty_like(logits)
     with L.on_device_of(logits):
