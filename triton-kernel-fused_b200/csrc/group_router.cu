@@ -187,6 +187,7 @@ __device__ __noinline__ void pick_exactly(const GroupParams& p, long long t, int
   }
 }
 
+// (At four CTAs an SM the softmax form spills: 48 bytes a thread at eight values a lane, 16 at four.)
 template <class T, bool SOFTMAX, int V>
 __global__ void __launch_bounds__(32 * kGroupWarps, V > 8 ? 1 : 4)
 group_topk_kernel(const __grid_constant__ GroupParams p) {
@@ -383,8 +384,9 @@ group_topk_kernel(const __grid_constant__ GroupParams p) {
 }
 
 // dz of w = s[idx] scale, or of w = s[idx] / (sum + 1e-20) scale: ds at the picks, then dz = ds s (1 - s), or s (ds - <ds, s>).
-// Bound by the one write of dz (and, softmax, the one read of z; sigmoid reads its k logits alone).  The k values meet their
-// experts in a row of shared memory.
+// Bound by the issue of instructions and by one token's loads at a time in a warp (the picks, then their logits): 32 768 tokens, 8 of 256 experts, bf16
+// 11.8 us by sigmoid scores, 184 warp instructions a token in 72 % of the cycles, where dz, the picks and their logits' sectors take 4.3; softmax, which reads
+// and sums the whole row, 400 in 61 %.  The k values meet their experts in a row of shared memory.
 template <class T, bool SOFTMAX, int V>
 __global__ void __launch_bounds__(32 * kGroupWarps)
 group_topk_bwd_kernel(const T* logits, const long long* idx, const float* grad_w, long long T_, int E, int k, int norm, int vec,
