@@ -1,5 +1,7 @@
 """GPU: the routers' top-k and losses and the block-scaled products under a tracer and under forward-mode gradients.  A traced call gives on other
 inputs, of another size too, what the plain call gives; an input with a tangent is refused."""
+import importlib
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fw
@@ -116,3 +118,19 @@ def test_quantisers_of_parameters(pkg):
     for fn in (pkg.fp8_block_quantize, pkg.fp8_block_quantize_weight):
         for a, b in zip(fn(p), fn(p.detach())):
             assert not a.requires_grad and torch.equal(a.float(), b.float())
+
+
+@pytest.mark.parametrize("compiled", [True, False])
+@pytest.mark.parametrize("name", NAMES)
+def test_inference_mode(pkg, monkeypatch, name, compiled):
+    """Results, and inputs made in inference mode and used outside it."""
+    if not compiled:
+        monkeypatch.setattr(importlib.import_module(pkg.__name__ + "._lib"), "fast", lambda: None)
+    fn, inputs = calls(pkg)[name]
+    want = flat(fn(*inputs(20)))
+    with torch.inference_mode():
+        args = inputs(20)
+        here = flat(fn(*args))
+    for got in (here, flat(fn(*args))):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    pkg.check_status()

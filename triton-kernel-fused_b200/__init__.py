@@ -16,4 +16,6 @@ from . import muon
 from .muon import DistributedMuon, FusedMuon, newton_schulz
 
 __all__ = ["moe", "moe_grouped", "moe_per_expert", "GROUPED_MIN_TOKENS", "fused_mlp_router", "fused_router", "FusedConvRouter",
-           "FusedMLPRouter", "router_bias_update", "fused_group_router", "group_topk", "router_losses", "MoELayer", "Fp8BlockMoELayer", "moe_mxfp8", "fp8_block_linear", "fp8_block_quantize", "fp8_block_quantize_weight", "moe_fp8_block", "ExpertParallelMoELayer", "ep_moe", "FusedMuon", "DistributedMuon", "newton_schulz", "muon", "ops", "build", "lib", "check_status"]
+           "FusedMLPRouter", "router_bias_update", "fused_group_router", "group_topk", "router_losses", "MoELayer", "Fp8BlockMoELayer",
+           "moe_mxfp8", "fp8_block_linear", "fp8_block_quantize", "fp8_block_quantize_weight", "moe_fp8_block", "ExpertParallelMoELayer",
+           "ep_moe", "FusedMuon", "DistributedMuon", "newton_schulz", "muon", "ops", "build", "lib", "check_status"]

@@ -105,7 +105,8 @@ def _product(x, w, scale, transposed):
 
 
 class _Fp8BlockLinear(torch.autograd.Function):
-    """Plain calls take its compiled form (csrc/fast.cpp).  x (M,K) through frozen weights; the gradient of x is the product of its own gradient, quantised like x, with the same codes."""
+    """x (M,K) through frozen weights; the gradient of x is the product of its own gradient, quantised like x, with the same codes.  Plain
+    calls take its compiled form (csrc/fast.cpp)."""
 
     @staticmethod
     def forward(ctx, x, w, scale):

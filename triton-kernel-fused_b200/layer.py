@@ -147,7 +147,8 @@ class MoELayer(LoadBalanceMixin, nn.Module):
                  group_score="top2", balance_loss=0.0, z_loss=0.0, balance_per_sequence=False):
         """act_codes: one activation code per expert (default all 0 = SiLU-GLU); Identity (3) / Zero (4)
         experts come last and carry no weights.  learnable_situ adds an (E,2) [alpha,gamma] parameter
-        for the code-5 experts.  scoring, num_groups, topk_groups, group_score: the router's scores and groups of experts (`group_topk`).
+        for the code-5 experts.  scoring, num_groups, topk_groups, group_score: the router's scores and groups of experts (`group_topk`);
+        with any of them, or a loss, E is a multiple of 8 (`fused_group_router`).
         balance_loss, z_loss: the coefficients of `router_losses`; a training forward leaves balance_loss * balance + z_loss * z of its
         batch in `aux_loss` (None otherwise), for the caller to add to the loss."""
         super().__init__()
@@ -242,8 +243,8 @@ class Fp8BlockMoELayer(nn.Module):
     """A layer for serving with 8-bit experts (`moe_fp8_block`): e4m3 stacks with fp32 scales per 128 x 128 block, as buffers, under
     the names that `MoELayer` has for its parameters, so a checkpoint of them loads by `load_state_dict`; `from_layer` quantises a bf16 one.
     Routes like `MoELayer`: by `fused_mlp_router` where scores are sigmoid over one group of experts, else by `fused_group_router`, which
-    exact_picks asks for in either case; `from_layer` does so for a layer with losses, whose router that is.  The gate, in bf16, is the one parameter and takes no gradient; `to(dtype)` and the like leave codes and scales as
-    they are."""
+    exact_picks asks for in either case; `from_layer` does so for a layer with losses, whose router that is.  (The state dict does not hold it.)
+    The gate, in bf16, is the one parameter and takes no gradient; `to(dtype)` and the like leave codes and scales as they are."""
 
     exact_picks = False
     _KEPT = ("gate_up_proj", "gate_up_scale", "down_proj", "down_scale", "bias")

@@ -181,7 +181,8 @@ _GROUP_SCORE = {"top2": 1, "max": 0}
 
 
 class _GroupTopk(torch.autograd.Function):
-    """Plain calls take the compiled form of this Function and of `_RouterLosses` (csrc/fast.cpp).  (idx (N,k) int64, weights (N,k) fp32, counts (E,) int32) of contiguous logits (N,E); only the weights are differentiable."""
+    """(idx (N,k) int64, weights (N,k) fp32, counts (E,) int32) of contiguous logits (N,E); only the weights are differentiable.  Plain
+    calls take the compiled form of this Function and of `_RouterLosses` (csrc/fast.cpp)."""
 
     @staticmethod
     def forward(ctx, logits, bias, top_k, groups, opened, scoring, top2, norm, scale):
@@ -209,7 +210,7 @@ def group_topk(logits, top_k, bias=None, num_groups=1, topk_groups=None, scoring
     a group's two best experts, or its best one (group_score "max").  The k best experts of the open groups are the picks, in
     descending order, equal values in the order of the experts, and their unbiased scores the weights: divided by their sum + 1e-20
     where norm_topk_prob and k > 1, times routed_scaling_factor.  Picks are decided as for real numbers: without a bias by the logits
-    themselves, with one in 64 bits where fp32 would round.  A row of -inf scores 0 everywhere; NaN ranks first.
+    themselves, with one, and for groups by two experts, in 64 bits where fp32 would round.  A row of -inf scores 0 everywhere; NaN ranks first.
     E <= 256, k <= 32 and at most the experts of the open groups.  Differentiable in the logits."""
     L.require(scoring in _SCORING, f"scoring must be 'sigmoid' or 'softmax', got {scoring!r}")
     L.require(group_score in _GROUP_SCORE, f"group_score must be 'top2' or 'max', got {group_score!r}")
@@ -270,7 +271,8 @@ class _RouterLogits(torch.autograd.Function):
 def fused_group_router(x, gate_weight, bias, top_k, num_experts, num_groups=1, topk_groups=None, scoring="sigmoid", group_score="top2",
                        norm_topk_prob=True, routed_scaling_factor=1.0, return_counts=False, return_logits=False):
     """`fused_mlp_router` with softmax or sigmoid scores and groups of experts (`group_topk`): x (B,S,H) or (N,H), gate_weight (E,H) ->
-    (idx, weights[, counts][, logits]).  The logits are bf16 and differentiable, for `router_losses`."""
+    (idx, weights[, counts][, logits]).  The logits are bf16 and differentiable, for `router_losses`.  E a multiple of 8 here
+    (`group_topk` takes any), x and gate_weight bf16."""
     L.require(num_experts is None or int(num_experts) == gate_weight.shape[0], "num_experts must equal gate_weight.shape[0]")
     flat = x.reshape(-1, x.shape[-1])
     if flat.shape[0] == 0:
