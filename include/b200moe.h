@@ -48,6 +48,8 @@ enum {
 enum { B200MOE_LOGITS_BF16 = 0, B200MOE_LOGITS_F32 = 1, B200MOE_SCORES_F32 = 2 };
 /* ... and by the group-limited top-k and the router losses: LOGITS_BF16, LOGITS_F32 and */
 enum { B200MOE_LOGITS_F16 = 3 };
+/* types of rows where several are served: the same numbers */
+enum { B200MOE_BF16 = 0, B200MOE_F32 = 1, B200MOE_F16 = 3 };
 /* their scores */
 enum { B200MOE_SIGMOID = 0, B200MOE_SOFTMAX = 1 };
 
@@ -366,12 +368,31 @@ int b200moe_fp8_block_quant_weight(const void* w, int64_t groups, int64_t N, int
 size_t b200moe_fp8_block_linear_ws_bytes(int64_t M, int64_t K);
 int b200moe_fp8_block_linear(const void* x, const void* w, const float* w_scale, int64_t M, int64_t N, int64_t K, int transposed,
                              void* ws, void* out, int32_t* status, b200moe_stream_t stream);
+/* The same from rows that are codes already: q (M,K), q_scale [k-block][scale_pitch], scale_pitch at least M rounded up to whole 128 and a
+ * multiple of 4, all of it readable. */
+int b200moe_fp8_block_linear_rows(const void* q, const float* q_scale, int64_t scale_pitch, const void* w, const float* w_scale, int64_t M,
+                                  int64_t N, int64_t K, void* out, int32_t* status, b200moe_stream_t stream);
 /* The experts on given picks, forward (SiLU-GLU): gate_up (E,2I,H) and down (E,H,I) e4m3 with their scales, x (T,H) bf16,
  * idx (T,k) int64, w (T,k) fp32, out (T,H) bf16; H and I multiples of 128.  silu(gate) * up is requantised from fp32. */
 size_t b200moe_moe_fp8_block_ws_bytes(int64_t T, int64_t H, int64_t I, int E, int k);
 int b200moe_moe_fp8_block_forward(const void* x, const int64_t* idx, const float* w, const void* gate_up, const float* gate_up_scale,
                                   const void* down, const float* down_scale, int64_t T, int64_t H, int64_t I, int E, int k,
                                   void* ws, void* out, int32_t* status, b200moe_stream_t stream);
+
+/* ---- root-mean-square norm (no counterpart in the reference) ------------------------------------
+ * h = x + residual in the rows' type (h = x without one), y = h / sqrt(mean(h^2) + eps) * weight.  type: B200MOE_BF16, _F16 or _F32,
+ * weight_type the same or B200MOE_F32; rows of K values, 1..16384, ldx / ldr elements apart; all sums fp32.
+ * y, h (both contiguous), q: each nullable, one at least; h only with a residual.  q (rows,K) e4m3 codes of y before it is rounded, K % 8 == 0,
+ * with scales [block of 128][scale_pitch >= rows] as b200moe_fp8_block_quant gives them. */
+int b200moe_rms_norm_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldr, int type, const void* weight, int weight_type,
+                         int64_t rows, int64_t K, float eps, void* y, void* h, void* q, float* scale, int64_t scale_pitch,
+                         b200moe_stream_t stream);
+/* The gradient: of h (of x and of the residual alike) grad_x = the norm's + grad_h (nullable: 0), and of the weight, summed over the rows in
+ * a fixed order; either may be NULL.  h: as the forward had it (x without a residual).  ws: for grad_weight. */
+size_t b200moe_rms_norm_bwd_ws_bytes(int64_t rows, int64_t K);
+int b200moe_rms_norm_bwd(const void* grad_y, const void* grad_h, const void* h, int64_t ldh, int type, const void* weight,
+                         int weight_type, int64_t rows, int64_t K, float eps, void* ws, void* grad_x, void* grad_weight,
+                         b200moe_stream_t stream);
 
 /* ---- combine -------------------------------------------------------------------------------- */
 /* Replaces _combine_scatter_kernel / index_add_ (kernels/sm75/moe.py:673-682, :593-595):

@@ -93,8 +93,13 @@ _SIGNATURES = {
     "b200moe_fp8_block_quant_weight": (c_int, [c_void_p] + [c_int64] * 3 + [c_void_p] * 3),
     "b200moe_fp8_block_linear_ws_bytes": (c_size_t, [c_int64, c_int64]),
     "b200moe_fp8_block_linear": (c_int, [c_void_p] * 3 + [c_int64] * 3 + [c_int] + [c_void_p] * 4),
+    "b200moe_fp8_block_linear_rows": (c_int, [c_void_p] * 2 + [c_int64] + [c_void_p] * 2 + [c_int64] * 3 + [c_void_p] * 3),
     "b200moe_moe_fp8_block_ws_bytes": (c_size_t, [c_int64] * 3 + [c_int] * 2),
     "b200moe_moe_fp8_block_forward": (c_int, [c_void_p] * 7 + [c_int64] * 3 + [c_int] * 2 + [c_void_p] * 4),
+    "b200moe_rms_norm_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int, c_int64, c_int64, c_float] + [c_void_p] * 4 +
+                             [c_int64, c_void_p]),
+    "b200moe_rms_norm_bwd_ws_bytes": (c_size_t, [c_int64, c_int64]),
+    "b200moe_rms_norm_bwd": (c_int, [c_void_p] * 3 + [c_int64, c_int, c_void_p, c_int, c_int64, c_int64, c_float] + [c_void_p] * 4),
     "b200moe_ep_plan": (c_int, [c_void_p, c_int, c_int, c_int] + [c_void_p] * 5 + [c_int64, c_void_p, c_void_p]),
     "b200moe_ep_local_rows": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]),
     "b200moe_ep_publish": (c_int, [c_void_p] * 4 + [c_int64, c_int, c_int, c_int, c_int64, c_int] + [c_void_p] * 5),

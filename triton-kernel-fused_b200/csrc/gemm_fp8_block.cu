@@ -910,8 +910,9 @@ struct BlockCarver {
 // chunks 16.4 / 18.5.
 static bool quant_inside(int64_t mean, int64_t weights) { return mean <= 4 && weights < (32LL << 20); }
 
-// out (M, N) = x (M, K) * w (N, K)^T, or (b_mn) out (M, K') = x (M, N') * w (N', K'): N and K of the params are of the product
-static int block_dense(const void* x, const void* w, const float* sw, int64_t M, int64_t N, int64_t K, int b_mn, void* ws, void* out, int32_t* status,
+// out (M, N) = x (M, K) * w (N, K)^T, or (b_mn) out (M, K') = x (M, N') * w (N', K'): N and K of the params are of the product.  x: bf16 rows that
+// are quantised here, or (x_scale) their codes
+static int block_dense(const void* x, const float* x_scale, int64_t x_pitch, const void* w, const float* sw, int64_t M, int64_t N, int64_t K, int b_mn, void* ws, void* out, int32_t* status,
                        cudaStream_t st) {
   BlockParams bp{};
   bp.g.sched = SCHED_DENSE; bp.g.M = (int)M; bp.g.N = (int)N; bp.g.K = (int)K; bp.g.num_groups = 1;
@@ -923,14 +924,19 @@ static int block_dense(const void* x, const void* w, const float* sw, int64_t M,
   const int nt = b_mn ? 0 : few_dense(M, N, K);
   const int64_t ldq = code_pitch(K);
   BlockCarver c{static_cast<char*>(ws)};
-  uint8_t* q = c.take<uint8_t>(M * ldq);
-  float* sx = c.take<float>(scale_pitch(M) * ceil_div(K, 128));
-  if (nt == 16 && M <= 16) {
+  const void* q = x;
+  if (x_scale != nullptr) {
+    bp.sx = x_scale;
+    bp.sx_pitch = x_pitch;
+  } else if (nt == 16 && M <= 16) {
     bp.x = reinterpret_cast<const __nv_bfloat16*>(x);
   } else {
+    uint8_t* codes = c.take<uint8_t>(M * ldq);
+    float* sx = c.take<float>(scale_pitch(M) * ceil_div(K, 128));
+    q = codes;
     bp.sx = sx;
     bp.sx_pitch = scale_pitch(M);
-    const int rc = fp8_block_quant(x, M, K, M, nullptr, 1, q, ldq, sx, bp.sx_pitch, st);
+    const int rc = fp8_block_quant(x, M, K, M, nullptr, 1, codes, ldq, sx, bp.sx_pitch, st);
     if (rc) return rc;
   }
   OpScope scope("fp8_block_linear", 1);
@@ -1004,7 +1010,20 @@ int b200moe_fp8_block_linear(const void* x, const void* w, const float* w_scale,
   B200_CHECK_ARG(x && w && w_scale && ws && out, B200MOE_E_NULL, "fp8_block_linear: null pointer");
   B200_CHECK_ARG(aligned16(x) && aligned16(w) && aligned16(ws) && aligned16(out), B200MOE_E_ALIGN,
                  "fp8_block_linear: tensors must be 16-byte aligned");
-  return block_dense(x, w, w_scale, M, transposed ? K : N, transposed ? N : K, transposed, ws, out, status, (cudaStream_t)stream);
+  return block_dense(x, nullptr, 0, w, w_scale, M, transposed ? K : N, transposed ? N : K, transposed, ws, out, status, (cudaStream_t)stream);
+}
+
+int b200moe_fp8_block_linear_rows(const void* q, const float* q_scale, int64_t scale_pitch_, const void* w, const float* w_scale, int64_t M, int64_t N,
+                                  int64_t K, void* out, int32_t* status, b200moe_stream_t stream) {
+  int rc = check_linear("fp8_block_linear_rows", M, N, K);
+  if (rc) return rc;
+  if (M == 0) return 0;
+  B200_CHECK_ARG(q && q_scale && w && w_scale && out, B200MOE_E_NULL, "fp8_block_linear_rows: null pointer");
+  B200_CHECK_ARG(scale_pitch_ >= scale_pitch(M) && scale_pitch_ % 4 == 0, B200MOE_E_BAD_SHAPE,
+                 "fp8_block_linear_rows: scales %lld apart, %lld rows rounded up to whole 128 are wanted", (long long)scale_pitch_, (long long)M);
+  B200_CHECK_ARG(aligned16(q) && aligned16(q_scale) && aligned16(w) && aligned16(out), B200MOE_E_ALIGN,
+                 "fp8_block_linear_rows: tensors must be 16-byte aligned");
+  return block_dense(q, q_scale, scale_pitch_, w, w_scale, M, N, K, 0, nullptr, out, status, (cudaStream_t)stream);
 }
 
 size_t b200moe_moe_fp8_block_ws_bytes(int64_t T, int64_t H, int64_t I, int E, int k) {

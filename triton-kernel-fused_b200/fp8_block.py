@@ -91,17 +91,30 @@ def fp8_block_quantize_weight(w):
     return _QuantizeWeight.apply(w.contiguous())
 
 
-def _product(x, w, scale, transposed):
-    """x (M,K) * w (N,K)^T, or x (M,N) * w"""
+def _product(x, w, scale, transposed, q=None, q_scale=None):
+    """x (M,K) * w (N,K)^T, or x (M,N) * w; or q (M,K) codes with q_scale [block][row] * w^T, x being a shape alone"""
     (N, K), M, dev = w.shape, x.shape[0], x.device
     lib = L.lib()
     with L.on_device_of(x):
         out = torch.empty(M, K if transposed else N, dtype=torch.bfloat16, device=dev)
-        if M:
+        if M and q is not None:
+            L.check(lib.b200moe_fp8_block_linear_rows(q.data_ptr(), q_scale.data_ptr(), q_scale.stride(0), w.data_ptr(), scale.data_ptr(), M, N, K,
+                                                      out.data_ptr(), L.status_word(dev).data_ptr(), L.stream_of(q)))
+        elif M:
             ws = L.workspace(lib.b200moe_fp8_block_linear_ws_bytes(M, N if transposed else K), dev)
             L.check(lib.b200moe_fp8_block_linear(x.data_ptr(), w.data_ptr(), scale.data_ptr(), M, N, K, int(transposed), ws.data_ptr(),
                                                  out.data_ptr(), L.status_word(dev).data_ptr(), L.stream_of(x)))
     return out
+
+
+def _scales_by_block(scale):
+    """scales (M, blocks) as the products read them, [block][row] at a pitch of whole 128 rows: as `rms_norm_fp8_block` left them, or a copy"""
+    (M, blocks), pitch = scale.shape, scale.stride(1)
+    rows = -(-M // BLOCK) * BLOCK
+    if ((M == 1 or scale.stride(0) == 1) and pitch % 4 == 0 and pitch >= rows and scale.data_ptr() % 16 == 0
+            and scale.untyped_storage().nbytes() >= 4 * (scale.storage_offset() + (blocks - 1) * pitch + rows)):
+        return scale.t()
+    return scale.new_zeros(blocks, rows)[:, :M].copy_(scale.t())
 
 
 class _Fp8BlockLinear(torch.autograd.Function):
@@ -109,22 +122,28 @@ class _Fp8BlockLinear(torch.autograd.Function):
     calls take its compiled form (csrc/fast.cpp)."""
 
     @staticmethod
-    def forward(ctx, x, w, scale):
-        x, w = _aligned(x), _aligned(w)      # in here: a tracer would keep the choice it saw
+    def forward(ctx, x, w, scale, q=None, q_scale=None):
+        w = _aligned(w)      # in here: a tracer would keep the choice it saw
         ctx.save_for_backward(w, scale)
-        return _product(x, w, scale, False)
+        if q is not None:
+            return _product(q, w, scale, False, _aligned(q), _scales_by_block(q_scale))
+        return _product(_aligned(x), w, scale, False)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         w, scale = ctx.saved_tensors
-        return _product(_aligned(grad.to(torch.bfloat16).contiguous()), w, scale, True), None, None
+        return _product(_aligned(grad.to(torch.bfloat16).contiguous()), w, scale, True), None, None, None, None
 
 
-def fp8_block_linear(x, weight, weight_scale):
+def fp8_block_linear(x, weight, weight_scale, quantized=None):
     """x (..., K) bf16 times weight (N, K) float8_e4m3fn with weight_scale (ceil(N/128), ceil(K/128)) fp32 -> (..., N) bf16.
     N a multiple of 8, K of 16.  Differentiable in x (its gradient is quantised along N); the weights are frozen: one that
-    requires a gradient is refused in grad mode."""
+    requires a gradient is refused in grad mode.
+    quantized: (codes (..., K), scales (..., ceil(K/128))) of x, from `rms_norm_fp8_block` or `fp8_block_quantize`; the product reads these and x is
+    what the gradient goes to, or None where there is none to go."""
+    if quantized is not None:
+        return _linear_of_codes(x, weight, weight_scale, *quantized)
     fast = L.fast() if x.is_cuda else None
     if fast is not None:
         out = fast.fp8_block_linear(x, weight, weight_scale, L.status_word(x.device))
@@ -139,6 +158,27 @@ def fp8_block_linear(x, weight, weight_scale):
     L.require(N % 8 == 0 and K % 16 == 0 and N > 0 and K > 0, f"weight must be (N, K) with N a multiple of 8 and K of 16, got ({N}, {K})")
     out = _Fp8BlockLinear.apply(x.reshape(-1, K).contiguous(), w, scale)
     return out if x.dim() == 2 else out.view(*x.shape[:-1], N)
+
+
+def _linear_of_codes(x, weight, weight_scale, q, q_scale):
+    L.require(q.is_cuda, "codes must be a CUDA tensor (this package has no CPU path)")
+    w, scale = _weight("weight", weight, weight_scale, q.device, 2)
+    N, K = w.shape
+    L.require(N % 8 == 0 and K % 16 == 0 and N > 0 and K > 0, f"weight must be (N, K) with N a multiple of 8 and K of 16, got ({N}, {K})")
+    L.require(q.dtype == torch.float8_e4m3fn and q.dim() >= 1 and q.shape[-1] == K, f"codes must be float8_e4m3fn (..., {K}), got {q.dtype} "
+              f"{tuple(q.shape)}")
+    want = (*q.shape[:-1], _blocks(K))
+    L.require(q_scale.device == q.device and q_scale.dtype == torch.float32 and tuple(q_scale.shape) == want, f"their scales must be float32 {want} "
+              f"on their device, got {q_scale.dtype} {tuple(q_scale.shape)}")
+    L.require(not (torch.is_grad_enabled() and (q.requires_grad or q_scale.requires_grad)), "codes and their scales take no gradient, x does")
+    if x is not None:
+        if torch.is_autocast_enabled("cuda") and x.is_floating_point():
+            x = x.to(torch.get_autocast_dtype("cuda"))
+        L.require_cuda_bf16("x", x)
+        L.require(x.device == q.device and x.shape == q.shape, f"x must have its codes' shape {tuple(q.shape)}, got {tuple(x.shape)}")
+        x = x.reshape(-1, K)
+    out = _Fp8BlockLinear.apply(x, w, scale, q.reshape(-1, K).contiguous(), q_scale.reshape(-1, _blocks(K)))
+    return out if q.dim() == 2 else out.view(*q.shape[:-1], N)
 
 
 class _Experts(_Frozen):
