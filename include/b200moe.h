@@ -394,6 +394,23 @@ int b200moe_rms_norm_bwd(const void* grad_y, const void* grad_h, const void* h, 
                          int weight_type, int64_t rows, int64_t K, float eps, void* ws, void* grad_x, void* grad_weight,
                          b200moe_stream_t stream);
 
+/* ---- low-rank adapters (no counterpart in the reference) -----------------------------------------
+ * out[t] = base[t] + s_l (x[t] A_l^T) B_l^T with l = index[t]: x (T,K), a (L,R,K), b (L,N,R), base (T,N, nullable: 0) and out (T,N) bf16, rows of x
+ * and base ldx / ldb elements apart (multiples of 8); index int32 or int64 (index_bytes 4 or 8), NULL: adapter 0 for every row; a negative one
+ * names none, one of L or more too and raises status 9.  s_l = scales[l], or scale where scales is NULL.  K and N multiples of 8, R of 8 up to
+ * 128, L up to 65536; tensors 16-byte aligned.  x A^T is rounded to bf16 where there are more than a few rows or keep is set; sums are fp32.
+ * keep: a backward follows, which reads ws. */
+size_t b200moe_lora_fwd_ws_bytes(int64_t T, int64_t R, int64_t L, int keep);
+int b200moe_lora_forward(const void* x, int64_t ldx, const void* a, const void* b, const void* index, int index_bytes, const float* scales,
+                         float scale, const void* base, int64_t ldb, int64_t T, int64_t K, int64_t N, int64_t R, int64_t L, int keep,
+                         void* ws, void* out, int32_t* status, b200moe_stream_t stream);
+/* grad_x (T,K) bf16, grad_a (L,R,K) and grad_b (L,N,R) bf16 or (grad_f32) fp32, each nullable, from grad_out (T,N) bf16; sums over rows in a
+ * fixed order, adapters without a row get zeros.  has_index: the forward had one.  fwd_ws: the forward's, made with keep. */
+size_t b200moe_lora_bwd_ws_bytes(int64_t T, int64_t K, int64_t N, int64_t R, int64_t L);
+int b200moe_lora_backward(const void* grad_out, const void* x, int64_t ldx, const void* a, const void* b, int has_index, const float* scales,
+                          float scale, int64_t T, int64_t K, int64_t N, int64_t R, int64_t L, const void* fwd_ws, void* ws, void* grad_x,
+                          void* grad_a, void* grad_b, int grad_f32, int32_t* status, b200moe_stream_t stream);
+
 /* ---- combine -------------------------------------------------------------------------------- */
 /* Replaces _combine_scatter_kernel / index_add_ (kernels/sm75/moe.py:673-682, :593-595):
  * out[t] = sum_j w[t,j] * rows[slot_row[t*k+j]], fp32 accumulate in slot order, bf16 store.

@@ -100,6 +100,12 @@ _SIGNATURES = {
                              [c_int64, c_void_p]),
     "b200moe_rms_norm_bwd_ws_bytes": (c_size_t, [c_int64, c_int64]),
     "b200moe_rms_norm_bwd": (c_int, [c_void_p] * 3 + [c_int64, c_int, c_void_p, c_int, c_int64, c_int64, c_float] + [c_void_p] * 4),
+    "b200moe_lora_fwd_ws_bytes": (c_size_t, [c_int64] * 3 + [c_int]),
+    "b200moe_lora_forward": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_float, c_void_p, c_int64] + [c_int64] * 5 +
+                             [c_int] + [c_void_p] * 4),
+    "b200moe_lora_bwd_ws_bytes": (c_size_t, [c_int64] * 5),
+    "b200moe_lora_backward": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_float] + [c_int64] * 5 + [c_void_p] * 5 +
+                              [c_int, c_void_p, c_void_p]),
     "b200moe_ep_plan": (c_int, [c_void_p, c_int, c_int, c_int] + [c_void_p] * 5 + [c_int64, c_void_p, c_void_p]),
     "b200moe_ep_local_rows": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]),
     "b200moe_ep_publish": (c_int, [c_void_p] * 4 + [c_int64, c_int, c_int, c_int, c_int64, c_int] + [c_void_p] * 5),

@@ -416,6 +416,15 @@ static EncodeTiledFn get_encode_fn() {
   return fn;
 }
 
+// A thread that has made no CUDA call yet (one of the autograd engine's, whose memory came from a cache) has no context, which the encoder wants
+template <class... A>
+static CUresult encode_tiled(EncodeTiledFn fn, A... a) {
+  CUresult r = fn(a...);
+  int device;
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess) r = fn(a...);
+  return r;
+}
+
 // bf16 (or byte) tensor seen as dims {inner, outer, groups}; strides in elements; 128B (or 64B) swizzle; zero OOB fill.
 static int make_map(CUtensorMap* tm, const void* base, uint64_t inner, uint64_t outer, uint64_t groups,
                     uint64_t outer_stride, uint64_t group_stride, uint32_t box_inner, uint32_t box_outer,
@@ -430,7 +439,7 @@ static int make_map(CUtensorMap* tm, const void* base, uint64_t inner, uint64_t 
   cuuint64_t strides[2] = {outer_stride * elem_bytes, group_stride * elem_bytes};
   cuuint32_t box[3] = {box_inner, box_outer, 1};
   cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = fn(tm, elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+  CUresult r = encode_tiled(fn, tm, elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE,
                   swizzle_bytes == 0 ? CU_TENSOR_MAP_SWIZZLE_NONE : swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -452,7 +461,7 @@ static inline int make_map_gate_up(CUtensorMap* tm, const void* base, uint64_t K
   cuuint64_t strides[4] = {K * 2, I * K * 2, 16 * K, 4 * I * K};
   cuuint32_t box[5] = {64, 8, 2, groups, 1};
   cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-  CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dims, strides, box, estr,
+  CUresult r = encode_tiled(fn, tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   B200_CHECK_ARG(r == CUDA_SUCCESS, B200MOE_E_CUDA, "cuTensorMapEncodeTiled failed (%d): gate|up stack of %llu x %llu x %llu", (int)r,

@@ -1,0 +1,1038 @@
+// Low-rank adapters of many requests beside a shared projection: row t of x has the adapter l = index[t], or none,
+//
+//   v[t] = s_l x[t] A_l^T          out[t] = base[t] + v[t] B_l^T           A (L,R,K), B (L,N,R)
+//
+// and backward   u[t] = s_l g[t] B_l,   grad_x[t] = u[t] A_l,   grad_A_l = sum_t u[t]^T x[t],   grad_B_l = sum_t g[t]^T v[t].
+//
+// Four products with one short side (R of at most 128), all bound by HBM: `shrink` (T,D) -> (T,R) reads x or g, `expand` (T,R) -> (T,D) reads
+// base and writes out or grad_x, `wgrad` reads x or g again.  Each is a tcgen05 kernel over tiles of 128 rows as they come, without sorting
+// them: a tile's distinct adapters are found on the way, each is multiplied with all rows of the tile into tensor memory of its own, and a
+// row takes the result of its adapter.  Rows of other adapters are never added to it, not even times zero, so an infinity or a NaN stays with
+// its own adapter or row.  Few rows (a decoding batch) run in one kernel of their own, a cluster a row.
+//
+// v and u are rounded to bf16, the operands' type, between the two products: 2^-9 of their size, as the result itself is rounded.  All sums are fp32.
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "gemm_common.cuh"
+
+namespace b200moe {
+
+constexpr int kLTile = 128;                      // rows of a tile
+constexpr int kLBox = 128 * 64 * 2;              // 128 rows x 64 values, 128-byte swizzle
+
+struct LoraIndex {
+  const void* index;      // T adapters, or nullptr: adapter 0 for every row
+  int bytes;              // of one: 4 or 8
+  int T, L;
+  int* status;
+};
+
+// A tile's adapters, found by all threads of the CTA: row -> slot (-1: none), slot -> adapter
+struct LoraSlots {
+  int of_row[kLTile];
+  int adapter[kLTile];
+  int slot[kLTile];
+  int warps[4];
+  int n;
+};
+
+__device__ __forceinline__ int lora_adapter(const LoraIndex& p, long long t) {
+  if (t >= p.T) return -1;
+  if (p.index == nullptr) return 0;
+  const long long l = p.bytes == 8 ? static_cast<const long long*>(p.index)[t] : static_cast<const int*>(p.index)[t];
+  if (l >= p.L) {
+    *p.status = ST_BAD_ADAPTER_INDEX;
+    return -1;
+  }
+  return l < 0 ? -1 : static_cast<int>(l);
+}
+
+// barriers inside: every thread of the CTA calls it
+__device__ __forceinline__ void lora_slots(const LoraIndex& p, int tile, LoraSlots& s) {
+  const int t = threadIdx.x;
+  int l = -1, at = -1;
+  if (t < kLTile) {
+    l = lora_adapter(p, static_cast<long long>(tile) * kLTile + t);
+    s.of_row[t] = l;
+  }
+  __syncthreads();
+  bool first = false;
+  unsigned firsts = 0;
+  if (t < kLTile) {
+    if (l >= 0) {
+      at = t;
+      for (int j = 0; j < t; ++j)
+        if (s.of_row[j] == l) {
+          at = j;
+          break;
+        }
+    }
+    first = l >= 0 && at == t;
+    firsts = __ballot_sync(0xffffffffu, first);
+    if ((t & 31) == 0) s.warps[t >> 5] = __popc(firsts);
+  }
+  __syncthreads();
+  if (t < kLTile && first) {
+    int n = __popc(firsts & ((1u << (t & 31)) - 1u));
+    for (int w = 0; w < (t >> 5); ++w) n += s.warps[w];
+    s.slot[t] = n;
+    s.adapter[n] = l;
+  }
+  if (t == 0) s.n = s.warps[0] + s.warps[1] + s.warps[2] + s.warps[3];
+  __syncthreads();
+  if (t < kLTile && !first) s.slot[t] = l >= 0 ? s.slot[at] : -1;
+  __syncthreads();
+}
+
+// columns of tensor memory -> registers, 32 or 16 at a time
+template <int N>
+__device__ __forceinline__ void lora_fetch(uint32_t taddr, bool mine, float (&v)[N]) {
+#pragma unroll
+  for (int c = 0; c < N; c += 16) {
+    uint32_t r[16];
+    tmem_ld16(taddr + c, r);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[c + i] = mine ? __uint_as_float(r[i]) : v[c + i];
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ shrink
+// v[t, r] = s_l sum_d X[t, d] W_l[r, d].  A cluster of `split` CTAs shares a tile's columns d and adds up its partial sums through distributed
+// shared memory.  WMN: W_l lies (D, R), reduction index first (the backward's B).  As many adapters as fit 128 accumulator columns a pass.
+constexpr int kShrinkStages = 3, kShrinkStage = 2 * kLBox, kShrinkThreads = 192;
+constexpr int kShrinkSmem = kShrinkStages * kShrinkStage + (2 * kShrinkStages + 2) * 8 + 16 + 1024;
+
+struct ShrinkParams {
+  LoraIndex ix;
+  int D, R, split;
+  const float* scales;       // (L,), or nullptr: `scale` for all
+  float scale;
+  __nv_bfloat16* v;          // (T, RP)
+  int* rows;                 // nullable: the rows' adapters as wgrad reads them
+  unsigned char* present;    // nullable: (tiles, L), bit h: rows of the tile's half h have the adapter
+};
+
+template <int RP, bool WMN>
+__global__ void __launch_bounds__(kShrinkThreads)
+lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const ShrinkParams p) {
+  constexpr int NB = WMN && RP < 64 ? 64 : RP;       // accumulator columns of an adapter: whole swizzle atoms where W is MN-major
+  constexpr int SLOTS = 128 / NB;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kShrinkStages * kShrinkStage);
+  const uint32_t bar_full = smem_u32(bars), bar_empty = smem_u32(bars + kShrinkStages);
+  const uint32_t bar_tfull = smem_u32(bars + 2 * kShrinkStages), bar_tempty = bar_tfull + 8;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kShrinkStages + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  __shared__ LoraSlots slots;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = p.split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int tile = blockIdx.x / p.split;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kShrinkStages; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    mbar_init(bar_tfull, 1);
+    mbar_init(bar_tempty, 4);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmX);
+    tma_prefetch_desc(&tmW);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), 128);
+    tmem_relinquish();
+  }
+  grid_dep_wait();
+  tc_fence_before();
+  lora_slots(p.ix, tile, slots);
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int nkb = (p.D + 63) / 64;
+  const int kb0 = static_cast<int>(static_cast<long long>(rank) * nkb / p.split), kb1 = static_cast<int>(static_cast<long long>(rank + 1) * nkb / p.split);
+  const int passes = (slots.n + SLOTS - 1) / SLOTS;
+  float v[RP];
+#pragma unroll
+  for (int i = 0; i < RP; ++i) v[i] = 0.0f;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int pass = 0; pass < passes && ok; ++pass) {
+        const int first = pass * SLOTS, n = min(SLOTS, slots.n - first);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, ST_WAIT_PRODUCER)) {
+            ok = false;
+            break;
+          }
+          const uint32_t full = bar_full + 8 * s, sx = smem_u32(smem + s * kShrinkStage), sw = sx + kLBox;
+          mbar_arrive_expect_tx(full, kLBox + n * NB * 128);
+          tma_load_3d(sx, &tmX, full, kb * 64, tile * kLTile, 0);
+          for (int j = 0; j < n; ++j) {
+            const int l = slots.adapter[first + j];
+            if constexpr (WMN) {
+#pragma unroll
+              for (int h = 0; h < NB / 64; ++h) tma_load_3d(sw + (j * (NB / 64) + h) * 8192, &tmW, full, 64 * h, kb * 64, l);
+            } else {
+              tma_load_3d(sw + j * NB * 128, &tmW, full, kb * 64, 0, l);
+            }
+          }
+          if (++s == kShrinkStages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+    }
+    grid_dep_launch();
+  } else if (warp == 1) {
+    if (elect_one()) {
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int pass = 0; pass < passes && ok; ++pass) {
+        const int n = min(SLOTS, slots.n - pass * SLOTS);
+        const uint32_t idesc = umma_idesc_bf16(n * NB, 0, WMN);
+        if (!mbar_wait(bar_tempty, (pass & 1) ^ 1, abort_flag, ST_WAIT_MMA_TMEM)) break;
+        tc_fence_after();
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(bar_full + 8 * s, ph, abort_flag, ST_WAIT_MMA_FULL)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sx = smem_u32(smem + s * kShrinkStage), sw = sx + kLBox;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_bf16(tmem, umma_desc_sw128(sx + 32 * k, 0, 1024), umma_desc_sw128(sw + (WMN ? 2048 : 32) * k, WMN ? 8192 : 0, 1024), idesc,
+                      kb != kb0 || k != 0);
+          umma_commit(bar_empty + 8 * s);
+          if (++s == kShrinkStages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+        if (ok) umma_commit(bar_tfull);
+      }
+    }
+  } else {
+    const int q = warp & 3, row = 32 * q + lane, mine = slots.slot[row];
+    const uint32_t taddr = tmem + (static_cast<uint32_t>(32 * q) << 16);
+    bool ok = true;
+    for (int pass = 0; pass < passes; ++pass) {
+      ok = ok && mbar_wait(bar_tfull, pass & 1, abort_flag, ST_WAIT_EPILOGUE);
+      __syncwarp();
+      tc_fence_after();
+      if (kb1 > kb0)
+        for (int j = 0; j < min(SLOTS, slots.n - pass * SLOTS); ++j) {
+          const bool me = mine == pass * SLOTS + j;
+          if (__any_sync(0xffffffffu, me)) lora_fetch<RP>(taddr + j * NB, me, v);
+        }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_tempty);
+    }
+    const long long t = static_cast<long long>(tile) * kLTile + row;
+    if (p.rows != nullptr && rank == 0 && t < p.ix.T) p.rows[t] = slots.of_row[row];
+    if (p.split == 1) {
+      const float s = mine < 0 ? 0.0f : p.scales != nullptr ? p.scales[slots.adapter[mine]] : p.scale;
+      if (t < p.ix.T) {
+#pragma unroll
+        for (int i = 0; i < RP; i += 8) {
+          uint32_t o[4];
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
+            o[h] = mine >= 0 && i < p.R ? pack_bf16x2(s * v[i + 2 * h], s * v[i + 2 * h + 1]) : 0u;      // R a multiple of 8
+          *reinterpret_cast<uint4*>(p.v + t * RP + i) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+      }
+    } else {      // every load of this CTA has been used: its stages are free
+      float* mine_s = reinterpret_cast<float*>(smem) + row * (RP + 1);
+#pragma unroll
+      for (int i = 0; i < RP; ++i) mine_s[i] = v[i];
+    }
+  }
+  __syncwarp();
+  if (p.present != nullptr && rank == 0)
+    for (int l = threadIdx.x; l < p.ix.L; l += kShrinkThreads) {
+      unsigned bits = 0;
+      for (int r = 0; r < kLTile; ++r) bits |= slots.of_row[r] == l ? 1u << (r >> 6) : 0u;
+      p.present[static_cast<long long>(tile) * p.ix.L + l] = static_cast<unsigned char>(bits);
+    }
+  if (p.split > 1) {
+    __syncwarp();
+    cluster_sync_all();
+    const int rows = kLTile / p.split;
+    for (int i = threadIdx.x; i < rows * (RP / 2); i += kShrinkThreads) {
+      const int row = rank * rows + i / (RP / 2), c = 2 * (i % (RP / 2)), mine = slots.slot[row];
+      const long long t = static_cast<long long>(tile) * kLTile + row;
+      float a = 0.0f, b = 0.0f;
+      for (int r = 0; r < p.split; ++r) {
+        const uint32_t at = mapa_shared(smem_u32(smem) + 4 * (row * (RP + 1) + c), r);
+        float a1, b1;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(a1) : "r"(at) : "memory");
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(b1) : "r"(at + 4) : "memory");
+        a += a1;
+        b += b1;
+      }
+      const float s = mine < 0 ? 0.0f : p.scales != nullptr ? p.scales[slots.adapter[mine]] : p.scale;
+      if (t < p.ix.T) *reinterpret_cast<uint32_t*>(p.v + t * RP + c) = mine >= 0 && c < p.R ? pack_bf16x2(s * a, s * b) : 0u;
+    }
+    __syncwarp();
+    cluster_sync_all();      // nobody leaves while another reads its sums
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, 128);
+  if (threadIdx.x == 0 && *abort_flag != 0) *p.ix.status = *abort_flag;
+}
+
+// ------------------------------------------------------------------------------------------------ expand
+// out[t, n] = base[t, n] + sum_r v[t, r] W_l[n, r]; WMN: W_l lies (R, N) (the backward's A).  Persistent CTAs over (row tile, 128 columns), a row
+// tile's columns one after another.  The base's boxes land where the result leaves from; tensor memory holds four (columns, adapter) products.
+constexpr int kExpEpi = 8, kExpThreads = 64 + 32 * kExpEpi, kExpBase = 3;
+constexpr int kExpOut = 128 * 128 * 2;
+template <int RP> constexpr int kExpW = (RP > 64 ? 2 : 1) * kLBox;               // one adapter's 128 columns
+template <int RP> constexpr int kExpWStages = RP > 64 ? 2 : 3;
+template <int RP> constexpr int kExpSmem = kExpBase * kExpOut + (kExpWStages<RP> + 1) * kExpW<RP> + (2 * kExpBase + 2 * kExpWStages<RP> + 9) * 8 + 16 + 1024;
+
+struct ExpandParams {
+  LoraIndex ix;
+  int N, has_base, per_cta;
+};
+
+template <int RP, bool WMN>
+__global__ void __launch_bounds__(kExpThreads, 1)
+lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmBase,
+                   const __grid_constant__ CUtensorMap tmOut, const ExpandParams p) {
+  constexpr int WS = kExpWStages<RP>, W = kExpW<RP>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t *s_w = smem + kExpBase * kExpOut, *s_v = s_w + WS * W;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_v + W);
+  const uint32_t bar_bfull = smem_u32(bars), bar_bempty = bar_bfull + 8 * kExpBase;
+  const uint32_t bar_wfull = bar_bempty + 8 * kExpBase, bar_wempty = bar_wfull + 8 * WS;
+  const uint32_t bar_tfull = bar_wempty + 8 * WS, bar_tempty = bar_tfull + 32, bar_v = bar_tempty + 32;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kExpBase + 2 * WS + 9);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  __shared__ LoraSlots slots;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kExpBase; ++s) {
+      mbar_init(bar_bfull + 8 * s, 1);
+      mbar_init(bar_bempty + 8 * s, kExpEpi);
+    }
+    for (int s = 0; s < WS; ++s) {
+      mbar_init(bar_wfull + 8 * s, 1);
+      mbar_init(bar_wempty + 8 * s, 1);
+    }
+    for (int b = 0; b < 4; ++b) {
+      mbar_init(bar_tfull + 8 * b, 1);
+      mbar_init(bar_tempty + 8 * b, kExpEpi);
+    }
+    mbar_init(bar_v, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmV);
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmBase);
+    tma_prefetch_desc(&tmOut);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  grid_dep_wait();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int nct = (p.N + 127) / 128;
+  const long long total = static_cast<long long>((p.ix.T + kLTile - 1) / kLTile) * nct;
+  long long item = static_cast<long long>(blockIdx.x) * p.per_cta;
+  const long long end = min(total, item + p.per_cta);
+  int bs = 0, ws = 0, buf = 0;                       // places in the rings, their phases
+  uint32_t bph = 0, wph = 0, tph = 0, vph = 0;
+  bool ok = true;
+  while (item < end) {
+    const int tile = static_cast<int>(item / nct), ct0 = static_cast<int>(item - static_cast<long long>(tile) * nct);
+    const int ct1 = static_cast<int>(min(static_cast<long long>(nct), ct0 + (end - item)));
+    item += ct1 - ct0;
+    lora_slots(p.ix, tile, slots);
+    const int n = slots.n;
+    if (warp == 0) {
+      if (elect_one()) {
+        if (n > 0) {
+          mbar_arrive_expect_tx(bar_v, W);
+          for (int h = 0; h < W / kLBox; ++h) tma_load_3d(smem_u32(s_v) + h * kLBox, &tmV, bar_v, 64 * h, tile * kLTile, 0);
+        }
+        for (int ct = ct0; ct < ct1 && ok; ++ct) {
+          if (p.has_base) {
+            ok = mbar_wait(bar_bempty + 8 * bs, bph ^ 1, abort_flag, ST_WAIT_PRODUCER);
+            if (!ok) break;
+            const uint32_t full = bar_bfull + 8 * bs, to = smem_u32(smem + bs * kExpOut);
+            mbar_arrive_expect_tx(full, kExpOut);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) tma_load_3d(to + i * 4096, &tmBase, full, ct * 128 + 64 * (i >> 2), tile * kLTile + 32 * (i & 3), 0);
+            if (++bs == kExpBase) {
+              bs = 0;
+              bph ^= 1;
+            }
+          }
+          for (int j = 0; j < n; ++j) {
+            ok = mbar_wait(bar_wempty + 8 * ws, wph ^ 1, abort_flag, ST_WAIT_PRODUCER);
+            if (!ok) break;
+            const uint32_t full = bar_wfull + 8 * ws, to = smem_u32(s_w + ws * W);
+            const int l = slots.adapter[j];
+            if constexpr (WMN) {      // RP rows of 64 columns each
+              mbar_arrive_expect_tx(full, 2 * RP * 128);
+              tma_load_3d(to, &tmW, full, ct * 128, 0, l);
+              tma_load_3d(to + RP * 128, &tmW, full, ct * 128 + 64, 0, l);
+            } else {
+              mbar_arrive_expect_tx(full, W);
+              for (int h = 0; h < W / kLBox; ++h) tma_load_3d(to + h * kLBox, &tmW, full, 64 * h, ct * 128, l);
+            }
+            if (++ws == WS) {
+              ws = 0;
+              wph ^= 1;
+            }
+          }
+        }
+      }
+    } else if (warp == 1) {
+      if (elect_one()) {
+        constexpr uint32_t idesc = umma_idesc_bf16(128, 0, WMN);
+        if (n > 0) {
+          ok = ok && mbar_wait(bar_v, vph, abort_flag, ST_WAIT_MMA_FULL);
+          vph ^= 1;
+        }
+        const uint32_t sv = smem_u32(s_v);
+        for (int i = 0; i < (ct1 - ct0) * n && ok; ++i) {
+          ok = mbar_wait(bar_tempty + 8 * buf, tph ^ 1, abort_flag, ST_WAIT_MMA_TMEM) &&
+               mbar_wait(bar_wfull + 8 * ws, wph, abort_flag, ST_WAIT_MMA_FULL);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sw = smem_u32(s_w + ws * W);
+#pragma unroll
+          for (int k = 0; k < RP / 16; ++k)
+            umma_bf16(tmem + 128 * buf, umma_desc_sw128(sv + (k >> 2) * kLBox + 32 * (k & 3), 0, 1024),
+                      WMN ? umma_desc_sw128(sw + 2048 * k, RP * 128, 1024) : umma_desc_sw128(sw + (k >> 2) * kLBox + 32 * (k & 3), 0, 1024), idesc,
+                      k != 0);
+          umma_commit(bar_wempty + 8 * ws);
+          umma_commit(bar_tfull + 8 * buf);
+          if (++ws == WS) {
+            ws = 0;
+            wph ^= 1;
+          }
+          if (++buf == 4) {
+            buf = 0;
+            tph ^= 1;
+          }
+        }
+      }
+    } else {
+      const int q = warp & 3, part = (warp - 2) >> 2, mine = slots.slot[32 * q + lane];
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(32 * q) << 16) + 64 * part;
+      for (int ct = ct0; ct < ct1; ++ct) {
+        float acc[64];
+#pragma unroll
+        for (int i = 0; i < 64; ++i) acc[i] = 0.0f;
+        for (int j = 0; j < n; ++j) {
+          ok = ok && mbar_wait(bar_tfull + 8 * buf, tph, abort_flag, ST_WAIT_EPILOGUE);
+          __syncwarp();
+          tc_fence_after();
+          if (__any_sync(0xffffffffu, mine == j)) lora_fetch<64>(taddr + 128 * buf, mine == j, acc);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_tempty + 8 * buf);
+          if (++buf == 4) {
+            buf = 0;
+            tph ^= 1;
+          }
+        }
+        uint8_t* box = smem + bs * kExpOut + (4 * part + q) * 4096;
+        if (p.has_base) ok = ok && mbar_wait(bar_bfull + 8 * bs, bph, abort_flag, ST_WAIT_EPILOGUE);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!p.has_base) {       // the box's result of three tiles ago has left
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kExpBase - 1) : "memory");
+          __syncwarp();
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint4* at = reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4));
+          uint32_t w[4] = {0u, 0u, 0u, 0u};
+          if (p.has_base) {
+            const uint4 b = *at;
+            w[0] = b.x; w[1] = b.y; w[2] = b.z; w[3] = b.w;
+          }
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const float2 f = unpack_bf16x2(w[h]);
+            w[h] = pack_bf16x2(f.x + acc[8 * j + 2 * h], f.y + acc[8 * j + 2 * h + 1]);
+          }
+          *at = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (ok && ct * 128 + 64 * part < p.N && tile * kLTile + 32 * q < p.ix.T) tma_store_3d(&tmOut, smem_u32(box), ct * 128 + 64 * part, tile * kLTile + 32 * q, 0);
+          bulk_commit_group();
+          if (p.has_base) {
+            bulk_wait_read_all();
+            mbar_arrive(bar_bempty + 8 * bs);
+          }
+        }
+        if (++bs == kExpBase) {
+          bs = 0;
+          bph ^= 1;
+        }
+      }
+    }
+    __syncwarp();
+    __syncthreads();       // the slots are made anew
+  }
+  grid_dep_launch();
+  if (warp >= 2 && lane == 0) bulk_wait_all();
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+  if (threadIdx.x == 0 && *abort_flag != 0) *p.ix.status = *abort_flag;
+}
+
+// ------------------------------------------------------------------------------------------------ gradients of the factors
+// P_l[d, r] = sum over the rows t of adapter l of Y[t, d] V[t, r].  A CTA: one adapter, 128 columns d, a share of the rows in blocks of 64, of
+// which it visits those that have the adapter.  Rows of others in such a block are set to zero in shared memory, in both operands.
+constexpr int kWgThreads = 192, kWgWords = 2048;       // blocks of one CTA as bits: 32 kWgWords of them
+template <int RP> constexpr int kWgV = (RP > 64 ? 2 : 1) * 8192;
+template <int RP> constexpr int kWgStages = RP > 64 ? 3 : 4;
+template <int RP> constexpr int kWgSmem = kWgStages<RP> * (kLBox + kWgV<RP>) + (3 * kWgStages<RP> + 1) * 8 + 16 + 1024;
+
+struct WgradParams {
+  int T, D, R, L, splits, transposed;      // transposed: P is (R, D), else (D, R)
+  const int* rows;                         // nullptr: all of them are adapter 0's
+  const unsigned char* present;
+  void* out;                               // (splits, L, ...) fp32; one split: the gradient itself
+  int out_f32;
+  int* status;
+};
+
+template <int RP>
+__global__ void __launch_bounds__(kWgThreads)
+lora_wgrad_kernel(const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmV, const WgradParams p) {
+  constexpr int NB = RP < 64 ? 64 : RP, ST = kWgStages<RP>, STAGE = kLBox + kWgV<RP>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + ST * STAGE);
+  const uint32_t bar_full = smem_u32(bars), bar_ready = bar_full + 8 * ST, bar_empty = bar_ready + 8 * ST, bar_tfull = bar_empty + 8 * ST;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * ST + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  __shared__ unsigned live[kWgWords];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int chunks = (p.D + 127) / 128;
+  const int chunk = blockIdx.x % chunks, l = blockIdx.x / chunks % p.L, split = blockIdx.x / chunks / p.L;
+  const int blocks = (p.T + 63) / 64;
+  const int b0 = static_cast<int>(static_cast<long long>(split) * blocks / p.splits), b1 = static_cast<int>(static_cast<long long>(split + 1) * blocks / p.splits);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_ready + 8 * s, 4);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    mbar_init(bar_tfull, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmY);
+    tma_prefetch_desc(&tmV);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), NB);
+    tmem_relinquish();
+  }
+  grid_dep_wait();
+  bool any = false;
+  for (int w = warp; w * 32 < b1 - b0; w += kWgThreads / 32) {
+    const int b = b0 + 32 * w + lane;
+    const bool has = b < b1 && (p.present == nullptr || (p.present[static_cast<long long>(b >> 1) * p.L + l] >> (b & 1) & 1) != 0);
+    const unsigned m = __ballot_sync(0xffffffffu, has);
+    if (lane == 0) live[w] = m;
+    any = any || m != 0;
+  }
+  tc_fence_before();
+  any = __syncthreads_or(any);
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int words = (b1 - b0 + 31) / 32;
+  // f(block) for each that has the adapter, in order, until it says no
+  auto each = [&](auto f) {
+    for (int w = 0; w < words; ++w)
+      for (unsigned m = live[w]; m != 0; m &= m - 1)
+        if (!f(b0 + 32 * w + __ffs(m) - 1)) return;
+  };
+  if (warp == 0) {
+    if (elect_one()) {
+      int s = 0;
+      uint32_t ph = 0;
+      each([&](int b) {
+        if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, ST_WAIT_PRODUCER)) return false;
+        const uint32_t full = bar_full + 8 * s, sy = smem_u32(smem + s * STAGE);
+        mbar_arrive_expect_tx(full, STAGE);
+        tma_load_3d(sy, &tmY, full, chunk * 128, 64 * b, 0);
+        tma_load_3d(sy + 8192, &tmY, full, chunk * 128 + 64, 64 * b, 0);
+        for (int h = 0; h < NB / 64; ++h) tma_load_3d(sy + kLBox + 8192 * h, &tmV, full, 64 * h, 64 * b, 0);
+        if (++s == ST) {
+          s = 0;
+          ph ^= 1;
+        }
+        return true;
+      });
+    }
+    grid_dep_launch();
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t idesc = umma_idesc_bf16(NB, 1, 1);
+      int s = 0;
+      uint32_t ph = 0, more = 0;
+      bool ok = true;
+      each([&](int) {
+        ok = mbar_wait(bar_ready + 8 * s, ph, abort_flag, ST_WAIT_MMA_FULL);
+        if (!ok) return false;
+        tc_fence_after();
+        const uint32_t sy = smem_u32(smem + s * STAGE), sv = sy + kLBox;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          umma_bf16(tmem, umma_desc_sw128(sy + 2048 * k, 8192, 1024), umma_desc_sw128(sv + 2048 * k, 8192, 1024), idesc, more);
+          more = 1;
+        }
+        umma_commit(bar_empty + 8 * s);
+        if (++s == ST) {
+          s = 0;
+          ph ^= 1;
+        }
+        return true;
+      });
+      if (ok && any) umma_commit(bar_tfull);
+    }
+  } else {
+    const int q = warp & 3;
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    each([&](int b) {
+      unsigned bad0 = 0, bad1 = 0;
+      if (p.rows != nullptr) {      // rows past the last one are zero already
+        const int t = 64 * b + lane;
+        bad0 = __ballot_sync(0xffffffffu, t < p.T && p.rows[min(t, p.T - 1)] != l);
+        bad1 = __ballot_sync(0xffffffffu, t + 32 < p.T && p.rows[min(t + 32, p.T - 1)] != l);
+      }
+      ok = ok && mbar_wait(bar_full + 8 * s, ph, abort_flag, ST_WAIT_MMA_FULL);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return false;
+      if ((bad0 | bad1) != 0) {
+        uint8_t* sy = smem + s * STAGE;
+        for (int r = q; r < 64; r += 4)
+          if (((r < 32 ? bad0 : bad1) >> (r & 31) & 1) != 0)
+            for (int c = lane; c < STAGE / 1024; c += 32)       // 16 bytes of a row: eight a box
+              *reinterpret_cast<uint4*>(sy + (c >> 3) * 8192 + r * 128 + 16 * (c & 7)) = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async_smem();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_ready + 8 * s);
+      if (++s == ST) {
+        s = 0;
+        ph ^= 1;
+      }
+      return true;
+    });
+    if (any) ok = ok && mbar_wait(bar_tfull, 0, abort_flag, ST_WAIT_EPILOGUE);
+    __syncwarp();
+    tc_fence_after();
+    const uint32_t taddr = tmem + (static_cast<uint32_t>(32 * q) << 16);
+    const int d = chunk * 128 + 32 * q + lane;
+    const long long at = (static_cast<long long>(split) * p.L + l) * p.D * p.R;
+#pragma unroll
+    for (int c = 0; c < RP; c += 16) {
+      float v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+      if (any) lora_fetch<16>(taddr + c, true, v);
+      if (d < p.D) {
+        if (p.transposed) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (c + i < p.R) {
+              const long long o = at + static_cast<long long>(c + i) * p.D + d;
+              if (p.out_f32) static_cast<float*>(p.out)[o] = v[i];
+              else static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(v[i]);
+            }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; i += 8)
+            if (c + i < p.R) {
+              const long long o = at + static_cast<long long>(d) * p.R + c + i;
+              if (p.out_f32) {
+                float4* to = reinterpret_cast<float4*>(static_cast<float*>(p.out) + o);
+                to[0] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                to[1] = make_float4(v[i + 4], v[i + 5], v[i + 6], v[i + 7]);
+              } else {
+                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + o) =
+                    make_uint4(pack_bf16x2(v[i], v[i + 1]), pack_bf16x2(v[i + 2], v[i + 3]), pack_bf16x2(v[i + 4], v[i + 5]), pack_bf16x2(v[i + 6], v[i + 7]));
+              }
+            }
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, NB);
+  if (threadIdx.x == 0 && *abort_flag != 0) *p.status = *abort_flag;
+}
+
+// the sum of the splits' shares, n values (a multiple of 4)
+__global__ void __launch_bounds__(256) lora_wgrad_sum_kernel(const float* part, int splits, long long n, void* out, int out_f32) {
+  grid_dep_begin();
+  for (long long i = 4 * (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x); i < n; i += 1024LL * gridDim.x) {
+    float4 v = *reinterpret_cast<const float4*>(part + i);
+    for (int s = 1; s < splits; ++s) {
+      const float4 o = *reinterpret_cast<const float4*>(part + s * n + i);
+      v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+    }
+    if (out_f32) *reinterpret_cast<float4*>(static_cast<float*>(out) + i) = v;
+    else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(out) + i) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ few rows
+// A cluster of eight CTAs a row (and share of the columns, where rows are fewer than SMs): each CTA multiplies an eighth of x with all R rows of
+// A_l, the sums meet in distributed shared memory, and each expands its columns from fp32 values that were never rounded.
+constexpr int kFewCluster = 8, kFewThreads = 256;
+
+struct FewLora {
+  LoraIndex ix;
+  const __nv_bfloat16 *x, *a, *b, *base;
+  __nv_bfloat16* out;
+  long long ldx, ldb;
+  int K, N, R, parts;
+  const float* scales;
+  float scale;
+};
+
+__device__ __forceinline__ float dot8(const uint4& a, const uint4& b, float s) {
+  const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = unpack_bf16x2(x[i]), g = unpack_bf16x2(y[i]);
+    s = fmaf(f.x, g.x, s);
+    s = fmaf(f.y, g.y, s);
+  }
+  return s;
+}
+
+__global__ void __launch_bounds__(kFewThreads) lora_few_kernel(const FewLora p) {
+  grid_dep_begin();
+  __shared__ float sums[128], v[128];
+  const int rank = static_cast<int>(cluster_ctarank()), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c = static_cast<int>(cluster_id_x()), part = c % p.parts;
+  const long long t = c / p.parts;
+  const int l = lora_adapter(p.ix, t);
+  if (l >= 0) {
+    const int vecs = p.K / 8, v0 = rank * vecs / kFewCluster, v1 = (rank + 1) * vecs / kFewCluster;
+    const uint4* x = reinterpret_cast<const uint4*>(p.x + t * p.ldx);
+    for (int r = warp; r < p.R; r += 2 * (kFewThreads / 32)) {       // two rows of A at a time
+      const int r2 = r + kFewThreads / 32;
+      const uint4* a = reinterpret_cast<const uint4*>(p.a + (static_cast<long long>(l) * p.R + r) * p.K);
+      const uint4* a2 = reinterpret_cast<const uint4*>(p.a + (static_cast<long long>(l) * p.R + min(r2, p.R - 1)) * p.K);
+      float s = 0.0f, s2 = 0.0f;
+#pragma unroll 2
+      for (int i = v0 + lane; i < v1; i += 32) {
+        const uint4 xv = x[i];
+        s = dot8(xv, a[i], s);
+        s2 = dot8(xv, a2[i], s2);
+      }
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, off);
+        s2 += __shfl_xor_sync(0xffffffffu, s2, off);
+      }
+      if (lane == 0) {
+        sums[r] = s;
+        if (r2 < p.R) sums[r2] = s2;
+      }
+    }
+  }
+  cluster_sync_all();
+  if (l >= 0 && static_cast<int>(threadIdx.x) < p.R) {
+    float s = 0.0f;
+    for (int r = 0; r < kFewCluster; ++r) {
+      float o;
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o) : "r"(mapa_shared(smem_u32(sums + threadIdx.x), r)) : "memory");
+      s += o;
+    }
+    v[threadIdx.x] = s * (p.scales != nullptr ? p.scales[l] : p.scale);
+  }
+  __syncthreads();
+  const int shares = p.parts * kFewCluster, share = part * kFewCluster + rank;
+  const int n0 = static_cast<int>(static_cast<long long>(share) * p.N / shares), n1 = static_cast<int>(static_cast<long long>(share + 1) * p.N / shares);
+  for (int n = n0 + threadIdx.x; n < n1; n += kFewThreads) {
+    float s = p.base != nullptr ? __bfloat162float(p.base[t * p.ldb + n]) : 0.0f;
+    if (l >= 0) {
+      const uint4* b = reinterpret_cast<const uint4*>(p.b + (static_cast<long long>(l) * p.N + n) * p.R);
+      float d = 0.0f;
+      for (int i = 0; i < p.R / 8; ++i) {
+        const uint4 w = b[i];
+        const uint32_t y[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const float2 f = unpack_bf16x2(y[h]);
+          d = fmaf(f.x, v[8 * i + 2 * h], d);
+          d = fmaf(f.y, v[8 * i + 2 * h + 1], d);
+        }
+      }
+      s += d;
+    }
+    p.out[t * p.N + n] = __float2bfloat16_rn(s);
+  }
+  cluster_sync_all();      // nobody leaves while another reads its sums
+}
+
+// ------------------------------------------------------------------------------------------------ host
+static int padded_rank(int64_t R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
+template <class F>
+static int by_rank(int rp, F f) {
+  if (rp == 16) return f(std::integral_constant<int, 16>());
+  if (rp == 32) return f(std::integral_constant<int, 32>());
+  if (rp == 64) return f(std::integral_constant<int, 64>());
+  return f(std::integral_constant<int, 128>());
+}
+
+// W: (L,R,D), or (wmn) (L,D,R)
+static int lora_shrink(const void* X, int64_t ldx, const void* W, bool wmn, ShrinkParams p, cudaStream_t st) {
+  return by_rank(padded_rank(p.R), [&](auto rp) -> int {
+    constexpr int RP = decltype(rp)::value;
+    CUtensorMap tmX, tmW;
+    int rc = make_map(&tmX, X, p.D, p.ix.T, 1, ldx, ldx * p.ix.T, 64, kLTile);
+    if (rc == 0) rc = wmn ? make_map(&tmW, W, p.R, p.D, p.ix.L, p.R, static_cast<int64_t>(p.R) * p.D, 64, 64)
+                          : make_map(&tmW, W, p.D, p.R, p.ix.L, p.D, static_cast<int64_t>(p.R) * p.D, 64, RP);
+    if (rc) return rc;
+    const int64_t tiles = ceil_div(p.ix.T, kLTile), blocks = ceil_div(p.D, 64);
+    p.split = 1;
+    while (p.split < 8 && tiles * p.split * 2 <= 2 * num_sms() && blocks >= 4 * p.split) p.split *= 2;
+    auto run = [&](auto mn) -> int {
+      constexpr bool MN = decltype(mn)::value;
+      static PerDevice allowed;
+      B200_CUDA(allow_smem(allowed, lora_shrink_kernel<RP, MN>, kShrinkSmem));
+      B200_CUDA(launch_chained(lora_shrink_kernel<RP, MN>, static_cast<int>(tiles * p.split), kShrinkThreads, kShrinkSmem, st, p.split, tmX, tmW, p));
+      return 0;
+    };
+    return wmn ? run(std::true_type()) : run(std::false_type());
+  });
+}
+
+// W: (L,N,R), or (wmn) (L,R,N)
+static int lora_expand(const void* V, const void* W, bool wmn, int64_t R, const void* base, int64_t ldb, void* out, ExpandParams p, cudaStream_t st) {
+  return by_rank(padded_rank(R), [&](auto rp) -> int {
+    constexpr int RP = decltype(rp)::value;
+    CUtensorMap tmV, tmW, tmB, tmO;
+    const int64_t T = p.ix.T, N = p.N;
+    int rc = make_map(&tmV, V, RP, T, 1, RP, T * RP, 64, kLTile);
+    if (rc == 0) rc = wmn ? make_map(&tmW, W, N, R, p.ix.L, N, N * R, 64, RP) : make_map(&tmW, W, R, N, p.ix.L, R, N * R, 64, 128);
+    if (rc == 0) rc = make_map(&tmO, out, N, T, 1, N, N * T, 64, 32);
+    tmB = tmO;
+    if (rc == 0 && base != nullptr) rc = make_map(&tmB, base, N, T, 1, ldb, ldb * T, 64, 32);
+    if (rc) return rc;
+    p.has_base = base != nullptr;
+    const int64_t items = ceil_div(T, kLTile) * ceil_div(N, 128);
+    p.per_cta = static_cast<int>(ceil_div(items, num_sms()));
+    const int grid = static_cast<int>(ceil_div(items, p.per_cta));
+    auto run = [&](auto mn) -> int {
+      constexpr bool MN = decltype(mn)::value;
+      static PerDevice allowed;
+      B200_CUDA(allow_smem(allowed, lora_expand_kernel<RP, MN>, kExpSmem<RP>));
+      B200_LAUNCH((lora_expand_kernel<RP, MN>), grid, kExpThreads, kExpSmem<RP>, st, tmV, tmW, tmB, tmO, p);
+      return 0;
+    };
+    return wmn ? run(std::true_type()) : run(std::false_type());
+  });
+}
+
+// Shares of the rows: as many as it takes for two CTAs an SM, each with eight blocks of rows at least
+static int wgrad_splits(int64_t T, int64_t D, int64_t L) {
+  const int64_t blocks = ceil_div(T, 64), ctas = ceil_div(D, 128) * L;
+  const int64_t s = std::max<int64_t>(1, std::min<int64_t>(2 * num_sms() / ctas, blocks / 8));
+  return static_cast<int>(std::max<int64_t>(s, ceil_div(blocks, 32 * kWgWords)));
+}
+static int lora_wgrad(const void* Y, int64_t ldy, const void* V, WgradParams p, float* ws, void* out, int out_f32, cudaStream_t st) {
+  return by_rank(padded_rank(p.R), [&](auto rp) -> int {
+    constexpr int RP = decltype(rp)::value;
+    CUtensorMap tmY, tmV;
+    int rc = make_map(&tmY, Y, p.D, p.T, 1, ldy, ldy * p.T, 64, 64);
+    if (rc == 0) rc = make_map(&tmV, V, RP, p.T, 1, RP, static_cast<int64_t>(p.T) * RP, 64, 64);
+    if (rc) return rc;
+    p.splits = wgrad_splits(p.T, p.D, p.L);
+    p.out = p.splits > 1 ? static_cast<void*>(ws) : out;
+    p.out_f32 = p.splits > 1 || out_f32;
+    static PerDevice allowed;
+    B200_CUDA(allow_smem(allowed, lora_wgrad_kernel<RP>, kWgSmem<RP>));
+    B200_LAUNCH(lora_wgrad_kernel<RP>, static_cast<int>(ceil_div(p.D, 128) * p.L * p.splits), kWgThreads, kWgSmem<RP>, st, tmY, tmV, p);
+    if (p.splits > 1) {
+      const long long n = static_cast<long long>(p.L) * p.D * p.R;
+      B200_LAUNCH(lora_wgrad_sum_kernel, static_cast<int>(std::min<long long>(ceil_div(n, 1024), 4 * num_sms())), 256, 0, st,
+                  static_cast<const float*>(ws), p.splits, n, out, out_f32);
+    }
+    return 0;
+  });
+}
+
+struct LoraCarver {
+  char* base;
+  size_t off = 0;
+  template <class T>
+  T* take(int64_t n) {
+    off = (off + 255) & ~static_cast<size_t>(255);
+    T* p = base != nullptr ? reinterpret_cast<T*>(base + off) : nullptr;
+    off += static_cast<size_t>(n) * sizeof(T);
+    return p;
+  }
+};
+struct LoraKept {
+  __nv_bfloat16* v;
+  int* rows;
+  unsigned char* present;
+};
+static LoraKept carve_lora(int64_t T, int64_t R, int64_t L, int keep, void* ws, size_t* bytes) {
+  LoraCarver c{static_cast<char*>(ws)};
+  LoraKept k{};
+  k.v = c.take<__nv_bfloat16>(T * padded_rank(R));
+  if (keep) {
+    k.rows = c.take<int>(T);
+    k.present = c.take<unsigned char>(ceil_div(T, kLTile) * L);
+  }
+  *bytes = c.off;
+  return k;
+}
+static bool lora_few(int64_t T, int keep) { return !keep && T <= 128; }
+
+}  // namespace b200moe
+
+using namespace b200moe;
+
+static int check_lora(const char* who, int64_t T, int64_t K, int64_t N, int64_t R, int64_t L) {
+  CHECK_DIM8(K);
+  CHECK_DIM8(N);
+  B200_CHECK_ARG(R >= 8 && R % 8 == 0 && R <= 128, B200MOE_E_UNSUPPORTED, "%s: rank %lld, supported are multiples of 8 up to 128", who, (long long)R);
+  B200_CHECK_ARG(T >= 0 && T < (1LL << 31) - 256 && K < (1LL << 31) - 256 && N < (1LL << 31) - 256, B200MOE_E_BAD_SHAPE,
+                 "%s: %lld rows, %lld -> %lld", who, (long long)T, (long long)K, (long long)N);
+  B200_CHECK_ARG(L >= 1 && L <= 65536, B200MOE_E_BAD_SHAPE, "%s: %lld adapters, supported 1..65536", who, (long long)L);
+  B200_CHECK_ARG(ceil_div(T, 128) * 8 < (1LL << 31) && ceil_div(std::max(K, N), 128) * L * 512 < (1LL << 31), B200MOE_E_BAD_SHAPE,
+                 "%s: %lld adapters of %lld -> %lld are too many", who, (long long)L, (long long)K, (long long)N);
+  return 0;
+}
+
+extern "C" {
+
+size_t b200moe_lora_fwd_ws_bytes(int64_t T, int64_t R, int64_t L, int keep) {
+  if (T <= 0 || R <= 0 || L <= 0) return 0;
+  size_t bytes = 0;
+  carve_lora(T, R, L, keep, nullptr, &bytes);
+  return bytes;
+}
+
+int b200moe_lora_forward(const void* x, int64_t ldx, const void* a, const void* b, const void* index, int index_bytes, const float* scales, float scale,
+                         const void* base, int64_t ldb, int64_t T, int64_t K, int64_t N, int64_t R, int64_t L, int keep, void* ws, void* out,
+                         int32_t* status, b200moe_stream_t stream) {
+  const int rc = check_lora("lora_forward", T, K, N, R, L);
+  if (rc) return rc;
+  B200_CHECK_ARG(ldx >= K && ldx % 8 == 0 && (base == nullptr || (ldb >= N && ldb % 8 == 0)), B200MOE_E_BAD_SHAPE,
+                 "lora_forward: rows of x %lld apart, of base %lld (multiples of 8, at least K and N)", (long long)ldx, (long long)ldb);
+  B200_CHECK_ARG(index == nullptr || index_bytes == 4 || index_bytes == 8, B200MOE_E_UNSUPPORTED, "lora_forward: an index of %d bytes", index_bytes);
+  if (T == 0) return 0;
+  B200_CHECK_ARG(x && a && b && ws && out && status, B200MOE_E_NULL, "lora_forward: null pointer");
+  B200_CHECK_ARG(aligned16(x) && aligned16(a) && aligned16(b) && aligned16(base) && aligned16(ws) && aligned16(out) &&
+                     reinterpret_cast<uintptr_t>(index) % 8 == 0,
+                 B200MOE_E_ALIGN, "lora_forward: tensors must be 16-byte aligned, the index 8");
+  cudaStream_t st = (cudaStream_t)stream;
+  const LoraIndex ix{index, index_bytes, static_cast<int>(T), static_cast<int>(L), status};
+  if (lora_few(T, keep)) {
+    const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(num_sms() / (T * kFewCluster), ceil_div(N, kFewCluster * kFewThreads))));
+    const FewLora p{ix, static_cast<const __nv_bfloat16*>(x), static_cast<const __nv_bfloat16*>(a), static_cast<const __nv_bfloat16*>(b),
+                    static_cast<const __nv_bfloat16*>(base), static_cast<__nv_bfloat16*>(out), ldx, ldb, static_cast<int>(K), static_cast<int>(N),
+                    static_cast<int>(R), parts, scales, scale};
+    OpScope scope("lora_few", 1);
+    B200_CUDA(launch_chained(lora_few_kernel, static_cast<int>(T * parts * kFewCluster), kFewThreads, 0, st, kFewCluster, p));
+    return 0;
+  }
+  size_t bytes;
+  const LoraKept k = carve_lora(T, R, L, keep, ws, &bytes);
+  {
+    OpScope scope("lora_shrink", 1);
+    const int rc2 = lora_shrink(x, ldx, a, false,
+                                ShrinkParams{ix, static_cast<int>(K), static_cast<int>(R), 1, scales, scale, k.v, k.rows, index != nullptr ? k.present : nullptr}, st);
+    if (rc2) return rc2;
+  }
+  OpScope scope("lora_expand", 1);
+  return lora_expand(k.v, b, false, R, base, ldb, out, ExpandParams{ix, static_cast<int>(N), 0, 0}, st);
+}
+
+size_t b200moe_lora_bwd_ws_bytes(int64_t T, int64_t K, int64_t N, int64_t R, int64_t L) {
+  if (T <= 0 || K <= 0 || N <= 0 || R <= 0 || L <= 0) return 0;
+  LoraCarver c{nullptr};
+  c.take<__nv_bfloat16>(T * padded_rank(R));
+  const int sa = wgrad_splits(T, K, L), sb = wgrad_splits(T, N, L);
+  c.take<float>(std::max(sa > 1 ? sa * L * R * K : 0, sb > 1 ? sb * L * R * N : 0));
+  return c.off;
+}
+
+int b200moe_lora_backward(const void* grad_out, const void* x, int64_t ldx, const void* a, const void* b, int has_index, const float* scales, float scale,
+                          int64_t T, int64_t K, int64_t N, int64_t R, int64_t L, const void* fwd_ws, void* ws, void* grad_x, void* grad_a, void* grad_b,
+                          int grad_f32, int32_t* status, b200moe_stream_t stream) {
+  const int rc = check_lora("lora_backward", T, K, N, R, L);
+  if (rc) return rc;
+  B200_CHECK_ARG(T >= 1, B200MOE_E_BAD_SHAPE, "lora_backward: no rows");
+  B200_CHECK_ARG(ldx >= K && ldx % 8 == 0, B200MOE_E_BAD_SHAPE, "lora_backward: rows of x %lld apart", (long long)ldx);
+  B200_CHECK_ARG(grad_out && x && a && b && fwd_ws && ws && status, B200MOE_E_NULL, "lora_backward: null pointer");
+  B200_CHECK_ARG(aligned16(grad_out) && aligned16(x) && aligned16(a) && aligned16(b) && aligned16(fwd_ws) && aligned16(ws) && aligned16(grad_x) &&
+                     aligned16(grad_a) && aligned16(grad_b),
+                 B200MOE_E_ALIGN, "lora_backward: tensors must be 16-byte aligned");
+  cudaStream_t st = (cudaStream_t)stream;
+  size_t bytes;
+  const LoraKept k = carve_lora(T, R, L, 1, const_cast<void*>(fwd_ws), &bytes);
+  LoraCarver c{static_cast<char*>(ws)};
+  __nv_bfloat16* u = c.take<__nv_bfloat16>(T * padded_rank(R));
+  float* part = c.take<float>(0);
+  const LoraIndex ix{has_index ? k.rows : nullptr, 4, static_cast<int>(T), static_cast<int>(L), status};
+  WgradParams w{static_cast<int>(T), 0, static_cast<int>(R), static_cast<int>(L), 1, 0, has_index ? k.rows : nullptr, has_index ? k.present : nullptr,
+                nullptr, 0, status};
+#define RUN(name, launches, call)     \
+  do {                                \
+    OpScope scope__(name, launches);  \
+    const int rc__ = (call);          \
+    if (rc__) return rc__;            \
+  } while (0)
+  if (grad_x || grad_a)
+    RUN("lora_shrink", 1,
+        lora_shrink(grad_out, N, b, true, ShrinkParams{ix, static_cast<int>(N), static_cast<int>(R), 1, scales, scale, u, nullptr, nullptr}, st));
+  if (grad_b) {
+    w.D = static_cast<int>(N);
+    w.transposed = 0;
+    RUN("lora_wgrad", wgrad_splits(T, N, L) > 1 ? 2 : 1, lora_wgrad(grad_out, N, k.v, w, part, grad_b, grad_f32, st));
+  }
+  if (grad_x)
+    RUN("lora_expand", 1, lora_expand(u, a, true, R, nullptr, 0, grad_x, ExpandParams{ix, static_cast<int>(K), 0, 0}, st));
+  if (grad_a) {
+    w.D = static_cast<int>(K);
+    w.transposed = 1;
+    RUN("lora_wgrad", wgrad_splits(T, K, L) > 1 ? 2 : 1, lora_wgrad(x, ldx, u, w, part, grad_a, grad_f32, st));
+  }
+#undef RUN
+  return 0;
+}
+
+}  // extern "C"

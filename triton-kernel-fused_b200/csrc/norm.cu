@@ -298,7 +298,6 @@ static int64_t norm_ctas(int64_t rows, int rows_cta, int threads, int threads_sm
 }
 
 constexpr int kBwdThreadsSm = 768;
-static int bwd_nv(int64_t K) { return K <= 1024 ? 4 : 2; }
 static int bwd_threads(int64_t K) { return K <= 1024 ? 256 : row_threads(K, 2); }
 static int64_t bwd_ctas(int64_t rows, int64_t K) {
   const int threads = bwd_threads(K);
