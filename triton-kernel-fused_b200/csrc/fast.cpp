@@ -1,6 +1,6 @@
-// Autograd functions of the layer, of the experts on given picks, of the conv router, of the group top-k, of the router losses and of
-// the block-scaled 8-bit products as compiled code: the host side of the Python Functions of the same name (layer.py, moe.py, router.py,
-// fp8_block.py) for plain calls.  Each function returns None for a call
+// Autograd functions of the layer, of the experts on given picks, of the conv router, of the group top-k, of the router losses, of
+// the block-scaled 8-bit products, of the root-mean-square norm and of the low-rank adapters as compiled code: the host side of the Python
+// Functions of the same name (layer.py, moe.py, router.py, fp8_block.py, norm.py, lora.py) for plain calls.  Each function returns None for a call
 // that is not plain (a tensor that would have to be cast or made contiguous, autocast, functorch transforms, forward-mode
 // gradients, dispatch modes, tensor subclasses, a shape that is an error), and the caller then takes the Python Function, which
 // casts, refuses or raises as it always did.
@@ -439,6 +439,21 @@ bool codes(const Tensor& w, const Tensor& scale, int64_t dim, c10::Device dev) {
 }
 bool aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 
+// Rows that are codes already, their scales at a pitch of whole 128 rows
+struct RowCodes {
+  Tensor q, scale;
+  int64_t pitch = 0;
+};
+Tensor rows_product(const RowCodes& r, const Tensor& w, const Tensor& scale, const Tensor& status) {
+  const int64_t N = w.size(0), K = w.size(1), M = r.q.numel() / K;
+  std::vector<int64_t> shape(r.q.sizes().begin(), r.q.sizes().end());
+  shape.back() = N;
+  Tensor out = at::empty(shape, r.q.options().dtype(at::kBFloat16));
+  check(b200moe_fp8_block_linear_rows(ptr(r.q), r.scale.data_ptr<float>(), r.pitch, ptr(w), scale.data_ptr<float>(), M, N, K, ptr(out),
+                                      status_ptr(status), stream_of(r.q)));
+  return out;
+}
+
 Tensor block_product(const Tensor& x, const Tensor& w, const Tensor& scale, const Tensor& status, bool transposed) {
   const int64_t N = w.size(0), K = w.size(1), M = x.numel() / (transposed ? N : K);
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
@@ -449,10 +464,10 @@ Tensor block_product(const Tensor& x, const Tensor& w, const Tensor& scale, cons
 }
 
 struct BlockLinear : torch::autograd::Function<BlockLinear> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& scale, const Tensor& status) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& scale, const Tensor& status, const RowCodes& rows) {
     ctx->save_for_backward({w, scale});
     ctx->saved_data["status"] = status;
-    return block_product(x, w, scale, status, false);
+    return rows.q.defined() ? rows_product(rows, w, scale, status) : block_product(x, w, scale, status, false);
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -460,7 +475,7 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
     const c10::cuda::CUDAGuard guard(s[0].device());
     Tensor g = grads[0].to(at::kBFloat16).contiguous();
     if (!aligned(g)) g = g.clone();
-    return once({block_product(g, s[0], s[1], ctx->saved_data["status"].toTensor(), true), Tensor(), Tensor(), Tensor()});
+    return once({block_product(g, s[0], s[1], ctx->saved_data["status"].toTensor(), true), Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 
@@ -471,8 +486,35 @@ optional<Tensor> fp8_block_linear(const Tensor& x, const Tensor& w, const Tensor
   if (!plain(x, at::kBFloat16, dev) || !codes(w, scale, 2, dev) || x.dim() < 1 || x.numel() == 0 || x.size(-1) != w.size(1)) return std::nullopt;
   if (w.size(0) % 8 != 0 || w.size(1) % 16 != 0 || !aligned(x) || !aligned(w)) return std::nullopt;
   const c10::cuda::CUDAGuard guard(dev);
-  if (at::GradMode::is_enabled() && x.requires_grad()) return BlockLinear::apply(x, w, scale, status);
+  if (at::GradMode::is_enabled() && x.requires_grad()) return BlockLinear::apply(x, w, scale, status, RowCodes());
   return block_product(x, w, scale, status, false);
+}
+
+// The same of rows that are codes; x: what the gradient goes to, if any
+optional<Tensor> fp8_block_linear_rows(const optional<Tensor>& x, const Tensor& q, const Tensor& q_scale, const Tensor& w, const Tensor& scale,
+                                       const Tensor& status) {
+  if (!plain_call(q)) return std::nullopt;
+  const auto dev = q.device();
+  if (!plain(q, at::kFloat8_e4m3fn, dev) || !codes(w, scale, 2, dev) || q.dim() < 1 || q.numel() == 0 || q.size(-1) != w.size(1)) return std::nullopt;
+  if (x.has_value() && (!plain(*x, at::kBFloat16, dev) || x->sizes() != q.sizes())) return std::nullopt;
+  if (w.size(0) % 8 != 0 || w.size(1) % 16 != 0 || !aligned(q) || !aligned(w) || q.requires_grad()) return std::nullopt;
+  // the scales as rms_norm_fp8_block left them: rows next to one another, blocks at a pitch
+  if (q_scale.scalar_type() != at::kFloat || q_scale.device() != dev || q_scale.layout() != at::kStrided || q_scale.dim() != q.dim() ||
+      q_scale.requires_grad() || q_scale._fw_grad(0).defined() || q_scale.key_set().has(c10::DispatchKey::Python))
+    return std::nullopt;
+  const int64_t blocks = (w.size(1) + 127) / 128, M = q.numel() / w.size(1), rows = (M + 127) / 128 * 128;
+  const int64_t pitch = blocks == 1 ? rows : q_scale.stride(-1);
+  if (q_scale.size(-1) != blocks || pitch % 4 != 0 || pitch < rows || !aligned(q_scale)) return std::nullopt;
+  int64_t stride = 1;
+  for (int64_t i = q.dim() - 2; i >= 0; --i) {
+    if (q_scale.size(i) != q.size(i) || (q.size(i) > 1 && q_scale.stride(i) != stride)) return std::nullopt;
+    stride *= q.size(i);
+  }
+  if (static_cast<int64_t>(q_scale.storage().nbytes()) < 4 * (q_scale.storage_offset() + (blocks - 1) * pitch + rows)) return std::nullopt;
+  const c10::cuda::CUDAGuard guard(dev);
+  const RowCodes r{q, q_scale, pitch};
+  if (x.has_value() && at::GradMode::is_enabled() && x->requires_grad()) return BlockLinear::apply(*x, w, scale, status, r);
+  return rows_product(r, w, scale, status);
 }
 
 // (N,H) bf16, or None
@@ -495,6 +537,184 @@ optional<Tensor> moe_fp8_block(const Tensor& x, const Tensor& idx, const Tensor&
   return out;
 }
 
+// ---------------------------------------------------------------------------- root-mean-square norm
+struct NormArgs {
+  optional<Tensor> residual;
+  Tensor q, scale;      // codes and [block][row] scales to be filled, or undefined
+  int type, w_type;
+  double eps;
+  bool want_y;
+};
+
+// y where it is wanted, then h where there is a residual
+variable_list norm_forward(const Tensor& x, const Tensor& w, const NormArgs& a) {
+  const int64_t K = x.size(-1), N = x.numel() / K;
+  Tensor y = a.want_y ? at::empty(x.sizes(), x.options()) : Tensor();
+  Tensor h = a.residual.has_value() ? at::empty(x.sizes(), x.options()) : Tensor();
+  check(b200moe_rms_norm_fwd(ptr(x), K, ptr(a.residual), K, a.type, ptr(w), a.w_type, N, K, static_cast<float>(a.eps), ptr(y), ptr(h), ptr(a.q),
+                             static_cast<float*>(ptr(a.scale)), a.scale.defined() ? a.scale.size(1) : 0, stream_of(x)));
+  variable_list r;
+  if (y.defined()) r.push_back(y);
+  if (h.defined()) r.push_back(h);
+  return r;
+}
+
+struct RmsNorm : torch::autograd::Function<RmsNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const optional<Tensor>& residual, const NormArgs& a) {
+    ctx->saved_data["residual"] = residual.has_value();      // an input only where there is one
+    variable_list r = norm_forward(x, w, a);
+    ctx->save_for_backward({residual.has_value() ? r.back() : x, w});
+    ctx->saved_data["y"] = a.want_y;
+    ctx->saved_data["type"] = a.type;
+    ctx->saved_data["w_type"] = a.w_type;
+    ctx->saved_data["eps"] = a.eps;
+    ctx->set_materialize_grads(false);
+    return r;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list res(4);
+    const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_r = ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(2);
+    const bool has_y = ctx->saved_data["y"].toBool(), has_h = ctx->saved_data["residual"].toBool();
+    const Tensor grad_y = has_y ? grads[0] : Tensor(), grad_h = has_h ? grads[has_y] : Tensor();
+    if (!grad_y.defined()) {      // the stream alone was used
+      if (need_x) res[0] = grad_h;
+      if (need_r) res[2] = grad_h;
+      return res;
+    }
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &h = s[0], &w = s[1];
+    const int64_t K = h.size(-1), N = h.numel() / K;
+    const c10::cuda::CUDAGuard guard(h.device());
+    const Tensor gy = grad_y.contiguous(), gh = grad_h.defined() ? grad_h.contiguous() : Tensor();
+    Tensor gx = need_x || need_r ? at::empty(h.sizes(), h.options()) : Tensor(), gw = need_w ? at::empty(w.sizes(), w.options()) : Tensor();
+    Tensor ws = need_w ? bytes(b200moe_rms_norm_bwd_ws_bytes(N, K), h) : Tensor();
+    check(b200moe_rms_norm_bwd(ptr(gy), ptr(gh), ptr(h), K, ctx->saved_data["type"].toInt(), ptr(w), ctx->saved_data["w_type"].toInt(), N, K,
+                               static_cast<float>(ctx->saved_data["eps"].toDouble()), ptr(ws), ptr(gx), ptr(gw), stream_of(h)));
+    if (need_x) res[0] = gx;
+    if (need_r) res[2] = gx;
+    res[1] = gw;
+    return once(res);
+  }
+};
+
+// (y, h, codes, scales): those that were asked for; or None
+optional<std::tuple<optional<Tensor>, optional<Tensor>, optional<Tensor>, optional<Tensor>>> rms_norm(const Tensor& x, const Tensor& w,
+                                                                                                      const optional<Tensor>& residual, double eps,
+                                                                                                      bool want_y, bool want_codes) {
+  if (!plain_call(x)) return std::nullopt;
+  const auto dev = x.device();
+  const auto type = logits_type(x), w_type = logits_type(w);
+  if (!type.has_value() || !w_type.has_value() || (*w_type != *type && *w_type != B200MOE_F32)) return std::nullopt;
+  if (!plain(x, x.scalar_type(), dev) || !plain(w, w.scalar_type(), dev) || !plain_or_none(residual, x.scalar_type(), dev)) return std::nullopt;
+  if (x.dim() < 1 || x.numel() == 0 || w.dim() != 1 || w.size(0) != x.size(-1) || (residual.has_value() && residual->sizes() != x.sizes())) return std::nullopt;
+  const int64_t K = x.size(-1), N = x.numel() / K;
+  if (K > 16384 || (want_codes && K % 8 != 0) || !(eps >= 0.0) || N >= (1LL << 31) - 256) return std::nullopt;
+  const c10::cuda::CUDAGuard guard(dev);
+  NormArgs a{residual, Tensor(), Tensor(), *type, *w_type, eps, want_y};
+  if (want_codes) {
+    a.q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+    a.scale = at::empty({(K + 127) / 128, (N + 127) / 128 * 128}, x.options().dtype(at::kFloat));
+  }
+  const bool grad = at::GradMode::is_enabled() && (want_y || residual.has_value()) && (x.requires_grad() || w.requires_grad() || (residual.has_value() && residual->requires_grad()));
+  const variable_list r = grad ? RmsNorm::apply(x, w, residual, a) : norm_forward(x, w, a);
+  std::tuple<optional<Tensor>, optional<Tensor>, optional<Tensor>, optional<Tensor>> out;
+  if (want_y) std::get<0>(out) = r[0];
+  if (residual.has_value()) std::get<1>(out) = r.back();
+  if (want_codes) {      // (..., blocks), rows next to one another
+    std::vector<int64_t> sizes(x.sizes().begin(), x.sizes().end()), strides(sizes.size());
+    sizes.back() = a.scale.size(0);
+    strides.back() = a.scale.size(1);
+    int64_t stride = 1;
+    for (int64_t i = x.dim() - 2; i >= 0; --i) {
+      strides[i] = stride;
+      stride *= sizes[i];
+    }
+    std::get<2>(out) = a.q;
+    std::get<3>(out) = a.scale.as_strided(sizes, strides);
+  }
+  return out;
+}
+
+// ---------------------------------------------------------------------------- low-rank adapters
+struct LoraArgs {
+  optional<Tensor> index, scales;
+  Tensor status;
+  double scale;
+};
+
+Tensor lora_forward(const Tensor& x, const Tensor& a, const Tensor& b, const optional<Tensor>& base, const LoraArgs& p, const Tensor& ws, bool keep) {
+  const int64_t L = a.size(0), R = a.size(1), K = a.size(2), N = b.size(1), T = x.numel() / K;
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = N;
+  Tensor out = at::empty(shape, x.options());
+  check(b200moe_lora_forward(ptr(x), K, ptr(a), ptr(b), ptr(p.index), p.index.has_value() ? p.index->element_size() : 0,
+                             static_cast<const float*>(ptr(p.scales)), static_cast<float>(p.scale), ptr(base), N, T, K, N, R, L, keep, ptr(ws),
+                             ptr(out), status_ptr(p.status), stream_of(x)));
+  return out;
+}
+
+struct Lora : torch::autograd::Function<Lora> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& a, const Tensor& b, const optional<Tensor>& base,
+                        const LoraArgs& p) {
+    const bool keep = x.requires_grad() || a.requires_grad() || b.requires_grad();
+    const Tensor ws = bytes(b200moe_lora_fwd_ws_bytes(x.numel() / a.size(2), a.size(1), a.size(0), keep), x);
+    Tensor out = lora_forward(x, a, b, base, p, ws, keep);
+    if (keep) ctx->save_for_backward({x, a, b, ws, p.scales.value_or(Tensor())});
+    ctx->saved_data["status"] = p.status;
+    ctx->saved_data["scale"] = p.scale;
+    ctx->saved_data["index"] = p.index.has_value();
+    ctx->saved_data["base"] = base.has_value();      // an input only where there is one
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list res(5);
+    if (ctx->saved_data["base"].toBool() && ctx->needs_input_grad(3)) res[3] = grads[0];
+    if (!ctx->needs_input_grad(0) && !ctx->needs_input_grad(1) && !ctx->needs_input_grad(2)) return once(res);
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &a = s[1], &b = s[2], &ws = s[3], &scales = s[4];
+    const int64_t L = a.size(0), R = a.size(1), K = a.size(2), N = b.size(1), T = x.numel() / K;
+    const c10::cuda::CUDAGuard guard(x.device());
+    Tensor g = grads[0].to(at::kBFloat16).contiguous();
+    if (!aligned(g)) g = g.clone();
+    for (int i = 0; i < 3; ++i) res[i] = grad_like(ctx->needs_input_grad(i), s[i]);
+    Tensor tmp = bytes(b200moe_lora_bwd_ws_bytes(T, K, N, R, L), x);
+    check(b200moe_lora_backward(ptr(g), ptr(x), K, ptr(a), ptr(b), ctx->saved_data["index"].toBool(), static_cast<const float*>(ptr(scales)),
+                                static_cast<float>(ctx->saved_data["scale"].toDouble()), T, K, N, R, L, ptr(ws), ptr(tmp), ptr(res[0]), ptr(res[1]),
+                                ptr(res[2]), 0, status_ptr(ctx->saved_data["status"].toTensor()), stream_of(x)));
+    return once(res);
+  }
+};
+
+// (..., N) bf16, or None
+optional<Tensor> lora_linear(const Tensor& x, const Tensor& a, const Tensor& b, const optional<Tensor>& index, const optional<Tensor>& scales,
+                             double scale, const optional<Tensor>& base, const Tensor& status) {
+  if (!plain_call(x)) return std::nullopt;
+  const auto dev = x.device();
+  if (!plain(x, at::kBFloat16, dev) || !plain(a, at::kBFloat16, dev) || !plain(b, at::kBFloat16, dev) || !plain_or_none(base, at::kBFloat16, dev) ||
+      !plain_or_none(scales, at::kFloat, dev))
+    return std::nullopt;
+  if (x.dim() < 1 || a.dim() != 3 || b.dim() != 3 || x.numel() == 0 || a.numel() == 0 || b.numel() == 0) return std::nullopt;
+  const int64_t L = a.size(0), R = a.size(1), K = a.size(2), N = b.size(1);
+  if (b.size(0) != L || b.size(2) != R || x.size(-1) != K || K % 8 != 0 || N % 8 != 0 || R % 8 != 0 || R > 128 || L > 65536) return std::nullopt;
+  const auto rows = x.sizes().slice(0, x.dim() - 1);
+  if (index.has_value()) {
+    const auto type = index->scalar_type();
+    if ((type != at::kInt && type != at::kLong) || !plain(*index, type, dev) || index->sizes() != rows) return std::nullopt;
+  } else if (L != 1) {
+    return std::nullopt;
+  }
+  if (scales.has_value() && (scales->dim() != 1 || scales->size(0) != L || (at::GradMode::is_enabled() && scales->requires_grad()))) return std::nullopt;
+  if (base.has_value() && (base->dim() != x.dim() || base->sizes().slice(0, x.dim() - 1) != rows || base->size(-1) != N || !aligned(*base))) return std::nullopt;
+  if (!aligned(x) || !aligned(a) || !aligned(b)) return std::nullopt;
+  const c10::cuda::CUDAGuard guard(dev);
+  const LoraArgs p{index, scales, status, scale};
+  if (at::GradMode::is_enabled() && (x.requires_grad() || a.requires_grad() || b.requires_grad() || (base.has_value() && base->requires_grad())))
+    return Lora::apply(x, a, b, base, p);
+  return lora_forward(x, a, b, base, p, bytes(b200moe_lora_fwd_ws_bytes(x.numel() / K, R, L, 0), x), false);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -505,5 +725,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("group_topk", torch::wrap_pybind_function_no_gil(group_topk));
   m.def("router_losses", torch::wrap_pybind_function_no_gil(router_losses));
   m.def("fp8_block_linear", torch::wrap_pybind_function_no_gil(fp8_block_linear));
+  m.def("fp8_block_linear_rows", torch::wrap_pybind_function_no_gil(fp8_block_linear_rows));
+  m.def("rms_norm", torch::wrap_pybind_function_no_gil(rms_norm));
+  m.def("lora_linear", torch::wrap_pybind_function_no_gil(lora_linear));
   m.def("moe_fp8_block", torch::wrap_pybind_function_no_gil(moe_fp8_block));
 }

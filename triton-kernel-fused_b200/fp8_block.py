@@ -162,6 +162,11 @@ def fp8_block_linear(x, weight, weight_scale, quantized=None):
 
 def _linear_of_codes(x, weight, weight_scale, q, q_scale):
     L.require(q.is_cuda, "codes must be a CUDA tensor (this package has no CPU path)")
+    fast = L.fast()
+    if fast is not None:
+        out = fast.fp8_block_linear_rows(x, q, q_scale, weight, weight_scale, L.status_word(q.device))
+        if out is not None:
+            return out
     w, scale = _weight("weight", weight, weight_scale, q.device, 2)
     N, K = w.shape
     L.require(N % 8 == 0 and K % 16 == 0 and N > 0 and K > 0, f"weight must be (N, K) with N a multiple of 8 and K of 16, got ({N}, {K})")

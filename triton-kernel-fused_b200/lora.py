@@ -29,7 +29,7 @@ def _aligned(t):
 
 
 class _Lora(torch.autograd.Function):
-    """base (..., N) or zeros, plus x (..., K) through each row's adapter of a (L,R,K), b (L,N,R)."""
+    """base (..., N) or zeros, plus x (..., K) through each row's adapter of a (L,R,K), b (L,N,R).  Plain calls take its compiled form (csrc/fast.cpp)."""
 
     @staticmethod
     def forward(ctx, x, a, b, base, index, scales, scale):
@@ -84,6 +84,12 @@ def lora_linear(x, lora_a, lora_b, index=None, scaling=1.0, base=None):
     128 (smaller ones of a stack are padded with zeros).  Adapters are bf16, or fp32 that is rounded to it and gets fp32 gradients.  x A^T is rounded
     to bf16 where a gradient is wanted or the rows are more than a few; sums are fp32 and the result is rounded once.  Rows and adapters
     do not mix: NaN in one stays there.  Differentiable in x, lora_a, lora_b and base; scaling takes no gradient."""
+    fast = L.fast() if x.is_cuda else None
+    if fast is not None:
+        wide = isinstance(scaling, torch.Tensor)
+        out = fast.lora_linear(x, lora_a, lora_b, index, scaling if wide else None, 1.0 if wide else scaling, base, L.status_word(x.device))
+        if out is not None:
+            return out
     if torch.is_autocast_enabled("cuda") and x.is_floating_point():
         dt = torch.get_autocast_dtype("cuda")
         x, base = x.to(dt), None if base is None else base.to(dt)

@@ -24,7 +24,7 @@ def _rows(t, K):
 
 class _RmsNorm(torch.autograd.Function):
     """(y, h, codes, scales [block][row]) of x (..., K), each None that is not asked for or (h) has no residual; scales lie at a pitch that the
-    products read without a copy."""
+    products read without a copy.  Plain calls take its compiled form (csrc/fast.cpp)."""
 
     @staticmethod
     def forward(ctx, x, residual, weight, eps, want_y, want_codes):
@@ -91,6 +91,11 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
     """x (..., K) bf16, fp16 or fp32, weight (K,) of x's type or fp32, residual like x -> y, or (y, h) with a residual: h = x + residual (rounded to
     x's type) and y = h / sqrt(mean(h^2) + eps) * weight.  K up to 16384; rows may lie at any distance.  Differentiable in x, residual and
     weight, through y and h."""
+    fast = L.fast() if x.is_cuda else None
+    if fast is not None:
+        res = fast.rms_norm(x, weight, residual, eps, True, False)
+        if res is not None:
+            return res[0] if residual is None else res[:2]
     eps = _check(x, weight, residual, eps, False)
     y, h, _, _ = _RmsNorm.apply(x, residual, weight, eps, True, False)
     return y if residual is None else (y, h)
@@ -101,6 +106,11 @@ def rms_norm_fp8_block(x, weight, residual=None, eps=1e-6, return_norm=False):
     the values being code * scale; y where return_norm, h where there is a residual.  K a multiple of 8.  Codes are the nearest to y before its
     rounding (`fp8_block_quantize(y)` rounds twice).  `fp8_block_linear(y, w, s, quantized=(codes, scales))` takes them; they carry no gradient,
     y and h do."""
+    fast = L.fast() if x.is_cuda else None
+    res = None if fast is None else fast.rms_norm(x, weight, residual, eps, bool(return_norm), True)
+    if res is not None:
+        y, h, q, scale = res
+        return (q, scale) + ((y,) if return_norm else ()) + ((h,) if residual is not None else ())
     eps = _check(x, weight, residual, eps, True)
     y, h, q, scale = _RmsNorm.apply(x, residual, weight, eps, bool(return_norm), True)
     scale = scale[:, : x.numel() // x.shape[-1]].t().reshape(*x.shape[:-1], scale.shape[0])
