@@ -386,13 +386,13 @@ int b200moe_moe_fp8_block_forward(const void* x, const int64_t* idx, const float
  * with scales [block of 128][scale_pitch >= rows] as b200moe_fp8_block_quant gives them. */
 int b200moe_rms_norm_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldr, int type, const void* weight, int weight_type,
                          int64_t rows, int64_t K, float eps, void* y, void* h, void* q, float* scale, int64_t scale_pitch,
-                         b200moe_stream_t stream);
+                         int32_t* status, b200moe_stream_t stream);
 /* The gradient: of h (of x and of the residual alike) grad_x = the norm's + grad_h (nullable: 0), and of the weight, summed over the rows in
  * a fixed order; either may be NULL.  h: as the forward had it (x without a residual).  ws: for grad_weight. */
 size_t b200moe_rms_norm_bwd_ws_bytes(int64_t rows, int64_t K);
 int b200moe_rms_norm_bwd(const void* grad_y, const void* grad_h, const void* h, int64_t ldh, int type, const void* weight,
                          int weight_type, int64_t rows, int64_t K, float eps, void* ws, void* grad_x, void* grad_weight,
-                         b200moe_stream_t stream);
+                         int32_t* status, b200moe_stream_t stream);
 
 /* ---- low-rank adapters (no counterpart in the reference) -----------------------------------------
  * out[t] = base[t] + s_l (x[t] A_l^T) B_l^T with l = index[t]: x (T,K), a (L,R,K), b (L,N,R), base (T,N, nullable: 0) and out (T,N) bf16, rows of x

@@ -10,8 +10,8 @@ P = 1 << 20      # an address that is never read
 def test_c_entry_points():
     lib = load_pkg().lib()
 
-    def fwd(x=P, ldx=64, r=P, ldr=64, t=0, w=P, wt=0, rows=4, K=64, eps=1e-6, y=P, h=P, q=P, s=P, pitch=128):
-        return lib.b200moe_rms_norm_fwd(x, ldx, r, ldr, t, w, wt, rows, K, eps, y, h, q, s, pitch, None)
+    def fwd(x=P, ldx=64, r=P, ldr=64, t=0, w=P, wt=0, rows=4, K=64, eps=1e-6, y=P, h=P, q=P, s=P, pitch=128, st=P):
+        return lib.b200moe_rms_norm_fwd(x, ldx, r, ldr, t, w, wt, rows, K, eps, y, h, q, s, pitch, st, None)
 
     assert fwd(rows=0) == 0
     assert fwd(x=None) == -6 and fwd(w=None) == -6 and fwd(s=None) == -6 and fwd(y=None, h=None, q=None) == -6 and fwd(r=None) == -6
@@ -19,10 +19,11 @@ def test_c_entry_points():
     assert fwd(K=0) == -1 and fwd(K=16385, ldx=1 << 20, ldr=1 << 20) == -1 and fwd(ldx=63) == -1 and fwd(ldr=8) == -1
     assert fwd(eps=-1.0) == -1 and fwd(eps=float("nan")) == -1 and fwd(K=60) == -1 and fwd(pitch=3) == -1 and fwd(q=P + 4) == -2
 
-    def bwd(gy=P, gh=P, h=P, ldh=64, t=0, w=P, wt=0, rows=4, K=64, ws=P, gx=P, gw=P):
-        return lib.b200moe_rms_norm_bwd(gy, gh, h, ldh, t, w, wt, rows, K, 1e-6, ws, gx, gw, None)
+    def bwd(gy=P, gh=P, h=P, ldh=64, t=0, w=P, wt=0, rows=4, K=64, ws=P, gx=P, gw=P, st=P):
+        return lib.b200moe_rms_norm_bwd(gy, gh, h, ldh, t, w, wt, rows, K, 1e-6, ws, gx, gw, st, None)
 
     assert bwd(rows=0, gw=None) == 0
+    assert fwd(st=None) == -6 and bwd(st=None) == -6 and bwd(ws=P + 8) == -2
     assert bwd(gy=None) == -6 and bwd(h=None) == -6 and bwd(w=None) == -6 and bwd(gx=None, gw=None) == -6 and bwd(ws=None) == -6
     assert bwd(t=7) == -3 and bwd(ldh=60) == -1 and bwd(K=0) == -1 and bwd(rows=-2) == -1
     assert lib.b200moe_rms_norm_bwd_ws_bytes(0, 64) == 0 and lib.b200moe_rms_norm_bwd_ws_bytes(4, 1 << 20) == 0

@@ -97,9 +97,9 @@ _SIGNATURES = {
     "b200moe_moe_fp8_block_ws_bytes": (c_size_t, [c_int64] * 3 + [c_int] * 2),
     "b200moe_moe_fp8_block_forward": (c_int, [c_void_p] * 7 + [c_int64] * 3 + [c_int] * 2 + [c_void_p] * 4),
     "b200moe_rms_norm_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int, c_int64, c_int64, c_float] + [c_void_p] * 4 +
-                             [c_int64, c_void_p]),
+                             [c_int64] + [c_void_p] * 2),
     "b200moe_rms_norm_bwd_ws_bytes": (c_size_t, [c_int64, c_int64]),
-    "b200moe_rms_norm_bwd": (c_int, [c_void_p] * 3 + [c_int64, c_int, c_void_p, c_int, c_int64, c_int64, c_float] + [c_void_p] * 4),
+    "b200moe_rms_norm_bwd": (c_int, [c_void_p] * 3 + [c_int64, c_int, c_void_p, c_int, c_int64, c_int64, c_float] + [c_void_p] * 5),
     "b200moe_lora_fwd_ws_bytes": (c_size_t, [c_int64] * 3 + [c_int]),
     "b200moe_lora_forward": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_float, c_void_p, c_int64] + [c_int64] * 5 +
                              [c_int] + [c_void_p] * 4),

@@ -21,6 +21,7 @@ enum : int {
   ST_BAD_EXPERT_INDEX = 5,// permute: an expert index outside [0, E)
   ST_SELFTEST_TIMEOUT = 6,// self-test: a wait that nothing completes ran out, as intended
   ST_WAIT_PEER = 7,       // cross-rank barrier: a peer's arrival never showed up within the limit
+  ST_WAIT_ROWS = 10,      // norm: a row's copy never arrived
   ST_BAD_ADAPTER_INDEX = 9,// adapters: a row names one that there is none of
   ST_EP_CAPACITY = 8      // expert parallel with fixed buffers: a rank would receive more rows than its buffers hold
 };

@@ -540,6 +540,7 @@ optional<Tensor> moe_fp8_block(const Tensor& x, const Tensor& idx, const Tensor&
 // ---------------------------------------------------------------------------- root-mean-square norm
 struct NormArgs {
   optional<Tensor> residual;
+  Tensor status;
   Tensor q, scale;      // codes and [block][row] scales to be filled, or undefined
   int type, w_type;
   double eps;
@@ -552,7 +553,7 @@ variable_list norm_forward(const Tensor& x, const Tensor& w, const NormArgs& a) 
   Tensor y = a.want_y ? at::empty(x.sizes(), x.options()) : Tensor();
   Tensor h = a.residual.has_value() ? at::empty(x.sizes(), x.options()) : Tensor();
   check(b200moe_rms_norm_fwd(ptr(x), K, ptr(a.residual), K, a.type, ptr(w), a.w_type, N, K, static_cast<float>(a.eps), ptr(y), ptr(h), ptr(a.q),
-                             static_cast<float*>(ptr(a.scale)), a.scale.defined() ? a.scale.size(1) : 0, stream_of(x)));
+                             static_cast<float*>(ptr(a.scale)), a.scale.defined() ? a.scale.size(1) : 0, status_ptr(a.status), stream_of(x)));
   variable_list r;
   if (y.defined()) r.push_back(y);
   if (h.defined()) r.push_back(h);
@@ -565,6 +566,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     variable_list r = norm_forward(x, w, a);
     ctx->save_for_backward({residual.has_value() ? r.back() : x, w});
     ctx->saved_data["y"] = a.want_y;
+    ctx->saved_data["status"] = a.status;
     ctx->saved_data["type"] = a.type;
     ctx->saved_data["w_type"] = a.w_type;
     ctx->saved_data["eps"] = a.eps;
@@ -590,7 +592,8 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     Tensor gx = need_x || need_r ? at::empty(h.sizes(), h.options()) : Tensor(), gw = need_w ? at::empty(w.sizes(), w.options()) : Tensor();
     Tensor ws = need_w ? bytes(b200moe_rms_norm_bwd_ws_bytes(N, K), h) : Tensor();
     check(b200moe_rms_norm_bwd(ptr(gy), ptr(gh), ptr(h), K, ctx->saved_data["type"].toInt(), ptr(w), ctx->saved_data["w_type"].toInt(), N, K,
-                               static_cast<float>(ctx->saved_data["eps"].toDouble()), ptr(ws), ptr(gx), ptr(gw), stream_of(h)));
+                               static_cast<float>(ctx->saved_data["eps"].toDouble()), ptr(ws), ptr(gx), ptr(gw),
+                               status_ptr(ctx->saved_data["status"].toTensor()), stream_of(h)));
     if (need_x) res[0] = gx;
     if (need_r) res[2] = gx;
     res[1] = gw;
@@ -601,7 +604,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
 // (y, h, codes, scales): those that were asked for; or None
 optional<std::tuple<optional<Tensor>, optional<Tensor>, optional<Tensor>, optional<Tensor>>> rms_norm(const Tensor& x, const Tensor& w,
                                                                                                       const optional<Tensor>& residual, double eps,
-                                                                                                      bool want_y, bool want_codes) {
+                                                                                                      bool want_y, bool want_codes, const Tensor& status) {
   if (!plain_call(x)) return std::nullopt;
   const auto dev = x.device();
   const auto type = logits_type(x), w_type = logits_type(w);
@@ -611,7 +614,7 @@ optional<std::tuple<optional<Tensor>, optional<Tensor>, optional<Tensor>, option
   const int64_t K = x.size(-1), N = x.numel() / K;
   if (K > 16384 || (want_codes && K % 8 != 0) || !(eps >= 0.0) || N >= (1LL << 31) - 256) return std::nullopt;
   const c10::cuda::CUDAGuard guard(dev);
-  NormArgs a{residual, Tensor(), Tensor(), *type, *w_type, eps, want_y};
+  NormArgs a{residual, status, Tensor(), Tensor(), *type, *w_type, eps, want_y};
   if (want_codes) {
     a.q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
     a.scale = at::empty({(K + 127) / 128, (N + 127) / 128 * 128}, x.options().dtype(at::kFloat));

@@ -42,7 +42,7 @@ class _RmsNorm(torch.autograd.Function):
             if N:
                 L.check(lib.b200moe_rms_norm_fwd(x2.data_ptr(), x2.stride(0), L.ptr(r2), 0 if r2 is None else r2.stride(0), ops._LOGITS[x.dtype],
                                                  weight.data_ptr(), ops._LOGITS[weight.dtype], N, K, eps, L.ptr(y), L.ptr(h), L.ptr(q), L.ptr(scale),
-                                                 pitch, L.stream_of(x)))
+                                                 pitch, L.status_word(dev).data_ptr(), L.stream_of(x)))
         ctx.save_for_backward(x if h is None else h, weight)
         ctx.eps = eps
         if want_codes:
@@ -68,7 +68,7 @@ class _RmsNorm(torch.autograd.Function):
             if N or need_w:
                 L.check(lib.b200moe_rms_norm_bwd(grad_y.data_ptr(), L.ptr(grad_h), h2.data_ptr(), max(h2.stride(0), K), ops._LOGITS[h.dtype],
                                                  weight.data_ptr(), ops._LOGITS[weight.dtype], N, K, ctx.eps, L.ptr(ws), L.ptr(gx), L.ptr(gw),
-                                                 L.stream_of(h)))
+                                                 L.status_word(dev).data_ptr(), L.stream_of(h)))
         return gx if need_x else None, gx if need_r else None, gw, None, None, None
 
 
@@ -93,7 +93,7 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
     weight, through y and h."""
     fast = L.fast() if x.is_cuda else None
     if fast is not None:
-        res = fast.rms_norm(x, weight, residual, eps, True, False)
+        res = fast.rms_norm(x, weight, residual, eps, True, False, L.status_word(x.device))
         if res is not None:
             return res[0] if residual is None else res[:2]
     eps = _check(x, weight, residual, eps, False)
@@ -107,7 +107,7 @@ def rms_norm_fp8_block(x, weight, residual=None, eps=1e-6, return_norm=False):
     rounding (`fp8_block_quantize(y)` rounds twice).  `fp8_block_linear(y, w, s, quantized=(codes, scales))` takes them; they carry no gradient,
     y and h do."""
     fast = L.fast() if x.is_cuda else None
-    res = None if fast is None else fast.rms_norm(x, weight, residual, eps, bool(return_norm), True)
+    res = None if fast is None else fast.rms_norm(x, weight, residual, eps, bool(return_norm), True, L.status_word(x.device))
     if res is not None:
         y, h, q, scale = res
         return (q, scale) + ((y,) if return_norm else ()) + ((h,) if residual is not None else ())
