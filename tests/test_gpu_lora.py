@@ -298,7 +298,7 @@ def test_traced_forward_gradients_and_autocast(pkg):
 
 
 def test_observer(pkg):
-    x, a, b, s, bs, index = make(300, 256, 64, 16, 3)
+    x, a, b, s, bs, index = make(3000, 256, 64, 16, 3)
 
     def seen(call):
         names = []

@@ -49,14 +49,25 @@ __device__ __forceinline__ int lora_adapter(const LoraIndex& p, long long t) {
   return l < 0 ? -1 : static_cast<int>(l);
 }
 
-// barriers inside: every thread of the CTA calls it
-__device__ __forceinline__ void lora_slots(const LoraIndex& p, int tile, LoraSlots& s) {
+// this thread's row's, asked for ahead
+__device__ __forceinline__ int lora_ahead(const LoraIndex& p, int tile) {
+  return threadIdx.x < kLTile ? lora_adapter(p, static_cast<long long>(tile) * kLTile + threadIdx.x) : -1;
+}
+// l: lora_ahead.  Barriers inside: every thread of the CTA calls it
+__device__ __forceinline__ void lora_slots(const LoraIndex& p, int l, LoraSlots& s) {
   const int t = threadIdx.x;
-  int l = -1, at = -1;
-  if (t < kLTile) {
-    l = lora_adapter(p, static_cast<long long>(tile) * kLTile + t);
-    s.of_row[t] = l;
+  if (p.index == nullptr) {
+    if (t < kLTile) {
+      s.of_row[t] = l;
+      s.slot[t] = l;
+      s.adapter[0] = 0;
+    }
+    if (t == 0) s.n = 1;
+    __syncthreads();
+    return;
   }
+  int at = -1;
+  if (t < kLTile) s.of_row[t] = l;
   __syncthreads();
   bool first = false;
   unsigned firsts = 0;
@@ -99,15 +110,35 @@ __device__ __forceinline__ void lora_fetch(uint32_t taddr, bool mine, float (&v)
   }
 }
 
+// four neighbouring sums of every CTA of the cluster, added up in their order: all loads on their way at once
+__device__ __forceinline__ float4 cluster_sum4(uint32_t at, int ctas) {
+  float4 v[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (k < ctas)
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(v[k].x), "=f"(v[k].y), "=f"(v[k].z), "=f"(v[k].w)
+                   : "r"(mapa_shared(at, k))
+                   : "memory");
+  }
+#pragma unroll
+  for (int k = 1; k < 8; ++k) {
+    v[0].x += v[k].x; v[0].y += v[k].y; v[0].z += v[k].z; v[0].w += v[k].w;
+  }
+  return v[0];
+}
+
 // ------------------------------------------------------------------------------------------------ shrink
 // v[t, r] = s_l sum_d X[t, d] W_l[r, d].  A cluster of `split` CTAs shares a tile's columns d and adds up its partial sums through distributed
 // shared memory.  WMN: W_l lies (D, R), reduction index first (the backward's B).  As many adapters as fit 128 accumulator columns a pass.
-constexpr int kShrinkStages = 3, kShrinkStage = 2 * kLBox, kShrinkThreads = 192;
-constexpr int kShrinkSmem = kShrinkStages * kShrinkStage + (2 * kShrinkStages + 2) * 8 + 16 + 1024;
+constexpr int kShrinkMost = 5, kShrinkThreads = 192, kShrinkRing = 96 << 10;      // stages: of X and of the adapters that a pass can have
+constexpr int kShrinkSmem = kShrinkRing + (2 * kShrinkMost + 2) * 8 + 16 + 1024;
 
 struct ShrinkParams {
   LoraIndex ix;
   int D, R, split;
+  int stages, stage;         // of the ring, bytes of one
   const float* scales;       // (L,), or nullptr: `scale` for all
   float scale;
   __nv_bfloat16* v;          // (T, RP)
@@ -122,18 +153,18 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
   constexpr int SLOTS = 128 / NB;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kShrinkStages * kShrinkStage);
-  const uint32_t bar_full = smem_u32(bars), bar_empty = smem_u32(bars + kShrinkStages);
-  const uint32_t bar_tfull = smem_u32(bars + 2 * kShrinkStages), bar_tempty = bar_tfull + 8;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kShrinkStages + 2);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kShrinkRing);
+  const uint32_t bar_full = smem_u32(bars), bar_empty = smem_u32(bars + kShrinkMost);
+  const uint32_t bar_tfull = smem_u32(bars + 2 * kShrinkMost), bar_tempty = bar_tfull + 8;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kShrinkMost + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   __shared__ LoraSlots slots;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = p.split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int tile = blockIdx.x / p.split;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kShrinkStages; ++s) {
-      mbar_init(bar_full + 8 * s, 1);
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(bar_full + 8 * s, 2);        // X, and the adapters
       mbar_init(bar_empty + 8 * s, 1);
     }
     mbar_init(bar_tfull, 1);
@@ -148,12 +179,18 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     tmem_relinquish();
   }
   grid_dep_wait();
-  tc_fence_before();
-  lora_slots(p.ix, tile, slots);
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
   const int nkb = (p.D + 63) / 64;
   const int kb0 = static_cast<int>(static_cast<long long>(rank) * nkb / p.split), kb1 = static_cast<int>(static_cast<long long>(rank + 1) * nkb / p.split);
+  const int ahead = min(p.stages, kb1 - kb0);
+  if (threadIdx.x == 0)      // rows of X are on their way while the tile's adapters are looked up
+    for (int s = 0; s < ahead; ++s) {
+      mbar_arrive_expect_tx(bar_full + 8 * s, kLBox);
+      tma_load_3d(smem_u32(smem + s * p.stage), &tmX, bar_full + 8 * s, (kb0 + s) * 64, tile * kLTile, 0);
+    }
+  tc_fence_before();
+  lora_slots(p.ix, lora_ahead(p.ix, tile), slots);
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
   const int passes = (slots.n + SLOTS - 1) / SLOTS;
   float v[RP];
 #pragma unroll
@@ -171,9 +208,12 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
             ok = false;
             break;
           }
-          const uint32_t full = bar_full + 8 * s, sx = smem_u32(smem + s * kShrinkStage), sw = sx + kLBox;
-          mbar_arrive_expect_tx(full, kLBox + n * NB * 128);
-          tma_load_3d(sx, &tmX, full, kb * 64, tile * kLTile, 0);
+          const uint32_t full = bar_full + 8 * s, sx = smem_u32(smem + s * p.stage), sw = sx + kLBox;
+          if (pass > 0 || kb - kb0 >= ahead) {
+            mbar_arrive_expect_tx(full, kLBox);
+            tma_load_3d(sx, &tmX, full, kb * 64, tile * kLTile, 0);
+          }
+          mbar_arrive_expect_tx(full, n * NB * 128);
           for (int j = 0; j < n; ++j) {
             const int l = slots.adapter[first + j];
             if constexpr (WMN) {
@@ -183,13 +223,20 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
               tma_load_3d(sw + j * NB * 128, &tmW, full, kb * 64, 0, l);
             }
           }
-          if (++s == kShrinkStages) {
+          if (++s == p.stages) {
             s = 0;
             ph ^= 1;
           }
         }
       }
     }
+    __syncwarp();
+    if (passes == 0 && lane == 0)      // nobody reads the rows that are on their way
+      for (int s = 0; s < ahead; ++s) {
+        mbar_arrive(bar_full + 8 * s);
+        mbar_wait(bar_full + 8 * s, 0, abort_flag, ST_WAIT_PRODUCER);
+      }
+    __syncwarp();
     grid_dep_launch();
   } else if (warp == 1) {
     if (elect_one()) {
@@ -207,13 +254,13 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
             break;
           }
           tc_fence_after();
-          const uint32_t sx = smem_u32(smem + s * kShrinkStage), sw = sx + kLBox;
+          const uint32_t sx = smem_u32(smem + s * p.stage), sw = sx + kLBox;
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             umma_bf16(tmem, umma_desc_sw128(sx + 32 * k, 0, 1024), umma_desc_sw128(sw + (WMN ? 2048 : 32) * k, WMN ? 8192 : 0, 1024), idesc,
                       kb != kb0 || k != 0);
           umma_commit(bar_empty + 8 * s);
-          if (++s == kShrinkStages) {
+          if (++s == p.stages) {
             s = 0;
             ph ^= 1;
           }
@@ -253,9 +300,9 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
         }
       }
     } else {      // every load of this CTA has been used: its stages are free
-      float* mine_s = reinterpret_cast<float*>(smem) + row * (RP + 1);
+      float4* to = reinterpret_cast<float4*>(smem + row * (RP + 4) * 4);
 #pragma unroll
-      for (int i = 0; i < RP; ++i) mine_s[i] = v[i];
+      for (int i = 0; i < RP; i += 4) to[i / 4] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
     }
   }
   __syncwarp();
@@ -269,20 +316,14 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     __syncwarp();
     cluster_sync_all();
     const int rows = kLTile / p.split;
-    for (int i = threadIdx.x; i < rows * (RP / 2); i += kShrinkThreads) {
-      const int row = rank * rows + i / (RP / 2), c = 2 * (i % (RP / 2)), mine = slots.slot[row];
+    for (int i = threadIdx.x; i < rows * (RP / 4); i += kShrinkThreads) {
+      const int row = rank * rows + i / (RP / 4), c = 4 * (i % (RP / 4)), mine = slots.slot[row];
       const long long t = static_cast<long long>(tile) * kLTile + row;
-      float a = 0.0f, b = 0.0f;
-      for (int r = 0; r < p.split; ++r) {
-        const uint32_t at = mapa_shared(smem_u32(smem) + 4 * (row * (RP + 1) + c), r);
-        float a1, b1;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(a1) : "r"(at) : "memory");
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(b1) : "r"(at + 4) : "memory");
-        a += a1;
-        b += b1;
-      }
+      const float4 v4 = cluster_sum4(smem_u32(smem) + 4 * (row * (RP + 4) + c), p.split);
       const float s = mine < 0 ? 0.0f : p.scales != nullptr ? p.scales[slots.adapter[mine]] : p.scale;
-      if (t < p.ix.T) *reinterpret_cast<uint32_t*>(p.v + t * RP + c) = mine >= 0 && c < p.R ? pack_bf16x2(s * a, s * b) : 0u;
+      if (t < p.ix.T)
+        *reinterpret_cast<uint2*>(p.v + t * RP + c) =
+            mine >= 0 && c < p.R ? make_uint2(pack_bf16x2(s * v4.x, s * v4.y), pack_bf16x2(s * v4.z, s * v4.w)) : make_uint2(0u, 0u);
     }
     __syncwarp();
     cluster_sync_all();      // nobody leaves while another reads its sums
@@ -295,12 +336,14 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
 
 // ------------------------------------------------------------------------------------------------ expand
 // out[t, n] = base[t, n] + sum_r v[t, r] W_l[n, r]; WMN: W_l lies (R, N) (the backward's A).  Persistent CTAs over (row tile, 128 columns), a row
-// tile's columns one after another.  The base's boxes land where the result leaves from; tensor memory holds four (columns, adapter) products.
-constexpr int kExpEpi = 8, kExpThreads = 64 + 32 * kExpEpi, kExpBase = 3;
+// tile's columns one after another.  The base's boxes land where the result leaves from: an epilogue warp fetches its own, a few tiles ahead whatever the
+// adapters' products wait for; tensor memory holds four (columns, adapter) products.
+constexpr int kExpEpi = 8, kExpThreads = 64 + 32 * kExpEpi;
 constexpr int kExpOut = 128 * 128 * 2;
+template <int RP> constexpr int kExpBase = RP > 64 ? 3 : 4;
 template <int RP> constexpr int kExpW = (RP > 64 ? 2 : 1) * kLBox;               // one adapter's 128 columns
-template <int RP> constexpr int kExpWStages = RP > 64 ? 2 : 3;
-template <int RP> constexpr int kExpSmem = kExpBase * kExpOut + (kExpWStages<RP> + 1) * kExpW<RP> + (2 * kExpBase + 2 * kExpWStages<RP> + 9) * 8 + 16 + 1024;
+template <int RP> constexpr int kExpWStages = RP > 64 ? 2 : 4;
+template <int RP> constexpr int kExpSmem = kExpBase<RP> * kExpOut + (kExpWStages<RP> + 1) * kExpW<RP> + (kExpEpi * kExpBase<RP> + 2 * kExpWStages<RP> + 9) * 8 + 16 + 1024;
 
 struct ExpandParams {
   LoraIndex ix;
@@ -311,23 +354,20 @@ template <int RP, bool WMN>
 __global__ void __launch_bounds__(kExpThreads, 1)
 lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmBase,
                    const __grid_constant__ CUtensorMap tmOut, const ExpandParams p) {
-  constexpr int WS = kExpWStages<RP>, W = kExpW<RP>;
+  constexpr int WS = kExpWStages<RP>, W = kExpW<RP>, BASES = kExpBase<RP>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t *s_w = smem + kExpBase * kExpOut, *s_v = s_w + WS * W;
+  uint8_t *s_w = smem + BASES * kExpOut, *s_v = s_w + WS * W;
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_v + W);
-  const uint32_t bar_bfull = smem_u32(bars), bar_bempty = bar_bfull + 8 * kExpBase;
-  const uint32_t bar_wfull = bar_bempty + 8 * kExpBase, bar_wempty = bar_wfull + 8 * WS;
+  const uint32_t bar_base = smem_u32(bars);      // [stage][epilogue warp]
+  const uint32_t bar_wfull = bar_base + 8 * kExpEpi * BASES, bar_wempty = bar_wfull + 8 * WS;
   const uint32_t bar_tfull = bar_wempty + 8 * WS, bar_tempty = bar_tfull + 32, bar_v = bar_tempty + 32;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kExpBase + 2 * WS + 9);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kExpEpi * BASES + 2 * WS + 9);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   __shared__ LoraSlots slots;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kExpBase; ++s) {
-      mbar_init(bar_bfull + 8 * s, 1);
-      mbar_init(bar_bempty + 8 * s, kExpEpi);
-    }
+    for (int s = 0; s < kExpEpi * BASES; ++s) mbar_init(bar_base + 8 * s, 1);
     for (int s = 0; s < WS; ++s) {
       mbar_init(bar_wfull + 8 * s, 1);
       mbar_init(bar_wempty + 8 * s, 1);
@@ -360,12 +400,27 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
   int bs = 0, ws = 0, buf = 0;                       // places in the rings, their phases
   uint32_t bph = 0, wph = 0, tph = 0, vph = 0;
   bool ok = true;
+  const int q = warp & 3, part = (warp - 2) >> 2;    // epilogue: the quarter of the rows, the half of the columns
+  const uint32_t my_box = smem_u32(smem) + (4 * part + q) * 4096;
+  auto fetch_base = [&](long long i, int stage) {
+    if (i >= end) return;
+    const int tile = static_cast<int>(i / nct), ct = static_cast<int>(i - static_cast<long long>(tile) * nct);
+    mbar_arrive_expect_tx(bar_base + 8 * (kExpEpi * stage + warp - 2), 4096);
+    tma_load_3d(my_box + stage * kExpOut, &tmBase, bar_base + 8 * (kExpEpi * stage + warp - 2), ct * 128 + 64 * part, tile * kLTile + 32 * q, 0);
+  };
+  if (p.has_base && warp >= 2 && lane == 0)
+    for (int i = 0; i < BASES; ++i) fetch_base(item + i, i);
+  __syncwarp();
+  const long long first_item = item;
+  long long now = item;                              // epilogue: the tile at hand
+  int mine_next = lora_ahead(p.ix, static_cast<int>(item / nct));
   while (item < end) {
     const int tile = static_cast<int>(item / nct), ct0 = static_cast<int>(item - static_cast<long long>(tile) * nct);
     const int ct1 = static_cast<int>(min(static_cast<long long>(nct), ct0 + (end - item)));
     item += ct1 - ct0;
-    lora_slots(p.ix, tile, slots);
+    lora_slots(p.ix, mine_next, slots);
     const int n = slots.n;
+    if (item < end) mine_next = lora_ahead(p.ix, tile + 1);
     if (warp == 0) {
       if (elect_one()) {
         if (n > 0) {
@@ -373,18 +428,6 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
           for (int h = 0; h < W / kLBox; ++h) tma_load_3d(smem_u32(s_v) + h * kLBox, &tmV, bar_v, 64 * h, tile * kLTile, 0);
         }
         for (int ct = ct0; ct < ct1 && ok; ++ct) {
-          if (p.has_base) {
-            ok = mbar_wait(bar_bempty + 8 * bs, bph ^ 1, abort_flag, ST_WAIT_PRODUCER);
-            if (!ok) break;
-            const uint32_t full = bar_bfull + 8 * bs, to = smem_u32(smem + bs * kExpOut);
-            mbar_arrive_expect_tx(full, kExpOut);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) tma_load_3d(to + i * 4096, &tmBase, full, ct * 128 + 64 * (i >> 2), tile * kLTile + 32 * (i & 3), 0);
-            if (++bs == kExpBase) {
-              bs = 0;
-              bph ^= 1;
-            }
-          }
           for (int j = 0; j < n; ++j) {
             ok = mbar_wait(bar_wempty + 8 * ws, wph ^ 1, abort_flag, ST_WAIT_PRODUCER);
             if (!ok) break;
@@ -437,17 +480,31 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
         }
       }
     } else {
-      const int q = warp & 3, part = (warp - 2) >> 2, mine = slots.slot[32 * q + lane];
+      const int mine = slots.slot[32 * q + lane];
       const uint32_t taddr = tmem + (static_cast<uint32_t>(32 * q) << 16) + 64 * part;
-      for (int ct = ct0; ct < ct1; ++ct) {
+      for (int ct = ct0; ct < ct1; ++ct, ++now) {
         float acc[64];
+        if (n != 1) {
 #pragma unroll
-        for (int i = 0; i < 64; ++i) acc[i] = 0.0f;
+          for (int i = 0; i < 64; ++i) acc[i] = 0.0f;
+        }
         for (int j = 0; j < n; ++j) {
           ok = ok && mbar_wait(bar_tfull + 8 * buf, tph, abort_flag, ST_WAIT_EPILOGUE);
           __syncwarp();
           tc_fence_after();
-          if (__any_sync(0xffffffffu, mine == j)) lora_fetch<64>(taddr + 128 * buf, mine == j, acc);
+          if (n == 1 || __any_sync(0xffffffffu, mine == j)) {
+            uint32_t r[2][32];
+            tmem_ld32(taddr + 128 * buf, r[0]);
+            tmem_ld32(taddr + 128 * buf + 32, r[1]);
+            tmem_ld_wait();
+            if (n == 1) {
+#pragma unroll
+              for (int i = 0; i < 64; ++i) acc[i] = mine == 0 ? __uint_as_float(r[i >> 5][i & 31]) : 0.0f;
+            } else {
+#pragma unroll
+              for (int i = 0; i < 64; ++i) acc[i] = mine == j ? __uint_as_float(r[i >> 5][i & 31]) : acc[i];
+            }
+          }
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_tempty + 8 * buf);
@@ -457,12 +514,9 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
           }
         }
         uint8_t* box = smem + bs * kExpOut + (4 * part + q) * 4096;
-        if (p.has_base) ok = ok && mbar_wait(bar_bfull + 8 * bs, bph, abort_flag, ST_WAIT_EPILOGUE);
+        if (p.has_base) ok = ok && mbar_wait(bar_base + 8 * (kExpEpi * bs + warp - 2), bph, abort_flag, ST_WAIT_EPILOGUE);
+        else if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(BASES - 1) : "memory");      // the box's result of a round ago has left
         ok = __all_sync(0xffffffffu, ok);
-        if (!p.has_base) {       // the box's result of three tiles ago has left
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kExpBase - 1) : "memory");
-          __syncwarp();
-        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           uint4* at = reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4));
@@ -483,12 +537,12 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
         if (lane == 0) {
           if (ok && ct * 128 + 64 * part < p.N && tile * kLTile + 32 * q < p.ix.T) tma_store_3d(&tmOut, smem_u32(box), ct * 128 + 64 * part, tile * kLTile + 32 * q, 0);
           bulk_commit_group();
-          if (p.has_base) {
-            bulk_wait_read_all();
-            mbar_arrive(bar_bempty + 8 * bs);
+          if (p.has_base && now > first_item) {      // the result before has left its box, which takes the base of a tile to come
+            asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+            fetch_base(now - 1 + BASES, bs == 0 ? BASES - 1 : bs - 1);
           }
         }
-        if (++bs == kExpBase) {
+        if (++bs == BASES) {
           bs = 0;
           bph ^= 1;
         }
@@ -653,67 +707,76 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap tmY, const __grid_constant
     if (any) ok = ok && mbar_wait(bar_tfull, 0, abort_flag, ST_WAIT_EPILOGUE);
     __syncwarp();
     tc_fence_after();
+    // this CTA's sums into shared memory, whose stages have all been used
     const uint32_t taddr = tmem + (static_cast<uint32_t>(32 * q) << 16);
-    const int d = chunk * 128 + 32 * q + lane;
-    const long long at = (static_cast<long long>(split) * p.L + l) * p.D * p.R;
+    float4* to = reinterpret_cast<float4*>(smem + (32 * q + lane) * (RP + 4) * 4);
 #pragma unroll
     for (int c = 0; c < RP; c += 16) {
       float v[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = 0.0f;
       if (any) lora_fetch<16>(taddr + c, true, v);
-      if (d < p.D) {
-        if (p.transposed) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (c + i < p.R) {
-              const long long o = at + static_cast<long long>(c + i) * p.D + d;
-              if (p.out_f32) static_cast<float*>(p.out)[o] = v[i];
-              else static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(v[i]);
-            }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; i += 8)
-            if (c + i < p.R) {
-              const long long o = at + static_cast<long long>(d) * p.R + c + i;
-              if (p.out_f32) {
-                float4* to = reinterpret_cast<float4*>(static_cast<float*>(p.out) + o);
-                to[0] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                to[1] = make_float4(v[i + 4], v[i + 5], v[i + 6], v[i + 7]);
-              } else {
-                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + o) =
-                    make_uint4(pack_bf16x2(v[i], v[i + 1]), pack_bf16x2(v[i + 2], v[i + 3]), pack_bf16x2(v[i + 4], v[i + 5]), pack_bf16x2(v[i + 6], v[i + 7]));
-              }
-            }
-        }
-      }
+      for (int i = 0; i < 16; i += 4) to[(c + i) / 4] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
     }
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  // ... and out of it, four r a thread
+  const int d0 = chunk * 128;
+  const long long at = (static_cast<long long>(split) * p.L + l) * p.D * p.R;
+  for (int i = threadIdx.x; i < 128 * (p.R / 4); i += kWgThreads) {
+    const int row = p.transposed ? i % 128 : i / (p.R / 4), r = 4 * (p.transposed ? i / 128 : i % (p.R / 4));
+    const float4 v = *reinterpret_cast<const float4*>(smem + 4 * (row * (RP + 4) + r));
+    if (d0 + row >= p.D) continue;
+    if (p.transposed) {
+      const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const long long o = at + static_cast<long long>(r + h) * p.D + d0 + row;
+        if (p.out_f32) static_cast<float*>(p.out)[o] = f[h];
+        else static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(f[h]);
+      }
+    } else {
+      const long long o = at + static_cast<long long>(d0 + row) * p.R + r;
+      if (p.out_f32) *reinterpret_cast<float4*>(static_cast<float*>(p.out) + o) = v;
+      else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + o) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+    }
+  }
   if (warp == 1) tmem_dealloc(tmem, NB);
   if (threadIdx.x == 0 && *abort_flag != 0) *p.status = *abort_flag;
 }
 
-// the sum of the splits' shares, n values (a multiple of 4)
-__global__ void __launch_bounds__(256) lora_wgrad_sum_kernel(const float* part, int splits, long long n, void* out, int out_f32) {
+// the sum of the splits' shares, n values (a multiple of 4), always in the same order; eight of them are on their way at a time
+__global__ void __launch_bounds__(128) lora_wgrad_sum_kernel(const float* part, int splits, long long n, void* out, int out_f32) {
   grid_dep_begin();
-  for (long long i = 4 * (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x); i < n; i += 1024LL * gridDim.x) {
-    float4 v = *reinterpret_cast<const float4*>(part + i);
-    for (int s = 1; s < splits; ++s) {
-      const float4 o = *reinterpret_cast<const float4*>(part + s * n + i);
-      v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+  const long long i = 4 * (static_cast<long long>(blockIdx.x) * 128 + threadIdx.x);
+  if (i >= n) return;
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int s = 0; s < splits; s += 8) {
+    float4 o[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) o[u] = s + u < splits ? *reinterpret_cast<const float4*>(part + (s + u) * n + i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      v.x += o[u].x; v.y += o[u].y; v.z += o[u].z; v.w += o[u].w;
     }
-    if (out_f32) *reinterpret_cast<float4*>(static_cast<float*>(out) + i) = v;
-    else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(out) + i) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
   }
+  if (out_f32) *reinterpret_cast<float4*>(static_cast<float*>(out) + i) = v;
+  else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(out) + i) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
-// A cluster of eight CTAs a row (and share of the columns, where rows are fewer than SMs): each CTA multiplies an eighth of x with all R rows of
-// A_l, the sums meet in distributed shared memory, and each expands its columns from fp32 values that were never rounded.
-constexpr int kFewCluster = 8, kFewThreads = 256;
+// A cluster of eight CTAs takes up to sixteen rows of one adapter (and a share of the columns, where such groups are fewer than SMs): each CTA multiplies
+// an eighth of the rows with all of A_l, the sums meet in distributed shared memory, and each expands its columns.  Both products are m16n8k16
+// instructions; the order of the reduction index within one is free as long as both operands have it, so a lane's share of x and A_l is 16 neighbouring
+// bytes of global memory, of B_l 8 of shared memory.  v is never rounded: it is split into two bf16 numbers that hold 16 bits of it.
+// Bound by latency: bulk copies of the first columns of B_l and of the base are on their way while x and A_l are multiplied, and the result leaves from
+// where the base landed.
+constexpr int kFewCluster = 8, kFewThreads = 256, kFewWarps = kFewThreads / 32, kFewRows = 16, kFewBlock = 128;
+constexpr int kFewChunk = 20 << 10;      // of two: columns of B_l, and of the base and the result of each row
+static int few_smem(int64_t R) { return static_cast<int>(2 * kFewChunk + kFewRows * R * 4 + std::max<int64_t>(4096, (R + 15) / 16 * 1024)); }
 
 struct FewLora {
   LoraIndex ix;
@@ -725,81 +788,244 @@ struct FewLora {
   float scale;
 };
 
-__device__ __forceinline__ float dot8(const uint4& a, const uint4& b, float s) {
-  const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = unpack_bf16x2(x[i]), g = unpack_bf16x2(y[i]);
-    s = fmaf(f.x, g.x, s);
-    s = fmaf(f.y, g.y, s);
-  }
-  return s;
+// A cluster's rows: found by every CTA of it.  The rows of a block of 128 are ranked among those of their adapter (or of none) in it; sixteen ranks make a
+// group, in the order of their first rows.  Returns the number of rows, 0: there is no such group in the block.  Barriers inside.
+struct __align__(16) FewGroup {
+  int adapter[kFewBlock];
+  int rank[kFewBlock];
+  unsigned first[kFewBlock / 32];      // rows that begin a group
+  int rows[kFewRows];
+  int n, l;
+};
+// groups of a block at most: one for each sixteen rows and one more for each adapter and for none
+__host__ __device__ inline int few_groups(const LoraIndex& ix) {
+  const int rows = ix.T < kFewBlock ? ix.T : kFewBlock, more = ix.index == nullptr || ix.T == 1 ? 0 : ix.L + 1;
+  return rows < (rows + kFewRows - 1) / kFewRows + more ? rows : (rows + kFewRows - 1) / kFewRows + more;
 }
-
-__global__ void __launch_bounds__(kFewThreads) lora_few_kernel(const FewLora p) {
-  grid_dep_begin();
-  __shared__ float sums[128], v[128];
-  const int rank = static_cast<int>(cluster_ctarank()), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int c = static_cast<int>(cluster_id_x()), part = c % p.parts;
-  const long long t = c / p.parts;
-  const int l = lora_adapter(p.ix, t);
-  if (l >= 0) {
-    const int vecs = p.K / 8, v0 = rank * vecs / kFewCluster, v1 = (rank + 1) * vecs / kFewCluster;
-    const uint4* x = reinterpret_cast<const uint4*>(p.x + t * p.ldx);
-    for (int r = warp; r < p.R; r += 2 * (kFewThreads / 32)) {       // two rows of A at a time
-      const int r2 = r + kFewThreads / 32;
-      const uint4* a = reinterpret_cast<const uint4*>(p.a + (static_cast<long long>(l) * p.R + r) * p.K);
-      const uint4* a2 = reinterpret_cast<const uint4*>(p.a + (static_cast<long long>(l) * p.R + min(r2, p.R - 1)) * p.K);
-      float s = 0.0f, s2 = 0.0f;
-#pragma unroll 2
-      for (int i = v0 + lane; i < v1; i += 32) {
-        const uint4 xv = x[i];
-        s = dot8(xv, a[i], s);
-        s2 = dot8(xv, a2[i], s2);
-      }
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) {
-        s += __shfl_xor_sync(0xffffffffu, s, off);
-        s2 += __shfl_xor_sync(0xffffffffu, s2, off);
-      }
-      if (lane == 0) {
-        sums[r] = s;
-        if (r2 < p.R) sums[r2] = s2;
-      }
-    }
+__device__ __forceinline__ int few_group(const LoraIndex& ix, int block, int group, FewGroup& s) {
+  const int row0 = block * kFewBlock, t = threadIdx.x, left = ix.T - row0;
+  if (ix.index == nullptr || ix.T == 1) {
+    const int n = max(0, min(kFewRows, left - kFewRows * group));
+    if (t == 0) s.l = lora_adapter(ix, 0);
+    if (t < n) s.rows[t] = row0 + kFewRows * group + t;
+    __syncthreads();
+    return n;
   }
-  cluster_sync_all();
-  if (l >= 0 && static_cast<int>(threadIdx.x) < p.R) {
-    float s = 0.0f;
-    for (int r = 0; r < kFewCluster; ++r) {
-      float o;
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o) : "r"(mapa_shared(smem_u32(sums + threadIdx.x), r)) : "memory");
-      s += o;
+  int l = -2, rank = 0;
+  if (t < kFewBlock) s.adapter[t] = l = t < left ? lora_adapter(ix, row0 + t) : -2;
+  if (t == 0) s.n = 0;
+  __syncthreads();
+  if (t < kFewBlock) {
+    const unsigned same = __match_any_sync(0xffffffffu, l);
+    rank = __popc(same & ((1u << (t & 31)) - 1u));
+#pragma unroll 4
+    for (int j = 0; j < (t >> 5) * 8; ++j) {      // the warps before
+      const int4 o = reinterpret_cast<const int4*>(s.adapter)[j];
+      rank += (o.x == l) + (o.y == l) + (o.z == l) + (o.w == l);
     }
-    v[threadIdx.x] = s * (p.scales != nullptr ? p.scales[l] : p.scale);
+    s.rank[t] = rank;
+    const unsigned m = __ballot_sync(0xffffffffu, t < left && rank % kFewRows == 0);
+    if ((t & 31) == 0) s.first[t >> 5] = m;
   }
   __syncthreads();
-  const int shares = p.parts * kFewCluster, share = part * kFewCluster + rank;
-  const int n0 = static_cast<int>(static_cast<long long>(share) * p.N / shares), n1 = static_cast<int>(static_cast<long long>(share + 1) * p.N / shares);
-  for (int n = n0 + threadIdx.x; n < n1; n += kFewThreads) {
-    float s = p.base != nullptr ? __bfloat162float(p.base[t * p.ldb + n]) : 0.0f;
-    if (l >= 0) {
-      const uint4* b = reinterpret_cast<const uint4*>(p.b + (static_cast<long long>(l) * p.N + n) * p.R);
-      float d = 0.0f;
-      for (int i = 0; i < p.R / 8; ++i) {
-        const uint4 w = b[i];
-        const uint32_t y[4] = {w.x, w.y, w.z, w.w};
+  int leader = -1, skip = group;      // the group-th of the bits
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const float2 f = unpack_bf16x2(y[h]);
-          d = fmaf(f.x, v[8 * i + 2 * h], d);
-          d = fmaf(f.y, v[8 * i + 2 * h + 1], d);
+  for (int w = 0; w < kFewBlock / 32; ++w) {
+    unsigned m = s.first[w];
+    const int c = __popc(m);
+    if (leader < 0 && skip < c) {
+      for (int i = 0; i < skip; ++i) m &= m - 1;
+      leader = 32 * w + __ffs(m) - 1;
+    }
+    skip -= c;
+  }
+  if (leader < 0) return 0;
+  const int from = s.rank[leader], of = s.adapter[leader];
+  if (t < kFewBlock && l == of && rank >= from && rank < from + kFewRows) {
+    s.rows[rank - from] = row0 + t;
+    atomicAdd(&s.n, 1);
+  }
+  if (t == 0) s.l = of;
+  __syncthreads();
+  return s.n;
+}
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// two fp32 numbers as bf16 and what that leaves of them, as bf16 too (nothing of an infinity)
+__device__ __forceinline__ void split_bf16x2(float2 f, uint32_t& hi, uint32_t& lo) {
+  hi = pack_bf16x2(f.x, f.y);
+  const float2 h = unpack_bf16x2(hi);
+  lo = pack_bf16x2(fabsf(h.x) == INFINITY ? 0.0f : f.x - h.x, fabsf(h.y) == INFINITY ? 0.0f : f.y - h.y);
+}
+
+__global__ void __launch_bounds__(kFewThreads, 4) lora_few_kernel(const FewLora p) {
+  extern __shared__ __align__(128) uint8_t smem[];                 // two chunks, sums, and (by turns) partial sums or v as fragments
+  __shared__ FewGroup group;
+  __shared__ __align__(8) uint64_t bars[2];
+  __shared__ int abort_word;
+  float* sums = reinterpret_cast<float*>(smem + 2 * kFewChunk);    // of this CTA, [row][r]
+  float* part = sums + kFewRows * p.R;                             // [warp][row][8 r]
+  uint32_t* frag = reinterpret_cast<uint32_t*>(part);              // [16 r][lane][4 upper, 4 lower halves]
+  const uint32_t bar = smem_u32(bars);
+  if (threadIdx.x == 0) {
+    mbar_init(bar, 1);
+    mbar_init(bar + 8, 1);
+    abort_word = 0;
+    fence_mbar_init();
+  }
+  grid_dep_begin();
+  const int rank = static_cast<int>(cluster_ctarank()), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, q = lane & 3;
+  const int c = static_cast<int>(cluster_id_x()), share = c % p.parts * kFewCluster + rank, shares = p.parts * kFewCluster;
+  const int groups = few_groups(p.ix), n = few_group(p.ix, c / p.parts / groups, c / p.parts % groups, group);
+  if (n == 0) return;                                              // the whole cluster
+  const int l = group.l;
+  const int col0 = 8 * static_cast<int>(static_cast<long long>(share) * (p.N / 8) / shares);
+  const int col1 = 8 * static_cast<int>(static_cast<long long>(share + 1) * (p.N / 8) / shares);
+  const int wide = kFewChunk / (2 * p.R + 2 * n) & ~7, chunks = (col1 - col0 + wide - 1) / wide, ksteps = (p.R + 15) / 16;
+  const int rows_at = wide * p.R * 2;                              // of the base's and the result's rows in a chunk
+
+  const bool copies = l >= 0 || p.base != nullptr;
+  auto fetch = [&](int i) {                                        // warp 0: a lane a row
+    const int col = col0 + i * wide, w = min(wide, col1 - col);
+    const uint32_t to = smem_u32(smem) + (i & 1) * kFewChunk, full = bar + 8 * (i & 1);
+    if (lane == 0) {
+      mbar_arrive_expect_tx(full, (l >= 0 ? w * p.R * 2 : 0) + (p.base != nullptr ? n * w * 2 : 0));
+      if (l >= 0) bulk_load_1d(to, p.b + (static_cast<long long>(l) * p.N + col) * p.R, w * p.R * 2, full);
+    }
+    __syncwarp();
+    if (p.base != nullptr && lane < n) bulk_load_1d(to + rows_at + lane * wide * 2, p.base + group.rows[lane] * p.ldb + col, w * 2, full);
+  };
+  if (warp == 0 && copies)
+    for (int i = 0; i < min(2, chunks); ++i) fetch(i);
+
+  if (l >= 0) {
+    const bool low = g < n, high = g + 8 < n;
+    const __nv_bfloat16 *x0 = p.x + (low ? group.rows[g] : 0) * p.ldx, *x1 = p.x + (high ? group.rows[g + 8] : 0) * p.ldx;
+    // tiles of eight r, and where these are fewer than warps, several warps a tile that split the columns
+    const int rt = p.R / 8, split = rt < kFewWarps ? kFewWarps / rt : 1;
+    const int steps = (p.K + 31) / 32;
+    const int s0 = rank * steps / kFewCluster, s1 = (rank + 1) * steps / kFewCluster;
+    for (int tile = warp % (rt * split) / split; tile < rt && warp < rt * split; tile += kFewWarps / split) {
+      const int w = split > 1 ? warp % split : 0;
+      const int first = s0 + w * (s1 - s0) / split, last = s0 + (w + 1) * (s1 - s0) / split;
+      const __nv_bfloat16* a = p.a + (static_cast<long long>(l) * p.R + 8 * tile + g) * p.K;
+      float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+      for (int s = first; s < last; ++s) {
+        const int k = 32 * s + 8 * q;
+        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+        const uint4 av = k < p.K ? *reinterpret_cast<const uint4*>(a + k) : zero;
+        const uint4 u0 = k < p.K && low ? *reinterpret_cast<const uint4*>(x0 + k) : zero;
+        const uint4 u1 = k < p.K && high ? *reinterpret_cast<const uint4*>(x1 + k) : zero;
+        mma_bf16(d, u0.x, u1.x, u0.y, u1.y, av.x, av.y);
+        mma_bf16(d, u0.z, u1.z, u0.w, u1.w, av.z, av.w);
+      }
+      // one warp a tile: to its place, else to the warps that add up
+      float* to = split > 1 ? part + warp * (kFewRows * 8) : sums + 8 * tile;
+      const int pitch = split > 1 ? 8 : p.R;
+      *reinterpret_cast<float2*>(to + g * pitch + 2 * q) = make_float2(d[0], d[1]);
+      *reinterpret_cast<float2*>(to + (g + 8) * pitch + 2 * q) = make_float2(d[2], d[3]);
+    }
+    if (split > 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < rt * kFewRows * 8; i += kFewThreads) {
+        const int tile = i >> 7, at = i & 127;
+        float s = 0.0f;
+        for (int w = 0; w < split; ++w) s += part[(tile * split + w) * (kFewRows * 8) + at];
+        sums[(at >> 3) * p.R + 8 * tile + (at & 7)] = s;
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();
+    // v of the whole row as the fragments that the second product reads: of each 16 r lane (g, q) holds 4 q ... 4 q + 3 of rows g and g + 8
+    const float scale = p.scales != nullptr ? p.scales[l] : p.scale;
+    for (int i = threadIdx.x; i < ksteps * 128; i += kFewThreads) {
+      const int h = i & 3, at = i >> 2 & 31, row = (at >> 2) + 8 * (h & 1), r = 16 * (i >> 7) + 4 * (at & 3) + 2 * (h >> 1);
+      float2 s = make_float2(0.0f, 0.0f);
+      if (row < n && r < p.R) {
+#pragma unroll
+        for (int k = 0; k < kFewCluster; ++k) {
+          float2 o;
+          asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+                       : "=f"(o.x), "=f"(o.y)
+                       : "r"(mapa_shared(smem_u32(sums + row * p.R + r), k))
+                       : "memory");
+          s.x += o.x;
+          s.y += o.y;
         }
       }
-      s += d;
+      split_bf16x2(make_float2(s.x * scale, s.y * scale), frag[(i >> 7) * 256 + at * 8 + h], frag[(i >> 7) * 256 + at * 8 + 4 + h]);
     }
-    p.out[t * p.N + n] = __float2bfloat16_rn(s);
+    __syncthreads();
   }
+
+  for (int i = 0; i < chunks; ++i) {
+    const int col = col0 + i * wide, w = min(wide, col1 - col);
+    uint8_t *chunk = smem + (i & 1) * kFewChunk, *rows = chunk + rows_at;
+    if (copies) mbar_wait(bar + 8 * (i & 1), i >> 1 & 1, &abort_word, ST_WAIT_ROWS);
+    __syncwarp();
+    constexpr int TILES = 4;                                       // of a warp at a time, fewer at the end
+    const bool half = (p.R & 8) != 0 && q >= 2;                    // the last 16 r have 8 that are not there
+    auto group_of_tiles = [&](int tile0, int tiles, auto whole) {
+      constexpr bool WHOLE = decltype(whole)::value;
+      float d[TILES][4] = {};
+      if (l >= 0) {
+        const uint8_t* b = chunk + (8 * tile0 + g) * p.R * 2 + 8 * q;
+        for (int k = 0; k < ksteps; ++k, b += 32) {
+          const bool in = !(half && k == ksteps - 1);
+          uint2 bw[TILES];
+#pragma unroll
+          for (int j = 0; j < TILES; ++j) bw[j] = in && (WHOLE || j < tiles) ? *reinterpret_cast<const uint2*>(b + 16 * j * p.R) : make_uint2(0u, 0u);
+          const uint4 hi = *reinterpret_cast<const uint4*>(frag + k * 256 + lane * 8), lo = *reinterpret_cast<const uint4*>(frag + k * 256 + lane * 8 + 4);
+#pragma unroll
+          for (int j = 0; j < TILES; ++j) mma_bf16(d[j], lo.x, lo.y, lo.z, lo.w, bw[j].x, bw[j].y);
+#pragma unroll
+          for (int j = 0; j < TILES; ++j) mma_bf16(d[j], hi.x, hi.y, hi.z, hi.w, bw[j].x, bw[j].y);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (8 * h >= n) break;
+        uint32_t* at = reinterpret_cast<uint32_t*>(rows + (g + 8 * h) * wide * 2 + (8 * tile0 + 2 * q) * 2);
+        if (g + 8 * h < n) {
+          uint32_t o[TILES] = {};
+          if (p.base != nullptr)
+#pragma unroll
+            for (int j = 0; j < TILES; ++j)
+              if (WHOLE || j < tiles) o[j] = at[4 * j];
+#pragma unroll
+          for (int j = 0; j < TILES; ++j) {
+            const float2 f = unpack_bf16x2(o[j]);
+            if (WHOLE || j < tiles) at[4 * j] = pack_bf16x2(f.x + d[j][2 * h], f.y + d[j][2 * h + 1]);
+          }
+        }
+      }
+    };
+    for (int tile0 = TILES * warp; tile0 < w / 8; tile0 += TILES * kFewWarps) {
+      if (tile0 + TILES <= w / 8) group_of_tiles(tile0, TILES, std::true_type());
+      else group_of_tiles(tile0, w / 8 - tile0, std::false_type());
+    }
+    fence_proxy_async_smem();
+    __syncthreads();
+    if (warp == 0) {
+      if (lane < n) bulk_store_1d(p.out + static_cast<long long>(group.rows[lane]) * p.N + col, smem_u32(rows) + lane * wide * 2, w * 2);
+      bulk_commit_group();
+      if (i + 2 < chunks) {
+        bulk_wait_read_all();
+        __syncwarp();
+        if (copies) fetch(i + 2);
+      }
+    }
+    if (!copies && i + 2 < chunks) __syncthreads();      // the chunk may be written to again
+  }
+  if (warp == 0) bulk_wait_all();
+  __syncwarp();
+  if (threadIdx.x == 0 && abort_word != 0) *p.ix.status = abort_word;
   cluster_sync_all();      // nobody leaves while another reads its sums
 }
 
@@ -825,6 +1051,9 @@ static int lora_shrink(const void* X, int64_t ldx, const void* W, bool wmn, Shri
     const int64_t tiles = ceil_div(p.ix.T, kLTile), blocks = ceil_div(p.D, 64);
     p.split = 1;
     while (p.split < 8 && tiles * p.split * 2 <= 2 * num_sms() && blocks >= 4 * p.split) p.split *= 2;
+    const int columns = wmn && RP < 64 ? 64 : RP;      // of an adapter; as many adapters as make 128 share a pass
+    p.stage = kLBox + static_cast<int>(std::min<int64_t>(128 / columns, p.ix.L)) * columns * 128;
+    p.stages = std::min(kShrinkMost, kShrinkRing / p.stage);
     auto run = [&](auto mn) -> int {
       constexpr bool MN = decltype(mn)::value;
       static PerDevice allowed;
@@ -884,8 +1113,7 @@ static int lora_wgrad(const void* Y, int64_t ldy, const void* V, WgradParams p, 
     B200_LAUNCH(lora_wgrad_kernel<RP>, static_cast<int>(ceil_div(p.D, 128) * p.L * p.splits), kWgThreads, kWgSmem<RP>, st, tmY, tmV, p);
     if (p.splits > 1) {
       const long long n = static_cast<long long>(p.L) * p.D * p.R;
-      B200_LAUNCH(lora_wgrad_sum_kernel, static_cast<int>(std::min<long long>(ceil_div(n, 1024), 4 * num_sms())), 256, 0, st,
-                  static_cast<const float*>(ws), p.splits, n, out, out_f32);
+      B200_LAUNCH(lora_wgrad_sum_kernel, static_cast<int>(ceil_div(n, 512)), 128, 0, st, static_cast<const float*>(ws), p.splits, n, out, out_f32);
     }
     return 0;
   });
@@ -918,7 +1146,7 @@ static LoraKept carve_lora(int64_t T, int64_t R, int64_t L, int keep, void* ws, 
   *bytes = c.off;
   return k;
 }
-static bool lora_few(int64_t T, int keep) { return !keep && T <= 128; }
+static bool lora_few(int64_t T, int keep) { return !keep && T <= 512; }
 
 }  // namespace b200moe
 
@@ -961,12 +1189,15 @@ int b200moe_lora_forward(const void* x, int64_t ldx, const void* a, const void* 
   cudaStream_t st = (cudaStream_t)stream;
   const LoraIndex ix{index, index_bytes, static_cast<int>(T), static_cast<int>(L), status};
   if (lora_few(T, keep)) {
-    const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(num_sms() / (T * kFewCluster), ceil_div(N, kFewCluster * kFewThreads))));
+    const int64_t groups = few_groups(ix) * ceil_div(T, kFewBlock);
+    const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(num_sms() / (groups * kFewCluster), ceil_div(N, 8 * kFewWarps * kFewCluster))));
     const FewLora p{ix, static_cast<const __nv_bfloat16*>(x), static_cast<const __nv_bfloat16*>(a), static_cast<const __nv_bfloat16*>(b),
                     static_cast<const __nv_bfloat16*>(base), static_cast<__nv_bfloat16*>(out), ldx, ldb, static_cast<int>(K), static_cast<int>(N),
                     static_cast<int>(R), parts, scales, scale};
+    static PerDevice allowed;
+    B200_CUDA(allow_smem(allowed, lora_few_kernel, few_smem(128)));
     OpScope scope("lora_few", 1);
-    B200_CUDA(launch_chained(lora_few_kernel, static_cast<int>(T * parts * kFewCluster), kFewThreads, 0, st, kFewCluster, p));
+    B200_CUDA(launch_chained(lora_few_kernel, static_cast<int>(groups * parts * kFewCluster), kFewThreads, few_smem(R), st, kFewCluster, p));
     return 0;
   }
   size_t bytes;
@@ -974,7 +1205,7 @@ int b200moe_lora_forward(const void* x, int64_t ldx, const void* a, const void* 
   {
     OpScope scope("lora_shrink", 1);
     const int rc2 = lora_shrink(x, ldx, a, false,
-                                ShrinkParams{ix, static_cast<int>(K), static_cast<int>(R), 1, scales, scale, k.v, k.rows, index != nullptr ? k.present : nullptr}, st);
+                                ShrinkParams{ix, static_cast<int>(K), static_cast<int>(R), 1, 0, 0, scales, scale, k.v, k.rows, index != nullptr ? k.present : nullptr}, st);
     if (rc2) return rc2;
   }
   OpScope scope("lora_expand", 1);
@@ -1018,7 +1249,7 @@ int b200moe_lora_backward(const void* grad_out, const void* x, int64_t ldx, cons
   } while (0)
   if (grad_x || grad_a)
     RUN("lora_shrink", 1,
-        lora_shrink(grad_out, N, b, true, ShrinkParams{ix, static_cast<int>(N), static_cast<int>(R), 1, scales, scale, u, nullptr, nullptr}, st));
+        lora_shrink(grad_out, N, b, true, ShrinkParams{ix, static_cast<int>(N), static_cast<int>(R), 1, 0, 0, scales, scale, u, nullptr, nullptr}, st));
   if (grad_b) {
     w.D = static_cast<int>(N);
     w.transposed = 0;
