@@ -772,65 +772,106 @@ __global__ void __launch_bounds__(128) lora_wgrad_sum_kernel(const float* part, 
 // an eighth of the rows with all of A_l, the sums meet in distributed shared memory, and each expands its columns.  Both products are m16n8k16
 // instructions; the order of the reduction index within one is free as long as both operands have it, so a lane's share of x and A_l is 16 neighbouring
 // bytes of global memory, of B_l 8 of shared memory.  v is never rounded: it is split into two bf16 numbers that hold 16 bits of it.
-// Bound by latency: bulk copies of the first columns of B_l and of the base are on their way while x and A_l are multiplied, and the result leaves from
-// where the base landed.
-constexpr int kFewCluster = 8, kFewThreads = 256, kFewWarps = kFewThreads / 32, kFewRows = 16, kFewBlock = 128;
-constexpr int kFewChunk = 20 << 10;      // of two: columns of B_l, and of the base and the result of each row
-static int few_smem(int64_t R) { return static_cast<int>(2 * kFewChunk + kFewRows * R * 4 + std::max<int64_t>(4096, (R + 15) / 16 * 1024)); }
+// Bound by latency: each warp's bulk copies of its first columns of B_l and of the base are on their way while x and A_l are multiplied, and its result
+// leaves from where the base landed.
+constexpr int kFewCluster = 8, kFewThreads = 256, kFewWarps = kFewThreads / 32, kFewRows = 16, kFewMost = 512, kFewInline = 128;
+constexpr int kFewChunk = 7680;          // of a warp: columns of B_l, and of the base and the result of each row
+static int few_smem(int64_t R) { return static_cast<int>(kFewWarps * kFewChunk + kFewRows * R * 4 + std::max<int64_t>(4096, (R + 15) / 16 * 1024)); }
 
-struct FewLora {
-  LoraIndex ix;
-  const __nv_bfloat16 *x, *a, *b, *base;
-  __nv_bfloat16* out;
-  long long ldx, ldb;
-  int K, N, R, parts;
-  const float* scales;
-  float scale;
-};
 
-// A cluster's rows: found by every CTA of it.  The rows of a block of 128 are ranked among those of their adapter (or of none) in it; sixteen ranks make a
-// group, in the order of their first rows.  Returns the number of rows, 0: there is no such group in the block.  Barriers inside.
+// A cluster's rows.  The rows are ranked among those of their adapter (or of none); sixteen ranks make a group, in the order of their first rows.  Up to
+// kFewInline rows every CTA finds its group by itself; of more a kernel before ranks them, which costs 3 us and in every CTA took up to 10.
+struct FewRank { int adapter, rank; };
 struct __align__(16) FewGroup {
-  int adapter[kFewBlock];
-  int rank[kFewBlock];
-  unsigned first[kFewBlock / 32];      // rows that begin a group
+  int adapter[kFewInline];
+  int rank[kFewInline];
+  unsigned first[kFewInline / 32];      // rows that begin a group
   int rows[kFewRows];
   int n, l;
 };
-// groups of a block at most: one for each sixteen rows and one more for each adapter and for none
-__host__ __device__ inline int few_groups(const LoraIndex& ix) {
-  const int rows = ix.T < kFewBlock ? ix.T : kFewBlock, more = ix.index == nullptr || ix.T == 1 ? 0 : ix.L + 1;
-  return rows < (rows + kFewRows - 1) / kFewRows + more ? rows : (rows + kFewRows - 1) / kFewRows + more;
+// groups at most: one for each sixteen rows and one more for each adapter and for none
+static int few_groups(const LoraIndex& ix) {
+  const int more = ix.index == nullptr || ix.T == 1 ? 0 : ix.L + 1;
+  return std::min(ix.T, (ix.T + kFewRows - 1) / kFewRows + more);
 }
-__device__ __forceinline__ int few_group(const LoraIndex& ix, int block, int group, FewGroup& s) {
-  const int row0 = block * kFewBlock, t = threadIdx.x, left = ix.T - row0;
+// a row's rank among those of its adapter, by a whole warp for its 32 rows
+__device__ __forceinline__ int few_rank(const int* adapters, int t) {
+  const int l = adapters[t];
+  int rank = __popc(__match_any_sync(0xffffffffu, l) & ((1u << (t & 31)) - 1u));
+#pragma unroll 4
+  for (int j = 0; j < (t >> 5) * 8; ++j) {      // the warps' rows before
+    const int4 o = reinterpret_cast<const int4*>(adapters)[j];
+    rank += (o.x == l) + (o.y == l) + (o.z == l) + (o.w == l);
+  }
+  return rank;
+}
+// one CTA: ranks (T), and of each of `groups` groups the adapter and the first rank, -1 where there is no such group
+__global__ void __launch_bounds__(kFewMost) lora_rank_kernel(const LoraIndex ix, FewRank* ranks, FewRank* leaders, int groups) {
+  grid_dep_wait();
+  __shared__ __align__(16) int adapters[kFewMost];
+  __shared__ int before[kFewMost / 32];
+  const int t = threadIdx.x;
+  const int l = t < ix.T ? lora_adapter(ix, t) : -2;
+  adapters[t] = l;
+  __syncthreads();
+  const int rank = few_rank(adapters, t);
+  const bool first = t < ix.T && rank % kFewRows == 0;
+  const unsigned m = __ballot_sync(0xffffffffu, first);
+  if ((t & 31) == 0) before[t >> 5] = __popc(m);
+  if (t < ix.T) ranks[t] = FewRank{l, rank};
+  __syncthreads();
+  int n = __popc(m & ((1u << (t & 31)) - 1u)), all = 0;
+  for (int w = 0; w < kFewMost / 32; ++w) {
+    if (w < (t >> 5)) n += before[w];
+    all += before[w];
+  }
+  if (first) leaders[n] = FewRank{l, rank};
+  if (t >= all && t < groups) leaders[t] = FewRank{-1, -1};
+  grid_dep_launch();
+}
+// Returns the number of the group's rows, 0: there is no such group.  Barriers inside.
+__device__ __forceinline__ int few_group(const LoraIndex& ix, const FewRank* ranks, const FewRank* leaders, int group, FewGroup& s) {
+  const int t = threadIdx.x;
   if (ix.index == nullptr || ix.T == 1) {
-    const int n = max(0, min(kFewRows, left - kFewRows * group));
+    const int n = max(0, min(kFewRows, ix.T - kFewRows * group));
     if (t == 0) s.l = lora_adapter(ix, 0);
-    if (t < n) s.rows[t] = row0 + kFewRows * group + t;
+    if (t < n) s.rows[t] = kFewRows * group + t;
     __syncthreads();
     return n;
   }
-  int l = -2, rank = 0;
-  if (t < kFewBlock) s.adapter[t] = l = t < left ? lora_adapter(ix, row0 + t) : -2;
   if (t == 0) s.n = 0;
-  __syncthreads();
-  if (t < kFewBlock) {
-    const unsigned same = __match_any_sync(0xffffffffu, l);
-    rank = __popc(same & ((1u << (t & 31)) - 1u));
-#pragma unroll 4
-    for (int j = 0; j < (t >> 5) * 8; ++j) {      // the warps before
-      const int4 o = reinterpret_cast<const int4*>(s.adapter)[j];
-      rank += (o.x == l) + (o.y == l) + (o.z == l) + (o.w == l);
+  if (ranks != nullptr) {
+    const FewRank lead = leaders[group];
+    FewRank r[kFewMost / kFewThreads];
+#pragma unroll
+    for (int i = 0; i < kFewMost / kFewThreads; ++i) {
+      r[i] = FewRank{-2, -2};
+      if (t + i * kFewThreads < ix.T) r[i] = ranks[t + i * kFewThreads];
     }
-    s.rank[t] = rank;
-    const unsigned m = __ballot_sync(0xffffffffu, t < left && rank % kFewRows == 0);
+    __syncthreads();
+    if (lead.rank < 0) return 0;
+#pragma unroll
+    for (int i = 0; i < kFewMost / kFewThreads; ++i)
+      if (r[i].adapter == lead.adapter && r[i].rank >= lead.rank && r[i].rank < lead.rank + kFewRows) {
+        s.rows[r[i].rank - lead.rank] = t + i * kFewThreads;
+        atomicAdd(&s.n, 1);
+      }
+    if (t == 0) s.l = lead.adapter;
+    __syncthreads();
+    return s.n;
+  }
+  int l = -2, rank = 0;
+  if (t < kFewInline) s.adapter[t] = l = t < ix.T ? lora_adapter(ix, t) : -2;
+  __syncthreads();
+  if (t < kFewInline) {
+    s.rank[t] = rank = few_rank(s.adapter, t);
+    const unsigned m = __ballot_sync(0xffffffffu, t < ix.T && rank % kFewRows == 0);
     if ((t & 31) == 0) s.first[t >> 5] = m;
   }
   __syncthreads();
   int leader = -1, skip = group;      // the group-th of the bits
 #pragma unroll
-  for (int w = 0; w < kFewBlock / 32; ++w) {
+  for (int w = 0; w < kFewInline / 32; ++w) {
     unsigned m = s.first[w];
     const int c = __popc(m);
     if (leader < 0 && skip < c) {
@@ -841,8 +882,8 @@ __device__ __forceinline__ int few_group(const LoraIndex& ix, int block, int gro
   }
   if (leader < 0) return 0;
   const int from = s.rank[leader], of = s.adapter[leader];
-  if (t < kFewBlock && l == of && rank >= from && rank < from + kFewRows) {
-    s.rows[rank - from] = row0 + t;
+  if (t < kFewInline && l == of && rank >= from && rank < from + kFewRows) {
+    s.rows[rank - from] = t;
     atomicAdd(&s.n, 1);
   }
   if (t == 0) s.l = of;
@@ -862,46 +903,57 @@ __device__ __forceinline__ void split_bf16x2(float2 f, uint32_t& hi, uint32_t& l
   lo = pack_bf16x2(fabsf(h.x) == INFINITY ? 0.0f : f.x - h.x, fabsf(h.y) == INFINITY ? 0.0f : f.y - h.y);
 }
 
-__global__ void __launch_bounds__(kFewThreads, 4) lora_few_kernel(const FewLora p) {
-  extern __shared__ __align__(128) uint8_t smem[];                 // two chunks, sums, and (by turns) partial sums or v as fragments
+struct FewLora {
+  LoraIndex ix;
+  const __nv_bfloat16 *x, *a, *b, *base;
+  __nv_bfloat16* out;
+  long long ldx, ldb;
+  const FewRank *ranks, *leaders;      // of lora_rank_kernel, or nullptr
+  int K, N, R, parts;
+  const float* scales;
+  float scale;
+};
+
+// KS: steps of 16 r, 0: any number of them
+template <int KS>
+__global__ void __launch_bounds__(kFewThreads, 3) lora_few_kernel(const FewLora p) {
+  extern __shared__ __align__(128) uint8_t smem[];                 // a chunk a warp, sums, and (by turns) partial sums or v as fragments
   __shared__ FewGroup group;
-  __shared__ __align__(8) uint64_t bars[2];
+  __shared__ __align__(8) uint64_t bars[kFewWarps];
   __shared__ int abort_word;
-  float* sums = reinterpret_cast<float*>(smem + 2 * kFewChunk);    // of this CTA, [row][r]
+  float* sums = reinterpret_cast<float*>(smem + kFewWarps * kFewChunk);    // of this CTA, [row][r]
   float* part = sums + kFewRows * p.R;                             // [warp][row][8 r]
   uint32_t* frag = reinterpret_cast<uint32_t*>(part);              // [16 r][lane][4 upper, 4 lower halves]
-  const uint32_t bar = smem_u32(bars);
   if (threadIdx.x == 0) {
-    mbar_init(bar, 1);
-    mbar_init(bar + 8, 1);
+    for (int i = 0; i < kFewWarps; ++i) mbar_init(smem_u32(bars + i), 1);
     abort_word = 0;
     fence_mbar_init();
   }
   grid_dep_begin();
   const int rank = static_cast<int>(cluster_ctarank()), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, q = lane & 3;
-  const int c = static_cast<int>(cluster_id_x()), share = c % p.parts * kFewCluster + rank, shares = p.parts * kFewCluster;
-  const int groups = few_groups(p.ix), n = few_group(p.ix, c / p.parts / groups, c / p.parts % groups, group);
+  const int c = static_cast<int>(cluster_id_x());
+  const int n = few_group(p.ix, p.ranks, p.leaders, c / p.parts, group);
   if (n == 0) return;                                              // the whole cluster
   const int l = group.l;
+  // this warp's columns, in chunks of `wide`
+  const int share = (c % p.parts * kFewCluster + rank) * kFewWarps + warp, shares = p.parts * kFewCluster * kFewWarps;
   const int col0 = 8 * static_cast<int>(static_cast<long long>(share) * (p.N / 8) / shares);
   const int col1 = 8 * static_cast<int>(static_cast<long long>(share + 1) * (p.N / 8) / shares);
-  const int wide = kFewChunk / (2 * p.R + 2 * n) & ~7, chunks = (col1 - col0 + wide - 1) / wide, ksteps = (p.R + 15) / 16;
-  const int rows_at = wide * p.R * 2;                              // of the base's and the result's rows in a chunk
-
+  const int wide = kFewChunk / (2 * p.R + 2 * n) & ~7, ksteps = KS > 0 ? KS : (p.R + 15) / 16;
+  uint8_t *chunk = smem + warp * kFewChunk, *rows = chunk + wide * p.R * 2;      // rows: the base's, then the result's
+  const uint32_t full = smem_u32(bars + warp);
   const bool copies = l >= 0 || p.base != nullptr;
-  auto fetch = [&](int i) {                                        // warp 0: a lane a row
-    const int col = col0 + i * wide, w = min(wide, col1 - col);
-    const uint32_t to = smem_u32(smem) + (i & 1) * kFewChunk, full = bar + 8 * (i & 1);
+  auto fetch = [&](int col) {                                      // a lane a row
+    const int w = min(wide, col1 - col);
     if (lane == 0) {
       mbar_arrive_expect_tx(full, (l >= 0 ? w * p.R * 2 : 0) + (p.base != nullptr ? n * w * 2 : 0));
-      if (l >= 0) bulk_load_1d(to, p.b + (static_cast<long long>(l) * p.N + col) * p.R, w * p.R * 2, full);
+      if (l >= 0) bulk_load_1d(smem_u32(chunk), p.b + (static_cast<long long>(l) * p.N + col) * p.R, w * p.R * 2, full);
     }
     __syncwarp();
-    if (p.base != nullptr && lane < n) bulk_load_1d(to + rows_at + lane * wide * 2, p.base + group.rows[lane] * p.ldb + col, w * 2, full);
+    if (p.base != nullptr && lane < n) bulk_load_1d(smem_u32(rows) + lane * wide * 2, p.base + group.rows[lane] * p.ldb + col, w * 2, full);
   };
-  if (warp == 0 && copies)
-    for (int i = 0; i < min(2, chunks); ++i) fetch(i);
+  if (copies && col0 < col1) fetch(col0);
 
   if (l >= 0) {
     const bool low = g < n, high = g + 8 < n;
@@ -964,10 +1016,18 @@ __global__ void __launch_bounds__(kFewThreads, 4) lora_few_kernel(const FewLora 
     __syncthreads();
   }
 
-  for (int i = 0; i < chunks; ++i) {
-    const int col = col0 + i * wide, w = min(wide, col1 - col);
-    uint8_t *chunk = smem + (i & 1) * kFewChunk, *rows = chunk + rows_at;
-    if (copies) mbar_wait(bar + 8 * (i & 1), i >> 1 & 1, &abort_word, ST_WAIT_ROWS);
+  uint4 hi[KS > 0 ? KS : 1], lo[KS > 0 ? KS : 1];
+  if (KS > 0 && l >= 0) {
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      hi[k] = *reinterpret_cast<const uint4*>(frag + k * 256 + lane * 8);
+      lo[k] = *reinterpret_cast<const uint4*>(frag + k * 256 + lane * 8 + 4);
+    }
+  }
+  uint32_t phase = 0;
+  for (int col = col0; col < col1; col += wide, phase ^= 1) {
+    const int w = min(wide, col1 - col);
+    if (copies) mbar_wait(full, phase, &abort_word, ST_WAIT_ROWS);
     __syncwarp();
     constexpr int TILES = 4;                                       // of a warp at a time, fewer at the end
     const bool half = (p.R & 8) != 0 && q >= 2;                    // the last 16 r have 8 that are not there
@@ -976,16 +1036,23 @@ __global__ void __launch_bounds__(kFewThreads, 4) lora_few_kernel(const FewLora 
       float d[TILES][4] = {};
       if (l >= 0) {
         const uint8_t* b = chunk + (8 * tile0 + g) * p.R * 2 + 8 * q;
-        for (int k = 0; k < ksteps; ++k, b += 32) {
+        const int pitch = 16 * p.R;
+        auto step = [&](int k, const uint4& u, const uint4& v) {
           const bool in = !(half && k == ksteps - 1);
           uint2 bw[TILES];
 #pragma unroll
-          for (int j = 0; j < TILES; ++j) bw[j] = in && (WHOLE || j < tiles) ? *reinterpret_cast<const uint2*>(b + 16 * j * p.R) : make_uint2(0u, 0u);
-          const uint4 hi = *reinterpret_cast<const uint4*>(frag + k * 256 + lane * 8), lo = *reinterpret_cast<const uint4*>(frag + k * 256 + lane * 8 + 4);
+          for (int j = 0; j < TILES; ++j) bw[j] = in && (WHOLE || j < tiles) ? *reinterpret_cast<const uint2*>(b + j * pitch + 32 * k) : make_uint2(0u, 0u);
 #pragma unroll
-          for (int j = 0; j < TILES; ++j) mma_bf16(d[j], lo.x, lo.y, lo.z, lo.w, bw[j].x, bw[j].y);
+          for (int j = 0; j < TILES; ++j) mma_bf16(d[j], v.x, v.y, v.z, v.w, bw[j].x, bw[j].y);
 #pragma unroll
-          for (int j = 0; j < TILES; ++j) mma_bf16(d[j], hi.x, hi.y, hi.z, hi.w, bw[j].x, bw[j].y);
+          for (int j = 0; j < TILES; ++j) mma_bf16(d[j], u.x, u.y, u.z, u.w, bw[j].x, bw[j].y);
+        };
+        if constexpr (KS > 0) {
+#pragma unroll
+          for (int k = 0; k < KS; ++k) step(k, hi[k], lo[k]);
+        } else {
+          for (int k = 0; k < ksteps; ++k)
+            step(k, *reinterpret_cast<const uint4*>(frag + k * 256 + lane * 8), *reinterpret_cast<const uint4*>(frag + k * 256 + lane * 8 + 4));
         }
       }
 #pragma unroll
@@ -1006,24 +1073,21 @@ __global__ void __launch_bounds__(kFewThreads, 4) lora_few_kernel(const FewLora 
         }
       }
     };
-    for (int tile0 = TILES * warp; tile0 < w / 8; tile0 += TILES * kFewWarps) {
+    for (int tile0 = 0; tile0 < w / 8; tile0 += TILES) {
       if (tile0 + TILES <= w / 8) group_of_tiles(tile0, TILES, std::true_type());
       else group_of_tiles(tile0, w / 8 - tile0, std::false_type());
     }
     fence_proxy_async_smem();
-    __syncthreads();
-    if (warp == 0) {
-      if (lane < n) bulk_store_1d(p.out + static_cast<long long>(group.rows[lane]) * p.N + col, smem_u32(rows) + lane * wide * 2, w * 2);
-      bulk_commit_group();
-      if (i + 2 < chunks) {
-        bulk_wait_read_all();
-        __syncwarp();
-        if (copies) fetch(i + 2);
-      }
+    __syncwarp();
+    if (lane < n) bulk_store_1d(p.out + static_cast<long long>(group.rows[lane]) * p.N + col, smem_u32(rows) + lane * wide * 2, w * 2);
+    bulk_commit_group();
+    if (col + wide < col1) {
+      bulk_wait_read_all();
+      __syncwarp();
+      if (copies) fetch(col + wide);
     }
-    if (!copies && i + 2 < chunks) __syncthreads();      // the chunk may be written to again
   }
-  if (warp == 0) bulk_wait_all();
+  bulk_wait_all();
   __syncwarp();
   if (threadIdx.x == 0 && abort_word != 0) *p.ix.status = abort_word;
   cluster_sync_all();      // nobody leaves while another reads its sums
@@ -1146,7 +1210,10 @@ static LoraKept carve_lora(int64_t T, int64_t R, int64_t L, int keep, void* ws, 
   *bytes = c.off;
   return k;
 }
-static bool lora_few(int64_t T, int keep) { return !keep && T <= 512; }
+// Whether the kernel of few rows takes a call.  us, few rows / row tiles, L2 warm.  One adapter, 4096 x 14336, rank 16: 16 rows 8.4 / 10.0, 128 rows 9.8 /
+// 10.5, 256 rows 14.4 / 11.8; 2048 x 2816, rank 64: 16 rows 9.3 / 9.5, 64 rows 11.4 / 9.4.  Several, 4096 x 4096, rank 16, rows of 32 adapters mixed:
+// 64 rows 9.6 / 35, 512 rows 16 / 43.
+static bool lora_few(int64_t T, int64_t R, int64_t L, int keep) { return !keep && T <= (L > 1 ? kFewMost : R <= 32 ? 128 : 16); }
 
 }  // namespace b200moe
 
@@ -1170,7 +1237,7 @@ size_t b200moe_lora_fwd_ws_bytes(int64_t T, int64_t R, int64_t L, int keep) {
   if (T <= 0 || R <= 0 || L <= 0) return 0;
   size_t bytes = 0;
   carve_lora(T, R, L, keep, nullptr, &bytes);
-  return bytes;
+  return std::max(bytes, T <= kFewMost ? 2 * T * sizeof(FewRank) : 0);
 }
 
 int b200moe_lora_forward(const void* x, int64_t ldx, const void* a, const void* b, const void* index, int index_bytes, const float* scales, float scale,
@@ -1188,17 +1255,23 @@ int b200moe_lora_forward(const void* x, int64_t ldx, const void* a, const void* 
                  B200MOE_E_ALIGN, "lora_forward: tensors must be 16-byte aligned, the index 8");
   cudaStream_t st = (cudaStream_t)stream;
   const LoraIndex ix{index, index_bytes, static_cast<int>(T), static_cast<int>(L), status};
-  if (lora_few(T, keep)) {
-    const int64_t groups = few_groups(ix) * ceil_div(T, kFewBlock);
+  if (lora_few(T, R, L, keep)) {
+    const int64_t groups = few_groups(ix);
+    FewRank *ranks = index != nullptr && T > kFewInline ? static_cast<FewRank*>(ws) : nullptr, *leaders = ranks != nullptr ? ranks + T : nullptr;
     const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(num_sms() / (groups * kFewCluster), ceil_div(N, 8 * kFewWarps * kFewCluster))));
     const FewLora p{ix, static_cast<const __nv_bfloat16*>(x), static_cast<const __nv_bfloat16*>(a), static_cast<const __nv_bfloat16*>(b),
-                    static_cast<const __nv_bfloat16*>(base), static_cast<__nv_bfloat16*>(out), ldx, ldb, static_cast<int>(K), static_cast<int>(N),
-                    static_cast<int>(R), parts, scales, scale};
-    static PerDevice allowed;
-    B200_CUDA(allow_smem(allowed, lora_few_kernel, few_smem(128)));
-    OpScope scope("lora_few", 1);
-    B200_CUDA(launch_chained(lora_few_kernel, static_cast<int>(groups * parts * kFewCluster), kFewThreads, few_smem(R), st, kFewCluster, p));
-    return 0;
+                    static_cast<const __nv_bfloat16*>(base), static_cast<__nv_bfloat16*>(out), ldx, ldb, ranks, leaders, static_cast<int>(K),
+                    static_cast<int>(N), static_cast<int>(R), parts, scales, scale};
+    OpScope scope("lora_few", ranks != nullptr ? 2 : 1);
+    if (ranks != nullptr) B200_LAUNCH(lora_rank_kernel, 1, kFewMost, 0, st, ix, ranks, leaders, static_cast<int>(groups));
+    auto run = [&](auto ks) -> int {
+      constexpr int KS = decltype(ks)::value;
+      static PerDevice allowed;
+      B200_CUDA(allow_smem(allowed, lora_few_kernel<KS>, few_smem(128)));
+      B200_CUDA(launch_chained(lora_few_kernel<KS>, static_cast<int>(groups * parts * kFewCluster), kFewThreads, few_smem(R), st, kFewCluster, p));
+      return 0;
+    };
+    return R <= 16 ? run(std::integral_constant<int, 1>()) : R <= 32 ? run(std::integral_constant<int, 2>()) : run(std::integral_constant<int, 0>());
   }
   size_t bytes;
   const LoraKept k = carve_lora(T, R, L, keep, ws, &bytes);
