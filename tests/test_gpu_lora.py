@@ -30,6 +30,9 @@ def make(T, K, N, R, n, how="mixed", seed=0, base=True, dtype=BF):
         index = None
     elif how == "mixed":
         index = torch.randint(-1, n, (T,), generator=g, device=DEV)
+    elif how == "tail":      # prompts, then rows of their own requests
+        index = torch.arange(T, device=DEV) * 5 // T
+        index[-150:] = torch.arange(150, device=DEV) % n
     elif how == "packed":
         ends = (torch.rand(n, generator=g, device=DEV) * T).long().sort().values
         index = (torch.randperm(n + 1, generator=g, device=DEV) - 1)[torch.searchsorted(ends, torch.arange(T, device=DEV), right=True)]
@@ -80,7 +83,7 @@ def close(got, ref, terms, rounded=True):
 SHAPES = [(1, 64, 64, 8, 1, "one"), (1, 4096, 4096, 16, 4, "mixed"), (5, 264, 136, 24, 3, "mixed"), (64, 1024, 2816, 16, 64, "mixed"), (127, 520, 680, 128, 5, "packed"),
           (128, 64, 8, 64, 2, "mixed"), (129, 8, 64, 8, 3, "mixed"), (300, 1040, 680, 8, 3, "packed"), (300, 1040, 680, 16, 40, "mixed"), (512, 2048, 2816, 32, 7, "mixed"),
           (1000, 2048, 1408, 64, 1, "one"), (1000, 512, 520, 128, 3, "packed"), (1000, 512, 520, 128, 3, "mixed"), (777, 4096, 1032, 48, 9, "packed"), (260, 256, 256, 16, 2, "none"),
-          (20000, 128, 72, 16, 5, "packed"), (40000, 64, 64, 8, 2, "packed"), (2100, 64, 14336, 40, 4, "packed")]
+          (1700, 520, 1032, 16, 200, "mixed"), (900, 264, 136, 128, 60, "mixed"), (3000, 136, 264, 32, 12, "tail"), (20000, 128, 72, 16, 5, "packed"), (40000, 64, 64, 8, 2, "packed"), (2100, 64, 14336, 40, 4, "packed")]
 
 
 @pytest.mark.parametrize("T,K,N,R,n,how", SHAPES)
@@ -311,10 +314,11 @@ def test_observer(pkg):
         return names
 
     assert seen(lambda: pkg.lora_linear(x[:4], a, b, index[:4], s)) == [("lora_few", 1)]
-    assert seen(lambda: pkg.lora_linear(x, a, b, index, s)) == [("lora_shrink", 1), ("lora_expand", 1)]
+    assert seen(lambda: pkg.lora_linear(x, a, b, index, s)) == [("lora_tiles", 1), ("lora_shrink", 1), ("lora_expand", 1)]
+    assert seen(lambda: pkg.lora_linear(x, a[:1], b[:1])) == [("lora_shrink", 1), ("lora_expand", 1)]
     x.requires_grad_(), a.requires_grad_(), b.requires_grad_()
     got = [n for n, _ in seen(lambda: pkg.lora_linear(x, a, b, index, s).float().sum().backward())]
-    assert sorted(got) == sorted(["lora_shrink", "lora_expand"] * 2 + ["lora_wgrad"] * 2)
+    assert sorted(got) == sorted(["lora_tiles"] + ["lora_shrink", "lora_expand"] * 2 + ["lora_wgrad"] * 2)
 
 
 def test_refusals(pkg):

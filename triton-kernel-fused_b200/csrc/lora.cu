@@ -6,7 +6,7 @@
 //
 // Four products with one short side (R of at most 128), all bound by HBM: `shrink` (T,D) -> (T,R) reads x or g, `expand` (T,R) -> (T,D) reads
 // base and writes out or grad_x, `wgrad` reads x or g again.  Each is a tcgen05 kernel over tiles of 128 rows as they come, without sorting
-// them: a tile's distinct adapters are found on the way, each is multiplied with all rows of the tile into tensor memory of its own, and a
+// them: a tile's distinct adapters are found by a kernel before, each is multiplied with all rows of the tile into tensor memory of its own, and a
 // row takes the result of its adapter.  Rows of other adapters are never added to it, not even times zero, so an infinity or a NaN stays with
 // its own adapter or row.  Few rows (a decoding batch) run in one kernel of their own, a cluster a row.
 //
@@ -29,15 +29,6 @@ struct LoraIndex {
   int* status;
 };
 
-// A tile's adapters, found by all threads of the CTA: row -> slot (-1: none), slot -> adapter
-struct LoraSlots {
-  int of_row[kLTile];
-  int adapter[kLTile];
-  int slot[kLTile];
-  int warps[4];
-  int n;
-};
-
 __device__ __forceinline__ int lora_adapter(const LoraIndex& p, long long t) {
   if (t >= p.T) return -1;
   if (p.index == nullptr) return 0;
@@ -49,51 +40,122 @@ __device__ __forceinline__ int lora_adapter(const LoraIndex& p, long long t) {
   return l < 0 ? -1 : static_cast<int>(l);
 }
 
-// this thread's row's, asked for ahead
-__device__ __forceinline__ int lora_ahead(const LoraIndex& p, int tile) {
-  return threadIdx.x < kLTile ? lora_adapter(p, static_cast<long long>(tile) * kLTile + threadIdx.x) : -1;
+// The adapters of each tile of 128 rows, each named once, in the order of its first row.  nullptr: adapter 0 for every row
+struct LoraTiles {
+  int* n;                    // (tiles): adapters of a tile
+  int* adapter;              // (tiles, 128)
+  short* slot;               // (tiles, 128): of a row, its adapter's place among them, -1: none
+  int T, tiles;
+};
+__device__ __forceinline__ int tile_n(const LoraTiles& p, int tile) { return p.n == nullptr ? 1 : p.n[tile]; }
+__device__ __forceinline__ int tile_adapter(const LoraTiles& p, int tile, int i) {
+  return p.n == nullptr ? 0 : p.adapter[static_cast<long long>(tile) * kLTile + i];
 }
-// l: lora_ahead.  Barriers inside: every thread of the CTA calls it
-__device__ __forceinline__ void lora_slots(const LoraIndex& p, int l, LoraSlots& s) {
-  const int t = threadIdx.x;
-  if (p.index == nullptr) {
-    if (t < kLTile) {
-      s.of_row[t] = l;
-      s.slot[t] = l;
-      s.adapter[0] = 0;
+__device__ __forceinline__ int tile_slot(const LoraTiles& p, int tile, int row) {
+  const long long t = static_cast<long long>(tile) * kLTile + row;
+  return p.n == nullptr ? (t < p.T ? 0 : -1) : p.slot[t];
+}
+
+// rows (T), nullable: the rows' adapters, -1: none; present (tiles, L), nullable: bit h where rows of the tile's half h have the adapter
+__global__ void __launch_bounds__(kLTile) lora_tiles_kernel(const LoraIndex ix, const LoraTiles p, int* rows, unsigned char* present) {
+  grid_dep_wait();
+  __shared__ __align__(16) int of_row[kLTile];
+  __shared__ int slot[kLTile], warps[kLTile / 32];
+  const int t = threadIdx.x, tile = blockIdx.x;
+  const long long row = static_cast<long long>(tile) * kLTile + t;
+  const int l = lora_adapter(ix, row);
+  of_row[t] = l;
+  __syncthreads();
+  // the first row of this thread's adapter: in this warp, or in one before
+  const unsigned same = __match_any_sync(0xffffffffu, l);
+  int at = (t & ~31) + __ffs(same) - 1;
+  for (int j = 0; j < (t >> 5) * 8; ++j) {
+    const int4 o = reinterpret_cast<const int4*>(of_row)[j];
+    const int i = o.x == l ? 0 : o.y == l ? 1 : o.z == l ? 2 : o.w == l ? 3 : 4;
+    if (i < 4) {
+      at = 4 * j + i;
+      break;
     }
-    if (t == 0) s.n = 1;
+  }
+  __syncwarp();
+  const bool first = l >= 0 && at == t;
+  const unsigned firsts = __ballot_sync(0xffffffffu, first);
+  if ((t & 31) == 0) warps[t >> 5] = __popc(firsts);
+  __syncthreads();
+  int n = __popc(firsts & ((1u << (t & 31)) - 1u));
+  for (int w = 0; w < (t >> 5); ++w) n += warps[w];
+  if (first) {
+    slot[t] = n;
+    p.adapter[static_cast<long long>(tile) * kLTile + n] = l;
+  }
+  if (t == 0) p.n[tile] = warps[0] + warps[1] + warps[2] + warps[3];
+  __syncthreads();
+  p.slot[row] = static_cast<short>(l >= 0 ? slot[at] : -1);
+  if (rows != nullptr && row < ix.T) rows[row] = l;
+  if (present != nullptr) {
+    unsigned char* to = present + static_cast<long long>(tile) * ix.L;
+    for (int i = t; i < ix.L; i += kLTile) to[i] = 0;
+    __syncthreads();
+    if (first) {
+      bool low = false, high = false;
+      for (int j = 0; j < kLTile / 2; ++j) {
+        low = low || of_row[j] == l;
+        high = high || of_row[j + kLTile / 2] == l;
+      }
+      to[l] = static_cast<unsigned char>((low ? 1 : 0) | (high ? 2 : 0));
+    }
+  }
+  grid_dep_launch();
+}
+
+// Where a share of the tiles' work begins and ends: tile t has weight f(its adapters), and a place is a tile and what of its weight is before.  All
+// threads of the CTA; barriers inside.
+struct LoraShare {
+  long long warps[32], rest[2];
+  int tile[2];
+};
+template <int THREADS, class F>
+__device__ __forceinline__ void lora_share(const LoraTiles& p, long long share, long long shares, F weight, LoraShare& s) {
+  const int t = threadIdx.x;
+  if (p.n == nullptr) {
+    if (t < 2) {
+      const long long w = weight(1), at = (share + t) * (p.tiles * w) / shares;
+      s.tile[t] = static_cast<int>(at / w);
+      s.rest[t] = at % w;
+    }
     __syncthreads();
     return;
   }
-  int at = -1;
-  if (t < kLTile) s.of_row[t] = l;
+  const int per = (p.tiles + THREADS - 1) / THREADS, t0 = min(p.tiles, t * per), t1 = min(p.tiles, t0 + per);
+  long long sum = 0;
+  for (int i = t0; i < t1; ++i) sum += weight(p.n[i]);
+  long long incl = sum;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const long long o = __shfl_up_sync(0xffffffffu, incl, off);
+    if ((t & 31) >= off) incl += o;
+  }
+  if ((t & 31) == 31) s.warps[t >> 5] = incl;
   __syncthreads();
-  bool first = false;
-  unsigned firsts = 0;
-  if (t < kLTile) {
-    if (l >= 0) {
-      at = t;
-      for (int j = 0; j < t; ++j)
-        if (s.of_row[j] == l) {
-          at = j;
-          break;
-        }
+  long long before = incl - sum, total = 0;
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < (t >> 5)) before += s.warps[w];
+    total += s.warps[w];
+  }
+  for (int e = 0; e < 2; ++e) {
+    const long long at = (share + e) * total / shares;
+    if (at >= before && at < before + sum) {
+      long long rest = at - before;
+      int i = t0;
+      for (; rest >= weight(p.n[i]); ++i) rest -= weight(p.n[i]);
+      s.tile[e] = i;
+      s.rest[e] = rest;
     }
-    first = l >= 0 && at == t;
-    firsts = __ballot_sync(0xffffffffu, first);
-    if ((t & 31) == 0) s.warps[t >> 5] = __popc(firsts);
+    if (at == total && t == 0) {
+      s.tile[e] = p.tiles;
+      s.rest[e] = 0;
+    }
   }
-  __syncthreads();
-  if (t < kLTile && first) {
-    int n = __popc(firsts & ((1u << (t & 31)) - 1u));
-    for (int w = 0; w < (t >> 5); ++w) n += s.warps[w];
-    s.slot[t] = n;
-    s.adapter[n] = l;
-  }
-  if (t == 0) s.n = s.warps[0] + s.warps[1] + s.warps[2] + s.warps[3];
-  __syncthreads();
-  if (t < kLTile && !first) s.slot[t] = l >= 0 ? s.slot[at] : -1;
   __syncthreads();
 }
 
@@ -130,20 +192,20 @@ __device__ __forceinline__ float4 cluster_sum4(uint32_t at, int ctas) {
 }
 
 // ------------------------------------------------------------------------------------------------ shrink
-// v[t, r] = s_l sum_d X[t, d] W_l[r, d].  A cluster of `split` CTAs shares a tile's columns d and adds up its partial sums through distributed
-// shared memory.  WMN: W_l lies (D, R), reduction index first (the backward's B).  As many adapters as fit 128 accumulator columns a pass.
-constexpr int kShrinkMost = 5, kShrinkThreads = 192, kShrinkRing = 96 << 10;      // stages: of X and of the adapters that a pass can have
+// v[t, r] = s_l sum_d X[t, d] W_l[r, d].  A unit of work is a row tile and as many of its adapters as fit 128 accumulator columns; a cluster of `split`
+// CTAs shares a unit's columns d and adds up its partial sums through distributed shared memory.  WMN: W_l lies (D, R), reduction index first (the
+// backward's B).
+constexpr int kShrinkMost = 5, kShrinkThreads = 192, kShrinkRing = 96 << 10;      // stages: of X and of the adapters that a unit can have
 constexpr int kShrinkSmem = kShrinkRing + (2 * kShrinkMost + 2) * 8 + 16 + 1024;
 
 struct ShrinkParams {
-  LoraIndex ix;
+  LoraTiles tiles;
   int D, R, split;
   int stages, stage;         // of the ring, bytes of one
   const float* scales;       // (L,), or nullptr: `scale` for all
   float scale;
   __nv_bfloat16* v;          // (T, RP)
-  int* rows;                 // nullable: the rows' adapters as wgrad reads them
-  unsigned char* present;    // nullable: (tiles, L), bit h: rows of the tile's half h have the adapter
+  int* status;
 };
 
 template <int RP, bool WMN>
@@ -158,10 +220,9 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
   const uint32_t bar_tfull = smem_u32(bars + 2 * kShrinkMost), bar_tempty = bar_tfull + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kShrinkMost + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  __shared__ LoraSlots slots;
+  __shared__ LoraShare share;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = p.split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  const int tile = blockIdx.x / p.split;
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(bar_full + 8 * s, 2);        // X, and the adapters
@@ -179,48 +240,45 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     tmem_relinquish();
   }
   grid_dep_wait();
-  const int nkb = (p.D + 63) / 64;
-  const int kb0 = static_cast<int>(static_cast<long long>(rank) * nkb / p.split), kb1 = static_cast<int>(static_cast<long long>(rank + 1) * nkb / p.split);
-  const int ahead = min(p.stages, kb1 - kb0);
-  if (threadIdx.x == 0)      // rows of X are on their way while the tile's adapters are looked up
-    for (int s = 0; s < ahead; ++s) {
-      mbar_arrive_expect_tx(bar_full + 8 * s, kLBox);
-      tma_load_3d(smem_u32(smem + s * p.stage), &tmX, bar_full + 8 * s, (kb0 + s) * 64, tile * kLTile, 0);
-    }
   tc_fence_before();
-  lora_slots(p.ix, lora_ahead(p.ix, tile), slots);
+  lora_share<kShrinkThreads>(p.tiles, blockIdx.x / p.split, gridDim.x / p.split, [](int n) { return max(1, (n + SLOTS - 1) / SLOTS); }, share);
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int passes = (slots.n + SLOTS - 1) / SLOTS;
-  float v[RP];
-#pragma unroll
-  for (int i = 0; i < RP; ++i) v[i] = 0.0f;
+  const int nkb = (p.D + 63) / 64;
+  const int kb0 = static_cast<int>(static_cast<long long>(rank) * nkb / p.split), kb1 = static_cast<int>(static_cast<long long>(rank + 1) * nkb / p.split);
+  int done = 0;              // blocks of the units before: the place in the ring
+  uint32_t unit_ph = 0;
+  bool ok = true;
 
-  if (warp == 0) {
-    if (elect_one()) {
-      int s = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      for (int pass = 0; pass < passes && ok; ++pass) {
-        const int first = pass * SLOTS, n = min(SLOTS, slots.n - first);
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, ST_WAIT_PRODUCER)) {
-            ok = false;
-            break;
-          }
+  for (int tile = share.tile[0], pass = static_cast<int>(share.rest[0]); tile < share.tile[1] || (tile == share.tile[1] && pass < static_cast<int>(share.rest[1]));) {
+    const int all = tile_n(p.tiles, tile), first = pass * SLOTS, n = min(SLOTS, all - first);      // n = 0: a tile without adapters
+    const int row0 = tile * kLTile;
+    float v[RP];
+#pragma unroll
+    for (int i = 0; i < RP; ++i) v[i] = 0.0f;
+    int mine = -1;
+    if (warp == 0) {
+      if (n > 0 && elect_one()) {
+        int s = done % p.stages;
+        uint32_t ph = done / p.stages & 1;
+        int of[SLOTS];
+#pragma unroll
+        for (int j = 0; j < SLOTS; ++j) of[j] = j < n ? tile_adapter(p.tiles, tile, first + j) : 0;
+        for (int kb = kb0; kb < kb1 && ok; ++kb) {
+          ok = mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, ST_WAIT_PRODUCER);
+          if (!ok) break;
           const uint32_t full = bar_full + 8 * s, sx = smem_u32(smem + s * p.stage), sw = sx + kLBox;
-          if (pass > 0 || kb - kb0 >= ahead) {
-            mbar_arrive_expect_tx(full, kLBox);
-            tma_load_3d(sx, &tmX, full, kb * 64, tile * kLTile, 0);
-          }
+          mbar_arrive_expect_tx(full, kLBox);
+          tma_load_3d(sx, &tmX, full, kb * 64, row0, 0);
           mbar_arrive_expect_tx(full, n * NB * 128);
-          for (int j = 0; j < n; ++j) {
-            const int l = slots.adapter[first + j];
+#pragma unroll
+          for (int j = 0; j < SLOTS; ++j) {
+            if (j >= n) break;
             if constexpr (WMN) {
 #pragma unroll
-              for (int h = 0; h < NB / 64; ++h) tma_load_3d(sw + (j * (NB / 64) + h) * 8192, &tmW, full, 64 * h, kb * 64, l);
+              for (int h = 0; h < NB / 64; ++h) tma_load_3d(sw + (j * (NB / 64) + h) * 8192, &tmW, full, 64 * h, kb * 64, of[j]);
             } else {
-              tma_load_3d(sw + j * NB * 128, &tmW, full, kb * 64, 0, l);
+              tma_load_3d(sw + j * NB * 128, &tmW, full, kb * 64, 0, of[j]);
             }
           }
           if (++s == p.stages) {
@@ -229,30 +287,16 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
           }
         }
       }
-    }
-    __syncwarp();
-    if (passes == 0 && lane == 0)      // nobody reads the rows that are on their way
-      for (int s = 0; s < ahead; ++s) {
-        mbar_arrive(bar_full + 8 * s);
-        mbar_wait(bar_full + 8 * s, 0, abort_flag, ST_WAIT_PRODUCER);
-      }
-    __syncwarp();
-    grid_dep_launch();
-  } else if (warp == 1) {
-    if (elect_one()) {
-      int s = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      for (int pass = 0; pass < passes && ok; ++pass) {
-        const int n = min(SLOTS, slots.n - pass * SLOTS);
+    } else if (warp == 1) {
+      if (n > 0 && elect_one()) {
+        int s = done % p.stages;
+        uint32_t ph = done / p.stages & 1;
         const uint32_t idesc = umma_idesc_bf16(n * NB, 0, WMN);
-        if (!mbar_wait(bar_tempty, (pass & 1) ^ 1, abort_flag, ST_WAIT_MMA_TMEM)) break;
+        ok = ok && mbar_wait(bar_tempty, unit_ph ^ 1, abort_flag, ST_WAIT_MMA_TMEM);
         tc_fence_after();
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait(bar_full + 8 * s, ph, abort_flag, ST_WAIT_MMA_FULL)) {
-            ok = false;
-            break;
-          }
+        for (int kb = kb0; kb < kb1 && ok; ++kb) {
+          ok = mbar_wait(bar_full + 8 * s, ph, abort_flag, ST_WAIT_MMA_FULL);
+          if (!ok) break;
           tc_fence_after();
           const uint32_t sx = smem_u32(smem + s * p.stage), sw = sx + kLBox;
 #pragma unroll
@@ -267,71 +311,73 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
         }
         if (ok) umma_commit(bar_tfull);
       }
-    }
-  } else {
-    const int q = warp & 3, row = 32 * q + lane, mine = slots.slot[row];
-    const uint32_t taddr = tmem + (static_cast<uint32_t>(32 * q) << 16);
-    bool ok = true;
-    for (int pass = 0; pass < passes; ++pass) {
-      ok = ok && mbar_wait(bar_tfull, pass & 1, abort_flag, ST_WAIT_EPILOGUE);
-      __syncwarp();
-      tc_fence_after();
-      if (kb1 > kb0)
-        for (int j = 0; j < min(SLOTS, slots.n - pass * SLOTS); ++j) {
-          const bool me = mine == pass * SLOTS + j;
+    } else {
+      const int q = warp & 3, row = 32 * q + lane;
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(32 * q) << 16);
+      mine = tile_slot(p.tiles, tile, row);
+      if (n > 0) {
+        ok = ok && mbar_wait(bar_tfull, unit_ph, abort_flag, ST_WAIT_EPILOGUE);
+        __syncwarp();
+        tc_fence_after();
+        for (int j = 0; j < n; ++j) {
+          const bool me = mine == first + j;
           if (__any_sync(0xffffffffu, me)) lora_fetch<RP>(taddr + j * NB, me, v);
         }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_tempty);
-    }
-    const long long t = static_cast<long long>(tile) * kLTile + row;
-    if (p.rows != nullptr && rank == 0 && t < p.ix.T) p.rows[t] = slots.of_row[row];
-    if (p.split == 1) {
-      const float s = mine < 0 ? 0.0f : p.scales != nullptr ? p.scales[slots.adapter[mine]] : p.scale;
-      if (t < p.ix.T) {
-#pragma unroll
-        for (int i = 0; i < RP; i += 8) {
-          uint32_t o[4];
-#pragma unroll
-          for (int h = 0; h < 4; ++h)
-            o[h] = mine >= 0 && i < p.R ? pack_bf16x2(s * v[i + 2 * h], s * v[i + 2 * h + 1]) : 0u;      // R a multiple of 8
-          *reinterpret_cast<uint4*>(p.v + t * RP + i) = make_uint4(o[0], o[1], o[2], o[3]);
-        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_tempty);
       }
-    } else {      // every load of this CTA has been used: its stages are free
-      float4* to = reinterpret_cast<float4*>(smem + row * (RP + 4) * 4);
+      const long long t = static_cast<long long>(row0) + row;
+      if (p.split == 1) {
+        // a row is written by the unit of its adapter, or without one by the tile's first
+        if (t < p.tiles.T && (mine < 0 ? pass == 0 : mine >= first && mine < first + n)) {
+          const float s = mine < 0 ? 0.0f : p.scales != nullptr ? p.scales[tile_adapter(p.tiles, tile, mine)] : p.scale;
 #pragma unroll
-      for (int i = 0; i < RP; i += 4) to[i / 4] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          for (int i = 0; i < RP; i += 8) {
+            uint32_t o[4];
+#pragma unroll
+            for (int h = 0; h < 4; ++h)
+              o[h] = mine >= 0 && i < p.R ? pack_bf16x2(s * v[i + 2 * h], s * v[i + 2 * h + 1]) : 0u;      // R a multiple of 8
+            *reinterpret_cast<uint4*>(p.v + t * RP + i) = make_uint4(o[0], o[1], o[2], o[3]);
+          }
+        }
+      } else {      // every load of this CTA has been used: its stages are free
+        float4* to = reinterpret_cast<float4*>(smem + row * (RP + 4) * 4);
+#pragma unroll
+        for (int i = 0; i < RP; i += 4) to[i / 4] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+      }
     }
-  }
-  __syncwarp();
-  if (p.present != nullptr && rank == 0)
-    for (int l = threadIdx.x; l < p.ix.L; l += kShrinkThreads) {
-      unsigned bits = 0;
-      for (int r = 0; r < kLTile; ++r) bits |= slots.of_row[r] == l ? 1u << (r >> 6) : 0u;
-      p.present[static_cast<long long>(tile) * p.ix.L + l] = static_cast<unsigned char>(bits);
-    }
-  if (p.split > 1) {
     __syncwarp();
-    cluster_sync_all();
-    const int rows = kLTile / p.split;
-    for (int i = threadIdx.x; i < rows * (RP / 4); i += kShrinkThreads) {
-      const int row = rank * rows + i / (RP / 4), c = 4 * (i % (RP / 4)), mine = slots.slot[row];
-      const long long t = static_cast<long long>(tile) * kLTile + row;
-      const float4 v4 = cluster_sum4(smem_u32(smem) + 4 * (row * (RP + 4) + c), p.split);
-      const float s = mine < 0 ? 0.0f : p.scales != nullptr ? p.scales[slots.adapter[mine]] : p.scale;
-      if (t < p.ix.T)
+    if (p.split > 1) {
+      cluster_sync_all();
+      const int rows = kLTile / p.split;
+      for (int i = threadIdx.x; i < rows * (RP / 4); i += kShrinkThreads) {
+        const int row = rank * rows + i / (RP / 4), c = 4 * (i % (RP / 4)), slot = tile_slot(p.tiles, tile, row);
+        const long long t = static_cast<long long>(row0) + row;
+        if (t >= p.tiles.T || (slot < 0 ? pass > 0 : slot < first || slot >= first + n)) continue;
+        const float4 v4 = cluster_sum4(smem_u32(smem) + 4 * (row * (RP + 4) + c), p.split);
+        const float s = slot < 0 ? 0.0f : p.scales != nullptr ? p.scales[tile_adapter(p.tiles, tile, slot)] : p.scale;
         *reinterpret_cast<uint2*>(p.v + t * RP + c) =
-            mine >= 0 && c < p.R ? make_uint2(pack_bf16x2(s * v4.x, s * v4.y), pack_bf16x2(s * v4.z, s * v4.w)) : make_uint2(0u, 0u);
+            slot >= 0 && c < p.R ? make_uint2(pack_bf16x2(s * v4.x, s * v4.y), pack_bf16x2(s * v4.z, s * v4.w)) : make_uint2(0u, 0u);
+      }
+      fence_proxy_async_smem();      // before the next unit's rows land there
+      __syncwarp();
+      cluster_sync_all();            // nobody goes on while another reads its sums
     }
-    __syncwarp();
-    cluster_sync_all();      // nobody leaves while another reads its sums
+    if (n > 0) {
+      done += kb1 - kb0;
+      unit_ph ^= 1;
+    }
+    if (++pass * SLOTS >= all) {
+      pass = 0;
+      ++tile;
+    }
   }
+  if (warp == 0) grid_dep_launch();
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem, 128);
-  if (threadIdx.x == 0 && *abort_flag != 0) *p.ix.status = *abort_flag;
+  if (threadIdx.x == 0 && *abort_flag != 0) *p.status = *abort_flag;
 }
 
 // ------------------------------------------------------------------------------------------------ expand
@@ -343,11 +389,12 @@ constexpr int kExpOut = 128 * 128 * 2;
 template <int RP> constexpr int kExpBase = RP > 64 ? 3 : 4;
 template <int RP> constexpr int kExpW = (RP > 64 ? 2 : 1) * kLBox;               // one adapter's 128 columns
 template <int RP> constexpr int kExpWStages = RP > 64 ? 2 : 4;
-template <int RP> constexpr int kExpSmem = kExpBase<RP> * kExpOut + (kExpWStages<RP> + 1) * kExpW<RP> + (kExpEpi * kExpBase<RP> + 2 * kExpWStages<RP> + 9) * 8 + 16 + 1024;
+template <int RP> constexpr int kExpSmem = kExpBase<RP> * kExpOut + (kExpWStages<RP> + 1) * kExpW<RP> + (kExpEpi * kExpBase<RP> + 2 * kExpWStages<RP> + 10) * 8 + 16 + 1024;
 
 struct ExpandParams {
-  LoraIndex ix;
-  int N, has_base, per_cta;
+  LoraTiles tiles;
+  int N, has_base;
+  int* status;
 };
 
 template <int RP, bool WMN>
@@ -361,10 +408,10 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_v + W);
   const uint32_t bar_base = smem_u32(bars);      // [stage][epilogue warp]
   const uint32_t bar_wfull = bar_base + 8 * kExpEpi * BASES, bar_wempty = bar_wfull + 8 * WS;
-  const uint32_t bar_tfull = bar_wempty + 8 * WS, bar_tempty = bar_tfull + 32, bar_v = bar_tempty + 32;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kExpEpi * BASES + 2 * WS + 9);
+  const uint32_t bar_tfull = bar_wempty + 8 * WS, bar_tempty = bar_tfull + 32, bar_v = bar_tempty + 32, bar_vfree = bar_v + 8;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kExpEpi * BASES + 2 * WS + 10);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  __shared__ LoraSlots slots;
+  __shared__ LoraShare share;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kExpEpi * BASES; ++s) mbar_init(bar_base + 8 * s, 1);
@@ -377,6 +424,7 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
       mbar_init(bar_tempty + 8 * b, kExpEpi);
     }
     mbar_init(bar_v, 1);
+    mbar_init(bar_vfree, 1);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmV);
@@ -389,14 +437,24 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
     tmem_relinquish();
   }
   grid_dep_wait();
+  const int nct = (p.N + 127) / 128;
+  // a tile's columns take so much longer with each further adapter (8192 x 14336, rank 32: 1.7 us a tile with one, 0.25 more with each)
+  auto weight = [&](int n) { return 7 + max(0, n - 1); };
   tc_fence_before();
-  __syncthreads();
+  lora_share<kExpThreads>(p.tiles, blockIdx.x, gridDim.x, [&](int n) { return static_cast<long long>(nct) * weight(n); }, share);
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int nct = (p.N + 127) / 128;
-  const long long total = static_cast<long long>((p.ix.T + kLTile - 1) / kLTile) * nct;
-  long long item = static_cast<long long>(blockIdx.x) * p.per_cta;
-  const long long end = min(total, item + p.per_cta);
+  long long item, end;       // this CTA's (tile, columns): those that begin in its share
+  {
+    long long at[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int w = share.tile[e] < p.tiles.tiles ? weight(tile_n(p.tiles, share.tile[e])) : 1;
+      at[e] = static_cast<long long>(share.tile[e]) * nct + (share.rest[e] + w - 1) / w;
+    }
+    item = at[0];
+    end = at[1];
+  }
   int bs = 0, ws = 0, buf = 0;                       // places in the rings, their phases
   uint32_t bph = 0, wph = 0, tph = 0, vph = 0;
   bool ok = true;
@@ -413,26 +471,27 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
   __syncwarp();
   const long long first_item = item;
   long long now = item;                              // epilogue: the tile at hand
-  int mine_next = lora_ahead(p.ix, static_cast<int>(item / nct));
   while (item < end) {
     const int tile = static_cast<int>(item / nct), ct0 = static_cast<int>(item - static_cast<long long>(tile) * nct);
     const int ct1 = static_cast<int>(min(static_cast<long long>(nct), ct0 + (end - item)));
     item += ct1 - ct0;
-    lora_slots(p.ix, mine_next, slots);
-    const int n = slots.n;
-    if (item < end) mine_next = lora_ahead(p.ix, tile + 1);
+    const int n = tile_n(p.tiles, tile);
     if (warp == 0) {
       if (elect_one()) {
         if (n > 0) {
-          mbar_arrive_expect_tx(bar_v, W);
-          for (int h = 0; h < W / kLBox; ++h) tma_load_3d(smem_u32(s_v) + h * kLBox, &tmV, bar_v, 64 * h, tile * kLTile, 0);
+          ok = ok && mbar_wait(bar_vfree, vph ^ 1, abort_flag, ST_WAIT_PRODUCER);
+          vph ^= 1;
+          if (ok) {
+            mbar_arrive_expect_tx(bar_v, W);
+            for (int h = 0; h < W / kLBox; ++h) tma_load_3d(smem_u32(s_v) + h * kLBox, &tmV, bar_v, 64 * h, tile * kLTile, 0);
+          }
         }
         for (int ct = ct0; ct < ct1 && ok; ++ct) {
           for (int j = 0; j < n; ++j) {
             ok = mbar_wait(bar_wempty + 8 * ws, wph ^ 1, abort_flag, ST_WAIT_PRODUCER);
             if (!ok) break;
             const uint32_t full = bar_wfull + 8 * ws, to = smem_u32(s_w + ws * W);
-            const int l = slots.adapter[j];
+            const int l = tile_adapter(p.tiles, tile, j);
             if constexpr (WMN) {      // RP rows of 64 columns each
               mbar_arrive_expect_tx(full, 2 * RP * 128);
               tma_load_3d(to, &tmW, full, ct * 128, 0, l);
@@ -478,9 +537,10 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
             tph ^= 1;
           }
         }
+        if (n > 0 && ok) umma_commit(bar_vfree);
       }
     } else {
-      const int mine = slots.slot[32 * q + lane];
+      const int mine = tile_slot(p.tiles, tile, 32 * q + lane);
       const uint32_t taddr = tmem + (static_cast<uint32_t>(32 * q) << 16) + 64 * part;
       for (int ct = ct0; ct < ct1; ++ct, ++now) {
         float acc[64];
@@ -535,7 +595,7 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          if (ok && ct * 128 + 64 * part < p.N && tile * kLTile + 32 * q < p.ix.T) tma_store_3d(&tmOut, smem_u32(box), ct * 128 + 64 * part, tile * kLTile + 32 * q, 0);
+          if (ok && ct * 128 + 64 * part < p.N && tile * kLTile + 32 * q < p.tiles.T) tma_store_3d(&tmOut, smem_u32(box), ct * 128 + 64 * part, tile * kLTile + 32 * q, 0);
           bulk_commit_group();
           if (p.has_base && now > first_item) {      // the result before has left its box, which takes the base of a tile to come
             asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
@@ -549,7 +609,6 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
       }
     }
     __syncwarp();
-    __syncthreads();       // the slots are made anew
   }
   grid_dep_launch();
   if (warp >= 2 && lane == 0) bulk_wait_all();
@@ -557,7 +616,7 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem, 512);
-  if (threadIdx.x == 0 && *abort_flag != 0) *p.ix.status = *abort_flag;
+  if (threadIdx.x == 0 && *abort_flag != 0) *p.status = *abort_flag;
 }
 
 // ------------------------------------------------------------------------------------------------ gradients of the factors
@@ -1104,25 +1163,27 @@ static int by_rank(int rp, F f) {
 }
 
 // W: (L,R,D), or (wmn) (L,D,R)
-static int lora_shrink(const void* X, int64_t ldx, const void* W, bool wmn, ShrinkParams p, cudaStream_t st) {
+static int lora_shrink(const void* X, int64_t ldx, const void* W, bool wmn, int64_t L, ShrinkParams p, cudaStream_t st) {
   return by_rank(padded_rank(p.R), [&](auto rp) -> int {
     constexpr int RP = decltype(rp)::value;
+    const int64_t T = p.tiles.T, tiles = p.tiles.tiles, blocks = ceil_div(p.D, 64);
     CUtensorMap tmX, tmW;
-    int rc = make_map(&tmX, X, p.D, p.ix.T, 1, ldx, ldx * p.ix.T, 64, kLTile);
-    if (rc == 0) rc = wmn ? make_map(&tmW, W, p.R, p.D, p.ix.L, p.R, static_cast<int64_t>(p.R) * p.D, 64, 64)
-                          : make_map(&tmW, W, p.D, p.R, p.ix.L, p.D, static_cast<int64_t>(p.R) * p.D, 64, RP);
+    int rc = make_map(&tmX, X, p.D, T, 1, ldx, ldx * T, 64, kLTile);
+    if (rc == 0) rc = wmn ? make_map(&tmW, W, p.R, p.D, L, p.R, static_cast<int64_t>(p.R) * p.D, 64, 64)
+                          : make_map(&tmW, W, p.D, p.R, L, p.D, static_cast<int64_t>(p.R) * p.D, 64, RP);
     if (rc) return rc;
-    const int64_t tiles = ceil_div(p.ix.T, kLTile), blocks = ceil_div(p.D, 64);
+    const int columns = wmn && RP < 64 ? 64 : RP;      // of an adapter; as many adapters as make 128 share a unit
+    const int64_t slots = std::min<int64_t>(128 / columns, L), units = tiles * ceil_div(std::min<int64_t>(L, kLTile), slots);      // at most
     p.split = 1;
     while (p.split < 8 && tiles * p.split * 2 <= 2 * num_sms() && blocks >= 4 * p.split) p.split *= 2;
-    const int columns = wmn && RP < 64 ? 64 : RP;      // of an adapter; as many adapters as make 128 share a pass
-    p.stage = kLBox + static_cast<int>(std::min<int64_t>(128 / columns, p.ix.L)) * columns * 128;
+    const int64_t clusters = std::min<int64_t>(units, 2 * num_sms() / p.split);
+    p.stage = kLBox + static_cast<int>(slots) * columns * 128;
     p.stages = std::min(kShrinkMost, kShrinkRing / p.stage);
     auto run = [&](auto mn) -> int {
       constexpr bool MN = decltype(mn)::value;
       static PerDevice allowed;
       B200_CUDA(allow_smem(allowed, lora_shrink_kernel<RP, MN>, kShrinkSmem));
-      B200_CUDA(launch_chained(lora_shrink_kernel<RP, MN>, static_cast<int>(tiles * p.split), kShrinkThreads, kShrinkSmem, st, p.split, tmX, tmW, p));
+      B200_CUDA(launch_chained(lora_shrink_kernel<RP, MN>, static_cast<int>(clusters * p.split), kShrinkThreads, kShrinkSmem, st, p.split, tmX, tmW, p));
       return 0;
     };
     return wmn ? run(std::true_type()) : run(std::false_type());
@@ -1130,21 +1191,19 @@ static int lora_shrink(const void* X, int64_t ldx, const void* W, bool wmn, Shri
 }
 
 // W: (L,N,R), or (wmn) (L,R,N)
-static int lora_expand(const void* V, const void* W, bool wmn, int64_t R, const void* base, int64_t ldb, void* out, ExpandParams p, cudaStream_t st) {
+static int lora_expand(const void* V, const void* W, bool wmn, int64_t L, int64_t R, const void* base, int64_t ldb, void* out, ExpandParams p, cudaStream_t st) {
   return by_rank(padded_rank(R), [&](auto rp) -> int {
     constexpr int RP = decltype(rp)::value;
     CUtensorMap tmV, tmW, tmB, tmO;
-    const int64_t T = p.ix.T, N = p.N;
+    const int64_t T = p.tiles.T, N = p.N;
     int rc = make_map(&tmV, V, RP, T, 1, RP, T * RP, 64, kLTile);
-    if (rc == 0) rc = wmn ? make_map(&tmW, W, N, R, p.ix.L, N, N * R, 64, RP) : make_map(&tmW, W, R, N, p.ix.L, R, N * R, 64, 128);
+    if (rc == 0) rc = wmn ? make_map(&tmW, W, N, R, L, N, N * R, 64, RP) : make_map(&tmW, W, R, N, L, R, N * R, 64, 128);
     if (rc == 0) rc = make_map(&tmO, out, N, T, 1, N, N * T, 64, 32);
     tmB = tmO;
     if (rc == 0 && base != nullptr) rc = make_map(&tmB, base, N, T, 1, ldb, ldb * T, 64, 32);
     if (rc) return rc;
     p.has_base = base != nullptr;
-    const int64_t items = ceil_div(T, kLTile) * ceil_div(N, 128);
-    p.per_cta = static_cast<int>(ceil_div(items, num_sms()));
-    const int grid = static_cast<int>(ceil_div(items, p.per_cta));
+    const int grid = static_cast<int>(std::min<int64_t>(num_sms(), p.tiles.tiles * ceil_div(N, 128)));
     auto run = [&](auto mn) -> int {
       constexpr bool MN = decltype(mn)::value;
       static PerDevice allowed;
@@ -1196,16 +1255,26 @@ struct LoraCarver {
 };
 struct LoraKept {
   __nv_bfloat16* v;
+  LoraTiles tiles;
   int* rows;
   unsigned char* present;
 };
-static LoraKept carve_lora(int64_t T, int64_t R, int64_t L, int keep, void* ws, size_t* bytes) {
+// index: the call has one
+static LoraKept carve_lora(int64_t T, int64_t R, int64_t L, bool index, int keep, void* ws, size_t* bytes) {
   LoraCarver c{static_cast<char*>(ws)};
   LoraKept k{};
+  const int64_t tiles = ceil_div(T, kLTile);
   k.v = c.take<__nv_bfloat16>(T * padded_rank(R));
-  if (keep) {
-    k.rows = c.take<int>(T);
-    k.present = c.take<unsigned char>(ceil_div(T, kLTile) * L);
+  k.tiles.T = static_cast<int>(T);
+  k.tiles.tiles = static_cast<int>(tiles);
+  if (index) {
+    k.tiles.n = c.take<int>(tiles);
+    k.tiles.adapter = c.take<int>(tiles * kLTile);
+    k.tiles.slot = c.take<short>(tiles * kLTile);
+    if (keep) {
+      k.rows = c.take<int>(T);
+      k.present = c.take<unsigned char>(tiles * L);
+    }
   }
   *bytes = c.off;
   return k;
@@ -1236,7 +1305,7 @@ extern "C" {
 size_t b200moe_lora_fwd_ws_bytes(int64_t T, int64_t R, int64_t L, int keep) {
   if (T <= 0 || R <= 0 || L <= 0) return 0;
   size_t bytes = 0;
-  carve_lora(T, R, L, keep, nullptr, &bytes);
+  carve_lora(T, R, L, true, keep, nullptr, &bytes);
   return std::max(bytes, T <= kFewMost ? 2 * T * sizeof(FewRank) : 0);
 }
 
@@ -1274,15 +1343,18 @@ int b200moe_lora_forward(const void* x, int64_t ldx, const void* a, const void* 
     return R <= 16 ? run(std::integral_constant<int, 1>()) : R <= 32 ? run(std::integral_constant<int, 2>()) : run(std::integral_constant<int, 0>());
   }
   size_t bytes;
-  const LoraKept k = carve_lora(T, R, L, keep, ws, &bytes);
+  const LoraKept k = carve_lora(T, R, L, index != nullptr, keep, ws, &bytes);
+  if (index != nullptr) {
+    OpScope scope("lora_tiles", 1);
+    B200_LAUNCH(lora_tiles_kernel, k.tiles.tiles, kLTile, 0, st, ix, k.tiles, k.rows, k.present);
+  }
   {
     OpScope scope("lora_shrink", 1);
-    const int rc2 = lora_shrink(x, ldx, a, false,
-                                ShrinkParams{ix, static_cast<int>(K), static_cast<int>(R), 1, 0, 0, scales, scale, k.v, k.rows, index != nullptr ? k.present : nullptr}, st);
+    const int rc2 = lora_shrink(x, ldx, a, false, L, ShrinkParams{k.tiles, static_cast<int>(K), static_cast<int>(R), 1, 0, 0, scales, scale, k.v, status}, st);
     if (rc2) return rc2;
   }
   OpScope scope("lora_expand", 1);
-  return lora_expand(k.v, b, false, R, base, ldb, out, ExpandParams{ix, static_cast<int>(N), 0, 0}, st);
+  return lora_expand(k.v, b, false, L, R, base, ldb, out, ExpandParams{k.tiles, static_cast<int>(N), 0, status}, st);
 }
 
 size_t b200moe_lora_bwd_ws_bytes(int64_t T, int64_t K, int64_t N, int64_t R, int64_t L) {
@@ -1307,12 +1379,11 @@ int b200moe_lora_backward(const void* grad_out, const void* x, int64_t ldx, cons
                  B200MOE_E_ALIGN, "lora_backward: tensors must be 16-byte aligned");
   cudaStream_t st = (cudaStream_t)stream;
   size_t bytes;
-  const LoraKept k = carve_lora(T, R, L, 1, const_cast<void*>(fwd_ws), &bytes);
+  const LoraKept k = carve_lora(T, R, L, has_index != 0, 1, const_cast<void*>(fwd_ws), &bytes);
   LoraCarver c{static_cast<char*>(ws)};
   __nv_bfloat16* u = c.take<__nv_bfloat16>(T * padded_rank(R));
   float* part = c.take<float>(0);
-  const LoraIndex ix{has_index ? k.rows : nullptr, 4, static_cast<int>(T), static_cast<int>(L), status};
-  WgradParams w{static_cast<int>(T), 0, static_cast<int>(R), static_cast<int>(L), 1, 0, has_index ? k.rows : nullptr, has_index ? k.present : nullptr,
+  WgradParams w{static_cast<int>(T), 0, static_cast<int>(R), static_cast<int>(L), 1, 0, k.rows, k.present,
                 nullptr, 0, status};
 #define RUN(name, launches, call)     \
   do {                                \
@@ -1322,14 +1393,14 @@ int b200moe_lora_backward(const void* grad_out, const void* x, int64_t ldx, cons
   } while (0)
   if (grad_x || grad_a)
     RUN("lora_shrink", 1,
-        lora_shrink(grad_out, N, b, true, ShrinkParams{ix, static_cast<int>(N), static_cast<int>(R), 1, 0, 0, scales, scale, u, nullptr, nullptr}, st));
+        lora_shrink(grad_out, N, b, true, L, ShrinkParams{k.tiles, static_cast<int>(N), static_cast<int>(R), 1, 0, 0, scales, scale, u, status}, st));
   if (grad_b) {
     w.D = static_cast<int>(N);
     w.transposed = 0;
     RUN("lora_wgrad", wgrad_splits(T, N, L) > 1 ? 2 : 1, lora_wgrad(grad_out, N, k.v, w, part, grad_b, grad_f32, st));
   }
   if (grad_x)
-    RUN("lora_expand", 1, lora_expand(u, a, true, R, nullptr, 0, grad_x, ExpandParams{ix, static_cast<int>(K), 0, 0}, st));
+    RUN("lora_expand", 1, lora_expand(u, a, true, L, R, nullptr, 0, grad_x, ExpandParams{k.tiles, static_cast<int>(K), 0, status}, st));
   if (grad_a) {
     w.D = static_cast<int>(K);
     w.transposed = 1;
