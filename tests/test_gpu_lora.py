@@ -318,7 +318,7 @@ def test_observer(pkg):
     assert seen(lambda: pkg.lora_linear(x, a[:1], b[:1])) == [("lora_shrink", 1), ("lora_expand", 1)]
     x.requires_grad_(), a.requires_grad_(), b.requires_grad_()
     got = [n for n, _ in seen(lambda: pkg.lora_linear(x, a, b, index, s).float().sum().backward())]
-    assert sorted(got) == sorted(["lora_tiles"] + ["lora_shrink", "lora_expand"] * 2 + ["lora_wgrad"] * 2)
+    assert sorted(got) == sorted(["lora_tiles", "lora_shrink", "lora_expand", "lora_back", "lora_expand", "lora_wgrad"])
 
 
 def test_refusals(pkg):

@@ -208,19 +208,17 @@ struct ShrinkParams {
   int* status;
 };
 
+// one CTA of share `part` of `parts`, of a cluster or not
 template <int RP, bool WMN>
-__global__ void __launch_bounds__(kShrinkThreads)
-lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const ShrinkParams p) {
+__device__ __forceinline__ void shrink_rows(const CUtensorMap& tmX, const CUtensorMap& tmW, const ShrinkParams& p, int part, int parts, uint8_t* smem,
+                                            LoraShare& share) {
   constexpr int NB = WMN && RP < 64 ? 64 : RP;       // accumulator columns of an adapter: whole swizzle atoms where W is MN-major
   constexpr int SLOTS = 128 / NB;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kShrinkRing);
   const uint32_t bar_full = smem_u32(bars), bar_empty = smem_u32(bars + kShrinkMost);
   const uint32_t bar_tfull = smem_u32(bars + 2 * kShrinkMost), bar_tempty = bar_tfull + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kShrinkMost + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  __shared__ LoraShare share;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = p.split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   if (threadIdx.x == 0) {
@@ -241,7 +239,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
   }
   grid_dep_wait();
   tc_fence_before();
-  lora_share<kShrinkThreads>(p.tiles, blockIdx.x / p.split, gridDim.x / p.split, [](int n) { return max(1, (n + SLOTS - 1) / SLOTS); }, share);
+  lora_share<kShrinkThreads>(p.tiles, part, parts, [](int n) { return max(1, (n + SLOTS - 1) / SLOTS); }, share);
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int nkb = (p.D + 63) / 64;
@@ -378,6 +376,18 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem, 128);
   if (threadIdx.x == 0 && *abort_flag != 0) *p.status = *abort_flag;
+}
+
+__device__ __forceinline__ uint8_t* aligned_smem(uint8_t* raw) {
+  return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+}
+
+template <int RP, bool WMN>
+__global__ void __launch_bounds__(kShrinkThreads)
+lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const ShrinkParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ LoraShare share;
+  shrink_rows<RP, WMN>(tmX, tmW, p, blockIdx.x / p.split, gridDim.x / p.split, aligned_smem(smem_raw), share);
 }
 
 // ------------------------------------------------------------------------------------------------ expand
@@ -637,19 +647,15 @@ struct WgradParams {
 };
 
 template <int RP>
-__global__ void __launch_bounds__(kWgThreads)
-lora_wgrad_kernel(const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmV, const WgradParams p) {
+__device__ __forceinline__ void wgrad_rows(const CUtensorMap& tmY, const CUtensorMap& tmV, const WgradParams& p, int part, uint8_t* smem, unsigned* live) {
   constexpr int NB = RP < 64 ? 64 : RP, ST = kWgStages<RP>, STAGE = kLBox + kWgV<RP>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + ST * STAGE);
   const uint32_t bar_full = smem_u32(bars), bar_ready = bar_full + 8 * ST, bar_empty = bar_ready + 8 * ST, bar_tfull = bar_empty + 8 * ST;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * ST + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  __shared__ unsigned live[kWgWords];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int chunks = (p.D + 127) / 128;
-  const int chunk = blockIdx.x % chunks, l = blockIdx.x / chunks % p.L, split = blockIdx.x / chunks / p.L;
+  const int chunk = part % chunks, l = part / chunks % p.L, split = part / chunks / p.L;
   const int blocks = (p.T + 63) / 64;
   const int b0 = static_cast<int>(static_cast<long long>(split) * blocks / p.splits), b1 = static_cast<int>(static_cast<long long>(split + 1) * blocks / p.splits);
   if (threadIdx.x == 0) {
@@ -805,6 +811,33 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap tmY, const __grid_constant
   }
   if (warp == 1) tmem_dealloc(tmem, NB);
   if (threadIdx.x == 0 && *abort_flag != 0) *p.status = *abort_flag;
+}
+
+template <int RP>
+__global__ void __launch_bounds__(kWgThreads)
+lora_wgrad_kernel(const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmV, const WgradParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ unsigned live[kWgWords];
+  wgrad_rows<RP>(tmY, tmV, p, blockIdx.x, aligned_smem(smem_raw), live);
+}
+
+// Both products of the gradient g in one launch, shrink (u = g B) and wgrad (of B): by turns a cluster of the one and of the other, so that an SM has a
+// CTA of each, one waits for memory while the other computes, and what one has read the other finds in L2.
+constexpr int kBackThreads = kShrinkThreads;
+static_assert(kShrinkThreads == kWgThreads, "roles of one launch");
+template <int RP> constexpr int kBackSmem = kShrinkSmem > kWgSmem<RP> ? kShrinkSmem : kWgSmem<RP>;
+template <int RP>
+__global__ void __launch_bounds__(kBackThreads, 2)
+lora_back_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmY,
+                 const __grid_constant__ CUtensorMap tmV, const ShrinkParams p, const WgradParams w, int shrinks, int wgrads) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ LoraShare share;
+  __shared__ unsigned live[kWgWords];
+  const int c = blockIdx.x / p.split, both = 2 * min(shrinks, wgrads);      // clusters of the roles
+  const bool shrink = c < both ? (c & 1) == 0 : shrinks > wgrads;
+  const int part = c < both ? c >> 1 : c - both / 2;
+  if (shrink) shrink_rows<RP, true>(tmX, tmW, p, part, shrinks, aligned_smem(smem_raw), share);
+  else wgrad_rows<RP>(tmY, tmV, w, part * p.split + blockIdx.x % p.split, aligned_smem(smem_raw), live);
 }
 
 // the sum of the splits' shares, n values (a multiple of 4), always in the same order; eight of them are on their way at a time
@@ -1162,11 +1195,18 @@ static int by_rank(int rp, F f) {
   return f(std::integral_constant<int, 128>());
 }
 
-// W: (L,R,D), or (wmn) (L,D,R)
+// CTAs that share the columns of a unit, for so many CTAs at a time
+static int shrink_split(int64_t T, int64_t D, int64_t ctas) {
+  const int64_t tiles = ceil_div(T, kLTile), blocks = ceil_div(D, 64);
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= ctas && blocks >= 4 * split) split *= 2;
+  return split;
+}
+// W: (L,R,D), or (wmn) (L,D,R); split: 0, or that of the gradients' launch
 static int lora_shrink(const void* X, int64_t ldx, const void* W, bool wmn, int64_t L, ShrinkParams p, cudaStream_t st) {
   return by_rank(padded_rank(p.R), [&](auto rp) -> int {
     constexpr int RP = decltype(rp)::value;
-    const int64_t T = p.tiles.T, tiles = p.tiles.tiles, blocks = ceil_div(p.D, 64);
+    const int64_t T = p.tiles.T, tiles = p.tiles.tiles;
     CUtensorMap tmX, tmW;
     int rc = make_map(&tmX, X, p.D, T, 1, ldx, ldx * T, 64, kLTile);
     if (rc == 0) rc = wmn ? make_map(&tmW, W, p.R, p.D, L, p.R, static_cast<int64_t>(p.R) * p.D, 64, 64)
@@ -1174,8 +1214,7 @@ static int lora_shrink(const void* X, int64_t ldx, const void* W, bool wmn, int6
     if (rc) return rc;
     const int columns = wmn && RP < 64 ? 64 : RP;      // of an adapter; as many adapters as make 128 share a unit
     const int64_t slots = std::min<int64_t>(128 / columns, L), units = tiles * ceil_div(std::min<int64_t>(L, kLTile), slots);      // at most
-    p.split = 1;
-    while (p.split < 8 && tiles * p.split * 2 <= 2 * num_sms() && blocks >= 4 * p.split) p.split *= 2;
+    if (p.split == 0) p.split = shrink_split(T, p.D, 2 * num_sms());
     const int64_t clusters = std::min<int64_t>(units, 2 * num_sms() / p.split);
     p.stage = kLBox + static_cast<int>(slots) * columns * 128;
     p.stages = std::min(kShrinkMost, kShrinkRing / p.stage);
@@ -1221,14 +1260,24 @@ static int wgrad_splits(int64_t T, int64_t D, int64_t L) {
   const int64_t s = std::max<int64_t>(1, std::min<int64_t>(2 * num_sms() / ctas, blocks / 8));
   return static_cast<int>(std::max<int64_t>(s, ceil_div(blocks, 32 * kWgWords)));
 }
-static int lora_wgrad(const void* Y, int64_t ldy, const void* V, WgradParams p, float* ws, void* out, int out_f32, cudaStream_t st) {
+// The same for the gradient of B, which shares its launch with u = g B where that is wanted: one CTA an SM of either role, in whole clusters.  By itself it
+// has as many shares, so that its bits do not depend on what else is asked for.
+static int back_wgrad_splits(int64_t T, int64_t D, int64_t L) {
+  const int64_t blocks = ceil_div(T, 64), ctas = ceil_div(D, 128) * L;
+  const int64_t s = std::max<int64_t>(1, std::min<int64_t>(num_sms() / ctas, blocks / 8));
+  const int split = shrink_split(T, D, num_sms());
+  int64_t n = std::max<int64_t>(s, ceil_div(blocks, 32 * kWgWords));
+  while (n * ctas % split != 0) ++n;
+  return static_cast<int>(n);
+}
+static int lora_wgrad(const void* Y, int64_t ldy, const void* V, int splits, WgradParams p, float* ws, void* out, int out_f32, cudaStream_t st) {
   return by_rank(padded_rank(p.R), [&](auto rp) -> int {
     constexpr int RP = decltype(rp)::value;
     CUtensorMap tmY, tmV;
     int rc = make_map(&tmY, Y, p.D, p.T, 1, ldy, ldy * p.T, 64, 64);
     if (rc == 0) rc = make_map(&tmV, V, RP, p.T, 1, RP, static_cast<int64_t>(p.T) * RP, 64, 64);
     if (rc) return rc;
-    p.splits = wgrad_splits(p.T, p.D, p.L);
+    p.splits = splits;
     p.out = p.splits > 1 ? static_cast<void*>(ws) : out;
     p.out_f32 = p.splits > 1 || out_f32;
     static PerDevice allowed;
@@ -1237,6 +1286,38 @@ static int lora_wgrad(const void* Y, int64_t ldy, const void* V, WgradParams p, 
     if (p.splits > 1) {
       const long long n = static_cast<long long>(p.L) * p.D * p.R;
       B200_LAUNCH(lora_wgrad_sum_kernel, static_cast<int>(ceil_div(n, 512)), 128, 0, st, static_cast<const float*>(ws), p.splits, n, out, out_f32);
+    }
+    return 0;
+  });
+}
+
+// The launch of both: an SM holds a CTA of each role
+static int lora_back(const void* G, const void* B, const void* V, int64_t L, ShrinkParams p, WgradParams w, float* ws, void* out, int out_f32, cudaStream_t st) {
+  return by_rank(padded_rank(p.R), [&](auto rp) -> int {
+    constexpr int RP = decltype(rp)::value;
+    const int64_t T = p.tiles.T, D = p.D, tiles = p.tiles.tiles;
+    CUtensorMap tmX, tmW, tmY, tmV;
+    int rc = make_map(&tmX, G, D, T, 1, D, D * T, 64, kLTile);
+    if (rc == 0) rc = make_map(&tmW, B, p.R, D, L, p.R, static_cast<int64_t>(p.R) * D, 64, 64);
+    if (rc == 0) rc = make_map(&tmY, G, D, T, 1, D, D * T, 64, 64);
+    if (rc == 0) rc = make_map(&tmV, V, RP, T, 1, RP, T * RP, 64, 64);
+    if (rc) return rc;
+    const int columns = RP < 64 ? 64 : RP;
+    const int64_t slots = std::min<int64_t>(128 / columns, L), units = tiles * ceil_div(std::min<int64_t>(L, kLTile), slots);
+    const int64_t shrinks = std::min<int64_t>(units, num_sms() / p.split);
+    p.stage = kLBox + static_cast<int>(slots) * columns * 128;
+    p.stages = std::min(kShrinkMost, kShrinkRing / p.stage);
+    w.splits = back_wgrad_splits(T, D, L);
+    w.out = w.splits > 1 ? static_cast<void*>(ws) : out;
+    w.out_f32 = w.splits > 1 || out_f32;
+    const int64_t wgrads = ceil_div(D, 128) * L * w.splits / p.split;
+    static PerDevice allowed;
+    B200_CUDA(allow_smem(allowed, lora_back_kernel<RP>, kBackSmem<RP>));
+    B200_CUDA(launch_chained(lora_back_kernel<RP>, static_cast<int>((shrinks + wgrads) * p.split), kBackThreads, kBackSmem<RP>, st, p.split, tmX, tmW, tmY, tmV,
+                             p, w, static_cast<int>(shrinks), static_cast<int>(wgrads)));
+    if (w.splits > 1) {
+      const long long n = static_cast<long long>(L) * D * p.R;
+      B200_LAUNCH(lora_wgrad_sum_kernel, static_cast<int>(ceil_div(n, 512)), 128, 0, st, static_cast<const float*>(ws), w.splits, n, out, out_f32);
     }
     return 0;
   });
@@ -1350,7 +1431,7 @@ int b200moe_lora_forward(const void* x, int64_t ldx, const void* a, const void* 
   }
   {
     OpScope scope("lora_shrink", 1);
-    const int rc2 = lora_shrink(x, ldx, a, false, L, ShrinkParams{k.tiles, static_cast<int>(K), static_cast<int>(R), 1, 0, 0, scales, scale, k.v, status}, st);
+    const int rc2 = lora_shrink(x, ldx, a, false, L, ShrinkParams{k.tiles, static_cast<int>(K), static_cast<int>(R), 0, 0, 0, scales, scale, k.v, status}, st);
     if (rc2) return rc2;
   }
   OpScope scope("lora_expand", 1);
@@ -1361,7 +1442,7 @@ size_t b200moe_lora_bwd_ws_bytes(int64_t T, int64_t K, int64_t N, int64_t R, int
   if (T <= 0 || K <= 0 || N <= 0 || R <= 0 || L <= 0) return 0;
   LoraCarver c{nullptr};
   c.take<__nv_bfloat16>(T * padded_rank(R));
-  const int sa = wgrad_splits(T, K, L), sb = wgrad_splits(T, N, L);
+  const int sa = wgrad_splits(T, K, L), sb = back_wgrad_splits(T, N, L);
   c.take<float>(std::max(sa > 1 ? sa * L * R * K : 0, sb > 1 ? sb * L * R * N : 0));
   return c.off;
 }
@@ -1373,7 +1454,7 @@ int b200moe_lora_backward(const void* grad_out, const void* x, int64_t ldx, cons
   if (rc) return rc;
   B200_CHECK_ARG(T >= 1, B200MOE_E_BAD_SHAPE, "lora_backward: no rows");
   B200_CHECK_ARG(ldx >= K && ldx % 8 == 0, B200MOE_E_BAD_SHAPE, "lora_backward: rows of x %lld apart", (long long)ldx);
-  B200_CHECK_ARG(grad_out && x && a && b && fwd_ws && ws && status, B200MOE_E_NULL, "lora_backward: null pointer");
+  B200_CHECK_ARG(grad_out && x && a && b && fwd_ws && ws && status && (grad_x || grad_a || grad_b), B200MOE_E_NULL, "lora_backward: null pointer");
   B200_CHECK_ARG(aligned16(grad_out) && aligned16(x) && aligned16(a) && aligned16(b) && aligned16(fwd_ws) && aligned16(ws) && aligned16(grad_x) &&
                      aligned16(grad_a) && aligned16(grad_b),
                  B200MOE_E_ALIGN, "lora_backward: tensors must be 16-byte aligned");
@@ -1391,20 +1472,23 @@ int b200moe_lora_backward(const void* grad_out, const void* x, int64_t ldx, cons
     const int rc__ = (call);          \
     if (rc__) return rc__;            \
   } while (0)
-  if (grad_x || grad_a)
-    RUN("lora_shrink", 1,
-        lora_shrink(grad_out, N, b, true, L, ShrinkParams{k.tiles, static_cast<int>(N), static_cast<int>(R), 1, 0, 0, scales, scale, u, status}, st));
-  if (grad_b) {
+  const ShrinkParams sp{k.tiles, static_cast<int>(N), static_cast<int>(R), shrink_split(T, N, num_sms()), 0, 0, scales, scale, u, status};
+  const int sa = wgrad_splits(T, K, L), sb = back_wgrad_splits(T, N, L);
+  if (grad_b && (grad_x || grad_a)) {
     w.D = static_cast<int>(N);
-    w.transposed = 0;
-    RUN("lora_wgrad", wgrad_splits(T, N, L) > 1 ? 2 : 1, lora_wgrad(grad_out, N, k.v, w, part, grad_b, grad_f32, st));
+    RUN("lora_back", sb > 1 ? 2 : 1, lora_back(grad_out, b, k.v, L, sp, w, part, grad_b, grad_f32, st));
+  } else if (grad_b) {
+    w.D = static_cast<int>(N);
+    RUN("lora_wgrad", sb > 1 ? 2 : 1, lora_wgrad(grad_out, N, k.v, sb, w, part, grad_b, grad_f32, st));
+  } else {
+    RUN("lora_shrink", 1, lora_shrink(grad_out, N, b, true, L, sp, st));
   }
   if (grad_x)
     RUN("lora_expand", 1, lora_expand(u, a, true, L, R, nullptr, 0, grad_x, ExpandParams{k.tiles, static_cast<int>(K), 0, status}, st));
   if (grad_a) {
     w.D = static_cast<int>(K);
     w.transposed = 1;
-    RUN("lora_wgrad", wgrad_splits(T, K, L) > 1 ? 2 : 1, lora_wgrad(x, ldx, u, w, part, grad_a, grad_f32, st));
+    RUN("lora_wgrad", sa > 1 ? 2 : 1, lora_wgrad(x, ldx, u, sa, w, part, grad_a, grad_f32, st));
   }
 #undef RUN
   return 0;
