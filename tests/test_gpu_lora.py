@@ -285,6 +285,27 @@ def test_streams_and_graphs(pkg, T):
     pkg.check_status()
 
 
+@pytest.mark.parametrize("T", [30, 200, 900])
+def test_inference_mode_and_two_calls_at_once(pkg, T):
+    """Calls on two streams at a time have workspaces of their own."""
+    x, a, b, s, bs, index = make(T, 512, 264, 16, 6)
+    x2, a2, b2, s2, bs2, index2 = make(T, 1024, 520, 32, 9, seed=4)
+    want, want2 = pkg.lora_linear(x, a, b, index, s, bs), pkg.lora_linear(x2, a2, b2, index2, s2, bs2)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    with torch.inference_mode():
+        for _ in range(10):
+            with torch.cuda.stream(streams[0]):
+                got[0].append(pkg.lora_linear(x, a, b, index, s, bs))
+            with torch.cuda.stream(streams[1]):
+                got[1].append(pkg.lora_linear(x2, a2, b2, index2, s2, bs2))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in got[0]) and all(torch.equal(o, want2) for o in got[1])
+    pkg.check_status()
+
+
 @pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning", "ignore::DeprecationWarning")
 def test_traced_forward_gradients_and_autocast(pkg):
     x, a, b, s, bs, index = make(40, 256, 64, 16, 3)

@@ -179,6 +179,32 @@ def test_layouts(pkg, K):
     assert one.grad.shape == (K,) and torch.isfinite(one.grad).all()
 
 
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("T,K", [(6, 2048), (600, 2048), (600, 1037)])
+@pytest.mark.parametrize("size", [1e-17, 1e15])
+def test_small_and_large_rows(pkg, dt, T, K, size):
+    """Without eps, rows whose squares are near the ends of fp32's range and whose gradients are as far at the other end."""
+    x, _, w = make(T, K, dt, F32, 6)
+    x = (x.float() * size).to(dt).requires_grad_()
+    gy = torch.randn(T, K, generator=gen(8), device=DEV).to(dt)
+    y = pkg.rms_norm(x, w, eps=0)
+    h = x.detach().double()
+    rstd = 1 / torch.sqrt(h.square().mean(-1, keepdim=True))
+    n, d = h * rstd, gy.double() * w.double()
+    close(y.detach(), n * w.double(), (n * w.double()).abs(), 2.0 ** -19)
+    gx, = torch.autograd.grad(y, x, gy)
+    back = (d * n).mean(-1, keepdim=True)
+    close(gx, rstd * (d - n * back), rstd * (d.abs() + n.abs() * (d * n).abs().mean(-1, keepdim=True)), 2.0 ** -17)
+
+
+def test_inference_mode(pkg):
+    x, r, w = make(200, 256, BF)
+    with torch.inference_mode():
+        q, s, y, h = pkg.rms_norm_fp8_block(x, w, r, EPS, return_norm=True)
+    want = pkg.rms_norm_fp8_block(x, w, r, EPS, return_norm=True)
+    assert all(torch.equal(a.float(), b.float()) for a, b in zip((q, s, y, h), want))
+
+
 def test_empty_and_unused(pkg):
     x, r, w = (t.requires_grad_() for t in make(0, 64, BF))
     y, h = pkg.rms_norm(x, w, r)

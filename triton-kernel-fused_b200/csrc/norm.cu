@@ -324,7 +324,9 @@ __global__ void __launch_bounds__(THREADS) rms_norm_bwd_kernel(const NormBwd a) 
 // ------------------------------------------------------------------------------------------------ rows through shared memory
 // A CTA takes up to `group` rows a turn.  Bulk copies keep a ring of `stages` turns full; `tpr` threads share the columns of a row, NV vectors each, and
 // have R rows of a turn at once, so that what is done once a turn (shuffles, a barrier, roots, addresses) is spread over 32
-// values a thread: what bounds these kernels next to HBM is the number of instructions a value.
+// values a thread: what bounds these kernels next to HBM is the number of instructions a value.  us, of the floor at the rate of a plain copy: 16384 x 4096
+// with residual to codes 74 (72), 16384 x 2048 forward 38 (41: part of the result is still in L2), backward 44 (41).  With one vector of one row a thread
+// 113, 49 and 85; with rows in registers and no ring 97, 42 and 74.
 struct NormPlan {
   int threads, tpr, group, stages;
   long long ctas;
@@ -639,8 +641,8 @@ __global__ void __launch_bounds__(512, 1) rms_norm_bwd_rows_kernel(const NormBwd
       const float mine = turn_sums<2 * R>(s, part[flip][g], warps_row, warp_row) / static_cast<float>(a.K);
       if (threadIdx.x == 0 && before >= 0 && p.stages > 1) ring.refill(first + (p.stages - 1) * step, before, before_phase);
       const float other = __shfl_xor_sync(0xffffffffu, mine, 32 / (2 * R));
-      // in a row's first lanes: rstd, and what h is multiplied with, -rstd mean(d n) rstd
-      const float root = inverse_root(mine + a.eps), slope = -root * root * root * other;
+      // in a row's first lanes: rstd, and what n is multiplied with, -rstd mean(d n)
+      const float root = inverse_root(mine + a.eps), slope = -root * (root * other);
       flip ^= 1;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
@@ -658,8 +660,9 @@ __global__ void __launch_bounds__(512, 1) rms_norm_bwd_rows_kernel(const NormBwd
           pairs8(add ? shared8<T>(x + 2 * tensor_bytes + 8 * SIZE * j * p.tpr) : zeros8<T>(), of);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            acc[j][i] = fma2(gf[i], mul2(hf[i], rstd), acc[j][i]);
-            of[i] = fma2(mul2(gf[i], w[j][i]), rstd, fma2(hf[i], back, of[i]));
+            const float2 m = mul2(hf[i], rstd);
+            acc[j][i] = fma2(gf[i], m, acc[j][i]);
+            of[i] = fma2(mul2(gf[i], w[j][i]), rstd, fma2(m, back, of[i]));
           }
           if (a.gx != nullptr) put8(static_cast<T*>(a.gx) + row * a.K + c, a.K - c, from_pairs8<T>(of));
         }
