@@ -109,8 +109,8 @@ __global__ void __launch_bounds__(kLTile) lora_tiles_kernel(const LoraIndex ix, 
   grid_dep_launch();
 }
 
-// Where a share of the tiles' work begins and ends: tile t has weight f(its adapters), and a place is a tile and what of its weight is before.  All
-// threads of the CTA; barriers inside.
+// Where a cluster's share of the units of work begins and ends: tile t has weight f(its adapters), and a place is a tile and what of its weight is
+// before.  All threads of the CTA; barriers inside.
 struct LoraShare {
   long long warps[32], rest[2];
   int tile[2];
@@ -208,6 +208,7 @@ struct ShrinkParams {
   const float* scales;       // (L,), or nullptr: `scale` for all
   float scale;
   __nv_bfloat16* v;          // (T, RP)
+  int* counter;              // of the expand behind it, set to zero
   int* status;
 };
 
@@ -241,6 +242,7 @@ __device__ __forceinline__ void shrink_rows(const CUtensorMap& tmX, const CUtens
     tmem_relinquish();
   }
   grid_dep_wait();
+  if (part == 0 && rank == 0 && threadIdx.x == 0) *p.counter = 0;
   tc_fence_before();
   lora_share<kShrinkThreads>(p.tiles, part, parts, [](int n) { return max(1, (n + SLOTS - 1) / SLOTS); }, share);
   tc_fence_after();
@@ -394,23 +396,30 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
 }
 
 // ------------------------------------------------------------------------------------------------ expand
-// out[t, n] = base[t, n] + sum_r v[t, r] W_l[n, r]; WMN: W_l lies (R, N) (the backward's A).  Persistent CTAs over (row tile, 128 columns), a row
-// tile's columns one after another.  The base's boxes land where the result leaves from: an epilogue warp fetches its own, a few tiles ahead whatever the
-// adapters' products wait for; tensor memory holds four (columns, adapter) products.
-// 8192 x 14336 with one adapter takes 86 us whatever its rank; a kernel that does nothing but move the same boxes takes 84 to 86 (5.5 TB/s), with any
-// number of them on their way and in any order.  Without a base, writing alone, 61 (3.85 TB/s, all that such a stream gets here).  Nine stretches of
-// rows with an adapter each or none 96: tiles of two adapters occupy two of the four products.
-constexpr int kExpEpi = 8, kExpThreads = 64 + 32 * kExpEpi;
+// out[t, n] = base[t, n] + sum_r v[t, r] W_l[n, r]; WMN: W_l lies (R, N) (the backward's A).  Persistent CTAs take items of a row tile and 256 columns (128
+// where there is one for an SM at most) from a counter: SMs do not get equal shares of the memory's rate, and a copy of 470 MB that deals tiles out in
+// turns takes 82 us, one that takes them from a counter 75.  What is claimed ahead is kept short: four items; with eight the half of a small call is dealt
+// out at its start (16384 x 2816, rank 64: 36 and 39).  The base's boxes land where the result leaves from: an epilogue warp fetches its own, a few columns
+// ahead whatever the adapters' products wait for; tensor memory holds four (columns, adapter) products.
+// us: 8192 x 14336, rank 32, nine stretches of rows with an adapter each or none 82 (92 in equal shares by weight, 90 in items of 128 columns), 72 at the
+// rate of a plain copy; 16384 x 2816, rank 64, 36; 16384 x 2048 without a base 22, 10 at that rate, but writing alone gets 3.85 TB/s here: 17.
+constexpr int kExpEpi = 8, kExpThreads = 96 + 32 * kExpEpi;      // warps: loads, products, epilogue, items
 constexpr int kExpOut = 128 * 128 * 2;
 template <int RP> constexpr int kExpBase = RP > 64 ? 3 : 4;
 template <int RP> constexpr int kExpW = (RP > 64 ? 2 : 1) * kLBox;               // one adapter's 128 columns
 template <int RP> constexpr int kExpWStages = RP > 64 ? 2 : 4;
-template <int RP> constexpr int kExpSmem = kExpBase<RP> * kExpOut + (kExpWStages<RP> + 1) * kExpW<RP> + (kExpEpi * kExpBase<RP> + 2 * kExpWStages<RP> + 10) * 8 + 16 + 1024;
+constexpr int kExpQueue = 4;                     // items known ahead: as many as bases are fetched ahead, of single columns each
+template <int RP> constexpr int kExpBars = kExpEpi * kExpBase<RP> + 2 * kExpWStages<RP> + 2 * kExpQueue + 12;
+template <int RP> constexpr int kExpSmem = kExpBase<RP> * kExpOut + (kExpWStages<RP> + 2) * kExpW<RP> + kExpBars<RP> * 8 + 16 + 1024;
 
 struct ExpandParams {
   LoraTiles tiles;
-  int N, has_base;
+  int N, chunk, items, has_base;      // an item: `chunk` times 128 columns of a row tile, or what is left of them
+  int* counter;                       // items that have been handed out, besides each CTA's first
   int* status;
+};
+struct ExpandItem {
+  int tile, ct0, ct1, n;              // row tile (-1: no more), columns from 128 ct0 to 128 ct1, adapters
 };
 
 template <int RP, bool WMN>
@@ -421,13 +430,15 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t *s_w = smem + BASES * kExpOut, *s_v = s_w + WS * W;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_v + W);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_v + 2 * W);
   const uint32_t bar_base = smem_u32(bars);      // [stage][epilogue warp]
   const uint32_t bar_wfull = bar_base + 8 * kExpEpi * BASES, bar_wempty = bar_wfull + 8 * WS;
-  const uint32_t bar_tfull = bar_wempty + 8 * WS, bar_tempty = bar_tfull + 32, bar_v = bar_tempty + 32, bar_vfree = bar_v + 8;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kExpEpi * BASES + 2 * WS + 10);
+  const uint32_t bar_tfull = bar_wempty + 8 * WS, bar_tempty = bar_tfull + 32, bar_v = bar_tempty + 32, bar_vfree = bar_v + 16;
+  const uint32_t bar_qfull = bar_vfree + 16, bar_qempty = bar_qfull + 8 * kExpQueue;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kExpBars<RP>);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  __shared__ LoraShare share;
+  __shared__ ExpandItem queue[kExpQueue];
+  __shared__ __align__(4) signed char slots[kExpQueue][kLTile];      // of the item's rows
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kExpEpi * BASES; ++s) mbar_init(bar_base + 8 * s, 1);
@@ -439,8 +450,14 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
       mbar_init(bar_tfull + 8 * b, 1);
       mbar_init(bar_tempty + 8 * b, kExpEpi);
     }
-    mbar_init(bar_v, 1);
-    mbar_init(bar_vfree, 1);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar_v + 8 * b, 1);
+      mbar_init(bar_vfree + 8 * b, 1);
+    }
+    for (int s = 0; s < kExpQueue; ++s) {
+      mbar_init(bar_qfull + 8 * s, 1);
+      mbar_init(bar_qempty + 8 * s, 2 + kExpEpi);
+    }
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmV);
@@ -454,52 +471,80 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
   }
   grid_dep_wait();
   const int nct = (p.N + 127) / 128;
-  // a tile's columns take so much longer with each further adapter (8192 x 14336, rank 32: 1.7 us a tile with one, 0.25 more with each)
-  auto weight = [&](int n) { return 7 + max(0, n - 1); };
   tc_fence_before();
-  lora_share<kExpThreads>(p.tiles, blockIdx.x, gridDim.x, [&](int n) { return static_cast<long long>(nct) * weight(n); }, share);
+  __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  long long item, end;       // this CTA's (tile, columns): those that begin in its share
-  {
-    long long at[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int w = share.tile[e] < p.tiles.tiles ? weight(tile_n(p.tiles, share.tile[e])) : 1;
-      at[e] = static_cast<long long>(share.tile[e]) * nct + (share.rest[e] + w - 1) / w;
-    }
-    item = at[0];
-    end = at[1];
-  }
-  int bs = 0, ws = 0, buf = 0;                       // places in the rings, their phases
-  uint32_t bph = 0, wph = 0, tph = 0, vph = 0;
+  int ws = 0, buf = 0;                               // places in the rings, their phases
+  uint32_t wph = 0, tph = 0, vs = 0;
   bool ok = true;
+
+  if (warp == kExpThreads / 32 - 1) {                // hands out the items, the one after the next asked for already
+    const int per_tile = (nct + p.chunk - 1) / p.chunk;
+    int at = blockIdx.x, next = 0;
+    for (int e = 0;; ++e) {
+      if (lane == 0) next = atomicAdd(p.counter, 1) + gridDim.x;
+      ExpandItem it{-1, 0, 0, 0};
+      uint32_t slot4 = 0;
+      if (at < p.items) {
+        it.tile = at / per_tile;
+        it.ct0 = (at - it.tile * per_tile) * p.chunk;
+        it.ct1 = min(nct, it.ct0 + p.chunk);
+        it.n = tile_n(p.tiles, it.tile);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) slot4 |= (static_cast<uint32_t>(tile_slot(p.tiles, it.tile, 4 * lane + i)) & 0xffu) << (8 * i);
+      }
+      const int s = e % kExpQueue;
+      if (!__all_sync(0xffffffffu, mbar_wait(bar_qempty + 8 * s, (e / kExpQueue & 1) ^ 1, abort_flag, ST_WAIT_PRODUCER))) break;
+      if (lane == 0) queue[s] = it;
+      reinterpret_cast<uint32_t*>(slots[s])[lane] = slot4;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_qfull + 8 * s);
+      if (it.tile < 0) break;
+      at = __shfl_sync(0xffffffffu, next, 0);
+    }
+    __syncwarp();
+  }
   const int q = warp & 3, part = (warp - 2) >> 2;    // epilogue: the quarter of the rows, the half of the columns
   const uint32_t my_box = smem_u32(smem) + (4 * part + q) * 4096;
-  auto fetch_base = [&](long long i, int stage) {
-    if (i >= end) return;
-    const int tile = static_cast<int>(i / nct), ct = static_cast<int>(i - static_cast<long long>(tile) * nct);
-    mbar_arrive_expect_tx(bar_base + 8 * (kExpEpi * stage + warp - 2), 4096);
-    tma_load_3d(my_box + stage * kExpOut, &tmBase, bar_base + 8 * (kExpEpi * stage + warp - 2), ct * 128 + 64 * part, tile * kLTile + 32 * q, 0);
+  const bool epilogue = warp >= 2 && warp < 2 + kExpEpi;
+  // lane 0 of an epilogue warp: the base of the columns after those it fetched last
+  ExpandItem ahead{0, 0, 0, 0};
+  int ahead_e = -1;
+  auto fetch_base = [&](int stage) {
+    if (ahead.tile < 0) return;
+    if (ahead.ct0 == ahead.ct1) {
+      ++ahead_e;
+      const bool known = mbar_wait(bar_qfull + 8 * (ahead_e % kExpQueue), ahead_e / kExpQueue & 1, abort_flag, ST_WAIT_EPILOGUE);
+      ahead.tile = -1;
+      if (known) ahead = queue[ahead_e % kExpQueue];
+      if (ahead.tile < 0) return;
+    }
+    const uint32_t bar = bar_base + 8 * (kExpEpi * stage + warp - 2);
+    mbar_arrive_expect_tx(bar, 4096);
+    tma_load_3d(my_box + stage * kExpOut, &tmBase, bar, ahead.ct0 * 128 + 64 * part, ahead.tile * kLTile + 32 * q, 0);
+    ++ahead.ct0;
   };
-  if (p.has_base && warp >= 2 && lane == 0)
-    for (int i = 0; i < BASES; ++i) fetch_base(item + i, i);
+  if (p.has_base && epilogue && lane == 0)
+    for (int i = 0; i < BASES; ++i) fetch_base(i);
   __syncwarp();
-  const long long first_item = item;
-  long long now = item;                              // epilogue: the tile at hand
-  while (item < end) {
-    const int tile = static_cast<int>(item / nct), ct0 = static_cast<int>(item - static_cast<long long>(tile) * nct);
-    const int ct1 = static_cast<int>(min(static_cast<long long>(nct), ct0 + (end - item)));
-    item += ct1 - ct0;
-    const int n = tile_n(p.tiles, tile);
+  int bs = 0;
+  uint32_t bph = 0;
+  bool before = false;                               // epilogue: there is a result before this one
+  for (int e = 0; warp < 2 + kExpEpi; ++e) {
+    const int qs = e % kExpQueue;
+    if (!__all_sync(0xffffffffu, mbar_wait(bar_qfull + 8 * qs, e / kExpQueue & 1, abort_flag, ST_WAIT_PRODUCER))) break;
+    const ExpandItem it = queue[qs];
+    if (it.tile < 0) break;
+    const int tile = it.tile, ct0 = it.ct0, ct1 = it.ct1, n = it.n;
+    __syncwarp();
     if (warp == 0) {
       if (elect_one()) {
         if (n > 0) {
-          ok = ok && mbar_wait(bar_vfree, vph ^ 1, abort_flag, ST_WAIT_PRODUCER);
-          vph ^= 1;
+          ok = ok && mbar_wait(bar_vfree + 8 * (vs & 1), (vs >> 1 & 1) ^ 1, abort_flag, ST_WAIT_PRODUCER);
           if (ok) {
-            mbar_arrive_expect_tx(bar_v, W);
-            for (int h = 0; h < W / kLBox; ++h) tma_load_3d(smem_u32(s_v) + h * kLBox, &tmV, bar_v, 64 * h, tile * kLTile, 0);
+            mbar_arrive_expect_tx(bar_v + 8 * (vs & 1), W);
+            for (int h = 0; h < W / kLBox; ++h) tma_load_3d(smem_u32(s_v + (vs & 1) * W) + h * kLBox, &tmV, bar_v + 8 * (vs & 1), 64 * h, tile * kLTile, 0);
           }
         }
         for (int ct = ct0; ct < ct1 && ok; ++ct) {
@@ -527,10 +572,9 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
       if (elect_one()) {
         constexpr uint32_t idesc = umma_idesc_bf16(128, 0, WMN);
         if (n > 0) {
-          ok = ok && mbar_wait(bar_v, vph, abort_flag, ST_WAIT_MMA_FULL);
-          vph ^= 1;
+          ok = ok && mbar_wait(bar_v + 8 * (vs & 1), vs >> 1 & 1, abort_flag, ST_WAIT_MMA_FULL);
         }
-        const uint32_t sv = smem_u32(s_v);
+        const uint32_t sv = smem_u32(s_v + (vs & 1) * W);
         for (int i = 0; i < (ct1 - ct0) * n && ok; ++i) {
           ok = mbar_wait(bar_tempty + 8 * buf, tph ^ 1, abort_flag, ST_WAIT_MMA_TMEM) &&
                mbar_wait(bar_wfull + 8 * ws, wph, abort_flag, ST_WAIT_MMA_FULL);
@@ -553,12 +597,12 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
             tph ^= 1;
           }
         }
-        if (n > 0 && ok) umma_commit(bar_vfree);
+        if (n > 0 && ok) umma_commit(bar_vfree + 8 * (vs & 1));
       }
     } else {
-      const int mine = tile_slot(p.tiles, tile, 32 * q + lane);
+      const int mine = slots[qs][32 * q + lane];
       const uint32_t taddr = tmem + (static_cast<uint32_t>(32 * q) << 16) + 64 * part;
-      for (int ct = ct0; ct < ct1; ++ct, ++now) {
+      for (int ct = ct0; ct < ct1; ++ct) {
         float acc[64];
         if (n != 1) {
 #pragma unroll
@@ -613,21 +657,24 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
         if (lane == 0) {
           if (ok && ct * 128 + 64 * part < p.N && tile * kLTile + 32 * q < p.tiles.T) tma_store_3d(&tmOut, smem_u32(box), ct * 128 + 64 * part, tile * kLTile + 32 * q, 0);
           bulk_commit_group();
-          if (p.has_base && now > first_item) {      // the result before has left its box, which takes the base of a tile to come
+          if (p.has_base && before) {      // the result before has left its box, which takes the base of columns to come
             asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-            fetch_base(now - 1 + BASES, bs == 0 ? BASES - 1 : bs - 1);
+            fetch_base(bs == 0 ? BASES - 1 : bs - 1);
           }
         }
+        before = true;
         if (++bs == BASES) {
           bs = 0;
           bph ^= 1;
         }
       }
     }
+    if (n > 0) ++vs;
     __syncwarp();
+    if (lane == 0) mbar_arrive(bar_qempty + 8 * qs);
   }
   grid_dep_launch();
-  if (warp >= 2 && lane == 0) bulk_wait_all();
+  if (epilogue && lane == 0) bulk_wait_all();
   __syncwarp();
   tc_fence_before();
   __syncthreads();
@@ -1251,7 +1298,9 @@ static int lora_expand(const void* V, const void* W, bool wmn, int64_t L, int64_
     if (rc == 0 && base != nullptr) rc = make_map(&tmB, base, N, T, 1, ldb, ldb * T, 64, 32);
     if (rc) return rc;
     p.has_base = base != nullptr;
-    const int grid = static_cast<int>(std::min<int64_t>(num_sms(), p.tiles.tiles * ceil_div(N, 128)));
+    p.chunk = p.tiles.tiles * ceil_div(N, 128) <= num_sms() ? 1 : 2;
+    p.items = static_cast<int>(p.tiles.tiles * ceil_div(ceil_div(N, 128), p.chunk));
+    const int grid = static_cast<int>(std::min<int64_t>(num_sms(), p.items));
     auto run = [&](auto mn) -> int {
       constexpr bool MN = decltype(mn)::value;
       static PerDevice allowed;
@@ -1348,6 +1397,7 @@ struct LoraKept {
   LoraTiles tiles;
   int* rows;
   unsigned char* present;
+  int* counter;
 };
 // index: the call has one
 static LoraKept carve_lora(int64_t T, int64_t R, int64_t L, bool index, int keep, void* ws, size_t* bytes) {
@@ -1355,6 +1405,7 @@ static LoraKept carve_lora(int64_t T, int64_t R, int64_t L, bool index, int keep
   LoraKept k{};
   const int64_t tiles = ceil_div(T, kLTile);
   k.v = c.take<__nv_bfloat16>(T * padded_rank(R));
+  k.counter = c.take<int>(1);
   k.tiles.T = static_cast<int>(T);
   k.tiles.tiles = static_cast<int>(tiles);
   if (index) {
@@ -1371,7 +1422,7 @@ static LoraKept carve_lora(int64_t T, int64_t R, int64_t L, bool index, int keep
 }
 // Whether the kernel of few rows takes a call.  us, few rows / row tiles, L2 warm.  One adapter, 4096 x 14336, rank 16: 16 rows 8.4 / 10.0, 128 rows 9.8 /
 // 10.5, 256 rows 14.4 / 11.8; 2048 x 2816, rank 64: 16 rows 9.3 / 9.5, 64 rows 11.4 / 9.4.  Several, 4096 x 4096, rank 16, rows of 32 adapters mixed:
-// 64 rows 9.6 / 35, 512 rows 16 / 43.
+// 64 rows 8.6 / 23, 512 rows 16 / 29.
 static bool lora_few(int64_t T, int64_t R, int64_t L, int keep) { return !keep && T <= (L > 1 ? kFewMost : R <= 32 ? 128 : 16); }
 
 }  // namespace b200moe
@@ -1385,7 +1436,8 @@ static int check_lora(const char* who, int64_t T, int64_t K, int64_t N, int64_t 
   B200_CHECK_ARG(T >= 0 && T < (1LL << 31) - 256 && K < (1LL << 31) - 256 && N < (1LL << 31) - 256, B200MOE_E_BAD_SHAPE,
                  "%s: %lld rows, %lld -> %lld", who, (long long)T, (long long)K, (long long)N);
   B200_CHECK_ARG(L >= 1 && L <= 65536, B200MOE_E_BAD_SHAPE, "%s: %lld adapters, supported 1..65536", who, (long long)L);
-  B200_CHECK_ARG(ceil_div(T, 128) * 8 < (1LL << 31) && ceil_div(std::max(K, N), 128) * L * 512 < (1LL << 31), B200MOE_E_BAD_SHAPE,
+  B200_CHECK_ARG(ceil_div(T, 128) * 8 < (1LL << 31) && ceil_div(std::max(K, N), 128) * L * 512 < (1LL << 31) &&
+                     ceil_div(T, 128) * ceil_div(std::max(K, N), 128) < (1LL << 31) - 65536, B200MOE_E_BAD_SHAPE,
                  "%s: %lld adapters of %lld -> %lld are too many", who, (long long)L, (long long)K, (long long)N);
   return 0;
 }
@@ -1440,17 +1492,18 @@ int b200moe_lora_forward(const void* x, int64_t ldx, const void* a, const void* 
   }
   {
     OpScope scope("lora_shrink", 1);
-    const int rc2 = lora_shrink(x, ldx, a, false, L, ShrinkParams{k.tiles, static_cast<int>(K), static_cast<int>(R), 0, 0, 0, scales, scale, k.v, status}, st);
+    const int rc2 = lora_shrink(x, ldx, a, false, L, ShrinkParams{k.tiles, static_cast<int>(K), static_cast<int>(R), 0, 0, 0, scales, scale, k.v, k.counter, status}, st);
     if (rc2) return rc2;
   }
   OpScope scope("lora_expand", 1);
-  return lora_expand(k.v, b, false, L, R, base, ldb, out, ExpandParams{k.tiles, static_cast<int>(N), 0, status}, st);
+  return lora_expand(k.v, b, false, L, R, base, ldb, out, ExpandParams{k.tiles, static_cast<int>(N), 0, 0, 0, k.counter, status}, st);
 }
 
 size_t b200moe_lora_bwd_ws_bytes(int64_t T, int64_t K, int64_t N, int64_t R, int64_t L) {
   if (T <= 0 || K <= 0 || N <= 0 || R <= 0 || L <= 0) return 0;
   LoraCarver c{nullptr};
   c.take<__nv_bfloat16>(T * padded_rank(R));
+  c.take<int>(1);
   const int sa = wgrad_splits(T, K, L), sb = back_wgrad_splits(T, N, L);
   c.take<float>(std::max(sa > 1 ? sa * L * R * K : 0, sb > 1 ? sb * L * R * N : 0));
   return c.off;
@@ -1472,6 +1525,7 @@ int b200moe_lora_backward(const void* grad_out, const void* x, int64_t ldx, cons
   const LoraKept k = carve_lora(T, R, L, has_index != 0, 1, const_cast<void*>(fwd_ws), &bytes);
   LoraCarver c{static_cast<char*>(ws)};
   __nv_bfloat16* u = c.take<__nv_bfloat16>(T * padded_rank(R));
+  int* counter = c.take<int>(1);
   float* part = c.take<float>(0);
   WgradParams w{static_cast<int>(T), 0, static_cast<int>(R), static_cast<int>(L), 1, 0, k.rows, k.present,
                 nullptr, 0, status};
@@ -1481,7 +1535,7 @@ int b200moe_lora_backward(const void* grad_out, const void* x, int64_t ldx, cons
     const int rc__ = (call);          \
     if (rc__) return rc__;            \
   } while (0)
-  const ShrinkParams sp{k.tiles, static_cast<int>(N), static_cast<int>(R), shrink_split(T, N, num_sms()), 0, 0, scales, scale, u, status};
+  const ShrinkParams sp{k.tiles, static_cast<int>(N), static_cast<int>(R), shrink_split(T, N, num_sms()), 0, 0, scales, scale, u, counter, status};
   const int sa = wgrad_splits(T, K, L), sb = back_wgrad_splits(T, N, L);
   if (grad_b && (grad_x || grad_a)) {
     w.D = static_cast<int>(N);
@@ -1493,7 +1547,7 @@ int b200moe_lora_backward(const void* grad_out, const void* x, int64_t ldx, cons
     RUN("lora_shrink", 1, lora_shrink(grad_out, N, b, true, L, sp, st));
   }
   if (grad_x)
-    RUN("lora_expand", 1, lora_expand(u, a, true, L, R, nullptr, 0, grad_x, ExpandParams{k.tiles, static_cast<int>(K), 0, status}, st));
+    RUN("lora_expand", 1, lora_expand(u, a, true, L, R, nullptr, 0, grad_x, ExpandParams{k.tiles, static_cast<int>(K), 0, 0, 0, counter, status}, st));
   if (grad_a) {
     w.D = static_cast<int>(K);
     w.transposed = 1;
