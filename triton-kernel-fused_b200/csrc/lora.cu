@@ -10,8 +10,8 @@
 // row takes the result of its adapter.  Rows of other adapters are never added to it, not even times zero, so an infinity or a NaN stays with
 // its own adapter or row.  Few rows (a decoding batch) run in one kernel of their own, a cluster for up to sixteen rows of an adapter.
 //
-// v and u are rounded to bf16, the operands' type, between the two products of row tiles: by at most 2^-8 of their size, as the result itself is, which
-// makes the error of a result without a base 0.0024 in the norm in place of 0.0017.  All sums are fp32.
+// v and u, which go from one product to the next, are two bf16 numbers each, the nearest and what that leaves, side by side: 16 bits, so that results are as
+// exact as those of an fp32 v.  (Rounded to one number the error of a result without a base was 0.0024 in the norm in place of 0.0017.)  All sums are fp32.
 #include <cuda.h>
 
 #include <algorithm>
@@ -160,6 +160,13 @@ __device__ __forceinline__ void lora_share(const LoraTiles& p, long long share, 
   __syncthreads();
 }
 
+// two fp32 numbers as bf16 and what that leaves of them, as bf16 too (nothing of an infinity)
+__device__ __forceinline__ void split_bf16x2(float2 f, uint32_t& hi, uint32_t& lo) {
+  hi = pack_bf16x2(f.x, f.y);
+  const float2 h = unpack_bf16x2(hi);
+  lo = pack_bf16x2(fabsf(h.x) == INFINITY ? 0.0f : f.x - h.x, fabsf(h.y) == INFINITY ? 0.0f : f.y - h.y);
+}
+
 // columns of tensor memory -> registers, 32 or 16 at a time
 template <int N>
 __device__ __forceinline__ void lora_fetch(uint32_t taddr, bool mine, float (&v)[N]) {
@@ -207,7 +214,7 @@ struct ShrinkParams {
   int stages, stage;         // of the ring, bytes of one
   const float* scales;       // (L,), or nullptr: `scale` for all
   float scale;
-  __nv_bfloat16* v;          // (T, RP)
+  __nv_bfloat16* v;          // (T, 2 RP): nearest, rests
   int* counter;              // of the expand behind it, set to zero
   int* status;
 };
@@ -337,11 +344,13 @@ __device__ __forceinline__ void shrink_rows(const CUtensorMap& tmX, const CUtens
           const float s = mine < 0 ? 0.0f : p.scales != nullptr ? p.scales[tile_adapter(p.tiles, tile, mine)] : p.scale;
 #pragma unroll
           for (int i = 0; i < RP; i += 8) {
-            uint32_t o[4];
+            uint32_t hi[4] = {0u, 0u, 0u, 0u}, lo[4] = {0u, 0u, 0u, 0u};
+            if (mine >= 0 && i < p.R) {      // R a multiple of 8
 #pragma unroll
-            for (int h = 0; h < 4; ++h)
-              o[h] = mine >= 0 && i < p.R ? pack_bf16x2(s * v[i + 2 * h], s * v[i + 2 * h + 1]) : 0u;      // R a multiple of 8
-            *reinterpret_cast<uint4*>(p.v + t * RP + i) = make_uint4(o[0], o[1], o[2], o[3]);
+              for (int h = 0; h < 4; ++h) split_bf16x2(make_float2(s * v[i + 2 * h], s * v[i + 2 * h + 1]), hi[h], lo[h]);
+            }
+            *reinterpret_cast<uint4*>(p.v + t * (2 * RP) + i) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(p.v + t * (2 * RP) + RP + i) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
           }
         }
       } else {      // every load of this CTA has been used: its stages are free
@@ -360,8 +369,13 @@ __device__ __forceinline__ void shrink_rows(const CUtensorMap& tmX, const CUtens
         if (t >= p.tiles.T || (slot < 0 ? pass > 0 : slot < first || slot >= first + n)) continue;
         const float4 v4 = cluster_sum4(smem_u32(smem) + 4 * (row * (RP + 4) + c), p.split);
         const float s = slot < 0 ? 0.0f : p.scales != nullptr ? p.scales[tile_adapter(p.tiles, tile, slot)] : p.scale;
-        *reinterpret_cast<uint2*>(p.v + t * RP + c) =
-            slot >= 0 && c < p.R ? make_uint2(pack_bf16x2(s * v4.x, s * v4.y), pack_bf16x2(s * v4.z, s * v4.w)) : make_uint2(0u, 0u);
+        uint2 hi = make_uint2(0u, 0u), lo = make_uint2(0u, 0u);
+        if (slot >= 0 && c < p.R) {
+          split_bf16x2(make_float2(s * v4.x, s * v4.y), hi.x, lo.x);
+          split_bf16x2(make_float2(s * v4.z, s * v4.w), hi.y, lo.y);
+        }
+        *reinterpret_cast<uint2*>(p.v + t * (2 * RP) + c) = hi;
+        *reinterpret_cast<uint2*>(p.v + t * (2 * RP) + RP + c) = lo;
       }
       fence_proxy_async_smem();      // before the next unit's rows land there
       __syncwarp();
@@ -405,12 +419,14 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
 // rate of a plain copy; 16384 x 2816, rank 64, 36; 16384 x 2048 without a base 22, 10 at that rate, but writing alone gets 3.85 TB/s here: 17.
 constexpr int kExpEpi = 8, kExpThreads = 96 + 32 * kExpEpi;      // warps: loads, products, epilogue, items
 constexpr int kExpOut = 128 * 128 * 2;
-template <int RP> constexpr int kExpBase = RP > 64 ? 3 : 4;
+template <int RP> constexpr int kExpBase = RP > 32 ? 3 : 4;
 template <int RP> constexpr int kExpW = (RP > 64 ? 2 : 1) * kLBox;               // one adapter's 128 columns
+template <int RP> constexpr int kExpV = (RP > 32 ? RP / 32 : 1) * kLBox;         // both halves of v
+template <int RP> constexpr int kExpVs = RP > 64 ? 1 : 2;
 template <int RP> constexpr int kExpWStages = RP > 64 ? 2 : 4;
 constexpr int kExpQueue = 4;                     // items known ahead: as many as bases are fetched ahead, of single columns each
 template <int RP> constexpr int kExpBars = kExpEpi * kExpBase<RP> + 2 * kExpWStages<RP> + 2 * kExpQueue + 12;
-template <int RP> constexpr int kExpSmem = kExpBase<RP> * kExpOut + (kExpWStages<RP> + 2) * kExpW<RP> + kExpBars<RP> * 8 + 16 + 1024;
+template <int RP> constexpr int kExpSmem = kExpBase<RP> * kExpOut + kExpWStages<RP> * kExpW<RP> + kExpVs<RP> * kExpV<RP> + kExpBars<RP> * 8 + 16 + 1024;
 
 struct ExpandParams {
   LoraTiles tiles;
@@ -426,11 +442,11 @@ template <int RP, bool WMN>
 __global__ void __launch_bounds__(kExpThreads, 1)
 lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmBase,
                    const __grid_constant__ CUtensorMap tmOut, const ExpandParams p) {
-  constexpr int WS = kExpWStages<RP>, W = kExpW<RP>, BASES = kExpBase<RP>;
+  constexpr int WS = kExpWStages<RP>, W = kExpW<RP>, BASES = kExpBase<RP>, V = kExpV<RP>, VS = kExpVs<RP>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t *s_w = smem + BASES * kExpOut, *s_v = s_w + WS * W;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_v + 2 * W);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_v + VS * V);
   const uint32_t bar_base = smem_u32(bars);      // [stage][epilogue warp]
   const uint32_t bar_wfull = bar_base + 8 * kExpEpi * BASES, bar_wempty = bar_wfull + 8 * WS;
   const uint32_t bar_tfull = bar_wempty + 8 * WS, bar_tempty = bar_tfull + 32, bar_v = bar_tempty + 32, bar_vfree = bar_v + 16;
@@ -450,7 +466,7 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
       mbar_init(bar_tfull + 8 * b, 1);
       mbar_init(bar_tempty + 8 * b, kExpEpi);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < VS; ++b) {
       mbar_init(bar_v + 8 * b, 1);
       mbar_init(bar_vfree + 8 * b, 1);
     }
@@ -541,10 +557,10 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
     if (warp == 0) {
       if (elect_one()) {
         if (n > 0) {
-          ok = ok && mbar_wait(bar_vfree + 8 * (vs & 1), (vs >> 1 & 1) ^ 1, abort_flag, ST_WAIT_PRODUCER);
+          ok = ok && mbar_wait(bar_vfree + 8 * (vs % VS), (vs / VS & 1) ^ 1, abort_flag, ST_WAIT_PRODUCER);
           if (ok) {
-            mbar_arrive_expect_tx(bar_v + 8 * (vs & 1), W);
-            for (int h = 0; h < W / kLBox; ++h) tma_load_3d(smem_u32(s_v + (vs & 1) * W) + h * kLBox, &tmV, bar_v + 8 * (vs & 1), 64 * h, tile * kLTile, 0);
+            mbar_arrive_expect_tx(bar_v + 8 * (vs % VS), V);
+            for (int h = 0; h < V / kLBox; ++h) tma_load_3d(smem_u32(s_v + vs % VS * V) + h * kLBox, &tmV, bar_v + 8 * (vs % VS), 64 * h, tile * kLTile, 0);
           }
         }
         for (int ct = ct0; ct < ct1 && ok; ++ct) {
@@ -572,20 +588,22 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
       if (elect_one()) {
         constexpr uint32_t idesc = umma_idesc_bf16(128, 0, WMN);
         if (n > 0) {
-          ok = ok && mbar_wait(bar_v + 8 * (vs & 1), vs >> 1 & 1, abort_flag, ST_WAIT_MMA_FULL);
+          ok = ok && mbar_wait(bar_v + 8 * (vs % VS), vs / VS & 1, abort_flag, ST_WAIT_MMA_FULL);
         }
-        const uint32_t sv = smem_u32(s_v + (vs & 1) * W);
-        for (int i = 0; i < (ct1 - ct0) * n && ok; ++i) {
+        const uint32_t sv = smem_u32(s_v + vs % VS * V);
+        for (int u = 0; u < (ct1 - ct0) * n && ok; ++u) {
           ok = mbar_wait(bar_tempty + 8 * buf, tph ^ 1, abort_flag, ST_WAIT_MMA_TMEM) &&
                mbar_wait(bar_wfull + 8 * ws, wph, abort_flag, ST_WAIT_MMA_FULL);
           if (!ok) break;
           tc_fence_after();
           const uint32_t sw = smem_u32(s_w + ws * W);
 #pragma unroll
-          for (int k = 0; k < RP / 16; ++k)
-            umma_bf16(tmem + 128 * buf, umma_desc_sw128(sv + (k >> 2) * kLBox + 32 * (k & 3), 0, 1024),
+          for (int i = 0; i < RP / 8; ++i) {      // the nearest, then the rests
+            const int k = i % (RP / 16);
+            umma_bf16(tmem + 128 * buf, umma_desc_sw128(sv + (i >> 2) * kLBox + 32 * (i & 3), 0, 1024),
                       WMN ? umma_desc_sw128(sw + 2048 * k, RP * 128, 1024) : umma_desc_sw128(sw + (k >> 2) * kLBox + 32 * (k & 3), 0, 1024), idesc,
-                      k != 0);
+                      i != 0);
+          }
           umma_commit(bar_wempty + 8 * ws);
           umma_commit(bar_tfull + 8 * buf);
           if (++ws == WS) {
@@ -597,7 +615,7 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
             tph ^= 1;
           }
         }
-        if (n > 0 && ok) umma_commit(bar_vfree + 8 * (vs & 1));
+        if (n > 0 && ok) umma_commit(bar_vfree + 8 * (vs % VS));
       }
     } else {
       const int mine = slots[qs][32 * q + lane];
@@ -688,8 +706,8 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
 // 16384 x 2048, rank 64: 16 us, 10.3 at the copy rate, and 3 for the shares' sum.  Shares added up in clusters of eight instead took 31: so many large CTAs
 // of one cluster do not find room at once.
 constexpr int kWgThreads = 192, kWgWords = 2048;       // blocks of one CTA as bits: 32 kWgWords of them
-template <int RP> constexpr int kWgV = (RP > 64 ? 2 : 1) * 8192;
-template <int RP> constexpr int kWgStages = RP > 64 ? 3 : 4;
+template <int RP> constexpr int kWgV = (RP > 32 ? RP / 32 : 1) * 8192;
+template <int RP> constexpr int kWgStages = RP > 64 ? 2 : RP > 32 ? 3 : 4;
 template <int RP> constexpr int kWgSmem = kWgStages<RP> * (kLBox + kWgV<RP>) + (3 * kWgStages<RP> + 1) * 8 + 16 + 1024;
 
 struct WgradParams {
@@ -703,7 +721,7 @@ struct WgradParams {
 
 template <int RP>
 __device__ __forceinline__ void wgrad_rows(const CUtensorMap& tmY, const CUtensorMap& tmV, const WgradParams& p, int part, uint8_t* smem, unsigned* live) {
-  constexpr int NB = RP < 64 ? 64 : RP, ST = kWgStages<RP>, STAGE = kLBox + kWgV<RP>;
+  constexpr int NB = RP < 32 ? 64 : 2 * RP, ST = kWgStages<RP>, STAGE = kLBox + kWgV<RP>;      // columns: of V its nearest, then its rests
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + ST * STAGE);
   const uint32_t bar_full = smem_u32(bars), bar_ready = bar_full + 8 * ST, bar_empty = bar_ready + 8 * ST, bar_tfull = bar_empty + 8 * ST;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * ST + 1);
@@ -836,8 +854,12 @@ __device__ __forceinline__ void wgrad_rows(const CUtensorMap& tmY, const CUtenso
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = 0.0f;
       if (any) lora_fetch<16>(taddr + c, true, v);
+      float rest[16];
 #pragma unroll
-      for (int i = 0; i < 16; i += 4) to[(c + i) / 4] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+      for (int i = 0; i < 16; ++i) rest[i] = 0.0f;
+      if (any) lora_fetch<16>(taddr + RP + c, true, rest);
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) to[(c + i) / 4] = make_float4(v[i] + rest[i], v[i + 1] + rest[i + 1], v[i + 2] + rest[i + 2], v[i + 3] + rest[i + 3]);
     }
   }
   __syncwarp();
@@ -1044,13 +1066,6 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// two fp32 numbers as bf16 and what that leaves of them, as bf16 too (nothing of an infinity)
-__device__ __forceinline__ void split_bf16x2(float2 f, uint32_t& hi, uint32_t& lo) {
-  hi = pack_bf16x2(f.x, f.y);
-  const float2 h = unpack_bf16x2(hi);
-  lo = pack_bf16x2(fabsf(h.x) == INFINITY ? 0.0f : f.x - h.x, fabsf(h.y) == INFINITY ? 0.0f : f.y - h.y);
-}
-
 struct FewLora {
   LoraIndex ix;
   const __nv_bfloat16 *x, *a, *b, *base;
@@ -1291,7 +1306,7 @@ static int lora_expand(const void* V, const void* W, bool wmn, int64_t L, int64_
     constexpr int RP = decltype(rp)::value;
     CUtensorMap tmV, tmW, tmB, tmO;
     const int64_t T = p.tiles.T, N = p.N;
-    int rc = make_map(&tmV, V, RP, T, 1, RP, T * RP, 64, kLTile);
+    int rc = make_map(&tmV, V, 2 * RP, T, 1, 2 * RP, T * (2 * RP), 64, kLTile);
     if (rc == 0) rc = wmn ? make_map(&tmW, W, N, R, L, N, N * R, 64, RP) : make_map(&tmW, W, R, N, L, R, N * R, 64, 128);
     if (rc == 0) rc = make_map(&tmO, out, N, T, 1, N, N * T, 64, 32);
     tmB = tmO;
@@ -1333,7 +1348,7 @@ static int lora_wgrad(const void* Y, int64_t ldy, const void* V, int splits, Wgr
     constexpr int RP = decltype(rp)::value;
     CUtensorMap tmY, tmV;
     int rc = make_map(&tmY, Y, p.D, p.T, 1, ldy, ldy * p.T, 64, 64);
-    if (rc == 0) rc = make_map(&tmV, V, RP, p.T, 1, RP, static_cast<int64_t>(p.T) * RP, 64, 64);
+    if (rc == 0) rc = make_map(&tmV, V, 2 * RP, p.T, 1, 2 * RP, static_cast<int64_t>(p.T) * (2 * RP), 64, 64);
     if (rc) return rc;
     p.splits = splits;
     p.out = p.splits > 1 ? static_cast<void*>(ws) : out;
@@ -1358,7 +1373,7 @@ static int lora_back(const void* G, const void* B, const void* V, int64_t L, Shr
     int rc = make_map(&tmX, G, D, T, 1, D, D * T, 64, kLTile);
     if (rc == 0) rc = make_map(&tmW, B, p.R, D, L, p.R, static_cast<int64_t>(p.R) * D, 64, 64);
     if (rc == 0) rc = make_map(&tmY, G, D, T, 1, D, D * T, 64, 64);
-    if (rc == 0) rc = make_map(&tmV, V, RP, T, 1, RP, T * RP, 64, 64);
+    if (rc == 0) rc = make_map(&tmV, V, 2 * RP, T, 1, 2 * RP, T * (2 * RP), 64, 64);
     if (rc) return rc;
     const int columns = RP < 64 ? 64 : RP;
     const int64_t slots = std::min<int64_t>(128 / columns, L), units = tiles * ceil_div(std::min<int64_t>(L, kLTile), slots);
@@ -1404,7 +1419,7 @@ static LoraKept carve_lora(int64_t T, int64_t R, int64_t L, bool index, int keep
   LoraCarver c{static_cast<char*>(ws)};
   LoraKept k{};
   const int64_t tiles = ceil_div(T, kLTile);
-  k.v = c.take<__nv_bfloat16>(T * padded_rank(R));
+  k.v = c.take<__nv_bfloat16>(2 * T * padded_rank(R));
   k.counter = c.take<int>(1);
   k.tiles.T = static_cast<int>(T);
   k.tiles.tiles = static_cast<int>(tiles);
@@ -1502,7 +1517,7 @@ int b200moe_lora_forward(const void* x, int64_t ldx, const void* a, const void* 
 size_t b200moe_lora_bwd_ws_bytes(int64_t T, int64_t K, int64_t N, int64_t R, int64_t L) {
   if (T <= 0 || K <= 0 || N <= 0 || R <= 0 || L <= 0) return 0;
   LoraCarver c{nullptr};
-  c.take<__nv_bfloat16>(T * padded_rank(R));
+  c.take<__nv_bfloat16>(2 * T * padded_rank(R));
   c.take<int>(1);
   const int sa = wgrad_splits(T, K, L), sb = back_wgrad_splits(T, N, L);
   c.take<float>(std::max(sa > 1 ? sa * L * R * K : 0, sb > 1 ? sb * L * R * N : 0));
@@ -1524,7 +1539,7 @@ int b200moe_lora_backward(const void* grad_out, const void* x, int64_t ldx, cons
   size_t bytes;
   const LoraKept k = carve_lora(T, R, L, has_index != 0, 1, const_cast<void*>(fwd_ws), &bytes);
   LoraCarver c{static_cast<char*>(ws)};
-  __nv_bfloat16* u = c.take<__nv_bfloat16>(T * padded_rank(R));
+  __nv_bfloat16* u = c.take<__nv_bfloat16>(2 * T * padded_rank(R));
   int* counter = c.take<int>(1);
   float* part = c.take<float>(0);
   WgradParams w{static_cast<int>(T), 0, static_cast<int>(R), static_cast<int>(L), 1, 0, k.rows, k.present,
