@@ -1,7 +1,8 @@
 """GPU: low-rank adapters of many requests, against 64 bits.
 
 Bounds.  The tensor cores add in fp32 and may cut off instead of rounding: a sum of n products is off by n 2^-23 of the products' sizes.  x A^T
-(and g B) is rounded to bf16, 2^-8 of its size at most, unless few rows run without a backward; the result is off by half a step of its type more.
+(and g B) goes on as two bf16 numbers; most tests here allow for one, 2^-8 of its size, and `test_what_goes_on_holds_sixteen_bits` does not.  The result
+is off by half a step of its type more.
 What is off in the first product goes through the second: `spread` is its sizes times the sizes of the second factor."""
 import importlib
 
@@ -105,6 +106,24 @@ def test_forward(pkg, T, K, N, R, n, how, base):
 def test_few_rows_are_not_rounded_in_the_middle(pkg):
     x, a, b, s, bs, index = make(100, 1024, 512, 32, 6, base=False)
     close(pkg.lora_linear(x, a, b, index, s), reference(x, a, b, s, None, index)["y"], 1024, rounded=False)
+
+
+@pytest.mark.parametrize("R", [8, 16, 32, 48, 64, 128])
+@pytest.mark.parametrize("how,n", [("one", 1), ("mixed", 3)])
+@pytest.mark.parametrize("T", [20, 300])
+def test_what_goes_on_holds_sixteen_bits(pkg, T, R, how, n):
+    """x A^T and g B are two bf16 numbers, the second off by 2^-8 of at most 2^-8 of the value, on row tiles and with a gradient too.  Short sums, so that
+    their bounds are far below what one rounded number would be off."""
+    x, a, b, s, _, index = make(T, 16, 24, R, n, how, seed=11, base=False, dtype=F32)
+    go = torch.randn(T, 24, generator=gen(12), device=DEV).to(BF)
+    leaves = [t.requires_grad_() for t in (x, a, b)]
+    y = pkg.lora_linear(x, a, b, index, s)
+    got = {"y": y.detach(), **dict(zip(("gx", "ga", "gb"), torch.autograd.grad(y, leaves, go)))}
+    ref = reference(x.detach(), a.detach(), b.detach(), s, None, index, go)
+    for name, terms in (("y", R), ("gx", R), ("ga", T), ("gb", T)):
+        value, middle, sums = ref[name]
+        close(got[name], (value, middle * 2.0 ** -8, sums), terms)
+    pkg.check_status()
 
 
 @pytest.mark.parametrize("T,K,N,R,n,how", SHAPES)

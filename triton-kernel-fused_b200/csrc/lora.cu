@@ -416,7 +416,8 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
 // out at its start (16384 x 2816, rank 64: 36 and 39).  The base's boxes land where the result leaves from: an epilogue warp fetches its own, a few columns
 // ahead whatever the adapters' products wait for; tensor memory holds four (columns, adapter) products.
 // us: 8192 x 14336, rank 32, nine stretches of rows with an adapter each or none 82 (92 in equal shares by weight, 90 in items of 128 columns), 72 at the
-// rate of a plain copy; 16384 x 2816, rank 64, 36; 16384 x 2048 without a base 22, 10 at that rate, but writing alone gets 3.85 TB/s here: 17.
+// rate of a plain copy; 16384 x 2816, rank 64, 37 (36 with v rounded to one number, which leaves room for one base more); 16384 x 2048 without a base 23, 10
+// at that rate, but writing alone gets 3.85 TB/s here: 17.
 constexpr int kExpEpi = 8, kExpThreads = 96 + 32 * kExpEpi;      // warps: loads, products, epilogue, items
 constexpr int kExpOut = 128 * 128 * 2;
 template <int RP> constexpr int kExpBase = RP > 32 ? 3 : 4;
@@ -703,7 +704,8 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
 // ------------------------------------------------------------------------------------------------ gradients of the factors
 // P_l[d, r] = sum over the rows t of adapter l of Y[t, d] V[t, r].  A CTA: one adapter, 128 columns d, a share of the rows in blocks of 64, of
 // which it visits those that have the adapter.  Rows of others in such a block are set to zero in shared memory, in both operands.
-// 16384 x 2048, rank 64: 16 us, 10.3 at the copy rate, and 3 for the shares' sum.  Shares added up in clusters of eight instead took 31: so many large CTAs
+// 16384 x 2048, rank 64: 17 us, 10.3 at the copy rate, and 3 for the shares' sum.  V's rests are columns of their own, so its 16 KB a block are read for each 128
+// columns (16 us with the nearest numbers alone; 256 columns a CTA would need twice the shares and their sums).  Shares added up in clusters of eight instead took 31: so many large CTAs
 // of one cluster do not find room at once.
 constexpr int kWgThreads = 192, kWgWords = 2048;       // blocks of one CTA as bits: 32 kWgWords of them
 template <int RP> constexpr int kWgV = (RP > 32 ? RP / 32 : 1) * 8192;
@@ -899,8 +901,8 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap tmY, const __grid_constant
 }
 
 // Both products of the gradient g in one launch, shrink (u = g B) and wgrad (of B): by turns a cluster of the one and of the other, so that an SM has a
-// CTA of each, one waits for memory while the other computes, and what one has read the other finds in L2.  16384 x 2816, rank 64: 27 us, one after the
-// other 21 and 19.
+// CTA of each, one waits for memory while the other computes, and what one has read the other finds in L2.  16384 x 2816, rank 64: 31 us, one after the
+// other 21 and 20.
 constexpr int kBackThreads = kShrinkThreads;
 static_assert(kShrinkThreads == kWgThreads, "roles of one launch");
 template <int RP> constexpr int kBackSmem = kShrinkSmem > kWgSmem<RP> ? kShrinkSmem : kWgSmem<RP>;

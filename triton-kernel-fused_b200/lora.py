@@ -81,9 +81,9 @@ def lora_linear(x, lora_a, lora_b, index=None, scaling=1.0, base=None):
 
     index: int32 or int64 of x's leading shape; a negative one is a row without an adapter, whose out is its base (one of L or more too, and it
     raises the status word).  None: one adapter (L = 1) for every row.  scaling: a number, or fp32 (L,).  K and N multiples of 8, the rank R of 8 up to
-    128 (smaller ones of a stack are padded with zeros).  Adapters are bf16, or fp32 that is rounded to it and gets fp32 gradients.  x A^T is rounded
-    to bf16 where a gradient is wanted or the rows are more than a few; sums are fp32 and the result is rounded once.  Rows and adapters
-    do not mix: NaN in one stays there.  Differentiable in x, lora_a, lora_b and base; scaling takes no gradient."""
+    128 (smaller ones of a stack are padded with zeros).  Adapters are bf16, or fp32 that is rounded to it and gets fp32 gradients.  Sums are fp32,
+    x A^T goes on in 16 bits or more (two bf16 numbers) and the result is rounded once.  Rows and adapters do not mix: NaN or an infinity in one stays
+    there (an infinity in lora_b may come out as NaN).  Differentiable in x, lora_a, lora_b and base; scaling takes no gradient."""
     fast = L.fast() if x.is_cuda else None
     if fast is not None:
         wide = isinstance(scaling, torch.Tensor)
