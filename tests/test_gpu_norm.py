@@ -369,3 +369,11 @@ def test_refusals(pkg):
                         ("take no gradient", lambda: pkg.fp8_block_linear(x, wq, ws, (q, s.clone().requires_grad_())))):
         with pytest.raises(ValueError, match=match):
             call()
+
+
+def test_an_infinite_eps_is_refused(pkg):
+    x, _, w = make(4, 128, BF)
+    for eps in (float("inf"), 1e39, float("nan")):
+        for call in (lambda: pkg.rms_norm(x, w, eps=eps), lambda: pkg.rms_norm(x[:, ::2], w[::2], eps=eps), lambda: pkg.rms_norm_fp8_block(x, w, eps=eps)):
+            with pytest.raises(ValueError, match="eps"):
+                call()

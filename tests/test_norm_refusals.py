@@ -43,3 +43,10 @@ def test_python_callables():
                  lambda: pkg.fp8_block_linear(x, q[:64], s, quantized=(q, s))):
         with pytest.raises(ValueError, match="CUDA"):
             call()
+
+
+def test_an_infinite_eps():
+    lib = load_pkg().lib()
+    for eps in (float("inf"), 1e39):      # the second is one in fp32
+        assert lib.b200moe_rms_norm_fwd(P, 64, None, 64, 0, P, 0, 4, 64, eps, P, None, None, None, 0, P, None) == -1
+        assert lib.b200moe_rms_norm_bwd(P, None, P, 64, 0, P, 0, 4, 64, eps, P, P, P, P, None) == -1

@@ -12,6 +12,7 @@
 // Of the operators below, host time of a call of 512 tokens, forward and backward: top-k 118 / 75, losses 141 / 84, an 8-bit product 154 / 89.
 //
 // Nothing is kept between calls but what autograd saves (saved-tensor hooks see it); the workspace of a forward is a saved tensor.
+#include <limits>
 #include <ATen/autocast_mode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -612,7 +613,7 @@ optional<std::tuple<optional<Tensor>, optional<Tensor>, optional<Tensor>, option
   if (!plain(x, x.scalar_type(), dev) || !plain(w, w.scalar_type(), dev) || !plain_or_none(residual, x.scalar_type(), dev)) return std::nullopt;
   if (x.dim() < 1 || x.numel() == 0 || w.dim() != 1 || w.size(0) != x.size(-1) || (residual.has_value() && residual->sizes() != x.sizes())) return std::nullopt;
   const int64_t K = x.size(-1), N = x.numel() / K;
-  if (K > 16384 || (want_codes && K % 8 != 0) || !(eps >= 0.0) || N >= (1LL << 31) - 256) return std::nullopt;
+  if (K > 16384 || (want_codes && K % 8 != 0) || !(eps >= 0.0 && eps <= std::numeric_limits<float>::max()) || N >= (1LL << 31) - 256) return std::nullopt;
   const c10::cuda::CUDAGuard guard(dev);
   NormArgs a{residual, status, Tensor(), Tensor(), *type, *w_type, eps, want_y};
   if (want_codes) {

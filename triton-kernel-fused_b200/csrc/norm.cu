@@ -10,6 +10,7 @@
 // Bound by HBM: a row is read once.  Three forms: rows through shared memory, which a ring of bulk copies keeps full (rms_norm_*_rows); few rows, where
 // latency counts, and rows off a vector's boundary through registers (rms_norm_*).
 #include <algorithm>
+#include <limits>
 
 #include "fp8_block.cuh"
 #include "logits.cuh"
@@ -775,7 +776,7 @@ static int check_norm(const char* who, int type, int w_type, int64_t rows, int64
                  w_type);
   B200_CHECK_ARG(rows >= 0 && rows < (1LL << 31) - 256, B200MOE_E_BAD_SHAPE, "%s: %lld rows", who, (long long)rows);
   B200_CHECK_ARG(K >= 1 && K <= kNormMaxK, B200MOE_E_BAD_SHAPE, "%s: rows of %lld values, supported 1..%d", who, (long long)K, kNormMaxK);
-  B200_CHECK_ARG(eps >= 0.0f, B200MOE_E_BAD_SHAPE, "%s: eps = %g must not be negative", who, (double)eps);
+  B200_CHECK_ARG(eps >= 0.0f && eps <= std::numeric_limits<float>::max(), B200MOE_E_BAD_SHAPE, "%s: eps = %g must be finite and not negative", who, (double)eps);
   return 0;
 }
 

@@ -83,7 +83,7 @@ def _check(x, weight, residual, eps, codes):
         L.require(residual.device == x.device and residual.dtype == x.dtype and residual.shape == x.shape,
                   f"residual must be {x.dtype} {tuple(x.shape)} on x's device, got {residual.dtype} {tuple(residual.shape)}")
     eps = float(eps)
-    L.require(0.0 <= eps < float("inf"), f"eps = {eps} must not be negative")
+    L.require(0.0 <= eps <= torch.finfo(torch.float32).max, f"eps = {eps} must be finite in fp32 and not negative")
     return eps
 
 
