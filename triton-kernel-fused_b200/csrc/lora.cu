@@ -818,16 +818,33 @@ __device__ __forceinline__ void wgrad_rows(const CUtensorMap& tmY, const CUtenso
     int s = 0;
     uint32_t ph = 0;
     bool ok = true;
-    each([&](int b) {
-      unsigned bad0 = 0, bad1 = 0;
-      if (p.rows != nullptr) {      // rows past the last one are zero already
-        const int t = 64 * b + lane;
-        bad0 = __ballot_sync(0xffffffffu, t < p.T && p.rows[min(t, p.T - 1)] != l);
-        bad1 = __ballot_sync(0xffffffffu, t + 32 < p.T && p.rows[min(t + 32, p.T - 1)] != l);
+    // the adapters of a block's rows, fetched a block ahead; rows past the last one are zero already, whoever's they are
+    int r0 = l, r1 = l;
+    auto adapters = [&](int b) {
+      if (p.rows == nullptr || b < 0) return;
+      const int t = 64 * b + lane;
+      r0 = t < p.T ? p.rows[t] : l;
+      r1 = t + 32 < p.T ? p.rows[t + 32] : l;
+    };
+    int w = 0;
+    unsigned m = words > 0 ? live[0] : 0;
+    auto next = [&]() {              // the block after those it gave before, -1: none
+      while (m == 0) {
+        if (++w >= words) return -1;
+        m = live[w];
       }
-      ok = ok && mbar_wait(bar_full + 8 * s, ph, abort_flag, ST_WAIT_MMA_FULL);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) return false;
+      const int b = b0 + 32 * w + __ffs(m) - 1;
+      m &= m - 1;
+      return b;
+    };
+    int ahead = next();
+    adapters(ahead);
+    while (ahead >= 0 && ok) {
+      const unsigned bad0 = __ballot_sync(0xffffffffu, r0 != l), bad1 = __ballot_sync(0xffffffffu, r1 != l);
+      ahead = next();
+      adapters(ahead);
+      ok = __all_sync(0xffffffffu, mbar_wait(bar_full + 8 * s, ph, abort_flag, ST_WAIT_MMA_FULL));
+      if (!ok) break;
       if ((bad0 | bad1) != 0) {
         uint8_t* sy = smem + s * STAGE;
         for (int r = q; r < 64; r += 4)
@@ -842,8 +859,7 @@ __device__ __forceinline__ void wgrad_rows(const CUtensorMap& tmY, const CUtenso
         s = 0;
         ph ^= 1;
       }
-      return true;
-    });
+    }
     if (any) ok = ok && mbar_wait(bar_tfull, 0, abort_flag, ST_WAIT_EPILOGUE);
     __syncwarp();
     tc_fence_after();
