@@ -57,54 +57,108 @@ __device__ __forceinline__ int tile_slot(const LoraTiles& p, int tile, int row) 
   return p.n == nullptr ? (t < p.T ? 0 : -1) : p.slot[t];
 }
 
-// rows (T), nullable: the rows' adapters, -1: none; present (tiles, L), nullable: bit h where rows of the tile's half h have the adapter
-__global__ void __launch_bounds__(kLTile) lora_tiles_kernel(const LoraIndex ix, const LoraTiles p, int* rows, unsigned char* present) {
+// The same for the lists, which the tiles' CTAs report for: no store between the loads, so that several are on their way
+__device__ __forceinline__ int named_adapter(const LoraIndex& p, long long t) {
+  const long long l = p.bytes == 8 ? static_cast<const long long*>(p.index)[t] : static_cast<const int*>(p.index)[t];
+  return l < 0 || l >= p.L ? -1 : static_cast<int>(l);
+}
+// The rows of each adapter, in their order, one adapter after another: those of l are order[bounds[l]] ... order[bounds[l + 1] - 1].
+struct LoraLists {
+  int* order;                // (T), nullptr: not asked for
+  int* bounds;               // (L + 1)
+};
+constexpr int kTilesThreads = 512, kTilesEach = kTilesThreads / kLTile;
+
+// one CTA: the list of adapter l.  Each warp counts in a stretch of the rows of its own, and then writes behind those before it.
+__device__ __forceinline__ void lora_list(const LoraIndex& ix, const LoraLists& p, int l) {
+  constexpr int WARPS = kTilesThreads / 32, U = 8;
+  __shared__ int found[2][WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long each = (static_cast<long long>(ix.T) + 32 * WARPS - 1) / (32 * WARPS) * 32, r0 = warp * each, r1 = min(static_cast<long long>(ix.T), r0 + each);
+  int here = 0, below = 0;
+  for (long long r = r0 + lane; r - lane < r1; r += 32 * U) {
+    int of[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) of[u] = r + 32 * u < r1 ? named_adapter(ix, r + 32 * u) : -1;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      here += of[u] == l;
+      below += of[u] >= 0 && of[u] < l;
+    }
+  }
+  here = __reduce_add_sync(0xffffffffu, here);
+  below = __reduce_add_sync(0xffffffffu, below);
+  if (lane == 0) {
+    found[0][warp] = here;
+    found[1][warp] = below;
+  }
+  __syncthreads();
+  int first = 0, at = 0, all = 0;
+  for (int w = 0; w < WARPS; ++w) {
+    first += found[1][w];
+    if (w < warp) at += found[0][w];
+    all += found[0][w];
+  }
+  at += first;
+  if (threadIdx.x == 0) {
+    p.bounds[l] = first;
+    if (l == ix.L - 1) p.bounds[l + 1] = first + all;
+  }
+  for (long long r = r0 + lane; here > 0 && r - lane < r1; r += 32 * U) {
+    int of[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) of[u] = r + 32 * u < r1 ? named_adapter(ix, r + 32 * u) : -1;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const unsigned m = __ballot_sync(0xffffffffu, of[u] == l);
+      if (of[u] == l) p.order[at + __popc(m & ((1u << lane) - 1u))] = static_cast<int>(r + 32 * u);
+      at += __popc(m);
+    }
+  }
+}
+
+// The first CTAs make a list each, where lists are asked for; the others take kTilesEach tiles each, 128 threads a tile.
+__global__ void __launch_bounds__(kTilesThreads) lora_tiles_kernel(const LoraIndex ix, const LoraTiles p, const LoraLists lists) {
   grid_dep_wait();
-  __shared__ __align__(16) int of_row[kLTile];
-  __shared__ int slot[kLTile], warps[kLTile / 32];
-  const int t = threadIdx.x, tile = blockIdx.x;
-  const long long row = static_cast<long long>(tile) * kLTile + t;
-  const int l = lora_adapter(ix, row);
-  of_row[t] = l;
-  __syncthreads();
-  // the first row of this thread's adapter: in this warp, or in one before
-  const unsigned same = __match_any_sync(0xffffffffu, l);
-  int at = (t & ~31) + __ffs(same) - 1;
-  for (int j = 0; j < (t >> 5) * 8; ++j) {
-    const int4 o = reinterpret_cast<const int4*>(of_row)[j];
-    const int i = o.x == l ? 0 : o.y == l ? 1 : o.z == l ? 2 : o.w == l ? 3 : 4;
-    if (i < 4) {
-      at = 4 * j + i;
-      break;
-    }
-  }
-  __syncwarp();
-  const bool first = l >= 0 && at == t;
-  const unsigned firsts = __ballot_sync(0xffffffffu, first);
-  if ((t & 31) == 0) warps[t >> 5] = __popc(firsts);
-  __syncthreads();
-  int n = __popc(firsts & ((1u << (t & 31)) - 1u));
-  for (int w = 0; w < (t >> 5); ++w) n += warps[w];
-  if (first) {
-    slot[t] = n;
-    p.adapter[static_cast<long long>(tile) * kLTile + n] = l;
-  }
-  if (t == 0) p.n[tile] = warps[0] + warps[1] + warps[2] + warps[3];
-  __syncthreads();
-  p.slot[row] = static_cast<short>(l >= 0 ? slot[at] : -1);
-  if (rows != nullptr && row < ix.T) rows[row] = l;
-  if (present != nullptr) {
-    unsigned char* to = present + static_cast<long long>(tile) * ix.L;
-    for (int i = t; i < ix.L; i += kLTile) to[i] = 0;
-    __syncthreads();
-    if (first) {
-      bool low = false, high = false;
-      for (int j = 0; j < kLTile / 2; ++j) {
-        low = low || of_row[j] == l;
-        high = high || of_row[j + kLTile / 2] == l;
+  __shared__ __align__(16) int all_rows[kTilesEach][kLTile];
+  __shared__ int slots[kTilesEach][kLTile], all_warps[kTilesEach][kLTile / 32];
+  const int n_lists = lists.order != nullptr ? ix.L : 0;
+  const int g = threadIdx.x / kLTile, t = threadIdx.x % kLTile;
+  const int tile = (static_cast<int>(blockIdx.x) - n_lists) * kTilesEach + g;
+  if (static_cast<int>(blockIdx.x) < n_lists) {
+    lora_list(ix, lists, blockIdx.x);
+  } else if (tile < p.tiles) {
+    auto sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(g + 1), "n"(kLTile) : "memory"); };
+    int *of_row = all_rows[g], *slot = slots[g], *warps = all_warps[g];
+    const long long row = static_cast<long long>(tile) * kLTile + t;
+    const int l = lora_adapter(ix, row);
+    of_row[t] = l;
+    sync();
+    // the first row of this thread's adapter: in this warp, or in one before
+    const unsigned same = __match_any_sync(0xffffffffu, l);
+    int at = (t & ~31) + __ffs(same) - 1;
+    for (int j = 0; j < (t >> 5) * 8; ++j) {
+      const int4 o = reinterpret_cast<const int4*>(of_row)[j];
+      const int i = o.x == l ? 0 : o.y == l ? 1 : o.z == l ? 2 : o.w == l ? 3 : 4;
+      if (i < 4) {
+        at = 4 * j + i;
+        break;
       }
-      to[l] = static_cast<unsigned char>((low ? 1 : 0) | (high ? 2 : 0));
     }
+    __syncwarp();
+    const bool first = l >= 0 && at == t;
+    const unsigned firsts = __ballot_sync(0xffffffffu, first);
+    if ((t & 31) == 0) warps[t >> 5] = __popc(firsts);
+    sync();
+    int n = __popc(firsts & ((1u << (t & 31)) - 1u));
+    for (int w = 0; w < (t >> 5); ++w) n += warps[w];
+    if (first) {
+      slot[t] = n;
+      p.adapter[static_cast<long long>(tile) * kLTile + n] = l;
+    }
+    if (t == 0) p.n[tile] = warps[0] + warps[1] + warps[2] + warps[3];
+    sync();
+    p.slot[row] = static_cast<short>(l >= 0 ? slot[at] : -1);
   }
   grid_dep_launch();
 }
@@ -702,41 +756,46 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
 }
 
 // ------------------------------------------------------------------------------------------------ gradients of the factors
-// P_l[d, r] = sum over the rows t of adapter l of Y[t, d] V[t, r].  A CTA: one adapter, 128 columns d, a share of the rows in blocks of 64, of
-// which it visits those that have the adapter.  Rows of others in such a block are set to zero in shared memory, in both operands.
+// P_l[d, r] = sum over the rows t of adapter l of Y[t, d] V[t, r].  A CTA: one adapter, 128 columns d, a share of the adapter's rows in blocks of 64.  A block of
+// neighbouring rows is two boxes of Y and those of V; of others four warps copy the 64 rows of the adapter's list into the same places, 16 bytes a lane.
 // 16384 x 2048, rank 64: 17 us, 10.3 at the copy rate, and 3 for the shares' sum.  V's rests are columns of their own, so its 16 KB a block are read for each 128
-// columns (16 us with the nearest numbers alone; 256 columns a CTA would need twice the shares and their sums).  Shares added up in clusters of eight instead took 31: so many large CTAs
-// of one cluster do not find room at once.
-constexpr int kWgThreads = 192, kWgWords = 2048;       // blocks of one CTA as bits: 32 kWgWords of them
+// columns (16 us with the nearest numbers alone; 256 columns a CTA would need twice the shares and their sums).  Shares added up in clusters of eight
+// instead took 31: so many large CTAs of one cluster do not find room at once.  8192 x 2048, rank 16, rows of 32 adapters mixed: 18 (267 where each adapter's CTAs visited every
+// block that has a row of it and set the others' rows to zero); 3001 rows of three adapters one after another 7.6 (11), by 16 bytes alone 14.
+constexpr int kWgThreads = 192;
 template <int RP> constexpr int kWgV = (RP > 32 ? RP / 32 : 1) * 8192;
 template <int RP> constexpr int kWgStages = RP > 64 ? 2 : RP > 32 ? 3 : 4;
-template <int RP> constexpr int kWgSmem = kWgStages<RP> * (kLBox + kWgV<RP>) + (3 * kWgStages<RP> + 1) * 8 + 16 + 1024;
+template <int RP> constexpr int kWgSmem = kWgStages<RP> * (kLBox + kWgV<RP>) + (2 * kWgStages<RP> + 1) * 8 + 16 + 1024;
 
 struct WgradParams {
   int T, D, R, L, splits, transposed;      // transposed: P is (R, D), else (D, R)
-  const int* rows;                         // nullptr: all of them are adapter 0's
-  const unsigned char* present;
+  LoraLists lists;                         // order: nullptr: all rows are adapter 0's
+  const __nv_bfloat16 *y, *v;              // (T, D) at ldy, (T, 2 RP)
+  long long ldy;
   void* out;                               // (splits, L, ...) fp32; one split: the gradient itself
   int out_f32;
   int* status;
 };
+// 16 bytes of global memory, or zeros, into shared memory
+__device__ __forceinline__ void copy_16(uint32_t to, const void* from, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(reinterpret_cast<uint64_t>(from)), "r"(there ? 16 : 0) : "memory");
+}
 
 template <int RP>
-__device__ __forceinline__ void wgrad_rows(const CUtensorMap& tmY, const CUtensorMap& tmV, const WgradParams& p, int part, uint8_t* smem, unsigned* live) {
+__device__ __forceinline__ void wgrad_rows(const CUtensorMap& tmY, const CUtensorMap& tmV, const WgradParams& p, int part, uint8_t* smem) {
   constexpr int NB = RP < 32 ? 64 : 2 * RP, ST = kWgStages<RP>, STAGE = kLBox + kWgV<RP>;      // columns: of V its nearest, then its rests
+  constexpr int AHEAD = ST - 1;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + ST * STAGE);
-  const uint32_t bar_full = smem_u32(bars), bar_ready = bar_full + 8 * ST, bar_empty = bar_ready + 8 * ST, bar_tfull = bar_empty + 8 * ST;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * ST + 1);
+  const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * ST, bar_tfull = bar_empty + 8 * ST;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * ST + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool listed = p.lists.order != nullptr;
   const int chunks = (p.D + 127) / 128;
   const int chunk = part % chunks, l = part / chunks % p.L, split = part / chunks / p.L;
-  const int blocks = (p.T + 63) / 64;
-  const int b0 = static_cast<int>(static_cast<long long>(split) * blocks / p.splits), b1 = static_cast<int>(static_cast<long long>(split + 1) * blocks / p.splits);
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
-      mbar_init(bar_full + 8 * s, 1);
-      mbar_init(bar_ready + 8 * s, 4);
+      mbar_init(bar_full + 8 * s, listed ? 4 : 1);
       mbar_init(bar_empty + 8 * s, 1);
     }
     mbar_init(bar_tfull, 1);
@@ -750,116 +809,99 @@ __device__ __forceinline__ void wgrad_rows(const CUtensorMap& tmY, const CUtenso
     tmem_relinquish();
   }
   grid_dep_wait();
-  bool any = false;
-  for (int w = warp; w * 32 < b1 - b0; w += kWgThreads / 32) {
-    const int b = b0 + 32 * w + lane;
-    const bool has = b < b1 && (p.present == nullptr || (p.present[static_cast<long long>(b >> 1) * p.L + l] >> (b & 1) & 1) != 0);
-    const unsigned m = __ballot_sync(0xffffffffu, has);
-    if (lane == 0) live[w] = m;
-    any = any || m != 0;
-  }
   tc_fence_before();
-  any = __syncthreads_or(any);
+  __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int words = (b1 - b0 + 31) / 32;
-  // f(block) for each that has the adapter, in order, until it says no
-  auto each = [&](auto f) {
-    for (int w = 0; w < words; ++w)
-      for (unsigned m = live[w]; m != 0; m &= m - 1)
-        if (!f(b0 + 32 * w + __ffs(m) - 1)) return;
+  const int start = listed ? p.lists.bounds[l] : 0, rows = listed ? p.lists.bounds[l + 1] - start : p.T, all = (rows + 63) / 64;
+  const int b0 = static_cast<int>(static_cast<long long>(split) * all / p.splits), n = static_cast<int>(static_cast<long long>(split + 1) * all / p.splits) - b0;
+  const bool any = n > 0;
+  bool ok = true;
+  // one thread: a block of neighbouring rows
+  auto boxes = [&](int s, int row) {
+    const uint32_t full = bar_full + 8 * s, sy = smem_u32(smem + s * STAGE);
+    mbar_arrive_expect_tx(full, STAGE);
+    tma_load_3d(sy, &tmY, full, chunk * 128, row, 0);
+    tma_load_3d(sy + 8192, &tmY, full, chunk * 128 + 64, row, 0);
+    for (int h = 0; h < NB / 64; ++h) tma_load_3d(sy + kLBox + 8192 * h, &tmV, full, 64 * h, row, 0);
   };
   if (warp == 0) {
-    if (elect_one()) {
-      int s = 0;
-      uint32_t ph = 0;
-      each([&](int b) {
-        if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, ST_WAIT_PRODUCER)) return false;
-        const uint32_t full = bar_full + 8 * s, sy = smem_u32(smem + s * STAGE);
-        mbar_arrive_expect_tx(full, STAGE);
-        tma_load_3d(sy, &tmY, full, chunk * 128, 64 * b, 0);
-        tma_load_3d(sy + 8192, &tmY, full, chunk * 128 + 64, 64 * b, 0);
-        for (int h = 0; h < NB / 64; ++h) tma_load_3d(sy + kLBox + 8192 * h, &tmV, full, 64 * h, 64 * b, 0);
-        if (++s == ST) {
-          s = 0;
-          ph ^= 1;
-        }
-        return true;
-      });
-    }
+    if (!listed && elect_one())
+      for (int b = 0; b < n; ++b) {
+        if (!mbar_wait(bar_empty + 8 * (b % ST), (b / ST & 1) ^ 1, abort_flag, ST_WAIT_PRODUCER)) break;
+        boxes(b % ST, 64 * (b0 + b));
+      }
     grid_dep_launch();
   } else if (warp == 1) {
     if (elect_one()) {
       constexpr uint32_t idesc = umma_idesc_bf16(NB, 1, 1);
-      int s = 0;
-      uint32_t ph = 0, more = 0;
-      bool ok = true;
-      each([&](int) {
-        ok = mbar_wait(bar_ready + 8 * s, ph, abort_flag, ST_WAIT_MMA_FULL);
-        if (!ok) return false;
+      for (int b = 0; b < n && ok; ++b) {
+        const int s = b % ST;
+        ok = mbar_wait(bar_full + 8 * s, b / ST & 1, abort_flag, ST_WAIT_MMA_FULL);
+        if (!ok) break;
         tc_fence_after();
         const uint32_t sy = smem_u32(smem + s * STAGE), sv = sy + kLBox;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          umma_bf16(tmem, umma_desc_sw128(sy + 2048 * k, 8192, 1024), umma_desc_sw128(sv + 2048 * k, 8192, 1024), idesc, more);
-          more = 1;
-        }
+        for (int k = 0; k < 4; ++k)
+          umma_bf16(tmem, umma_desc_sw128(sy + 2048 * k, 8192, 1024), umma_desc_sw128(sv + 2048 * k, 8192, 1024), idesc, b > 0 || k > 0);
         umma_commit(bar_empty + 8 * s);
-        if (++s == ST) {
-          s = 0;
-          ph ^= 1;
-        }
-        return true;
-      });
+      }
       if (ok && any) umma_commit(bar_tfull);
     }
   } else {
-    const int q = warp & 3;
-    int s = 0;
-    uint32_t ph = 0;
-    bool ok = true;
-    // the adapters of a block's rows, fetched a block ahead; rows past the last one are zero already, whoever's they are
-    int r0 = l, r1 = l;
-    auto adapters = [&](int b) {
-      if (p.rows == nullptr || b < 0) return;
-      const int t = 64 * b + lane;
-      r0 = t < p.T ? p.rows[t] : l;
-      r1 = t + 32 < p.T ? p.rows[t + 32] : l;
-    };
-    int w = 0;
-    unsigned m = words > 0 ? live[0] : 0;
-    auto next = [&]() {              // the block after those it gave before, -1: none
-      while (m == 0) {
-        if (++w >= words) return -1;
-        m = live[w];
-      }
-      const int b = b0 + 32 * w + __ffs(m) - 1;
-      m &= m - 1;
-      return b;
-    };
-    int ahead = next();
-    adapters(ahead);
-    while (ahead >= 0 && ok) {
-      const unsigned bad0 = __ballot_sync(0xffffffffu, r0 != l), bad1 = __ballot_sync(0xffffffffu, r1 != l);
-      ahead = next();
-      adapters(ahead);
-      ok = __all_sync(0xffffffffu, mbar_wait(bar_full + 8 * s, ph, abort_flag, ST_WAIT_MMA_FULL));
-      if (!ok) break;
-      if ((bad0 | bad1) != 0) {
-        uint8_t* sy = smem + s * STAGE;
-        for (int r = q; r < 64; r += 4)
-          if (((r < 32 ? bad0 : bad1) >> (r & 31) & 1) != 0)
-            for (int c = lane; c < STAGE / 1024; c += 32)       // 16 bytes of a row: eight a box
-              *reinterpret_cast<uint4*>(sy + (c >> 3) * 8192 + r * 128 + 16 * (c & 7)) = make_uint4(0u, 0u, 0u, 0u);
+    if (listed) {            // a warp 16 rows of a block
+      const int w = warp - 2;
+      const int* order = p.lists.order + start;
+      // lanes below 16: a row; lanes 16 and 17: the block's first and last; -1: there is none
+      auto look = [&](int b) {
+        const int i = 64 * (b0 + b) + (lane < 16 ? 16 * w + lane : lane == 16 ? 0 : 63);
+        return b < n && i < rows ? order[i] : -1;
+      };
+      int next = look(0), sent = 0, b = 0;
+      unsigned whole = 0;    // which of the last blocks are boxes
+      auto arrived = [&](int upto) {
         fence_proxy_async_smem();
+        __syncwarp();
+        for (; sent < upto; ++sent)
+          if (lane == 0 && (whole >> (sent & 31) & 1) == 0) mbar_arrive(bar_full + 8 * (sent % ST));
+      };
+      for (; b < n; ++b) {
+        const int s = b % ST, mine = next;
+        next = look(b + 1);
+        const int head = __shfl_sync(0xffffffffu, mine, 16), tail = __shfl_sync(0xffffffffu, mine, 17);
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_empty + 8 * s, (b / ST & 1) ^ 1, abort_flag, ST_WAIT_PRODUCER));
+        if (!ok) break;
+        if (tail - head == 63 && tail >= 0) {
+          whole |= 1u << (b & 31);
+          if (lane == 0) {
+            if (w == 0) boxes(s, head);
+            else mbar_arrive(bar_full + 8 * s);
+          }
+        } else {
+          whole &= ~(1u << (b & 31));
+          const uint32_t sy = smem_u32(smem + s * STAGE), sv = sy + kLBox;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int r = (32 * k + lane) >> 4, c = lane & 15, at = __shfl_sync(0xffffffffu, mine, r);
+            const bool there = at >= 0 && chunk * 128 + 8 * c < p.D;
+            copy_16(sy + (c >> 3) * 8192 + (16 * w + r) * 128 + (((c ^ r) & 7) << 4), there ? p.y + at * p.ldy + chunk * 128 + 8 * c : p.y, there);
+          }
+#pragma unroll
+          for (int k = 0; k < RP / 8; ++k) {
+            const int r = (32 * k + lane) / (RP / 4), c = (32 * k + lane) % (RP / 4), at = __shfl_sync(0xffffffffu, mine, r);
+            copy_16(sv + (c >> 3) * 8192 + (16 * w + r) * 128 + (((c ^ r) & 7) << 4), at >= 0 ? p.v + static_cast<long long>(at) * (2 * RP) + 8 * c : p.v, at >= 0);
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (b >= AHEAD) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD) : "memory");
+          arrived(b - AHEAD + 1);
+        }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_ready + 8 * s);
-      if (++s == ST) {
-        s = 0;
-        ph ^= 1;
-      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      arrived(b);
     }
+    const int q = warp & 3;
     if (any) ok = ok && mbar_wait(bar_tfull, 0, abort_flag, ST_WAIT_EPILOGUE);
     __syncwarp();
     tc_fence_after();
@@ -912,8 +954,7 @@ template <int RP>
 __global__ void __launch_bounds__(kWgThreads)
 lora_wgrad_kernel(const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmV, const WgradParams p) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ unsigned live[kWgWords];
-  wgrad_rows<RP>(tmY, tmV, p, blockIdx.x, aligned_smem(smem_raw), live);
+  wgrad_rows<RP>(tmY, tmV, p, blockIdx.x, aligned_smem(smem_raw));
 }
 
 // Both products of the gradient g in one launch, shrink (u = g B) and wgrad (of B): by turns a cluster of the one and of the other, so that an SM has a
@@ -928,12 +969,11 @@ lora_back_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
                  const __grid_constant__ CUtensorMap tmV, const ShrinkParams p, const WgradParams w, int shrinks, int wgrads) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ LoraShare share;
-  __shared__ unsigned live[kWgWords];
   const int c = blockIdx.x / p.split, both = 2 * min(shrinks, wgrads);      // clusters of the roles
   const bool shrink = c < both ? (c & 1) == 0 : shrinks > wgrads;
   const int part = c < both ? c >> 1 : c - both / 2;
   if (shrink) shrink_rows<RP, true>(tmX, tmW, p, part, shrinks, aligned_smem(smem_raw), share);
-  else wgrad_rows<RP>(tmY, tmV, w, part * p.split + blockIdx.x % p.split, aligned_smem(smem_raw), live);
+  else wgrad_rows<RP>(tmY, tmV, w, part * p.split + blockIdx.x % p.split, aligned_smem(smem_raw));
 }
 
 // the sum of the splits' shares, n values (a multiple of 4), always in the same order; eight of them are on their way at a time
@@ -1348,16 +1388,14 @@ static int lora_expand(const void* V, const void* W, bool wmn, int64_t L, int64_
 // Shares of the rows: as many as it takes for two CTAs an SM, each with eight blocks of rows at least
 static int wgrad_splits(int64_t T, int64_t D, int64_t L) {
   const int64_t blocks = ceil_div(T, 64), ctas = ceil_div(D, 128) * L;
-  const int64_t s = std::max<int64_t>(1, std::min<int64_t>(2 * num_sms() / ctas, blocks / 8));
-  return static_cast<int>(std::max<int64_t>(s, ceil_div(blocks, 32 * kWgWords)));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2 * num_sms() / ctas, blocks / 8)));
 }
 // The same for the gradient of B, which shares its launch with u = g B where that is wanted: one CTA an SM of either role, in whole clusters.  By itself it
 // has as many shares, so that its bits do not depend on what else is asked for.
 static int back_wgrad_splits(int64_t T, int64_t D, int64_t L) {
   const int64_t blocks = ceil_div(T, 64), ctas = ceil_div(D, 128) * L;
-  const int64_t s = std::max<int64_t>(1, std::min<int64_t>(num_sms() / ctas, blocks / 8));
   const int split = shrink_split(T, D, num_sms());
-  int64_t n = std::max<int64_t>(s, ceil_div(blocks, 32 * kWgWords));
+  int64_t n = std::max<int64_t>(1, std::min<int64_t>(num_sms() / ctas, blocks / 8));
   while (n * ctas % split != 0) ++n;
   return static_cast<int>(n);
 }
@@ -1369,6 +1407,9 @@ static int lora_wgrad(const void* Y, int64_t ldy, const void* V, int splits, Wgr
     if (rc == 0) rc = make_map(&tmV, V, 2 * RP, p.T, 1, 2 * RP, static_cast<int64_t>(p.T) * (2 * RP), 64, 64);
     if (rc) return rc;
     p.splits = splits;
+    p.y = static_cast<const __nv_bfloat16*>(Y);
+    p.v = static_cast<const __nv_bfloat16*>(V);
+    p.ldy = ldy;
     p.out = p.splits > 1 ? static_cast<void*>(ws) : out;
     p.out_f32 = p.splits > 1 || out_f32;
     static PerDevice allowed;
@@ -1399,6 +1440,9 @@ static int lora_back(const void* G, const void* B, const void* V, int64_t L, Shr
     p.stage = kLBox + static_cast<int>(slots) * columns * 128;
     p.stages = std::min(kShrinkMost, kShrinkRing / p.stage);
     w.splits = back_wgrad_splits(T, D, L);
+    w.y = static_cast<const __nv_bfloat16*>(G);
+    w.v = static_cast<const __nv_bfloat16*>(V);
+    w.ldy = D;
     w.out = w.splits > 1 ? static_cast<void*>(ws) : out;
     w.out_f32 = w.splits > 1 || out_f32;
     const int64_t wgrads = ceil_div(D, 128) * L * w.splits / p.split;
@@ -1428,8 +1472,7 @@ struct LoraCarver {
 struct LoraKept {
   __nv_bfloat16* v;
   LoraTiles tiles;
-  int* rows;
-  unsigned char* present;
+  LoraLists lists;
   int* counter;
 };
 // index: the call has one
@@ -1446,8 +1489,8 @@ static LoraKept carve_lora(int64_t T, int64_t R, int64_t L, bool index, int keep
     k.tiles.adapter = c.take<int>(tiles * kLTile);
     k.tiles.slot = c.take<short>(tiles * kLTile);
     if (keep) {
-      k.rows = c.take<int>(T);
-      k.present = c.take<unsigned char>(tiles * L);
+      k.lists.order = c.take<int>(T);
+      k.lists.bounds = c.take<int>(L + 1);
     }
   }
   *bytes = c.off;
@@ -1521,7 +1564,7 @@ int b200moe_lora_forward(const void* x, int64_t ldx, const void* a, const void* 
   const LoraKept k = carve_lora(T, R, L, index != nullptr, keep, ws, &bytes);
   if (index != nullptr) {
     OpScope scope("lora_tiles", 1);
-    B200_LAUNCH(lora_tiles_kernel, k.tiles.tiles, kLTile, 0, st, ix, k.tiles, k.rows, k.present);
+    B200_LAUNCH(lora_tiles_kernel, static_cast<int>(ceil_div(k.tiles.tiles, kTilesEach) + (keep ? L : 0)), kTilesThreads, 0, st, ix, k.tiles, k.lists);
   }
   {
     OpScope scope("lora_shrink", 1);
@@ -1560,8 +1603,8 @@ int b200moe_lora_backward(const void* grad_out, const void* x, int64_t ldx, cons
   __nv_bfloat16* u = c.take<__nv_bfloat16>(2 * T * padded_rank(R));
   int* counter = c.take<int>(1);
   float* part = c.take<float>(0);
-  WgradParams w{static_cast<int>(T), 0, static_cast<int>(R), static_cast<int>(L), 1, 0, k.rows, k.present,
-                nullptr, 0, status};
+  WgradParams w{static_cast<int>(T), 0, static_cast<int>(R), static_cast<int>(L), 1, 0, k.lists,
+                nullptr, nullptr, 0, nullptr, 0, status};
 #define RUN(name, launches, call)     \
   do {                                \
     OpScope scope__(name, launches);  \
