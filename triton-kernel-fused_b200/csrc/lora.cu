@@ -996,14 +996,14 @@ __global__ void __launch_bounds__(128) lora_wgrad_sum_kernel(const float* part, 
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
-// A cluster of eight CTAs takes up to sixteen rows of one adapter (and a share of the columns, where such groups are fewer than SMs): each CTA multiplies
-// an eighth of the rows with all of A_l, the sums meet in distributed shared memory, and each expands its columns.  Both products are m16n8k16
+// A cluster of eight CTAs (four, where there are many groups) takes up to sixteen rows of one adapter, and a share of the columns, where such groups are fewer than
+// SMs: each CTA multiplies an eighth of the rows with all of A_l, the sums meet in distributed shared memory, and each expands its columns.  Both products are m16n8k16
 // instructions; the order of the reduction index within one is free as long as both operands have it, so a lane's share of x and A_l is 16 neighbouring
 // bytes of global memory, of B_l 8 of shared memory.  v is never rounded: it is split into two bf16 numbers that hold 16 bits of it.
 // Bound by latency: each warp's bulk copies of its first columns of B_l and of the base are on their way while x and A_l are multiplied, and its result
 // leaves from where the base landed.  us, L2 warm: one row, 4096 x 4096, rank 16 4.9; 64 rows of 32 adapters, 4096 x 14336 12.9 (17.9 with columns handed out
 // to the CTA's warps in turns, 30 with columns fetched into registers four tiles ahead).
-constexpr int kFewCluster = 8, kFewThreads = 256, kFewWarps = kFewThreads / 32, kFewRows = 16, kFewMost = 512, kFewInline = 128;
+constexpr int kFewThreads = 256, kFewSm = 3, kFewWarps = kFewThreads / 32, kFewRows = 16, kFewMost = 512, kFewInline = 128;
 constexpr int kFewChunk = 7680;          // of a warp: columns of B_l, and of the base and the result of each row
 static int few_smem(int64_t R) { return static_cast<int>(kFewWarps * kFewChunk + kFewRows * R * 4 + std::max<int64_t>(4096, (R + 15) / 16 * 1024)); }
 
@@ -1135,9 +1135,9 @@ struct FewLora {
   float scale;
 };
 
-// KS: steps of 16 r, 0: any number of them
-template <int KS>
-__global__ void __launch_bounds__(kFewThreads, 3) lora_few_kernel(const FewLora p) {
+// KS: steps of 16 r, 0: any number of them; CTAS: of a cluster
+template <int KS, int CTAS>
+__global__ void __launch_bounds__(kFewThreads, kFewSm) lora_few_kernel(const FewLora p) {
   extern __shared__ __align__(128) uint8_t smem[];                 // a chunk a warp, sums, and (by turns) partial sums or v as fragments
   __shared__ FewGroup group;
   __shared__ __align__(8) uint64_t bars[kFewWarps];
@@ -1158,7 +1158,7 @@ __global__ void __launch_bounds__(kFewThreads, 3) lora_few_kernel(const FewLora 
   if (n == 0) return;                                              // the whole cluster
   const int l = group.l;
   // this warp's columns, in chunks of `wide`
-  const int share = (c % p.parts * kFewCluster + rank) * kFewWarps + warp, shares = p.parts * kFewCluster * kFewWarps;
+  const int share = (c % p.parts * CTAS + rank) * kFewWarps + warp, shares = p.parts * CTAS * kFewWarps;
   const int col0 = 8 * static_cast<int>(static_cast<long long>(share) * (p.N / 8) / shares);
   const int col1 = 8 * static_cast<int>(static_cast<long long>(share + 1) * (p.N / 8) / shares);
   const int wide = kFewChunk / (2 * p.R + 2 * n) & ~7, ksteps = KS > 0 ? KS : (p.R + 15) / 16;
@@ -1182,7 +1182,7 @@ __global__ void __launch_bounds__(kFewThreads, 3) lora_few_kernel(const FewLora 
     // tiles of eight r, and where these are fewer than warps, several warps a tile that split the columns
     const int rt = p.R / 8, split = rt < kFewWarps ? kFewWarps / rt : 1;
     const int steps = (p.K + 31) / 32;
-    const int s0 = rank * steps / kFewCluster, s1 = (rank + 1) * steps / kFewCluster;
+    const int s0 = rank * steps / CTAS, s1 = (rank + 1) * steps / CTAS;
     for (int tile = warp % (rt * split) / split; tile < rt && warp < rt * split; tile += kFewWarps / split) {
       const int w = split > 1 ? warp % split : 0;
       const int first = s0 + w * (s1 - s0) / split, last = s0 + (w + 1) * (s1 - s0) / split;
@@ -1222,7 +1222,7 @@ __global__ void __launch_bounds__(kFewThreads, 3) lora_few_kernel(const FewLora 
       float2 s = make_float2(0.0f, 0.0f);
       if (row < n && r < p.R) {
 #pragma unroll
-        for (int k = 0; k < kFewCluster; ++k) {
+        for (int k = 0; k < CTAS; ++k) {
           float2 o;
           asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
                        : "=f"(o.x), "=f"(o.y)
@@ -1501,6 +1501,15 @@ static LoraKept carve_lora(int64_t T, int64_t R, int64_t L, bool index, int keep
 // 64 rows 8.6 / 23, 512 rows 16 / 29.
 static bool lora_few(int64_t T, int64_t R, int64_t L, int keep) { return !keep && T <= (L > 1 ? kFewMost : R <= 32 ? 128 : 16); }
 
+// CTAs of a cluster: eight, and four where the clusters of all groups there may be would not be on the SMs at once although a warp's columns fit one chunk, or
+// would come round twice.  us, eight / four: 2048 x 2816, rank 16, 512 rows of 32 adapters 14.9 / 13.1, 128 rows of 128 16.8 / 9.5, 64 rows of 8 7.6 / 7.7; 4096 x
+// 14336, 64 rows of 64 12.8 / 16.6, 512 rows of 32 26 / 29, 128 rows of 128 27 / 22; 4096 x 4096, 512 rows of 32 15.7 / 17.0, 256 rows of 128 27.5 / 24.0.
+static int few_cluster(int64_t T, int64_t N, int64_t R, int64_t L, int64_t groups) {
+  const int64_t room = static_cast<int64_t>(num_sms()) * kFewSm, rows = std::min<int64_t>(kFewRows, ceil_div(T, L));
+  const bool fits = N * 2 * (R + rows) <= 4 * kFewWarps * kFewChunk;
+  return groups * 8 > (fits ? room : 2 * room) ? 4 : 8;
+}
+
 }  // namespace b200moe
 
 using namespace b200moe;
@@ -1545,20 +1554,24 @@ int b200moe_lora_forward(const void* x, int64_t ldx, const void* a, const void* 
   if (lora_few(T, R, L, keep)) {
     const int64_t groups = few_groups(ix);
     FewRank *ranks = index != nullptr && T > kFewInline ? static_cast<FewRank*>(ws) : nullptr, *leaders = ranks != nullptr ? ranks + T : nullptr;
-    const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(num_sms() / (groups * kFewCluster), ceil_div(N, 8 * kFewWarps * kFewCluster))));
+    const int ctas = few_cluster(T, N, R, L, groups);
+    const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(num_sms() / (groups * ctas), ceil_div(N, 8 * kFewWarps * ctas))));
     const FewLora p{ix, static_cast<const __nv_bfloat16*>(x), static_cast<const __nv_bfloat16*>(a), static_cast<const __nv_bfloat16*>(b),
                     static_cast<const __nv_bfloat16*>(base), static_cast<__nv_bfloat16*>(out), ldx, ldb, ranks, leaders, static_cast<int>(K),
                     static_cast<int>(N), static_cast<int>(R), parts, scales, scale};
     OpScope scope("lora_few", ranks != nullptr ? 2 : 1);
     if (ranks != nullptr) B200_LAUNCH(lora_rank_kernel, 1, kFewMost, 0, st, ix, ranks, leaders, static_cast<int>(groups));
-    auto run = [&](auto ks) -> int {
-      constexpr int KS = decltype(ks)::value;
+    auto run = [&](auto ks, auto of) -> int {
+      constexpr int KS = decltype(ks)::value, CTAS = decltype(of)::value;
       static PerDevice allowed;
-      B200_CUDA(allow_smem(allowed, lora_few_kernel<KS>, few_smem(128)));
-      B200_CUDA(launch_chained(lora_few_kernel<KS>, static_cast<int>(groups * parts * kFewCluster), kFewThreads, few_smem(R), st, kFewCluster, p));
+      B200_CUDA(allow_smem(allowed, lora_few_kernel<KS, CTAS>, few_smem(128)));
+      B200_CUDA(launch_chained(lora_few_kernel<KS, CTAS>, static_cast<int>(groups * parts * CTAS), kFewThreads, few_smem(R), st, CTAS, p));
       return 0;
     };
-    return R <= 16 ? run(std::integral_constant<int, 1>()) : R <= 32 ? run(std::integral_constant<int, 2>()) : run(std::integral_constant<int, 0>());
+    auto run_of = [&](auto of) -> int {
+      return R <= 16 ? run(std::integral_constant<int, 1>(), of) : R <= 32 ? run(std::integral_constant<int, 2>(), of) : run(std::integral_constant<int, 0>(), of);
+    };
+    return ctas == 8 ? run_of(std::integral_constant<int, 8>()) : run_of(std::integral_constant<int, 4>());
   }
   size_t bytes;
   const LoraKept k = carve_lora(T, R, L, index != nullptr, keep, ws, &bytes);
