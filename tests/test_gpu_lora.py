@@ -420,3 +420,15 @@ def test_first_call_of_a_thread(pkg):
     t.join()
     L.check(rc[0])
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("T", [40, 700])
+def test_rows_of_a_larger_batch(pkg, T):
+    """Everything a slice from the second row on: int32 indices lie at no multiple of eight bytes then."""
+    x, a, b, s, bs, index = make(T + 1, 64, 72, 16, 3, seed=21)
+    want = pkg.lora_linear(x[1:].clone(), a, b, index[1:].clone(), s, bs[1:].clone())
+    for i in (index[1:], index.int()[1:]):
+        assert torch.equal(pkg.lora_linear(x[1:], a, b, i, s, bs[1:]), want)
+    n = torch.stack([index, index], 1).int()[:, 1]      # and every second of them
+    assert torch.equal(pkg.lora_linear(x, a, b, n, s, bs), pkg.lora_linear(x, a, b, index, s, bs))
+    pkg.check_status()

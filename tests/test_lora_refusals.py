@@ -37,3 +37,9 @@ def test_python_callable():
     x, a, b = (torch.zeros(*s, dtype=torch.bfloat16) for s in ((4, 64), (1, 8, 64), (1, 64, 8)))
     with pytest.raises(ValueError, match="CUDA"):
         pkg.lora_linear(x, a, b)
+
+
+def test_an_index_off_its_type():
+    lib = load_pkg().lib()
+    for bytes_, off in ((4, 2), (8, 4)):
+        assert lib.b200moe_lora_forward(P, 64, P, P, P + off, bytes_, None, 1.0, P, 64, 4, 64, 64, 8, 2, 0, P, P, P, None) == -2

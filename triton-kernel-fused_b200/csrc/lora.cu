@@ -1547,8 +1547,8 @@ int b200moe_lora_forward(const void* x, int64_t ldx, const void* a, const void* 
   if (T == 0) return 0;
   B200_CHECK_ARG(x && a && b && ws && out && status, B200MOE_E_NULL, "lora_forward: null pointer");
   B200_CHECK_ARG(aligned16(x) && aligned16(a) && aligned16(b) && aligned16(base) && aligned16(ws) && aligned16(out) &&
-                     reinterpret_cast<uintptr_t>(index) % 8 == 0,
-                 B200MOE_E_ALIGN, "lora_forward: tensors must be 16-byte aligned, the index 8");
+                     (index == nullptr || reinterpret_cast<uintptr_t>(index) % index_bytes == 0),
+                 B200MOE_E_ALIGN, "lora_forward: tensors must be 16-byte aligned, the index as its type");
   cudaStream_t st = (cudaStream_t)stream;
   const LoraIndex ix{index, index_bytes, static_cast<int>(T), static_cast<int>(L), status};
   if (lora_few(T, R, L, keep)) {
