@@ -432,3 +432,23 @@ def test_rows_of_a_larger_batch(pkg, T):
     n = torch.stack([index, index], 1).int()[:, 1]      # and every second of them
     assert torch.equal(pkg.lora_linear(x, a, b, n, s, bs), pkg.lora_linear(x, a, b, index, s, bs))
     pkg.check_status()
+
+
+def test_offsets_beyond_32_bits(pkg):
+    """x, base, the result and both gradients have more than 2^31 values; only the last rows have a gradient, so those are all that the sums hold."""
+    T, K, N, R, n, m = 270_000, 8192, 8200, 16, 3, 1000
+    x, bs = (torch.empty(T, d, dtype=BF, device=DEV).normal_(generator=gen(31)) for d in (K, N))
+    _, a, b, s, _, _ = make(1, K, N, R, n, seed=32)
+    go = torch.zeros(T, N, dtype=BF, device=DEV)
+    go[-m:].normal_(generator=gen(33))
+    for index in (torch.arange(T, device=DEV) * n // T, torch.arange(T, device=DEV) * 7 % (n + 1) - 1):
+        leaves = [t.requires_grad_() for t in (x, a, b)]
+        y = pkg.lora_linear(x, a, b, index, s, bs)
+        gx, ga, gb = torch.autograd.grad(y, leaves, go)
+        ref = reference(x.detach()[-m:], a.detach(), b.detach(), s, bs[-m:], index[-m:], go[-m:])
+        close(y.detach()[-m:], ref["y"], K)
+        close(gx[-m:], ref["gx"], N)
+        close(ga, ref["ga"], N)
+        close(gb, ref["gb"], K)
+        del y, gx
+    pkg.check_status()

@@ -377,3 +377,29 @@ def test_an_infinite_eps_is_refused(pkg):
         for call in (lambda: pkg.rms_norm(x, w, eps=eps), lambda: pkg.rms_norm(x[:, ::2], w[::2], eps=eps), lambda: pkg.rms_norm_fp8_block(x, w, eps=eps)):
             with pytest.raises(ValueError, match="eps"):
                 call()
+
+
+def test_offsets_beyond_32_bits(pkg):
+    """More than 2^31 values; rows do not depend on where they lie."""
+    T, K, m = 135_000, 16_384, 1000
+    g = torch.Generator(device=DEV).manual_seed(41)
+    x, r = (torch.empty(T, K, dtype=BF, device=DEV).normal_(generator=g) for _ in range(2))
+    w = torch.empty(K, dtype=BF, device=DEV).normal_(generator=g)
+    few = [t[-m:].clone() for t in (x, r)]
+    q, s, y, h = pkg.rms_norm_fp8_block(x, w, r, return_norm=True)
+    for got, want in zip((q, s, y, h), pkg.rms_norm_fp8_block(few[0], w, few[1], return_norm=True)):
+        assert torch.equal(got[-m:].float(), want.float())
+    del q, s, y, h
+    gy = torch.zeros(T, K, dtype=BF, device=DEV)
+    gy[-m:].normal_(generator=g)
+    out = []
+    for rows in ((x, r, gy), (few[0], few[1], gy[-m:])):
+        p, res, go = rows[0].detach().requires_grad_(), rows[1], rows[2]
+        wl = w.detach().requires_grad_()
+        y, h = pkg.rms_norm(p, wl, res)
+        gx, gw = torch.autograd.grad([y, h], [p, wl], [go, go])
+        out.append((gx[-m:].clone(), gw.float()))
+        del y, h, gx
+    assert torch.equal(out[0][0], out[1][0])
+    assert float((out[0][1] - out[1][1]).norm()) <= 2.0 ** -7 * float(out[1][1].norm())      # each rounded to bf16 once, sums in another order
+    pkg.check_status()
