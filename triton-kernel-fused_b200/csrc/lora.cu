@@ -5,10 +5,10 @@
 // and backward   u[t] = s_l g[t] B_l,   grad_x[t] = u[t] A_l,   grad_A_l = sum_t u[t]^T x[t],   grad_B_l = sum_t g[t]^T v[t].
 //
 // Four products with one short side (R of at most 128), all bound by HBM: `shrink` (T,D) -> (T,R) reads x or g, `expand` (T,R) -> (T,D) reads
-// base and writes out or grad_x, `wgrad` reads x or g again.  Each is a tcgen05 kernel over tiles of 128 rows as they come, without sorting
+// base and writes out or grad_x, `wgrad` reads x or g again.  Each is a tcgen05 kernel.  The first two take tiles of 128 rows as they come, without sorting
 // them: a tile's distinct adapters are found by a kernel before, each is multiplied with all rows of the tile into tensor memory of its own, and a
-// row takes the result of its adapter.  Rows of other adapters are never added to it, not even times zero, so an infinity or a NaN stays with
-// its own adapter or row.  Few rows (a decoding batch) run in one kernel of their own, a cluster for up to sixteen rows of an adapter.
+// row takes the result of its adapter.  `wgrad` takes the rows of an adapter's list.  Rows of other adapters are never added to anything, not even times
+// zero, so an infinity or a NaN stays with its own adapter or row.  Few rows (a decoding batch) run in one kernel of their own, a cluster for up to sixteen rows of an adapter.
 //
 // v and u, which go from one product to the next, are two bf16 numbers each, the nearest and what that leaves, side by side: 16 bits, so that results are as
 // exact as those of an fp32 v.  (Rounded to one number the error of a result without a base was 0.0024 in the norm in place of 0.0017.)  All sums are fp32.
@@ -760,8 +760,8 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tmV, const __grid_constan
 // neighbouring rows is two boxes of Y and those of V; of others four warps copy the 64 rows of the adapter's list into the same places, 16 bytes a lane.
 // 16384 x 2048, rank 64: 17 us, 10.3 at the copy rate, and 3 for the shares' sum.  V's rests are columns of their own, so its 16 KB a block are read for each 128
 // columns (16 us with the nearest numbers alone; 256 columns a CTA would need twice the shares and their sums).  Shares added up in clusters of eight
-// instead took 31: so many large CTAs of one cluster do not find room at once.  8192 x 2048, rank 16, rows of 32 adapters mixed: 18 (267 where each adapter's CTAs visited every
-// block that has a row of it and set the others' rows to zero); 3001 rows of three adapters one after another 7.6 (11), by 16 bytes alone 14.
+// instead took 31: so many large CTAs of one cluster do not find room at once.  8192 x 2048, rank 16, rows of 32 adapters mixed: 18 (267 where each
+// adapter's CTAs visited every block that has a row of it and set the others' rows to zero); 3001 rows of three adapters one after another 7.6 (11).
 constexpr int kWgThreads = 192;
 template <int RP> constexpr int kWgV = (RP > 32 ? RP / 32 : 1) * 8192;
 template <int RP> constexpr int kWgStages = RP > 64 ? 2 : RP > 32 ? 3 : 4;
