@@ -813,7 +813,7 @@ __device__ __forceinline__ void wgrad_rows(const CUtensorMap& tmY, const CUtenso
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int start = listed ? p.lists.bounds[l] : 0, rows = listed ? p.lists.bounds[l + 1] - start : p.T, all = (rows + 63) / 64;
+  const int start = listed ? p.lists.bounds[l] : 0, rows = listed ? p.lists.bounds[l + 1] - start : l == 0 ? p.T : 0, all = (rows + 63) / 64;
   const int b0 = static_cast<int>(static_cast<long long>(split) * all / p.splits), n = static_cast<int>(static_cast<long long>(split + 1) * all / p.splits) - b0;
   const bool any = n > 0;
   bool ok = true;
