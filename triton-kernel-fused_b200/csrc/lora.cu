@@ -1310,8 +1310,8 @@ __global__ void __launch_bounds__(kFewThreads, kFewSm) lora_few_kernel(const Few
   }
   bulk_wait_all();
   __syncwarp();
+  cluster_sync_all();      // nobody leaves while another reads its sums, and every warp's waits are over
   if (threadIdx.x == 0 && abort_word != 0) *p.ix.status = abort_word;
-  cluster_sync_all();      // nobody leaves while another reads its sums
 }
 
 // ------------------------------------------------------------------------------------------------ host
