@@ -398,7 +398,7 @@ int b200moe_rms_norm_bwd(const void* grad_y, const void* grad_h, const void* h, 
  * out[t] = base[t] + s_l (x[t] A_l^T) B_l^T with l = index[t]: x (T,K), a (L,R,K), b (L,N,R), base (T,N, nullable: 0) and out (T,N) bf16, rows of x
  * and base ldx / ldb elements apart (multiples of 8); index int32 or int64 (index_bytes 4 or 8), NULL: adapter 0 for every row; a negative one
  * names none, one of L or more too and raises status 9.  s_l = scales[l], or scale where scales is NULL.  K and N multiples of 8, R of 8 up to
- * 128, L up to 65536; tensors 16-byte aligned.  Sums are fp32; x A^T goes on as two bf16 numbers, 16 bits of it.
+ * 128, L up to 65536 (a stack below 2^38 values); tensors 16-byte aligned.  Sums are fp32; x A^T goes on as two bf16 numbers, 16 bits of it.
  * keep: a backward follows, which reads ws. */
 size_t b200moe_lora_fwd_ws_bytes(int64_t T, int64_t R, int64_t L, int keep);
 int b200moe_lora_forward(const void* x, int64_t ldx, const void* a, const void* b, const void* index, int index_bytes, const float* scales,

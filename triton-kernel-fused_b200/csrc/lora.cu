@@ -1521,9 +1521,10 @@ static int check_lora(const char* who, int64_t T, int64_t K, int64_t N, int64_t 
   B200_CHECK_ARG(T >= 0 && T < (1LL << 31) - 256 && K < (1LL << 31) - 256 && N < (1LL << 31) - 256, B200MOE_E_BAD_SHAPE,
                  "%s: %lld rows, %lld -> %lld", who, (long long)T, (long long)K, (long long)N);
   B200_CHECK_ARG(L >= 1 && L <= 65536, B200MOE_E_BAD_SHAPE, "%s: %lld adapters, supported 1..65536", who, (long long)L);
-  B200_CHECK_ARG(ceil_div(T, 128) * 8 < (1LL << 31) && ceil_div(std::max(K, N), 128) * L * 512 < (1LL << 31) &&
-                     ceil_div(T, 128) * ceil_div(std::max(K, N), 128) < (1LL << 31) - 65536, B200MOE_E_BAD_SHAPE,
-                 "%s: %lld adapters of %lld -> %lld are too many", who, (long long)L, (long long)K, (long long)N);
+  // Tiles of the second product, in an int; and stacks that a GPU can hold at all, 0.5 TB each, which leaves the gradients' CTAs (one for 128 columns of an
+  // adapter) below 2^29.
+  B200_CHECK_ARG(ceil_div(T, 128) * ceil_div(std::max(K, N), 128) < (1LL << 31) - 65536 && L * R * std::max(K, N) < (1LL << 38), B200MOE_E_BAD_SHAPE,
+                 "%s: %lld rows, %lld adapters of %lld -> %lld are too many", who, (long long)T, (long long)L, (long long)K, (long long)N);
   return 0;
 }
 
