@@ -973,7 +973,8 @@ lora_back_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
   const bool shrink = c < both ? (c & 1) == 0 : shrinks > wgrads;
   const int part = c < both ? c >> 1 : c - both / 2;
   if (shrink) shrink_rows<RP, true>(tmX, tmW, p, part, shrinks, aligned_smem(smem_raw), share);
-  else wgrad_rows<RP>(tmY, tmV, w, part * p.split + blockIdx.x % p.split, aligned_smem(smem_raw));
+  else if (const int at = part * p.split + static_cast<int>(blockIdx.x) % p.split; at < (w.D + 127) / 128 * w.L * w.splits)      // the last cluster may have more CTAs
+    wgrad_rows<RP>(tmY, tmV, w, at, aligned_smem(smem_raw));
 }
 
 // the sum of the splits' shares, n values (a multiple of 4), always in the same order; eight of them are on their way at a time
@@ -1390,14 +1391,11 @@ static int wgrad_splits(int64_t T, int64_t D, int64_t L) {
   const int64_t blocks = ceil_div(T, 64), ctas = ceil_div(D, 128) * L;
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2 * num_sms() / ctas, blocks / 8)));
 }
-// The same for the gradient of B, which shares its launch with u = g B where that is wanted: one CTA an SM of either role, in whole clusters.  By itself it
-// has as many shares, so that its bits do not depend on what else is asked for.
+// The same for the gradient of B, which shares its launch with u = g B where that is wanted: one CTA an SM of either role.  By itself it has as many shares,
+// so that its bits do not depend on what else is asked for.
 static int back_wgrad_splits(int64_t T, int64_t D, int64_t L) {
   const int64_t blocks = ceil_div(T, 64), ctas = ceil_div(D, 128) * L;
-  const int split = shrink_split(T, D, num_sms());
-  int64_t n = std::max<int64_t>(1, std::min<int64_t>(num_sms() / ctas, blocks / 8));
-  while (n * ctas % split != 0) ++n;
-  return static_cast<int>(n);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(num_sms() / ctas, blocks / 8)));
 }
 static int lora_wgrad(const void* Y, int64_t ldy, const void* V, int splits, WgradParams p, float* ws, void* out, int out_f32, cudaStream_t st) {
   return by_rank(padded_rank(p.R), [&](auto rp) -> int {
@@ -1445,7 +1443,7 @@ static int lora_back(const void* G, const void* B, const void* V, int64_t L, Shr
     w.ldy = D;
     w.out = w.splits > 1 ? static_cast<void*>(ws) : out;
     w.out_f32 = w.splits > 1 || out_f32;
-    const int64_t wgrads = ceil_div(D, 128) * L * w.splits / p.split;
+    const int64_t wgrads = ceil_div(ceil_div(D, 128) * L * w.splits, p.split);
     static PerDevice allowed;
     B200_CUDA(allow_smem(allowed, lora_back_kernel<RP>, kBackSmem<RP>));
     B200_CUDA(launch_chained(lora_back_kernel<RP>, static_cast<int>((shrinks + wgrads) * p.split), kBackThreads, kBackSmem<RP>, st, p.split, tmX, tmW, tmY, tmV,
