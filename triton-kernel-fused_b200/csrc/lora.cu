@@ -1332,8 +1332,10 @@ static int shrink_split(int64_t T, int64_t D, int64_t ctas) {
   while (split < 8 && tiles * split * 2 <= ctas && blocks >= 4 * split) split *= 2;
   return split;
 }
+// `sms`: those that a call's grids are made for, gemm_cta_budget() at its start: the row tiles' kernels are persistent, and SMs reserved for an exchange are not
+// theirs.  Workspaces are sized for num_sms(), which never gives fewer shares.
 // W: (L,R,D), or (wmn) (L,D,R); split: 0, or that of the gradients' launch
-static int lora_shrink(const void* X, int64_t ldx, const void* W, bool wmn, int64_t L, ShrinkParams p, cudaStream_t st) {
+static int lora_shrink(const void* X, int64_t ldx, const void* W, bool wmn, int64_t L, ShrinkParams p, int sms, cudaStream_t st) {
   return by_rank(padded_rank(p.R), [&](auto rp) -> int {
     constexpr int RP = decltype(rp)::value;
     const int64_t T = p.tiles.T, tiles = p.tiles.tiles;
@@ -1344,8 +1346,8 @@ static int lora_shrink(const void* X, int64_t ldx, const void* W, bool wmn, int6
     if (rc) return rc;
     const int columns = wmn && RP < 64 ? 64 : RP;      // of an adapter; as many adapters as make 128 share a unit
     const int64_t slots = std::min<int64_t>(128 / columns, L), units = tiles * ceil_div(std::min<int64_t>(L, kLTile), slots);      // at most
-    if (p.split == 0) p.split = shrink_split(T, p.D, 2 * num_sms());
-    const int64_t clusters = std::min<int64_t>(units, 2 * num_sms() / p.split);
+    if (p.split == 0) p.split = shrink_split(T, p.D, 2 * sms);
+    const int64_t clusters = std::min<int64_t>(units, 2 * sms / p.split);
     p.stage = kLBox + static_cast<int>(slots) * columns * 128;
     p.stages = std::min(kShrinkMost, kShrinkRing / p.stage);
     auto run = [&](auto mn) -> int {
@@ -1360,7 +1362,7 @@ static int lora_shrink(const void* X, int64_t ldx, const void* W, bool wmn, int6
 }
 
 // W: (L,N,R), or (wmn) (L,R,N)
-static int lora_expand(const void* V, const void* W, bool wmn, int64_t L, int64_t R, const void* base, int64_t ldb, void* out, ExpandParams p, cudaStream_t st) {
+static int lora_expand(const void* V, const void* W, bool wmn, int64_t L, int64_t R, const void* base, int64_t ldb, void* out, ExpandParams p, int sms, cudaStream_t st) {
   return by_rank(padded_rank(R), [&](auto rp) -> int {
     constexpr int RP = decltype(rp)::value;
     CUtensorMap tmV, tmW, tmB, tmO;
@@ -1372,9 +1374,9 @@ static int lora_expand(const void* V, const void* W, bool wmn, int64_t L, int64_
     if (rc == 0 && base != nullptr) rc = make_map(&tmB, base, N, T, 1, ldb, ldb * T, 64, 32);
     if (rc) return rc;
     p.has_base = base != nullptr;
-    p.chunk = p.tiles.tiles * ceil_div(N, 128) <= num_sms() ? 1 : 2;
+    p.chunk = p.tiles.tiles * ceil_div(N, 128) <= sms ? 1 : 2;
     p.items = static_cast<int>(p.tiles.tiles * ceil_div(ceil_div(N, 128), p.chunk));
-    const int grid = static_cast<int>(std::min<int64_t>(num_sms(), p.items));
+    const int grid = static_cast<int>(std::min<int64_t>(sms, p.items));
     auto run = [&](auto mn) -> int {
       constexpr bool MN = decltype(mn)::value;
       static PerDevice allowed;
@@ -1387,15 +1389,15 @@ static int lora_expand(const void* V, const void* W, bool wmn, int64_t L, int64_
 }
 
 // Shares of the rows: as many as it takes for two CTAs an SM, each with eight blocks of rows at least
-static int wgrad_splits(int64_t T, int64_t D, int64_t L) {
+static int wgrad_splits(int64_t T, int64_t D, int64_t L, int sms) {
   const int64_t blocks = ceil_div(T, 64), ctas = ceil_div(D, 128) * L;
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2 * num_sms() / ctas, blocks / 8)));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2 * sms / ctas, blocks / 8)));
 }
 // The same for the gradient of B, which shares its launch with u = g B where that is wanted: one CTA an SM of either role.  By itself it has as many shares,
 // so that its bits do not depend on what else is asked for.
-static int back_wgrad_splits(int64_t T, int64_t D, int64_t L) {
+static int back_wgrad_splits(int64_t T, int64_t D, int64_t L, int sms) {
   const int64_t blocks = ceil_div(T, 64), ctas = ceil_div(D, 128) * L;
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(num_sms() / ctas, blocks / 8)));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms / ctas, blocks / 8)));
 }
 static int lora_wgrad(const void* Y, int64_t ldy, const void* V, int splits, WgradParams p, float* ws, void* out, int out_f32, cudaStream_t st) {
   return by_rank(padded_rank(p.R), [&](auto rp) -> int {
@@ -1422,7 +1424,8 @@ static int lora_wgrad(const void* Y, int64_t ldy, const void* V, int splits, Wgr
 }
 
 // The launch of both: an SM holds a CTA of each role
-static int lora_back(const void* G, const void* B, const void* V, int64_t L, ShrinkParams p, WgradParams w, float* ws, void* out, int out_f32, cudaStream_t st) {
+static int lora_back(const void* G, const void* B, const void* V, int64_t L, ShrinkParams p, WgradParams w, int splits, int sms, float* ws, void* out, int out_f32,
+                     cudaStream_t st) {
   return by_rank(padded_rank(p.R), [&](auto rp) -> int {
     constexpr int RP = decltype(rp)::value;
     const int64_t T = p.tiles.T, D = p.D, tiles = p.tiles.tiles;
@@ -1434,10 +1437,10 @@ static int lora_back(const void* G, const void* B, const void* V, int64_t L, Shr
     if (rc) return rc;
     const int columns = RP < 64 ? 64 : RP;
     const int64_t slots = std::min<int64_t>(128 / columns, L), units = tiles * ceil_div(std::min<int64_t>(L, kLTile), slots);
-    const int64_t shrinks = std::min<int64_t>(units, num_sms() / p.split);
+    const int64_t shrinks = std::min<int64_t>(units, sms / p.split);
     p.stage = kLBox + static_cast<int>(slots) * columns * 128;
     p.stages = std::min(kShrinkMost, kShrinkRing / p.stage);
-    w.splits = back_wgrad_splits(T, D, L);
+    w.splits = splits;
     w.y = static_cast<const __nv_bfloat16*>(G);
     w.v = static_cast<const __nv_bfloat16*>(V);
     w.ldy = D;
@@ -1502,8 +1505,8 @@ static bool lora_few(int64_t T, int64_t R, int64_t L, int keep) { return !keep &
 // CTAs of a cluster: eight, and four where the clusters of all groups there may be would not be on the SMs at once although a warp's columns fit one chunk, or
 // would come round twice.  us, eight / four: 2048 x 2816, rank 16, 512 rows of 32 adapters 14.9 / 13.1, 128 rows of 128 16.8 / 9.5, 64 rows of 8 7.6 / 7.7; 4096 x
 // 14336, 64 rows of 64 12.8 / 16.6, 512 rows of 32 26 / 29, 128 rows of 128 27 / 22; 4096 x 4096, 512 rows of 32 15.7 / 17.0, 256 rows of 128 27.5 / 24.0.
-static int few_cluster(int64_t T, int64_t N, int64_t R, int64_t L, int64_t groups) {
-  const int64_t room = static_cast<int64_t>(num_sms()) * kFewSm, rows = std::min<int64_t>(kFewRows, ceil_div(T, L));
+static int few_cluster(int64_t T, int64_t N, int64_t R, int64_t L, int64_t groups, int sms) {
+  const int64_t room = static_cast<int64_t>(sms) * kFewSm, rows = std::min<int64_t>(kFewRows, ceil_div(T, L));
   const bool fits = N * 2 * (R + rows) <= 4 * kFewWarps * kFewChunk;
   return groups * 8 > (fits ? room : 2 * room) ? 4 : 8;
 }
@@ -1549,12 +1552,13 @@ int b200moe_lora_forward(const void* x, int64_t ldx, const void* a, const void* 
                      (index == nullptr || reinterpret_cast<uintptr_t>(index) % index_bytes == 0),
                  B200MOE_E_ALIGN, "lora_forward: tensors must be 16-byte aligned, the index as its type");
   cudaStream_t st = (cudaStream_t)stream;
+  const int sms = gemm_cta_budget();
   const LoraIndex ix{index, index_bytes, static_cast<int>(T), static_cast<int>(L), status};
   if (lora_few(T, R, L, keep)) {
     const int64_t groups = few_groups(ix);
     FewRank *ranks = index != nullptr && T > kFewInline ? static_cast<FewRank*>(ws) : nullptr, *leaders = ranks != nullptr ? ranks + T : nullptr;
-    const int ctas = few_cluster(T, N, R, L, groups);
-    const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(num_sms() / (groups * ctas), ceil_div(N, 8 * kFewWarps * ctas))));
+    const int ctas = few_cluster(T, N, R, L, groups, sms);
+    const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms / (groups * ctas), ceil_div(N, 8 * kFewWarps * ctas))));
     const FewLora p{ix, static_cast<const __nv_bfloat16*>(x), static_cast<const __nv_bfloat16*>(a), static_cast<const __nv_bfloat16*>(b),
                     static_cast<const __nv_bfloat16*>(base), static_cast<__nv_bfloat16*>(out), ldx, ldb, ranks, leaders, static_cast<int>(K),
                     static_cast<int>(N), static_cast<int>(R), parts, scales, scale};
@@ -1580,11 +1584,11 @@ int b200moe_lora_forward(const void* x, int64_t ldx, const void* a, const void* 
   }
   {
     OpScope scope("lora_shrink", 1);
-    const int rc2 = lora_shrink(x, ldx, a, false, L, ShrinkParams{k.tiles, static_cast<int>(K), static_cast<int>(R), 0, 0, 0, scales, scale, k.v, k.counter, status}, st);
+    const int rc2 = lora_shrink(x, ldx, a, false, L, ShrinkParams{k.tiles, static_cast<int>(K), static_cast<int>(R), 0, 0, 0, scales, scale, k.v, k.counter, status}, sms, st);
     if (rc2) return rc2;
   }
   OpScope scope("lora_expand", 1);
-  return lora_expand(k.v, b, false, L, R, base, ldb, out, ExpandParams{k.tiles, static_cast<int>(N), 0, 0, 0, k.counter, status}, st);
+  return lora_expand(k.v, b, false, L, R, base, ldb, out, ExpandParams{k.tiles, static_cast<int>(N), 0, 0, 0, k.counter, status}, sms, st);
 }
 
 size_t b200moe_lora_bwd_ws_bytes(int64_t T, int64_t K, int64_t N, int64_t R, int64_t L) {
@@ -1592,7 +1596,7 @@ size_t b200moe_lora_bwd_ws_bytes(int64_t T, int64_t K, int64_t N, int64_t R, int
   LoraCarver c{nullptr};
   c.take<__nv_bfloat16>(2 * T * padded_rank(R));
   c.take<int>(1);
-  const int sa = wgrad_splits(T, K, L), sb = back_wgrad_splits(T, N, L);
+  const int sa = wgrad_splits(T, K, L, num_sms()), sb = back_wgrad_splits(T, N, L, num_sms());
   c.take<float>(std::max(sa > 1 ? sa * L * R * K : 0, sb > 1 ? sb * L * R * N : 0));
   return c.off;
 }
@@ -1609,6 +1613,7 @@ int b200moe_lora_backward(const void* grad_out, const void* x, int64_t ldx, cons
                      aligned16(grad_a) && aligned16(grad_b),
                  B200MOE_E_ALIGN, "lora_backward: tensors must be 16-byte aligned");
   cudaStream_t st = (cudaStream_t)stream;
+  const int sms = gemm_cta_budget();
   size_t bytes;
   const LoraKept k = carve_lora(T, R, L, has_index != 0, 1, const_cast<void*>(fwd_ws), &bytes);
   LoraCarver c{static_cast<char*>(ws)};
@@ -1623,19 +1628,19 @@ int b200moe_lora_backward(const void* grad_out, const void* x, int64_t ldx, cons
     const int rc__ = (call);          \
     if (rc__) return rc__;            \
   } while (0)
-  const ShrinkParams sp{k.tiles, static_cast<int>(N), static_cast<int>(R), shrink_split(T, N, num_sms()), 0, 0, scales, scale, u, counter, status};
-  const int sa = wgrad_splits(T, K, L), sb = back_wgrad_splits(T, N, L);
+  const ShrinkParams sp{k.tiles, static_cast<int>(N), static_cast<int>(R), shrink_split(T, N, sms), 0, 0, scales, scale, u, counter, status};
+  const int sa = wgrad_splits(T, K, L, sms), sb = back_wgrad_splits(T, N, L, sms);
   if (grad_b && (grad_x || grad_a)) {
     w.D = static_cast<int>(N);
-    RUN("lora_back", sb > 1 ? 2 : 1, lora_back(grad_out, b, k.v, L, sp, w, part, grad_b, grad_f32, st));
+    RUN("lora_back", sb > 1 ? 2 : 1, lora_back(grad_out, b, k.v, L, sp, w, sb, sms, part, grad_b, grad_f32, st));
   } else if (grad_b) {
     w.D = static_cast<int>(N);
     RUN("lora_wgrad", sb > 1 ? 2 : 1, lora_wgrad(grad_out, N, k.v, sb, w, part, grad_b, grad_f32, st));
   } else {
-    RUN("lora_shrink", 1, lora_shrink(grad_out, N, b, true, L, sp, st));
+    RUN("lora_shrink", 1, lora_shrink(grad_out, N, b, true, L, sp, sms, st));
   }
   if (grad_x)
-    RUN("lora_expand", 1, lora_expand(u, a, true, L, R, nullptr, 0, grad_x, ExpandParams{k.tiles, static_cast<int>(K), 0, 0, 0, counter, status}, st));
+    RUN("lora_expand", 1, lora_expand(u, a, true, L, R, nullptr, 0, grad_x, ExpandParams{k.tiles, static_cast<int>(K), 0, 0, 0, counter, status}, sms, st));
   if (grad_a) {
     w.D = static_cast<int>(K);
     w.transposed = 1;

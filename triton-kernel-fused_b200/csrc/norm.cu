@@ -734,14 +734,16 @@ static int by_types(int type, int w_type, F f) {
 static bool vectors(const void* p, int64_t ld, int type) { return aligned16(p) && (ld * type_bytes(type)) % 16 == 0; }
 
 static int row_threads(int64_t K, int nv) { return static_cast<int>((K + 8 * nv * 32 - 1) / (8 * nv * 32)) * 32; }
-static int64_t norm_ctas(int64_t rows, int rows_cta, int threads, int threads_sm) {
-  return std::max<int64_t>(1, std::min<int64_t>((rows + rows_cta - 1) / rows_cta, static_cast<int64_t>(num_sms()) * (threads_sm / threads)));
+// `sms`: gemm_cta_budget() of the call, since these grids stay until their rows are done and SMs reserved for an exchange are not theirs.  The workspace of the
+// weight's gradient is sized for num_sms().
+static int64_t norm_ctas(int64_t rows, int rows_cta, int threads, int threads_sm, int sms) {
+  return std::max<int64_t>(1, std::min<int64_t>((rows + rows_cta - 1) / rows_cta, static_cast<int64_t>(sms) * (threads_sm / threads)));
 }
 
 // Threads, rows a turn and turns in the ring for rows through shared memory: a vector of a row a thread up to 2048 values, two up to 4096, else four; as many
 // CTAs an SM as have two turns in the ring and 512 threads between them
 static int rows_nv(int64_t K) { return K <= 2048 ? 1 : K <= 4096 ? 2 : 4; }
-static NormPlan norm_plan(int64_t rows, int64_t K, int64_t row_bytes, int size) {
+static NormPlan norm_plan(int64_t rows, int64_t K, int64_t row_bytes, int size, int sms) {
   const int nv = rows_nv(K), r = nv >= 4 ? 1 : (size == 4 ? 2 : 4) / nv;      // kNormR
   NormPlan p;
   p.tpr = row_threads(K, nv);
@@ -749,10 +751,10 @@ static NormPlan norm_plan(int64_t rows, int64_t K, int64_t row_bytes, int size) 
   p.threads = p.tpr * groups;
   p.group = groups * r;
   int ctas = std::max(1, 512 / p.threads);
-  while (p.group > 1 && p.group * static_cast<int64_t>(ctas) * num_sms() > rows) p.group = (p.group + 1) / 2;
+  while (p.group > 1 && p.group * static_cast<int64_t>(ctas) * sms > rows) p.group = (p.group + 1) / 2;
   while (ctas > 1 && 2 * p.group * row_bytes * ctas > kNormRing) --ctas;
   p.stages = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(8, kNormRing / ctas / (p.group * row_bytes))));
-  p.ctas = std::max<int64_t>(1, std::min<int64_t>((rows + p.group - 1) / p.group, static_cast<int64_t>(ctas) * num_sms()));
+  p.ctas = std::max<int64_t>(1, std::min<int64_t>((rows + p.group - 1) / p.group, static_cast<int64_t>(ctas) * sms));
   return p;
 }
 template <class F>
@@ -762,9 +764,9 @@ static int by_rows_nv(int64_t K, F f) {
 }
 // of the backward through registers
 static int bwd_threads(int64_t K) { return K <= 512 ? 256 : row_threads(K, K > 8192 ? 4 : 2); }
-static int64_t bwd_ctas(int64_t rows, int64_t K) {
+static int64_t bwd_ctas(int64_t rows, int64_t K, int sms) {
   const int threads = bwd_threads(K);
-  return norm_ctas(rows, K <= 512 ? 8 : 1, threads, std::max(512, threads));
+  return norm_ctas(rows, K <= 512 ? 8 : 1, threads, std::max(512, threads), sms);
 }
 
 }  // namespace b200moe
@@ -797,12 +799,13 @@ int b200moe_rms_norm_fwd(const void* x, int64_t ldx, const void* residual, int64
   const bool vec = K % 8 == 0 && vectors(x, ldx, type) && (residual == nullptr || vectors(residual, ldr, type)) && aligned16(weight) &&
                    (y == nullptr || vectors(y, K, type)) && (h == nullptr || vectors(h, K, type));
   const NormFwd a{x, residual, weight, ldx, ldr, y, h, static_cast<uint8_t*>(q), scale, scale_pitch_, rows, static_cast<int>(K), eps};
+  const int sms = gemm_cta_budget();
   OpScope scope("rms_norm_fwd", 1);
   return by_types(type, weight_type, [&](auto t, auto w) -> int {
     using T = decltype(t);
     using W = decltype(w);
     auto run = [&](auto kernel, int rows_cta, int threads) -> int {
-      B200_LAUNCH(kernel, static_cast<int>(norm_ctas(rows, rows_cta, threads, 1024)), threads, 0, stream, a);
+      B200_LAUNCH(kernel, static_cast<int>(norm_ctas(rows, rows_cta, threads, 1024, sms)), threads, 0, stream, a);
       return 0;
     };
     auto run_rows = [&](auto nv) -> int {
@@ -810,7 +813,7 @@ int b200moe_rms_norm_fwd(const void* x, int64_t ldx, const void* residual, int64
       static PerDevice allowed;
       B200_CUDA(allow_smem(allowed, rms_norm_fwd_rows_kernel<T, W, NV>, kNormRing));
       const int64_t row_bytes = K * static_cast<int64_t>(sizeof(T)) * (residual != nullptr ? 2 : 1);
-      const NormPlan p = norm_plan(rows, K, row_bytes, type_bytes(type));
+      const NormPlan p = norm_plan(rows, K, row_bytes, type_bytes(type), sms);
       B200_LAUNCH((rms_norm_fwd_rows_kernel<T, W, NV>), static_cast<int>(p.ctas), p.threads, p.stages * p.group * row_bytes, stream, a, p, status);
       return 0;
     };
@@ -824,7 +827,7 @@ int b200moe_rms_norm_fwd(const void* x, int64_t ldx, const void* residual, int64
 
 size_t b200moe_rms_norm_bwd_ws_bytes(int64_t rows, int64_t K) {
   if (rows <= 0 || K < 1 || K > kNormMaxK) return 0;
-  return static_cast<size_t>(std::max(bwd_ctas(rows, K), static_cast<int64_t>(8) * num_sms())) * K * sizeof(float);
+  return static_cast<size_t>(std::max(bwd_ctas(rows, K, num_sms()), static_cast<int64_t>(8) * num_sms())) * K * sizeof(float);
 }
 
 int b200moe_rms_norm_bwd(const void* grad_y, const void* grad_h, const void* h, int64_t ldh, int type, const void* weight, int weight_type, int64_t rows,
@@ -840,8 +843,9 @@ int b200moe_rms_norm_bwd(const void* grad_y, const void* grad_h, const void* h, 
                    (grad_h == nullptr || vectors(grad_h, K, type)) && (grad_x == nullptr || vectors(grad_x, K, type));
   const NormBwd a{grad_y, grad_h, h, weight, ldh, grad_x, grad_weight != nullptr ? static_cast<float*>(ws) : nullptr, rows, static_cast<int>(K), eps};
   const int64_t row_bytes = K * type_bytes(type) * (grad_h != nullptr ? 3 : 2);
-  const NormPlan p = norm_plan(rows, K, row_bytes, type_bytes(type));
-  const int64_t ctas = rows == 0 ? 0 : vec ? p.ctas : bwd_ctas(rows, K);
+  const int sms = gemm_cta_budget();
+  const NormPlan p = norm_plan(rows, K, row_bytes, type_bytes(type), sms);
+  const int64_t ctas = rows == 0 ? 0 : vec ? p.ctas : bwd_ctas(rows, K, sms);
   OpScope scope("rms_norm_bwd", (rows > 0) + (grad_weight != nullptr));
   return by_types(type, weight_type, [&](auto t, auto w) -> int {
     using T = decltype(t);
