@@ -70,8 +70,8 @@ int b200moe_selftest_bounded_wait(int32_t* status, int64_t limit_cycles, b200moe
  * 1 after they are queued.  NULL = none.  Process-wide; for measurement. */
 typedef void (*b200moe_observer_t)(const char* name, int launches, int phase);
 int b200moe_set_observer(b200moe_observer_t observer);
-/* host: keep `n` SMs free of the persistent GEMM kernels (process-wide, default 0) so that
- * communication kernels queued on another stream can run beside them.  No reference counterpart. */
+/* host: keep `n` SMs free of the persistent GEMM kernels, the adapters' row tiles among them, and of the norms
+ * (process-wide, default 0) so that communication kernels queued on another stream can run beside them.  No reference counterpart. */
 int b200moe_set_reserved_sms(int n);
 /* host: let b200moe_ep_combine_pull occupy at most `n` SMs (one 1024-thread CTA each; 0 = all SMs), the
  * counterpart of b200moe_set_reserved_sms when a pull runs beside a GEMM.  No reference counterpart. */

@@ -1498,8 +1498,10 @@ static LoraKept carve_lora(int64_t T, int64_t R, int64_t L, bool index, int keep
   return k;
 }
 // Whether the kernel of few rows takes a call.  us, few rows / row tiles, L2 warm.  One adapter, 4096 x 14336, rank 16: 16 rows 8.4 / 10.0, 128 rows 9.8 /
-// 10.5, 256 rows 14.4 / 11.8; 2048 x 2816, rank 64: 16 rows 9.3 / 9.5, 64 rows 11.4 / 9.4.  Several, 4096 x 4096, rank 16, rows of 32 adapters mixed:
-// 64 rows 8.6 / 23, 512 rows 16 / 29.
+// 10.5, 256 rows 14.4 / 11.8; 2048 x 2816, rank 64: 16 rows 9.3 / 9.5, 64 rows 11.4 / 9.4.  Several, 4096 x 4096, rank 16: rows of 32 adapters mixed 64 rows
+// 8.7 / 22.5, 512 rows 15.9 / 28.7; of two packed 7.6 / 13.6 and 13.1 / 14.5.  The rule does not see that few adapters of a high rank are better in row tiles.  Up to 128
+// rows it loses nothing up to rank 64 (4096 x 4096, rank 64, 128 rows of two packed 15.5 / 15.4) and a tenth at rank 128, but 2048 x 2816, two packed, 256 and 512 rows: rank 32 13.5 / 13.4 and 14.4 / 13.8, rank 64 17.8 / 14.3 and 18.8 / 14.9, rank 128
+// 26.2 / 15.9 and 28.2 / 16.7; eight mixed, 512 rows: rank 64 20.1 / 18.1, rank 128 38.1 / 23.8.  With 32 mixed it is right at every rank: 24.0 / 40.0 and 47.7 / 73.1.
 static bool lora_few(int64_t T, int64_t R, int64_t L, int keep) { return !keep && T <= (L > 1 ? kFewMost : R <= 32 ? 128 : 16); }
 
 // CTAs of a cluster: eight, and four where the clusters of all groups there may be would not be on the SMs at once although a warp's columns fit one chunk, or

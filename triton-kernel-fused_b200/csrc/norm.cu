@@ -7,8 +7,9 @@
 // The norm is taken of h as it goes on, rounded, so that the backward, which has h alone, computes the gradient of what the forward computed; rstd
 // is computed again there, from a row that is read anyway.  Codes are made from y in fp32, not from its rounding.  All sums are fp32.
 //
-// Bound by HBM: a row is read once.  Three forms: rows through shared memory, which a ring of bulk copies keeps full (rms_norm_*_rows); few rows, where
-// latency counts, and rows off a vector's boundary through registers (rms_norm_*).
+// Bound by HBM: a row is read once.  Three forms: rows through shared memory, which a ring of bulk copies keeps full (rms_norm_*_rows_kernel); few rows of a
+// forward, where latency counts, as vectors through registers (rms_norm_fwd_kernel with VEC); and rows off a vector's boundary value by value through registers
+// (rms_norm_*_kernel without).  The last is bound by its loads: 16384 x 2047 forward and backward 315 us, 16384 x 2048 through shared memory 85, of 82.
 #include <algorithm>
 #include <limits>
 
@@ -325,9 +326,9 @@ __global__ void __launch_bounds__(THREADS) rms_norm_bwd_kernel(const NormBwd a) 
 // ------------------------------------------------------------------------------------------------ rows through shared memory
 // A CTA takes up to `group` rows a turn.  Bulk copies keep a ring of `stages` turns full; `tpr` threads share the columns of a row, NV vectors each, and
 // have R rows of a turn at once, so that what is done once a turn (shuffles, a barrier, roots, addresses) is spread over 32
-// values a thread: what bounds these kernels next to HBM is the number of instructions a value.  us, of the floor at the rate of a plain copy: 16384 x 4096
-// with residual to codes 74 (72), 16384 x 2048 forward 38 (41: part of the result is still in L2), backward 44 (41).  With one vector of one row a thread
-// 113, 49 and 85; with rows in registers and no ring 97, 42 and 74.
+// values a thread: what bounds these kernels next to HBM is the number of instructions a value.  us from a cold cache, and the floor at the rate of a plain copy:
+// 16384 x 4096 with residual to codes 75.7 (72), 16384 x 2048 forward 40 (41: part of the result is still in L2), backward 44.5 (41).  With one vector of one row a
+// thread 113, 49 and 85; with rows in registers and no ring 97, 42 and 74.  fp32, 16384 x 2048, forward, backward and the weight's sum 175 (164).
 struct NormPlan {
   int threads, tpr, group, stages;
   long long ctas;

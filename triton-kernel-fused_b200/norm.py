@@ -103,8 +103,9 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
 
 def rms_norm_fp8_block(x, weight, residual=None, eps=1e-6, return_norm=False):
     """`rms_norm` whose rows leave as the block-scaled products read them: (codes float8_e4m3fn (..., K), scales fp32 (..., ceil(K/128))[, y][, h]),
-    the values being code * scale; y where return_norm, h where there is a residual.  K a multiple of 8.  Codes are the nearest to y before its
-    rounding (`fp8_block_quantize(y)` rounds twice).  `fp8_block_linear(y, w, s, quantized=(codes, scales))` takes them; they carry no gradient,
+    the values being code * scale; y where return_norm, h where there is a residual.  K a multiple of 8.  Codes are made from y before its
+    rounding (`fp8_block_quantize(y)` rounds twice) and are the nearest up to fp32's roundings of y and of the scale: a value in the middle between two
+    codes may take either.  `fp8_block_linear(y, w, s, quantized=(codes, scales))` takes them; they carry no gradient,
     y and h do."""
     fast = L.fast() if x.is_cuda else None
     res = None if fast is None else fast.rms_norm(x, weight, residual, eps, bool(return_norm), True, L.status_word(x.device))
